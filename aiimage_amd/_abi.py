@@ -120,6 +120,23 @@ class DecoderConfig(ctypes.Structure):
                 ("rope_sin", ctypes.c_void_p), ("workgroups", ctypes.c_int)]
 
 
+class PagedKv(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("heads_kv", ctypes.c_int),
+                ("head_dim", ctypes.c_int), ("table", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("sequences", ctypes.c_int),
+                ("table_width", ctypes.c_int)]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("rows", ctypes.c_int),
+                ("rotary_dim", ctypes.c_int), ("axes", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("section0", ctypes.c_int),
+                ("section1", ctypes.c_int), ("section2", ctypes.c_int),
+                ("section3", ctypes.c_int)]
+
+
 _lib = None
 
 
@@ -149,6 +166,7 @@ def _declare(L):
     PP = ctypes.POINTER(ctypes.c_void_p)
     TP = ctypes.POINTER(Tensor)
     AP = ctypes.POINTER(LinearArgs)
+    KP, RP, i64 = ctypes.POINTER(PagedKv), ctypes.POINTER(Rope), ctypes.c_int64
     sig = {
         "aexq_abi_version": (i32, []),
         "aexq_last_error": (ctypes.c_char_p, []),
@@ -184,6 +202,12 @@ def _declare(L):
         "aexq_attention_decode_rope_at": (i32, [P, P, P, P, P, P, i32, i32, i32, i32, P, P, P,
                                                 f32, P]),
         "aexq_decode_advance": (i32, [P, P, P, P, P, i32]),
+        "aexq_rope_append_paged": (i32, [P, KP, RP, P, i32, i32, P, i64, P, i64, P, i64, P, i64]),
+        "aexq_attention_prompt": (i32, [P, P, i64, P, i64, P, i64, P, P, i32, i32, i32, i32, i32,
+                                        i32, i32, f32, P, i64]),
+        "aexq_attention_prompt_paged": (i32, [P, KP, P, i64, P, i32, i32, f32, P, i64]),
+        "aexq_attention_decode_paged": (i32, [P, KP, P, i64, i32, f32, P, i64]),
+        "aexq_logprobs": (i32, [P, TP, P, P, P, i32, P, P]),
         "aexq_decoder_create": (i32, [P, ctypes.POINTER(DecoderConfig), ctypes.POINTER(DecoderLayer),
                                       i32, P, PP]),
         "aexq_decoder_run": (i32, [P, P, P, P]),

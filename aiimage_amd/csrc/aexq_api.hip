@@ -64,6 +64,16 @@ struct aexq_ctx {
   long long attn_cap = 0;
   int* attn_count = nullptr;  // per kv head: splits finished in the running launch
   long long attn_count_cap = 0;
+  // partial rows and run plan of decode attention over a paged cache
+  float* paged_part = nullptr;
+  long long paged_part_cap = 0;
+  int* paged_plan = nullptr;
+  long long paged_plan_cap = 0;
+  // per part of a logits row: sums, and its best logits
+  float* logprob_stats = nullptr;
+  long long logprob_stats_cap = 0;
+  unsigned long long* logprob_keys = nullptr;
+  long long logprob_keys_cap = 0;
   // split-K partial planes of the MFMA kernels
   float* sk_part = nullptr;
   long long sk_cap = 0;
@@ -197,6 +207,10 @@ extern "C" void aexq_destroy(aexq_ctx* ctx) {
   (void)hipFree(ctx->gather_scratch);
   (void)hipFree(ctx->attn_part);
   (void)hipFree(ctx->attn_count);
+  (void)hipFree(ctx->paged_part);
+  (void)hipFree(ctx->paged_plan);
+  (void)hipFree(ctx->logprob_stats);
+  (void)hipFree(ctx->logprob_keys);
   (void)hipFree(ctx->sk_part);
   (void)hipFree(ctx->am_tagged);
   (void)hipFree(ctx->am_epoch);
@@ -2011,6 +2025,321 @@ extern "C" aexq_status aexq_decode_advance(aexq_ctx* ctx, int32_t* position, int
   hipError_t e = decode_advance_launch(position, token, argmax, tokens_out,
                                        tokens_out ? tokens_cap : 0, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "advance launch");
+  return AEXQ_OK;
+}
+
+// ---------------------------------------------------------------------------
+// many sequences: a paged cache, prompts, log probabilities
+// ---------------------------------------------------------------------------
+static bool is_head_dim(int d) { return d == 64 || d == 128 || d == 256; }
+
+// A cache descriptor as the kernels take it.
+static aexq_status view_paged(const aexq_paged_kv* kv, const char* op, PagedView* v) {
+  if (!kv || !kv->k || !kv->v || !kv->table || !kv->lengths)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL in the paged cache");
+  if (kv->pages <= 0 || kv->heads_kv <= 0 || kv->sequences <= 0 || kv->table_width <= 0)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op,
+                "pages=%d heads_kv=%d sequences=%d table_width=%d", kv->pages, kv->heads_kv,
+                kv->sequences, kv->table_width);
+  if (!is_head_dim(kv->head_dim))
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "head_dim=%d (64, 128 or 256) | layer=SDPA",
+                kv->head_dim);
+  const int ps = kv->page_size;
+  if (ps < 16 || ps > 4096 || (ps & (ps - 1)))
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "page_size=%d (a power of two, 16 to 4096)", ps);
+  if (kv->sequences > 65535)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "sequences=%d (at most 65535)", kv->sequences);
+  if ((long long)kv->table_width * ps > 0x7fffffffLL - 4096)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "table_width=%d pages of %d hold 2^31 positions or more",
+                kv->table_width, ps);
+  if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "pages not 16-byte aligned");
+  v->k = (const _Float16*)kv->k;
+  v->v = (const _Float16*)kv->v;
+  v->table = kv->table;
+  v->lengths = kv->lengths;
+  v->pages = kv->pages;
+  v->shift = __builtin_ctz(ps);
+  v->width = kv->table_width;
+  v->n = kv->sequences;
+  v->hkv = kv->heads_kv;
+  return AEXQ_OK;
+}
+
+// `heads` heads of `d` per row, rows `stride` elements apart.
+static aexq_status check_rows(const char* op, const char* name, const void* data, int64_t stride,
+                              int heads, int d) {
+  if (!data) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "%s is NULL", name);
+  if (stride < (int64_t)heads * d)
+    return fail(AEXQ_ERR_SHAPE, op, "%s rows %lld elements apart hold %d heads of %d", name,
+                (long long)stride, heads, d);
+  if ((uintptr_t)data % 16 || stride % 8)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%s rows not 16-byte aligned (stride %lld)", name,
+                (long long)stride);
+  return AEXQ_OK;
+}
+
+// Query heads over key heads, and the scale.
+static aexq_status check_heads(const char* op, int heads_q, int heads_kv, float scale) {
+  if (heads_kv <= 0 || heads_q <= 0 || heads_q % heads_kv != 0)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "heads_q=%d heads_kv=%d", heads_q, heads_kv);
+  if ((long long)heads_q * 256 > 0x7fffffffLL || heads_kv > 65535)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "heads_q=%d heads_kv=%d", heads_q, heads_kv);
+  if (!(scale > 0.0f) || !(scale <= 3.0e38f))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "scale=%g (positive and finite)", (double)scale);
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv,
+                                              const aexq_rope* rope, const int32_t* offsets,
+                                              int tokens, int heads_q, const void* q,
+                                              int64_t q_stride, const void* k, int64_t k_stride,
+                                              const void* v, int64_t v_stride, void* q_out,
+                                              int64_t q_out_stride) {
+  const char* op = "aexq_rope_append_paged";
+  if (!ctx || !rope || !offsets || !rope->cos_table || !rope->sin_table)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  RopeAppendParams p{};
+  aexq_status st = view_paged(kv, op, &p.kv);
+  if (!st && (tokens <= 0 || tokens > 1 << 23))
+    st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens=%d (1 to 2^23)", tokens);
+  if (!st) st = check_heads(op, heads_q, heads_q, 1.0f);
+  if (!st) st = check_rows(op, "q", q, q_stride, heads_q, kv->head_dim);
+  if (!st) st = check_rows(op, "k", k, k_stride, kv->heads_kv, kv->head_dim);
+  if (!st) st = check_rows(op, "v", v, v_stride, kv->heads_kv, kv->head_dim);
+  if (!st) st = check_rows(op, "q_out", q_out, q_out_stride, heads_q, kv->head_dim);
+  if (st) return st;
+  const int half = rope->rotary_dim / 2;
+  if (rope->rotary_dim <= 0 || rope->rotary_dim % 16 || rope->rotary_dim > kv->head_dim)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "rotary_dim=%d (a multiple of 16, at most head_dim=%d)",
+                rope->rotary_dim, kv->head_dim);
+  if (rope->rows <= 0 || rope->axes < 1 || rope->axes > 4)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "rows=%d axes=%d", rope->rows, rope->axes);
+  if (!rope->positions && rope->axes != 1)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "axes=%d need positions", rope->axes);
+  const int sections[4] = {rope->section0, rope->section1, rope->section2, rope->section3};
+  int sum = 0;
+  for (int a = 0; a < rope->axes; ++a) {
+    // (interleaved, the last pair of axis a > 0 is a + axes (sections[a] - 1))
+    if (sections[a] < 0 || sections[a] > half ||
+        (rope->interleaved && a && sections[a] &&
+         a + rope->axes * (sections[a] - 1) >= half))
+      return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "section %d of %d pairs does not fit %d", a,
+                  sections[a], half);
+    sum += sections[a];
+  }
+  if (sum != half)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "sections hold %d pairs of %d", sum, half);
+  p.kp = (_Float16*)kv->k;
+  p.vp = (_Float16*)kv->v;
+  p.offsets = offsets;
+  p.tokens = tokens;
+  p.hq = heads_q;
+  p.d = kv->head_dim;
+  p.q = (const _Float16*)q;
+  p.k = (const _Float16*)k;
+  p.v = (const _Float16*)v;
+  p.q_out = (_Float16*)q_out;
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.q_out_stride = q_out_stride;
+  p.cos_table = rope->cos_table;
+  p.sin_table = rope->sin_table;
+  p.positions = rope->positions;
+  p.rows = rope->rows;
+  p.rot = rope->rotary_dim;
+  p.axes = rope->axes;
+  p.interleaved = rope->interleaved;
+  memcpy(p.sections, sections, sizeof(sections));
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = rope_append_launch(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "rope append launch");
+  return AEXQ_OK;
+}
+
+// The two prompt entry points behind their descriptors.
+static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, int heads_q,
+                              int head_dim, float scale) {
+  if (p.n <= 0 || p.tokens <= 0)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "sequences=%d tokens=%d", p.n, p.tokens);
+  p.group = heads_q / p.hkv;
+  p.scale2 = scale * 1.4426950408889634f;
+  // rows of one sequence are counted in 31 bits, tiles are a grid's second axis
+  if ((long long)p.tokens * p.group > 0x7fffffffLL - 4096 ||
+      prompt_tiles(p.tokens, p.n, p.group) > 65535)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "tokens=%d of %d heads per key head in one call",
+                p.tokens, p.group);
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = prompt_launch(p, head_dim, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "attention launch");
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64_t q_stride,
+                                             const void* k, int64_t k_stride, const void* v,
+                                             int64_t v_stride, const int32_t* q_offsets,
+                                             const int32_t* kv_offsets, int sequences, int tokens,
+                                             int kv_tokens, int heads_q, int heads_kv,
+                                             int head_dim, int causal, float scale, void* out,
+                                             int64_t out_stride) {
+  const char* op = "aexq_attention_prompt";
+  if (!ctx || !q_offsets) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  if (!is_head_dim(head_dim))
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "head_dim=%d (64, 128 or 256) | layer=SDPA", head_dim);
+  aexq_status st = check_heads(op, heads_q, heads_kv, scale);
+  if (!st) st = check_rows(op, "q", q, q_stride, heads_q, head_dim);
+  if (!st) st = check_rows(op, "k", k, k_stride, heads_kv, head_dim);
+  if (!st) st = check_rows(op, "v", v, v_stride, heads_kv, head_dim);
+  if (!st) st = check_rows(op, "out", out, out_stride, heads_q, head_dim);
+  if (!st && (kv_tokens <= 0 || (!kv_offsets && kv_tokens != tokens)))
+    st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "kv_tokens=%d tokens=%d", kv_tokens, tokens);
+  if (!st && sequences > 65535)
+    st = fail(AEXQ_ERR_UNSUPPORTED, op, "sequences=%d (at most 65535)", sequences);
+  if (st) return st;
+  PromptParams p{};
+  p.q = (const _Float16*)q;
+  p.k = (const _Float16*)k;
+  p.v = (const _Float16*)v;
+  p.out = (_Float16*)out;
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.out_stride = out_stride;
+  p.q_offsets = q_offsets;
+  p.kv_offsets = kv_offsets ? kv_offsets : q_offsets;
+  p.n = sequences;
+  p.tokens = tokens;
+  p.kv_tokens = kv_tokens;
+  p.hkv = heads_kv;
+  p.causal = causal != 0;
+  return prompt_run(ctx, op, p, heads_q, head_dim, scale);
+}
+
+extern "C" aexq_status aexq_attention_prompt_paged(aexq_ctx* ctx, const aexq_paged_kv* kv,
+                                                   const void* q, int64_t q_stride,
+                                                   const int32_t* offsets, int tokens, int heads_q,
+                                                   float scale, void* out, int64_t out_stride) {
+  const char* op = "aexq_attention_prompt_paged";
+  if (!ctx || !offsets) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  PromptParams p{};
+  aexq_status st = view_paged(kv, op, &p.kv);
+  if (!st) st = check_heads(op, heads_q, kv->heads_kv, scale);
+  if (!st) st = check_rows(op, "q", q, q_stride, heads_q, kv->head_dim);
+  if (!st) st = check_rows(op, "out", out, out_stride, heads_q, kv->head_dim);
+  if (st) return st;
+  p.q = (const _Float16*)q;
+  p.out = (_Float16*)out;
+  p.q_stride = q_stride;
+  p.out_stride = out_stride;
+  p.q_offsets = offsets;
+  p.n = kv->sequences;
+  p.tokens = tokens;
+  p.hkv = kv->heads_kv;
+  p.causal = 1;
+  return prompt_run(ctx, op, p, heads_q, kv->head_dim, scale);
+}
+
+extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_paged_kv* kv,
+                                                   const void* q, int64_t q_stride, int heads_q,
+                                                   float scale, void* out, int64_t out_stride) {
+  const char* op = "aexq_attention_decode_paged";
+  if (!ctx) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "ctx is NULL");
+  DecodePagedParams p{};
+  aexq_status st = view_paged(kv, op, &p.kv);
+  if (!st) st = check_heads(op, heads_q, kv->heads_kv, scale);
+  if (!st) st = check_rows(op, "q", q, q_stride, heads_q, kv->head_dim);
+  if (!st) st = check_rows(op, "out", out, out_stride, heads_q, kv->head_dim);
+  if (!st && out == q)
+    st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is q, which other workgroups still read");
+  if (st) return st;
+  p.q = (const _Float16*)q;
+  p.out = (_Float16*)out;
+  p.q_stride = q_stride;
+  p.out_stride = out_stride;
+  p.group = heads_q / kv->heads_kv;
+  p.blocks = (p.group + 15) / 16;
+  p.scale2 = scale * 1.4426950408889634f;
+  p.min_run = 1;
+  const long long bound = (long long)kv->table_width * kv->page_size;
+  const int grid = decode_paged_split(bound) ? decode_paged_grid(ctx->cus) : 0;
+  // runs count units of all sequences in 31 bits
+  const long long units =
+      (bound / 128 + 1) * kv->sequences * (long long)(kv->heads_kv * p.blocks);
+  if (units > 0x7fffffffLL - (1 << 20))
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d sequences of up to %lld positions in one call",
+                kv->sequences, bound);
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  if (grid) {
+    st = grow_scratch(ctx, (void**)&ctx->paged_part, &ctx->paged_part_cap,
+                      decode_paged_part_floats(kv->head_dim, grid) * (long long)sizeof(float), op,
+                      "paged attention partials");
+    if (!st)
+      st = grow_scratch(ctx, (void**)&ctx->paged_plan, &ctx->paged_plan_cap,
+                        (1LL + kv->sequences) * (long long)sizeof(int), op,
+                        "paged attention plan");
+    if (st) return st;
+    p.part = ctx->paged_part;
+    p.plan = ctx->paged_plan;
+  }
+  const hipError_t e = decode_paged_launch(p, kv->head_dim, grid, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "attention launch");
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_logprobs(aexq_ctx* ctx, const aexq_tensor* logits,
+                                     const int32_t* tokens, float* logprob, float* entropy,
+                                     int top, int32_t* top_ids, float* top_logprobs) {
+  const char* op = "aexq_logprobs";
+  if (!ctx) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "ctx is NULL");
+  TensorView v;
+  aexq_status st = view_tensor(logits, op, "logits", &v);
+  if (st) return st;
+  if (v.head_dim || v.batch > 1)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "head-packed or batched logits | rejectedFallback=layout");
+  if (logprob && !tokens)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "log probabilities of which tokens?");
+  if (top < 0 || top > 64 || top > v.width)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "top=%d (0 to 64, at most the %d logits)", top,
+                v.width);
+  if (!logprob && !entropy && !(top && (top_ids || top_logprobs)))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "no output asked for");
+  const int esize = v.dtype == AEXQ_DTYPE_F16 ? 2 : 4;
+  if ((uintptr_t)v.data % esize)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "logits not aligned to their type");
+  if (v.width > 1 << 30 || v.rows > 1 << 23)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d rows of %d logits (at most 2^23 of 2^30)", v.rows,
+                v.width);
+  LogprobParams p{};
+  p.x = v.data;
+  p.f16 = esize == 2;
+  p.rows = v.rows;
+  p.rstride = v.rstride;
+  p.n = v.width;
+  p.tokens = tokens;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top = top;
+  p.ids = top_ids;
+  p.values = top_logprobs;
+  p.parts = logprob_parts(p.rows, p.n, esize, ctx->cus);
+  const int ve = 16 / esize;  // chunks of a row that starts anywhere in one
+  p.cols = (int)(((long long)p.n + 2 * ve - 2) / ve / p.parts + 1);
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  if (p.parts > 1) {
+    const long long n = p.rows * p.parts;
+    st = grow_scratch(ctx, (void**)&ctx->logprob_stats, &ctx->logprob_stats_cap,
+                      n * 4 * (long long)sizeof(float), op, "log probability sums");
+    if (!st)
+      st = grow_scratch(ctx, (void**)&ctx->logprob_keys, &ctx->logprob_keys_cap,
+                        (n * top + 1) * (long long)sizeof(unsigned long long), op,
+                        "log probability alternatives");
+    if (st) return st;
+    p.stats = ctx->logprob_stats;
+    p.keys = ctx->logprob_keys;
+  }
+  const hipError_t e = logprob_launch(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "log probability launch");
   return AEXQ_OK;
 }
 

@@ -1,0 +1,312 @@
+// Log probabilities of given tokens, entropy and top alternatives of rows of
+// logits (gfx950).
+#include <math.h>
+
+#include "aexq_device.hpp"
+
+namespace aexq {
+
+// ---------------------------------------------------------------------------
+// One pass over a row of logits x with a running maximum m, in log2 units:
+//   Z = sum e^(x - m),  T = sum e^(x - m) (x - m) log2 e
+//   log p[t] = (x[t] - m) - ln Z,   H = ln Z - T ln 2 / Z
+// (x - m is taken before anything is rounded, so large logits lose nothing).
+// Lanes take 16-byte chunks in turn; what a lane keeps for the alternatives is
+// its best chunk (by its largest logit) and the largest logit of the others.
+//
+// The K best of the row, by logit and then by index: among the 256 lanes' best
+// chunks the K-th is a bound that at least K logits reach, so only chunks that
+// reach it are read again (mostly about K of them), and a lane's whole share
+// only where its second chunk reaches it too.  Those logits go through a sorted
+// list per wave, an entry a lane; the four lists are merged by counting, for
+// each entry, the entries above it.
+//
+// Reading the logits bounds it (HBM).  Few rows are cut into parts of chunks, a
+// workgroup each, whose (m, Z, T, K best) a second launch joins in the same way.
+// ---------------------------------------------------------------------------
+typedef unsigned long long u64;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// x - m of a logit that weighs nothing (-inf among them), in log2 units
+constexpr float kFar = -300.0f;
+
+// Order of the alternatives: the larger logit, then the lower index.  0 is below
+// every logit.
+__device__ __forceinline__ u64 top_key(float x, int index) {
+  return (u64)argmax_ord(x) << 32 | (uint32_t)~index;
+}
+
+struct Stats {
+  float m, z, t;
+};
+// The sums of two parts on their common maximum; parts of weight 0 add 0.
+__device__ __forceinline__ Stats join(Stats a, Stats b) {
+  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
+  const float da = fmaxf((a.m - base) * kLog2e, kFar), db = fmaxf((b.m - base) * kLog2e, kFar);
+  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+  Stats r;
+  r.m = m;
+  r.z = a.z * fa + b.z * fb;
+  r.t = fa * fmaf(a.z, da, a.t) + fb * fmaf(b.z, db, b.t);
+  return r;
+}
+__device__ __forceinline__ Stats join_wave(Stats a) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    Stats b;
+    b.m = __shfl_xor(a.m, off, 64);
+    b.z = __shfl_xor(a.z, off, 64);
+    b.t = __shfl_xor(a.t, off, 64);
+    a = join(a, b);
+  }
+  return a;
+}
+
+// A row's outputs by its workgroup: thread r < top has the r-th key.  A row
+// whose logits have no finite sum of exponentials (a NaN, a +inf, or only -inf)
+// has no probabilities: NaN, and alternatives -1.
+template <typename E>
+__device__ __forceinline__ void row_outputs(const LogprobParams& p, int row, const E* x, Stats s,
+                                            u64 key) {
+  const bool sound = s.z > 0.0f && s.z < INFINITY;
+  const float ln = logf(s.z), nan = __builtin_nanf("");
+  if (threadIdx.x == 0) {
+    if (p.logprob) {
+      const int token = p.tokens[row];
+      float v = token == -1 ? 0.0f : nan;
+      if (sound && token >= 0 && token < p.n) v = ((float)x[token] - s.m) - ln;
+      p.logprob[row] = v;
+    }
+    if (p.entropy) p.entropy[row] = sound ? ln - s.t * kLn2 / s.z : nan;
+  }
+  if ((int)threadIdx.x < p.top) {
+    const long long at = (long long)row * p.top + threadIdx.x;
+    if (p.ids) p.ids[at] = sound ? (int)~(uint32_t)key : -1;
+    if (p.values) p.values[at] = sound ? (argmax_unord((uint32_t)(key >> 32)) - s.m) - ln : nan;
+  }
+}
+
+// Puts `key` (wave-uniform) into the wave's sorted list, an entry a lane.
+__device__ __forceinline__ void list_insert(u64& entry, u64 key) {
+  const int at = __popcll(__ballot(entry > key)), lane = threadIdx.x & 63;
+  const u64 up = __shfl_up(entry, 1, 64);
+  entry = lane < at ? entry : lane == at ? key : up;
+}
+
+template <typename E>
+__global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p) {
+  constexpr int VE = 16 / (int)sizeof(E), U = 4;  // logits of a chunk, chunks in flight
+  __shared__ Stats wave_stats[kWaves];
+  __shared__ u64 keys[kThreads], sorted[64], bound;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const E* x = (const E*)p.x + (long long)row * p.rstride;
+  // chunks lie on 16-byte boundaries: chunk c starts at logit c VE - skew
+  const int skew = (int)((uintptr_t)x % 16 / sizeof(E));
+  const int chunks = (int)(((long long)p.n + skew + VE - 1) / VE);
+  const int c0 = min(part * p.cols, chunks), c1 = min(c0 + p.cols, chunks);
+
+  // chunk c; logits before the row's first or past its last read -inf
+  auto read = [&](int c, float* v) {
+    const int i0 = c * VE - skew;
+    if (i0 >= 0 && i0 <= p.n - VE) {
+      E e[VE];
+      __builtin_memcpy(e, __builtin_assume_aligned(x + i0, 16), 16);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[i] = (float)e[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        v[i] = -INFINITY;
+        if (i0 + i >= 0 && i0 + i < p.n) v[i] = (float)x[i0 + i];
+      }
+    }
+  };
+
+  Stats s = {-INFINITY, 0.0f, 0.0f};
+  float best = -INFINITY, second = -INFINITY;
+  int best_chunk = c0 + tid;
+  for (int c = c0 + tid; c < c1; c += U * kThreads) {
+    float v[U][VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (c + u * kThreads < c1) {
+        read(c + u * kThreads, v[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[u][i] = -INFINITY;
+      }
+    }
+    float m = s.m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float top = v[u][0];
+#pragma unroll
+      for (int i = 1; i < VE; ++i) top = fmaxf(top, v[u][i]);
+      m = fmaxf(m, top);
+      second = fmaxf(second, fminf(best, top));
+      best_chunk = top > best ? c + u * kThreads : best_chunk;
+      best = fmaxf(best, top);
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    const float d = fmaxf((s.m - base) * kLog2e, kFar), f = __builtin_amdgcn_exp2f(d);
+    s.t = f * fmaf(s.z, d, s.t);
+    s.z *= f;
+    s.m = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const float y = (v[u][i] - base) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+        s.z += e;
+        s.t = fmaf(e, fmaxf(y, kFar), s.t);
+      }
+  }
+  s = join_wave(s);
+  if (lane == 0) wave_stats[wave] = s;
+
+  u64 key = 0;
+  if (p.top) {
+    const bool any = c0 + tid < c1;
+    // some logit of the best chunk is `best`, at the chunk's last index or before
+    const u64 mine = any ? top_key(best, min(best_chunk * VE - skew + VE, p.n) - 1) : 0;
+    keys[tid] = mine;
+    if (tid == 0) bound = 0;
+    if (tid < 64) sorted[tid] = 0;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < kThreads; ++i) above += keys[i] > mine;
+    if (any && above == p.top - 1) bound = mine;
+    __syncthreads();
+    const u64 least = bound;  // 0: fewer chunks than alternatives, so all of them
+    const bool all = any && argmax_ord(second) >= (uint32_t)(least >> 32);
+    const bool one = any && !all && top_key(best, max(best_chunk * VE - skew, 0)) >= least;
+    u64 entry = 0;
+    auto take = [&](int c, bool on) {
+      float v[VE];
+      if (on) read(c, v);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int at = c * VE - skew + i;
+        const bool in = on && at >= 0 && at < p.n && !__builtin_isnan(v[i]);
+        const u64 k = in ? top_key(v[i], at) : 0;
+        for (u64 left = __ballot(in && k >= least); left; left &= left - 1) {
+          const int from = __ffsll((unsigned long long)left) - 1;
+          const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(k >> 32), from);
+          const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)k, from);
+          list_insert(entry, (u64)hi << 32 | lo);
+        }
+      }
+    };
+    if (__any(one)) take(best_chunk, one);
+    for (u64 left = __ballot(all); left; left &= left - 1) {
+      // the whole share of one lane, by all lanes
+      const int from = __ffsll((unsigned long long)left) - 1;
+      for (int c = c0 + wave * 64 + from; c < c1; c += 64 * kThreads) {
+        const int at = c + lane * kThreads;
+        take(at, at < c1);
+      }
+    }
+    __syncthreads();
+    keys[tid] = lane < p.top ? entry : 0;
+    __syncthreads();
+    const u64 own = keys[tid];
+    above = 0;
+    for (int w = 0; w < kWaves; ++w)
+      for (int i = 0; i < p.top; ++i) above += keys[w * 64 + i] > own;
+    if (own && above < p.top) sorted[above] = own;
+  }
+  __syncthreads();
+  if (tid < p.top) key = sorted[tid];
+  s = wave_stats[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) s = join(s, wave_stats[w]);
+  if (p.parts == 1) {
+    row_outputs(p, row, x, s, key);
+    return;
+  }
+  if (tid == 0) {
+    float* to = p.stats + 4LL * blockIdx.x;
+    to[0] = s.m;
+    to[1] = s.z;
+    to[2] = s.t;
+  }
+  if (tid < p.top) p.keys[(long long)blockIdx.x * p.top + tid] = key;
+}
+
+// Joins the parts of a row (at most kThreads).
+template <typename E>
+__global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobParams p) {
+  __shared__ Stats wave_stats[kWaves];
+  __shared__ u64 first[kThreads], reach[64 * 64], sorted[64], bound;
+  __shared__ int count;
+  const int row = blockIdx.x, tid = threadIdx.x;
+  const u64* keys = p.keys + (long long)row * p.parts * p.top;
+  Stats s = {-INFINITY, 0.0f, 0.0f};
+  u64 mine = 0;
+  if (tid < p.parts) {
+    const float* from = p.stats + 4LL * (row * (long long)p.parts + tid);
+    s = Stats{from[0], from[1], from[2]};
+    if (p.top) mine = keys[(long long)tid * p.top];
+  }
+  s = join_wave(s);
+  if ((tid & 63) == 0) wave_stats[tid >> 6] = s;
+  u64 key = 0;
+  if (p.top) {
+    first[tid] = mine;
+    if (tid == 0) {
+      bound = 0;
+      count = 0;
+    }
+    if (tid < 64) sorted[tid] = 0;
+    __syncthreads();
+    int above = 0;
+    for (int i = 0; i < p.parts; ++i) above += first[i] > mine;
+    if (mine && above == p.top - 1) bound = mine;
+    __syncthreads();
+    const u64 least = bound;
+    // keys that reach the bound lie in at most top parts (top - 1 parts in all
+    // where there is no bound): no more than the buffer holds
+    for (int i = tid; i < p.parts * p.top; i += kThreads) {
+      const u64 k = keys[i];
+      if (k && k >= least) reach[atomicAdd(&count, 1)] = k;
+    }
+    __syncthreads();
+    const int n = count;
+    for (int i = tid; i < n; i += kThreads) {
+      const u64 own = reach[i];
+      above = 0;
+      for (int j = 0; j < n; ++j) above += reach[j] > own;
+      if (above < p.top) sorted[above] = own;
+    }
+  }
+  __syncthreads();
+  if (tid < p.top) key = sorted[tid];
+  s = wave_stats[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) s = join(s, wave_stats[w]);
+  row_outputs(p, row, (const E*)p.x + (long long)row * p.rstride, s, key);
+}
+
+// Parts of a row: enough for two workgroups per CU, each of at least 512 chunks.
+int logprob_parts(long long rows, int n, int esize, int cus) {
+  const long long chunks = ((long long)n * esize + 15) / 16;
+  const long long parts = (2LL * cus + rows - 1) / rows, most = (chunks + 511) / 512;
+  const long long r = parts < most ? parts : most;
+  return (int)(r < 1 ? 1 : r > kThreads ? kThreads : r);
+}
+
+template <typename E>
+static hipError_t dispatch(const LogprobParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(logprob_kernel<E>, dim3((unsigned)(p.rows * p.parts)), dim3(kThreads), 0,
+                     stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.parts == 1) return e;
+  hipLaunchKernelGGL(logprob_join_kernel<E>, dim3((unsigned)p.rows), dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t logprob_launch(const LogprobParams& p, hipStream_t stream) {
+  return p.f16 ? dispatch<f16>(p, stream) : dispatch<float>(p, stream);
+}
+
+}  // namespace aexq

@@ -1,0 +1,493 @@
+// Operators on a paged key/value cache (gfx950): rotary positions with the
+// append of packed tokens, and attention of one new token per sequence.
+//
+// The cache is a pool of fp16 pages [pages][heads_kv][page_size][head_dim]
+// for K and one for V; position x of sequence s is row x % page_size of page
+// table[s][x / page_size].  Lengths and tables live on the device, so a
+// captured launch follows them from step to step.
+#include <math.h>
+
+#include "aexq_paged.hpp"
+
+namespace aexq {
+
+// ---------------------------------------------------------------------------
+// Rotary positions and append.  One workgroup per packed token t: the cos and
+// sin of its head's pairs go to LDS once (pair j from the table row of its
+// axis' position), then each thread moves 16-byte pieces: eight pairs (j, j +
+// rot/2) of a q or k head, eight unrotated elements behind them, or eight of v.
+//   x'[j] = x[j] cos - x[j + rot/2] sin,  x'[j + rot/2] = x[j] sin + x[j + rot/2] cos
+// in fp32, rounded once to fp16.  Token t of a sequence with n new tokens and
+// length L (after the append) lands at position L - n + (t - first).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void rope_append_kernel(const RopeAppendParams p) {
+  __shared__ float cs[128], sn[128];
+  const int t = blockIdx.x, tid = threadIdx.x;
+  const int d = p.d, half = p.rot / 2;
+  const int r8 = half / 8, c8 = (d - p.rot) / 8, per_head = r8 + c8;
+  const int rotated = (p.hq + p.kv.hkv) * per_head, total = rotated + p.kv.hkv * (d / 8);
+
+  struct Piece {
+    u32x4 a, b;
+  };
+  auto source = [&](int id) -> const f16* {
+    if (id >= rotated)
+      return p.v + (long long)t * p.v_stride + (long long)(id - rotated) * 8;
+    const int head = id / per_head, sub = id % per_head;
+    const f16* row = head < p.hq ? p.q + (long long)t * p.q_stride + head * d
+                                 : p.k + (long long)t * p.k_stride + (head - p.hq) * d;
+    return row + (sub < r8 ? 8 * sub : p.rot + 8 * (sub - r8));
+  };
+  auto load = [&](int id) {
+    const f16* s = source(id);
+    Piece x;
+    x.a = *(const u32x4*)s;
+    x.b = x.a;
+    if (id < rotated && id % per_head < r8) x.b = *(const u32x4*)(s + half);
+    return x;
+  };
+  Piece x{};
+  if (tid < total) x = load(tid);  // before anything else is known of the token
+
+  const int s = packed_sequence(p.offsets, p.kv.n, t);
+  if (s >= p.kv.n) return;  // rows behind the last sequence stay as they were
+  const int first = p.offsets[s], count = p.offsets[s + 1] - first;
+  if (t < first) return;
+  const int pos = p.kv.lengths[s] - count + (t - first);
+  // where its k and v rows go; nowhere outside the table or the pool
+  int page = -1;
+  if (pos >= 0 && pos < p.kv.width << p.kv.shift)
+    page = p.kv.table[(long long)s * p.kv.width + (pos >> p.kv.shift)];
+  const bool keep = page >= 0 && page < p.kv.pages;
+  const int row = pos & ((1 << p.kv.shift) - 1);
+  if (tid < half) {
+    int axis = 0;
+    if (p.interleaved) {
+      axis = tid % p.axes;
+      if (tid >= p.axes * p.sections[axis]) axis = 0;
+    } else {
+      for (int a = 0, end = p.sections[0]; a + 1 < p.axes && tid >= end; end += p.sections[++a])
+        axis = a + 1;
+    }
+    int at = p.positions ? p.positions[(long long)axis * p.tokens + t] : pos;
+    at = min(max(at, 0), p.rows - 1);
+    cs[tid] = p.cos_table[(long long)at * half + tid];
+    sn[tid] = p.sin_table[(long long)at * half + tid];
+  }
+  __syncthreads();
+  for (int id = tid; id < total; id += kThreads) {
+    if (id != tid) x = load(id);
+    if (id >= rotated) {
+      if (!keep) continue;
+      const int g = (id - rotated) / (d / 8), e = (id - rotated) % (d / 8);
+      f16* to = p.vp + ((((long long)page * p.kv.hkv + g) << p.kv.shift) + row) * d;
+      *(u32x4*)(to + 8 * e) = x.a;
+      continue;
+    }
+    const int head = id / per_head, sub = id % per_head;
+    if (head >= p.hq && !keep) continue;
+    f16* to = head < p.hq
+                  ? p.q_out + (long long)t * p.q_out_stride + head * d
+                  : p.kp + ((((long long)page * p.kv.hkv + (head - p.hq)) << p.kv.shift) + row) * d;
+    if (sub >= r8) {
+      *(u32x4*)(to + p.rot + 8 * (sub - r8)) = x.a;
+      continue;
+    }
+    u32x4 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f16x2 a = as_h2(x.a[e]), b = as_h2(x.b[e]);
+      f16x2 u, w;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float c = cs[8 * sub + 2 * e + i], z = sn[8 * sub + 2 * e + i];
+        u[i] = (f16)((float)a[i] * c - (float)b[i] * z);
+        w[i] = (f16)((float)a[i] * z + (float)b[i] * c);
+      }
+      lo[e] = as_u(u);
+      hi[e] = as_u(w);
+    }
+    *(u32x4*)(to + 8 * sub) = lo;
+    *(u32x4*)(to + 8 * sub + half) = hi;
+  }
+}
+
+hipError_t rope_append_launch(const RopeAppendParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(rope_append_kernel, dim3(p.tokens), dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Attention of one new token per sequence, out = softmax(scale q K^T) V, for
+// the up to 16 query heads of a key/value head at a time (more take further
+// blocks).  A wave takes 32 positions a step with both products on matrix
+// instructions and K and V straight from the cache to registers:
+//   S^T = K q^T   16 positions x 16 heads x 32 dims: lane (c = l % 16, g = l / 16)
+//                 holds 8 dims of K row c; the result leaves lane (c, g) with
+//                 head c's scores of positions 4 g + r (+ 16 in the second half);
+//   O^T = V^T P^T those scores' weights are the right operand as they stand, if
+//                 its k index 8 g + i is position 4 g + i (i < 4) or 16 + 4 g + i
+//                 - 4.  So lane (c, g) loads D/16 consecutive dims of those 8 V
+//                 rows (16 lanes cover a row) and v_perm turns the 8 rows x D/16
+//                 dims into the left operands: product t has dims (D/16) m + t.
+// The waves of a workgroup take steps in turn and meet in LDS at the end.
+//
+// What bounds it is reading K and V once (HBM).  The work is cut into units of
+// kDecodeUnit positions of one (sequence, head block), laid end to end, and each
+// workgroup takes an equal run of units, so lengths may differ as they like and
+// the host need not know them.  A run that holds all of a (sequence, block)
+// writes its output; the others leave (max, sum, acc) rows that a second launch
+// joins.
+// ---------------------------------------------------------------------------
+constexpr int kDecodeUnit = 128;
+
+template <int D>
+struct DecodeLds {
+  static constexpr int HT = D / 16 < 8 ? D / 16 : 8;  // dims of a lane's run in one pass
+  static constexpr int W = 16 * HT;                   // dims of one pass
+  alignas(16) float o[kWaves][16][W + 4];
+  float m[kWaves][16], l[kWaves][16];
+  int seq, base, count[kWaves];
+};
+
+// One (sequence s, head block hb) over positions [p0, p1) of len, by the whole
+// workgroup.  `slot` null: the output, else the partial rows.
+template <int D>
+__device__ __forceinline__ void decode_piece(const DecodePagedParams& p, DecodeLds<D>& lds, int s,
+                                             int hb, int len, int p0, int p1, float* slot) {
+  constexpr int KS = D / 32, DPL = D / 16, HT = DecodeLds<D>::HT, W = DecodeLds<D>::W;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sreg(tid >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int h = hb / p.blocks, first = hb % p.blocks * 16;  // kv head, first query head of it
+  const int live = min(16, p.group - first);
+  const int mask = (1 << p.kv.shift) - 1;
+
+  f16x8 qf[KS];
+  {
+    const f16* row = p.q + (long long)s * p.q_stride + (h * p.group + first + min(c, live - 1)) * D;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+      qf[i] = c < live ? *(const f16x8*)(row + 32 * i + 8 * g) : f16x8{};
+  }
+  f32x4 acc[DPL];
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) acc[i] = f32x4{};
+  float m = -INFINITY, l = 0.0f;
+
+  for (int x = p0 + 32 * wave; x < p1; x += 32 * kWaves) {
+    // the two blocks of 16 positions; a block past the end repeats the last one
+    const int x1 = min(x + 16, (len - 1) & ~15);
+    const long long r0 =
+        (((long long)sreg(paged_page(p.kv, s, x >> p.kv.shift)) * p.kv.hkv + h) << p.kv.shift) +
+        (x & mask);
+    const long long r1 =
+        (((long long)sreg(paged_page(p.kv, s, x1 >> p.kv.shift)) * p.kv.hkv + h) << p.kv.shift) +
+        (x1 & mask);
+    f16x8 k0[KS], k1[KS];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      k0[i] = *(const f16x8*)(p.kv.k + r0 * D + c * D + 8 * g + 32 * i);
+      k1[i] = *(const f16x8*)(p.kv.k + r1 * D + c * D + 8 * g + 32 * i);
+    }
+    uint32_t v[8][DPL / 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const f16* row = p.kv.v + (i < 4 ? r0 : r1) * D + (4 * g + i % 4) * D + DPL * c;
+      __builtin_memcpy(v[i], __builtin_assume_aligned(row, 2 * DPL), 2 * DPL);
+    }
+    f32x4 s0 = f32x4{}, s1 = f32x4{};
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0[i], qf[i], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1[i], qf[i], s1, 0, 0, 0);
+    }
+    float sc[8];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sc[r] = s0[r] * p.scale2;
+      sc[r + 4] = s1[r] * p.scale2;
+    }
+    if (x + 32 > len) {
+      // rows past the end weigh 0 and, whatever the page holds there, read 0
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = x + (i < 4 ? 0 : 16) + 4 * g + i % 4 < len;
+        sc[i] = in ? sc[i] : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < DPL / 2; ++e) v[i][e] = in ? v[i][e] : 0u;
+      }
+    }
+    float top = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])),
+                      fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+    if (__any(top > m + kLag)) {
+      const float next = fmaxf(m, rows_max(top));
+      const float f = exp2_fast(m - (next == -INFINITY ? 0.0f : next));
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][r] *= f;
+      m = next;
+    }
+    // (where every score so far is -inf the weights are 0, not NaN)
+    const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+    f16x8 w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = exp2_fast(sc[i] - base);
+      l += e;
+      w[i] = (f16)e;  // the weights' one rounding below 32 bits
+    }
+#pragma unroll
+    for (int e = 0; e < DPL / 2; ++e) {
+      u32x4 lo, hi;
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        lo[a] = __builtin_amdgcn_perm(v[2 * a + 1][e], v[2 * a][e], 0x05040100u);
+        hi[a] = __builtin_amdgcn_perm(v[2 * a + 1][e], v[2 * a][e], 0x07060302u);
+      }
+      acc[2 * e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, lo), w,
+                                                          acc[2 * e], 0, 0, 0);
+      acc[2 * e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, hi), w,
+                                                              acc[2 * e + 1], 0, 0, 0);
+    }
+  }
+
+  // the waves' (max, sum, acc) meet, D / (16 HT) passes of W dims
+  l = rows_sum(l);
+  if (lane < 16) {
+    lds.m[wave][c] = m;
+    lds.l[wave][c] = l;
+  }
+#pragma unroll
+  for (int pass = 0; pass < DPL / HT; ++pass) {
+    // acc[t][r] is dim DPL (4 g + r) + t of head c
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int t = 0; t < HT; t += 4) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = acc[pass * HT + t + e][r];
+        *(f32x4*)&lds.o[wave][c][HT * (4 * g + r) + t] = y;
+      }
+    __syncthreads();
+    for (int i = tid; i < live * (W / 4); i += kThreads) {
+      const int q = i / (W / 4), y = i % (W / 4) * 4;
+      float top = lds.m[0][q];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds.m[w][q]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      f32x4 a = f32x4{};
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = exp2_fast(lds.m[w][q] - base);
+        sum = fmaf(lds.l[w][q], f, sum);
+        const f32x4 b = *(const f32x4*)&lds.o[w][q][y];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = fmaf(b[e], f, a[e]);
+      }
+      const int dim = y / HT * DPL + pass * HT + y % HT;
+      if (slot) {
+        float* to = slot + q * (D + 4);
+        *(f32x4*)(to + 4 + dim) = a;
+        if (y == 0 && pass == 0) {
+          to[0] = top;
+          to[1] = sum;
+        }
+      } else {
+        // (a sum of 0: every score was -inf, and the answer is NaN)
+        const float inv = 1.0f / sum;
+        f16x4 b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = (f16)(a[e] * inv);
+        *(f16x4*)(p.out + (long long)s * p.out_stride + (h * p.group + first + q) * D + dim) = b;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One workgroup per (head block, sequence), nothing to join.
+template <int D>
+__global__ __launch_bounds__(kThreads) void decode_paged_whole(const DecodePagedParams p) {
+  __shared__ DecodeLds<D> lds;
+  const int hb = blockIdx.x, s = blockIdx.y;
+  const int len = paged_length(p.kv, s);
+  if (len > 0) {
+    decode_piece<D>(p, lds, s, hb, len, 0, len, nullptr);
+    return;
+  }
+  const int h = hb / p.blocks, first = hb % p.blocks * 16, live = min(16, p.group - first);
+  for (int i = threadIdx.x; i < live * D; i += kThreads)
+    p.out[(long long)s * p.out_stride + (h * p.group + first) * D + i] = (f16)0.0f;
+}
+
+// Units of one head block of a sequence.
+__device__ __forceinline__ int decode_units(int len) {
+  return (len + kDecodeUnit - 1) / kDecodeUnit;
+}
+
+// Equal runs of units.  plan[0] takes the run's length, plan[1 + s] the first
+// unit of sequence s, for the joining launch.
+template <int D>
+__global__ __launch_bounds__(kThreads) void decode_paged_runs(const DecodePagedParams p) {
+  __shared__ DecodeLds<D> lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n = p.kv.n, heads = p.kv.hkv * p.blocks;
+  // thread t adds up the units of its share of the sequences
+  const int share = (n + kThreads - 1) / kThreads;
+  const int s0 = min(tid * share, n), s1 = min(s0 + share, n);
+  int mine = 0;
+  for (int s = s0; s < s1; ++s) mine += decode_units(paged_length(p.kv, s)) * heads;
+  int upto = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += v;
+  }
+  if (lane == 63) lds.count[wave] = upto;
+  __syncthreads();
+  int before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += lds.count[w];
+    total += lds.count[w];
+  }
+  const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_run);
+  const int u0 = blockIdx.x * run;  // (the host keeps grid * run within 31 bits)
+  if (blockIdx.x == 0 && tid == 0) p.plan[0] = run;
+  if (u0 >= total) return;
+  const int u1 = min(u0 + run, total);
+  if (before <= u0 && u0 < before + mine) {
+    int s = s0, base = before;
+    for (;; ++s) {
+      const int u = decode_units(paged_length(p.kv, s)) * heads;
+      if (u0 < base + u) break;
+      base += u;
+    }
+    lds.seq = s;
+    lds.base = base;
+  }
+  __syncthreads();
+  int s = sreg(lds.seq), base = sreg(lds.base);
+  for (int u = u0; u < u1;) {
+    const int len = paged_length(p.kv, s), per = decode_units(len);
+    if (u >= base + per * heads) {
+      base += per * heads;
+      ++s;
+      continue;
+    }
+    const int hb = (u - base) / per, at = (u - base) % per;
+    const int take = min(per - at, u1 - u);
+    if (hb == 0 && at == 0 && tid == 0) p.plan[1 + s] = base;
+    float* slot = take == per ? nullptr
+                              : p.part + (2LL * blockIdx.x + (u == u0 ? 0 : 1)) * 16 * (D + 4);
+    decode_piece<D>(p, lds, s, hb, len, at * kDecodeUnit, min(len, (at + take) * kDecodeUnit),
+                    slot);
+    u += take;
+  }
+}
+
+// Joins the partial rows of the (sequence, head)s that more than one run holds:
+// M = max m_i, out = sum acc_i 2^(m_i - M) / sum l_i 2^(m_i - M).  Also the zero
+// rows of empty sequences.
+template <int D>
+__global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedParams p) {
+  constexpr int T4 = D / 4, R = kThreads / T4;  // threads along a row, rows at a time
+  __shared__ float4 sums[R][T4];
+  __shared__ float tops[R], weights[R];
+  const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+  const int y = tid % T4, r = tid / T4;
+  const int len = paged_length(p.kv, s);
+  f16* out = p.out + (long long)s * p.out_stride + head * D;
+  if (len == 0) {
+    if (tid < T4) *(f16x4*)(out + 4 * y) = f16x4{};
+    return;
+  }
+  const int per = decode_units(len), run = p.plan[0];
+  const int h = head / p.group, q = head % p.group;
+  const int a = p.plan[1 + s] + (h * p.blocks + q / 16) * per, b = a + per - 1;
+  const int w0 = a / run, w1 = b / run;
+  if (w0 == w1) return;  // its one run wrote the output
+  auto row = [&](int w) {
+    const int side = w == w0 && a % run ? 1 : 0;
+    return p.part + ((2LL * w + side) * 16 + q % 16) * (D + 4);
+  };
+  float m = -INFINITY, l = 0.0f;
+  f32x4 acc = f32x4{};
+  for (int w = w0 + r; w <= w1; w += R) {
+    const float* x = row(w);
+    const f32x4 o = *(const f32x4*)(x + 4 + 4 * y);
+    const float mx = x[0], lx = x[1];
+    const float next = fmaxf(m, mx), base = next == -INFINITY ? 0.0f : next;
+    const float f = exp2_fast(m - base), fx = exp2_fast(mx - base);
+    l = l * f + lx * fx;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f + o[e] * fx;
+    m = next;
+  }
+  sums[r][y] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  if (y == 0) {
+    tops[r] = m;
+    weights[r] = l;
+  }
+  __syncthreads();
+  if (r) return;
+  float top = tops[0];
+#pragma unroll
+  for (int i = 1; i < R; ++i) top = fmaxf(top, tops[i]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  acc = f32x4{};
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const float f = exp2_fast(tops[i] - base);
+    const float4 o = sums[i][y];
+    l = fmaf(weights[i], f, l);
+    acc[0] = fmaf(o.x, f, acc[0]);
+    acc[1] = fmaf(o.y, f, acc[1]);
+    acc[2] = fmaf(o.z, f, acc[2]);
+    acc[3] = fmaf(o.w, f, acc[3]);
+  }
+  const float inv = 1.0f / l;
+  f16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (f16)(acc[e] * inv);
+  *(f16x4*)(out + 4 * y) = v;
+}
+
+// Workgroups of the runs' launch, and whether a launch over up to `bound`
+// positions of each sequence is split at all.
+int decode_paged_grid(int cus) { return 4 * cus; }
+bool decode_paged_split(long long bound) { return bound > 512; }
+long long decode_paged_part_floats(int head_dim, int grid) {
+  return 2LL * grid * 16 * (head_dim + 4);
+}
+
+template <int D>
+static hipError_t decode_launch(const DecodePagedParams& p, int grid, hipStream_t stream) {
+  if (!grid) {
+    hipLaunchKernelGGL(decode_paged_whole<D>, dim3(p.kv.hkv * p.blocks, p.kv.n), dim3(kThreads), 0,
+                       stream, p);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL(decode_paged_runs<D>, dim3(grid), dim3(kThreads), 0, stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(decode_paged_join<D>, dim3(p.kv.hkv * p.group, p.kv.n), dim3(kThreads), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
+hipError_t decode_paged_launch(const DecodePagedParams& p, int head_dim, int grid,
+                               hipStream_t stream) {
+  switch (head_dim) {
+    case 64: return decode_launch<64>(p, grid, stream);
+    case 128: return decode_launch<128>(p, grid, stream);
+    default: return decode_launch<256>(p, grid, stream);
+  }
+}
+
+}  // namespace aexq

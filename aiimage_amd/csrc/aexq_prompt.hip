@@ -1,0 +1,328 @@
+// Attention over prompts (gfx950): packed sequences of different lengths,
+// grouped heads, causal or over whole sequences, K and V packed like q or in a
+// paged cache (whose last rows the queries then are).
+#include <math.h>
+
+#include "aexq_paged.hpp"
+
+namespace aexq {
+
+// ---------------------------------------------------------------------------
+// out = softmax(scale q K^T over what a row sees) V, in one pass over K and V
+// with a running maximum and sum per row.
+//
+// The rows of a sequence and kv head are its (token, query head of the group)
+// pairs, token by token: row r is token r / group, head r % group.  A workgroup
+// takes 128 of them, 32 to a wave, so one K/V tile in LDS serves every head of
+// the group and short prompts still fill the tile.  Tiles of KT positions are
+// fetched LDS-direct, one ahead, 16-byte chunks of a row exchanged by swz() so
+// that neither product's reads meet in LDS banks.
+//   S^T = K q^T   32 positions x 32 rows x 16 dims a product: q stays in
+//                 registers as the right operand; lane (j = l % 32, h = l / 32)
+//                 ends with row j's scores of positions 8 (i / 4) + 4 h + i % 4;
+//   O^T = V^T P^T takes the weights as they stand as its right operand when its
+//                 k index 8 h + i is position 8 (i / 4) + 4 h + i % 4 of 16; the
+//                 left operand is V transposed on the way out of LDS
+//                 (ds_read_b64_tr_b16), 4 positions of 16 dims per 16 lanes.
+// So scores, weights, maximum and sum of a row never leave its two lanes.
+//
+// Sequences and their tiles are found on the device from the offsets; the tiles
+// with the most positions start first.
+// ---------------------------------------------------------------------------
+constexpr int kPromptRows = 128;
+
+template <int D>
+struct PromptLds {
+  static constexpr int KT = D == 256 ? 32 : 64;
+  alignas(1024) f16 k[2][KT * D];
+  alignas(1024) f16 v[2][KT * D];
+  int seq, tile, count[kWaves];
+  int odd[2][kWaves];  // a V tile holds an infinity or a NaN
+};
+
+// Where chunk c of row r of a tile lies: chunk c ^ swz(r) of that row.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+  return (r & 3) << 2 | (r >> 2 & 3);
+}
+
+// Lane i's 16 bytes at its own address to LDS byte lds + 16 i.
+__device__ __forceinline__ void dma_lane(const void* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(from)
+               : "memory", "m0");
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Of each 16 lanes, lane i reads 4 elements at its address; together a 4 x 16
+// block, row i / 4, columns 4 (i % 4) ..; lane i gets column i.
+__device__ __forceinline__ f16x4 read_transposed(const f16* p) {
+  return __builtin_bit_cast(
+      f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+template <int D, bool PAGED>
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(const PromptParams p) {
+  constexpr int KT = PromptLds<D>::KT, CH = D / 8, KS = D / 16, DB = D / 32, SB = KT / 32;
+  constexpr int RL = 512 / D;        // tile rows of one LDS-direct load
+  constexpr int NL = KT / 4 / RL;    // loads of a wave per K (or V) tile
+  __shared__ PromptLds<D> lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = sreg(tid >> 6);
+  const int n = p.n, group = p.group, head = blockIdx.x;
+
+  // 1. the workgroup's sequence and tile, the last tiles first
+  auto first_of = [&](int s) { return min(max(p.q_offsets[s], 0), p.tokens); };
+  auto rows_of = [&](int s) {
+    const int a = first_of(s);
+    return (min(max(p.q_offsets[s + 1], a), p.tokens) - a) * group;
+  };
+  const int share = (n + kThreads - 1) / kThreads;
+  const int sa = min(tid * share, n), sb = min(sa + share, n);
+  int mine = 0;
+  for (int s = sa; s < sb; ++s) mine += (rows_of(s) + kPromptRows - 1) / kPromptRows;
+  int upto = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(upto, off, 64);
+    if (lane >= off) upto += v;
+  }
+  if (lane == 63) lds.count[wave] = upto;
+  __syncthreads();
+  int before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += lds.count[w];
+    total += lds.count[w];
+  }
+  const int at = total - 1 - (int)blockIdx.y;
+  if (at < 0) return;
+  if (before <= at && at < before + mine) {
+    int s = sa, base = before;
+    for (;; ++s) {
+      const int u = (rows_of(s) + kPromptRows - 1) / kPromptRows;
+      if (at < base + u) break;
+      base += u;
+    }
+    lds.seq = s;
+    lds.tile = at - base;
+  }
+  __syncthreads();
+  const int seq = sreg(lds.seq), tile = sreg(lds.tile);
+  const int q0 = first_of(seq), rows = rows_of(seq), queries = rows / group;
+  int kv0 = 0, len;
+  if constexpr (PAGED) {
+    len = paged_length(p.kv, seq);
+  } else {
+    kv0 = min(max(p.kv_offsets[seq], 0), p.kv_tokens);
+    len = min(max(p.kv_offsets[seq + 1], kv0), p.kv_tokens) - kv0;
+  }
+  len = sreg(len);
+  // positions that the token of row r sees
+  auto seen = [&](int r) { return p.causal ? max(len - queries + r / group + 1, 0) : len; };
+
+  // 2. q: the lane's row as the right operand of S^T
+  const int j = lane & 31, h = lane >> 5;
+  const int row = tile * kPromptRows + wave * 32 + j, last = rows - 1;
+  const int rr = min(row, last);  // rows past the end repeat the last one, and store nothing
+  const long long token = q0 + rr / group;
+  const int qh = head * group + rr % group;
+  f16x8 qf[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    qf[s] = *(const f16x8*)(p.q + token * p.q_stride + qh * D + 16 * s + 8 * h);
+  const int vis = seen(rr);
+  // what the wave's rows see at least and at most, and the workgroup's
+  const int w0 = min(tile * kPromptRows + wave * 32, last);
+  const int lo = sreg(seen(w0)), hi = sreg(seen(min(w0 + 31, last)));
+  const int low = sreg(seen(tile * kPromptRows));
+  const int most = sreg(seen(min(tile * kPromptRows + kPromptRows - 1, last)));
+  const int tiles = (most + KT - 1) / KT;
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+  float m = -INFINITY, l = 0.0f;
+
+  auto fetch = [&](int t, int b) {
+    const int r0 = wave * (KT / 4);
+    long long page_row = 0;
+    if constexpr (PAGED) {
+      // a wave's rows lie in one block of 16 positions, so in one page
+      const int x = min(t * KT + r0, len - 1);
+      page_row = ((long long)sreg(paged_page(p.kv, seq, x >> p.kv.shift)) * p.kv.hkv + head)
+                 << p.kv.shift;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r = r0 + i * RL + lane / CH;
+      const int chunk = lane % CH ^ swz<D>(r);
+      const int x = min(t * KT + r, len - 1);  // rows past the end repeat the last one
+      const uint32_t to = (r0 + i * RL) * D * 2;
+      if constexpr (PAGED) {
+        const long long a = (page_row + (x & ((1 << p.kv.shift) - 1))) * D + 8 * chunk;
+        dma_lane(p.kv.k + a, lds_addr(lds.k[b]) + to);
+        dma_lane(p.kv.v + a, lds_addr(lds.v[b]) + to);
+      } else {
+        const long long a = kv0 + x;
+        dma_lane(p.k + a * p.k_stride + head * D + 8 * chunk, lds_addr(lds.k[b]) + to);
+        dma_lane(p.v + a * p.v_stride + head * D + 8 * chunk, lds_addr(lds.v[b]) + to);
+      }
+    }
+  };
+
+  const int ksw = swz<D>(j);
+  const int tg = lane >> 4 & 1, ti = lane & 15;  // transposed reads: 16-dim half, lane of 16
+
+  if (tiles > 0) fetch(0, 0);
+  for (int t = 0; t < tiles; ++t) {
+    const int b = t & 1, x0 = t * KT;
+    wait_vm<0>();
+    const bool edge = x0 + KT > low;  // some row of the workgroup does not see all of it
+    if (edge) {
+      // An infinity or a NaN in V reaches, through 0 * V, the rows that do not
+      // see it: each wave looks through the rows it fetched.
+      float z = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const u32x4 y = *(const u32x4*)((const char*)lds.v[b] +
+                                        (wave * (KT / 4) + i * RL) * D * 2 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z = dot2(y[e], 0u, z);
+      }
+      const bool odd = __any(z != 0.0f);
+      if (lane == 0) lds.odd[b][wave] = odd;
+      wait_lgkm0();
+    }
+    bar();
+    if (t + 1 < tiles) fetch(t + 1, b ^ 1);
+    if (x0 >= hi) continue;  // none of the wave's rows sees any of it
+
+    f32x16 sc[SB];
+#pragma unroll
+    for (int i = 0; i < SB; ++i) sc[i] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < SB; ++i) {
+        const f16x8 kf = *(const f16x8*)&lds.k[b][(32 * i + j) * D + 8 * ((2 * s + h) ^ ksw)];
+        sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], sc[i], 0, 0, 0);
+      }
+    const bool masked = x0 + KT > lo;
+    if (masked) {
+      const int left = vis - x0 - 4 * h;
+#pragma unroll
+      for (int i = 0; i < SB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          sc[i][r] = 32 * i + 8 * (r / 4) + r % 4 < left ? sc[i][r] : -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[i][r]);
+    top *= p.scale2;
+    if (__any(top > m + kLag)) {
+      const float next = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const float f = exp2_fast(m - (next == -INFINITY ? 0.0f : next));
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= f;
+      m = next;
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - kLift;
+#pragma unroll
+    for (int i = 0; i < SB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sc[i][r] = exp2_fast(fmaf(sc[i][r], p.scale2, -base));
+        l += sc[i][r];
+      }
+    if (masked && (lds.odd[b][0] | lds.odd[b][1] | lds.odd[b][2] | lds.odd[b][3])) {
+      // position by position, for the rows that see it
+      for (int x = 0; x < KT && x0 + x < hi; ++x) {
+        float w = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * i + 8 * (r / 4) + r % 4 + 4 * h == x) w = sc[i][r];
+        // (the half that does not hold position x has 0)
+        w += __shfl_xor(w, 32, 64);
+        const bool in = x0 + x < vis;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = 32 * i + 8 * (r / 4) + 4 * h + r % 4;
+            const f16 y = lds.v[b][x * D + 8 * ((d / 8) ^ swz<D>(x)) + d % 8];
+            o[i][r] = in ? fmaf(w, (float)y, o[i][r]) : o[i][r];
+          }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int y = 0; y < KT / 16; ++y) {
+      f16x8 w;  // the weights' one rounding below 32 bits
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = (f16)sc[y / 2][8 * (y % 2) + i];
+#pragma unroll
+      for (int i = 0; i < DB; ++i) {
+        f16x4 a[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int r = 16 * y + 8 * z + 4 * h + ti / 4;
+          const int chunk = (2 * tg + (ti & 3) / 2) ^ (4 * i) ^ swz<D>(8 * z + 4 * h + ti / 4);
+          a[z] = read_transposed(&lds.v[b][r * D + 8 * chunk + 4 * (ti & 1)]);
+        }
+        const f16x8 vf = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w, o[i], 0, 0, 0);
+      }
+    }
+  }
+
+  // 3. the row's two lanes hold half of its sum each; a row that sees nothing is
+  // 0, one whose every score was -inf (a sum of 0) NaN
+  l += __shfl_xor(l, 32, 64);
+  const float inv = vis > 0 ? 1.0f / l : 0.0f;
+  if (row > last) return;
+  f16* out = p.out + token * p.out_stride + qh * D;
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f16x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (f16)(o[i][4 * r + e] * inv);
+      *(f16x4*)(out + 32 * i + 8 * r + 4 * h) = y;
+    }
+}
+
+// Tiles that the rows of `tokens` packed tokens in n sequences need at most.
+long long prompt_tiles(long long tokens, int n, int group) {
+  return tokens * group / kPromptRows + n;
+}
+
+template <int D>
+static void prompt_dispatch(const PromptParams& p, dim3 grid, hipStream_t stream) {
+  if (p.kv.k)
+    hipLaunchKernelGGL((prompt_kernel<D, true>), grid, dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL((prompt_kernel<D, false>), grid, dim3(kThreads), 0, stream, p);
+}
+
+hipError_t prompt_launch(const PromptParams& p, int head_dim, hipStream_t stream) {
+  const dim3 grid(p.hkv, (unsigned)prompt_tiles(p.tokens, p.n, p.group));
+  switch (head_dim) {
+    case 64: prompt_dispatch<64>(p, grid, stream); break;
+    case 128: prompt_dispatch<128>(p, grid, stream); break;
+    default: prompt_dispatch<256>(p, grid, stream); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace aexq

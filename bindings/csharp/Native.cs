@@ -150,6 +150,24 @@ namespace Aexis.Hip
         [FieldOffset(40)] public int workgroups;
     }
 
+    /// <summary>aexq_paged_kv: a pool of fp16 pages and the sequences' tables (device pointers).</summary>
+    [StructLayout(LayoutKind.Sequential)]
+    public struct AexqPagedKv
+    {
+        public IntPtr k, v;
+        public int pages, pageSize, headsKv, headDim;
+        public IntPtr table, lengths;
+        public int sequences, tableWidth;
+    }
+
+    /// <summary>aexq_rope: rotary tables and the positions of a call's tokens (device pointers).</summary>
+    [StructLayout(LayoutKind.Sequential)]
+    public struct AexqRope
+    {
+        public IntPtr cosTable, sinTable, positions;
+        public int rows, rotaryDim, axes, interleaved, section0, section1, section2, section3;
+    }
+
     /// <summary>The DllImports of include/aexq.h (one per declared function).</summary>
     public static class Native
     {
@@ -223,6 +241,22 @@ namespace Aexis.Hip
             IntPtr position /* device int32 */, IntPtr cosTable, IntPtr sinTable, float scale, IntPtr outF16);
         [DllImport(Lib)] public static extern int aexq_decode_advance(IntPtr ctx, IntPtr position, IntPtr token,
             IntPtr argmax, IntPtr tokensOut, int tokensCap);
+
+        // ---- many sequences: a paged key/value cache, prompts, probabilities; strides in elements
+        [DllImport(Lib)] public static extern int aexq_rope_append_paged(IntPtr ctx, ref AexqPagedKv kv,
+            ref AexqRope rope, IntPtr offsets, int tokens, int headsQ, IntPtr q, long qStride, IntPtr k,
+            long kStride, IntPtr v, long vStride, IntPtr qOut, long qOutStride);
+        [DllImport(Lib)] public static extern int aexq_attention_prompt(IntPtr ctx, IntPtr q, long qStride,
+            IntPtr k, long kStride, IntPtr v, long vStride, IntPtr qOffsets, IntPtr kvOffsets /* or 0 */,
+            int sequences, int tokens, int kvTokens, int headsQ, int headsKv, int headDim, int causal,
+            float scale, IntPtr outF16, long outStride);
+        [DllImport(Lib)] public static extern int aexq_attention_prompt_paged(IntPtr ctx, ref AexqPagedKv kv,
+            IntPtr q, long qStride, IntPtr offsets, int tokens, int headsQ, float scale, IntPtr outF16,
+            long outStride);
+        [DllImport(Lib)] public static extern int aexq_attention_decode_paged(IntPtr ctx, ref AexqPagedKv kv,
+            IntPtr q, long qStride, int headsQ, float scale, IntPtr outF16, long outStride);
+        [DllImport(Lib)] public static extern int aexq_logprobs(IntPtr ctx, ref AexqTensor logits,
+            IntPtr tokens, IntPtr logprob, IntPtr entropy, int top, IntPtr topIds, IntPtr topLogprobs);
 
         // ---- the decoder layers of a decode step in one launch
         [DllImport(Lib)] public static extern int aexq_decoder_create(IntPtr ctx, ref AexqDecoderConfig cfg,

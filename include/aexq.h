@@ -351,6 +351,102 @@ aexq_status aexq_attention_decode_rope_at(aexq_ctx* ctx, const void* q, const vo
 aexq_status aexq_decode_advance(aexq_ctx* ctx, int32_t* position, int32_t* token,
                                 const int32_t* argmax, int32_t* tokens_out, int tokens_cap);
 
+/* ---- many sequences: a paged key/value cache, prompts, probabilities -------- */
+/* No counterpart in the reference, which decodes one sequence.  Head dimensions
+ * 64, 128 and 256; rows of one token's heads are dense ([heads][head_dim]) and
+ * lie `stride` elements apart, so q, k and v may be views into one buffer; bases
+ * are 16-byte aligned and strides multiples of 8.  Outputs share no memory with
+ * inputs, but where it says so. */
+
+/* A pool of fp16 pages shared by `sequences` sequences.  Position x of sequence
+ * s is row x % page_size of page table[s][x / page_size].  `table` and `lengths`
+ * are read on the device when a launch runs, so a captured graph follows them.
+ * Reads are kept inside the pool: a length below 0 is 0, one past the table's
+ * width its end, a page entry below 0 page 0, one past the pool its last page. */
+typedef struct aexq_paged_kv {
+  void* k;                 /* device fp16 [pages][heads_kv][page_size][head_dim] */
+  void* v;
+  int pages;
+  int page_size;           /* a power of two, 16 to 4096 */
+  int heads_kv, head_dim;
+  const int32_t* table;    /* device [sequences][table_width] */
+  const int32_t* lengths;  /* device [sequences]: positions kept, those of the call included */
+  int sequences;           /* at most 65535 */
+  int table_width;
+} aexq_paged_kv;
+
+/* Rotary positions (rotate-half pairs (j, j + rotary_dim / 2); elements past
+ * rotary_dim stay).  Pair j is turned by the table row of its axis' position:
+ * axis a has sections[a] pairs, one section after the other, or, interleaved,
+ * pair j belongs to axis j % axes while j < axes * sections[j % axes] and to
+ * axis 0 otherwise.  Rows are clamped to the table. */
+typedef struct aexq_rope {
+  const float* cos_table;    /* device fp32 [rows][rotary_dim / 2] */
+  const float* sin_table;
+  const int32_t* positions;  /* device [axes][tokens]; NULL with one axis: the place in the cache */
+  int rows;
+  int rotary_dim;            /* a multiple of 16, at most head_dim */
+  int axes;                  /* 1 to 4 */
+  int interleaved;
+  int section0, section1, section2, section3; /* pairs per axis; their sum is rotary_dim / 2 */
+} aexq_rope;
+
+/* aexq_rope_kv_append for packed tokens of many sequences: the new tokens of
+ * sequence s are rows offsets[s] .. offsets[s + 1] - 1 (device int32
+ * [sequences + 1], not decreasing) and become its last positions, the ones
+ * before lengths[s].  q is rotated into q_out (which may be q), k rotated and v
+ * copied into their pages.  A position outside the table, or whose page entry
+ * lies outside the pool, is not stored.  Rows behind the last sequence are not
+ * touched.  Two tokens that name the same cache row in one call leave either's
+ * values, piece by piece. */
+aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const aexq_rope* rope,
+                                   const int32_t* offsets, int tokens, int heads_q, const void* q,
+                                   int64_t q_stride, const void* k, int64_t k_stride,
+                                   const void* v, int64_t v_stride, void* q_out,
+                                   int64_t q_out_stride);
+
+/* Attention over packed prompts: out = softmax(scale q k^T) v per sequence and
+ * query head (key head h / (heads_q / heads_kv)), the softmax as in
+ * aexq_attention_decode.  Sequence s has query rows q_offsets[s] ..
+ * q_offsets[s + 1] - 1 and key rows kv_offsets[s] .. kv_offsets[s + 1] - 1
+ * (device int32 [sequences + 1]; NULL kv_offsets: the same).  causal: the
+ * queries are the sequence's last positions and see those up to their own.  A
+ * row that sees no position is 0; what a row does not see does not reach it,
+ * infinities and NaN in k or v included.  Rows behind the last sequence are not
+ * touched.  scale > 0. */
+aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64_t q_stride, const void* k,
+                                  int64_t k_stride, const void* v, int64_t v_stride,
+                                  const int32_t* q_offsets, const int32_t* kv_offsets,
+                                  int sequences, int tokens, int kv_tokens, int heads_q,
+                                  int heads_kv, int head_dim, int causal, float scale, void* out,
+                                  int64_t out_stride);
+
+/* The causal form over a paged cache: the query rows of sequence s are its last
+ * positions, those before lengths[s] (a whole prompt, or a chunk of one whose
+ * first part is in the cache already). */
+aexq_status aexq_attention_prompt_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const void* q,
+                                        int64_t q_stride, const int32_t* offsets, int tokens,
+                                        int heads_q, float scale, void* out, int64_t out_stride);
+
+/* aexq_attention_decode for every sequence of a paged cache: row s of q attends
+ * over the lengths[s] positions of sequence s; no position, a zero row.  Uses
+ * the context's scratch (launches on one context run in stream order, replays of
+ * graphs captured from it included). */
+aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const void* q,
+                                        int64_t q_stride, int heads_q, float scale, void* out,
+                                        int64_t out_stride);
+
+/* Log probabilities over rows of fp32 or fp16 logits (not head-packed):
+ * logprob[r] (nullable) of token tokens[r] (device int32; 0 for token -1, NaN
+ * for another one outside the row), entropy[r] (nullable, nats), and the `top`
+ * (0 to 64) largest logits of the row, equal ones by the lower index: top_ids
+ * [rows][top] and top_logprobs [rows][top] (each nullable).  Logits of -inf
+ * weigh nothing; a row with a NaN, a +inf, or nothing but -inf has no
+ * probabilities: NaN, and alternatives of -1.  Uses the context's scratch. */
+aexq_status aexq_logprobs(aexq_ctx* ctx, const aexq_tensor* logits, const int32_t* tokens,
+                          float* logprob, float* entropy, int top, int32_t* top_ids,
+                          float* top_logprobs);
+
 /* ---- the decoder layers of a decode step in one launch -------------------- */
 /* Qwen35DecoderSession.DecodeCore's per-layer chain (DEC:463-585: RMSNorm,
  * q/k/v, RoPE, K/V append, SDPA, o_proj + residual, RMSNorm, gate/up + SwiGLU,
