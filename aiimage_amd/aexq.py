@@ -128,34 +128,41 @@ def new_activation(rows: int, width: int, dtype=torch.float16, layout: int = LAY
 
 # ---------------------------------------------------------------- many sequences
 
-def _want(ok: bool, message: str):
-    if not ok:
-        raise _abi.ArgumentError(_abi.ERR_INVALID_ARGUMENT, message)
+def _refuse(message: str):
+    raise _abi.ArgumentError(_abi.ERR_INVALID_ARGUMENT, message)
 
 
-def _device_array(t: torch.Tensor, name: str, dtype, shape: tuple, device=None) -> int:
-    """Address of a dense device array (None in `shape` matches any size)."""
-    _want(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} is not a device tensor")
-    _want(t.dtype == dtype, f"{name} is {t.dtype}, not {dtype}")
-    _want(t.dim() == len(shape) and all(w is None or w == g for w, g in zip(shape, t.shape)),
-          f"{name} has shape {tuple(t.shape)}, not {shape}")
-    _want(t.is_contiguous(), f"{name} is not contiguous")
-    _want(device is None or t.device == device, f"{name} is on {t.device}, not on {device}")
+# (These run before every launch of a few microseconds: the plain comparisons come
+# first, what is wrong is worked out once something is.)
+
+def _device_array(t: torch.Tensor, name: str, dtype, shape: tuple, device: int) -> int:
+    """Address of a dense array on GPU `device`."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
+            and t.get_device() == device and t.is_contiguous()):
+        what = (f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}"
+                if isinstance(t, torch.Tensor) else type(t).__name__)
+        _refuse(f"{name} is {what}, not a dense {dtype} {tuple(shape)} on GPU {device}")
     return t.data_ptr()
 
 
-def _head_rows(t: torch.Tensor, name: str, rows, heads, head_dim, device) -> int:
-    """Row stride in elements of fp16 rows [rows][heads][head_dim] whose heads are
-    dense; the rows may be a view into a wider buffer."""
-    _want(isinstance(t, torch.Tensor) and t.is_cuda and t.device == device,
-          f"{name} is not a tensor on {device}")
-    _want(t.dtype == torch.float16, f"{name} is {t.dtype}, not torch.float16")
-    _want(t.dim() == 3 and t.shape[0] == rows and t.shape[2] == head_dim
-          and (heads is None or t.shape[1] == heads),
-          f"{name} has shape {tuple(t.shape)}, not ({rows}, {heads or 'heads'}, {head_dim})")
-    _want(t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == head_dim),
-          f"{name}'s heads are not dense (strides {t.stride()})")
-    return t.stride(0) if rows > 1 else t.shape[1] * head_dim
+def _head_rows(t: torch.Tensor, name: str, shape: tuple, device: int) -> int:
+    """Row stride in elements of fp16 rows of `shape` [rows][heads][head_dim] whose
+    heads are dense; the rows may be a view into a wider buffer."""
+    if isinstance(t, torch.Tensor) and t.shape == shape:
+        row, head, one = t.stride()
+        rows, heads, dim = shape
+        if (t.dtype is torch.float16 and t.get_device() == device and one == 1
+                and (head == dim or heads == 1)):
+            return row if rows > 1 else heads * dim
+    what = (f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}"
+            if isinstance(t, torch.Tensor) else type(t).__name__)
+    _refuse(f"{name} is {what}, not fp16 rows {tuple(shape)} of dense heads on GPU {device}")
+
+
+def _head_shape(t: torch.Tensor, name: str) -> tuple:
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        _refuse(f"{name} is not [rows][heads][head_dim]")
+    return t.shape
 
 
 def paged_kv(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
@@ -163,14 +170,18 @@ def paged_kv(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor,
     """aexq_paged_kv of a pool k, v [pages][heads_kv][page_size][head_dim] (fp16),
     the sequences' page table [sequences][width] and lengths [sequences] (int32,
     read on the device when a launch runs)."""
-    d = _abi.PagedKv()
-    d.k = _device_array(k, "k", torch.float16, (None,) * 4)
-    d.v = _device_array(v, "v", torch.float16, tuple(k.shape), k.device)
-    d.table = _device_array(table, "table", torch.int32, (None, None), k.device)
-    d.lengths = _device_array(lengths, "lengths", torch.int32, (table.shape[0],), k.device)
+    if not (isinstance(k, torch.Tensor) and k.dim() == 4 and k.is_cuda):
+        _refuse("k is not a pool [pages][heads_kv][page_size][head_dim] on a GPU")
+    if not (isinstance(table, torch.Tensor) and table.dim() == 2):
+        _refuse("table is not [sequences][width]")
+    d, device = _abi.PagedKv(), k.get_device()
+    d.k = _device_array(k, "k", torch.float16, k.shape, device)
+    d.v = _device_array(v, "v", torch.float16, k.shape, device)
+    d.table = _device_array(table, "table", torch.int32, table.shape, device)
+    d.lengths = _device_array(lengths, "lengths", torch.int32, (table.shape[0],), device)
     d.pages, d.heads_kv, d.page_size, d.head_dim = k.shape
     d.sequences, d.table_width = table.shape
-    d._keep = (k, v, table, lengths)
+    d._keep, d._device = (k, v, table, lengths), device
     return d
 
 
@@ -179,20 +190,24 @@ def rope(cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor]
     """aexq_rope of tables cos, sin [rows][rotary_dim / 2] (fp32) and positions
     [axes][tokens] (int32; None: each token's place in the cache).  `sections`
     holds the pairs of each axis, one after the other or, interleaved, in turn."""
-    d = _abi.Rope()
-    d.cos_table = _device_array(cos, "cos", torch.float32, (None, None))
-    d.sin_table = _device_array(sin, "sin", torch.float32, tuple(cos.shape), cos.device)
-    d.positions = (_device_array(positions, "positions", torch.int32, (None, None), cos.device)
-                   if positions is not None else None)
+    if not (isinstance(cos, torch.Tensor) and cos.dim() == 2 and cos.is_cuda):
+        _refuse("cos is not [rows][rotary_dim / 2] on a GPU")
+    if positions is not None and not (isinstance(positions, torch.Tensor) and positions.dim() == 2):
+        _refuse("positions is not [axes][tokens]")
+    d, device = _abi.Rope(), cos.get_device()
+    d.cos_table = _device_array(cos, "cos", torch.float32, cos.shape, device)
+    d.sin_table = _device_array(sin, "sin", torch.float32, cos.shape, device)
     d.rows, d.rotary_dim = cos.shape[0], 2 * cos.shape[1]
-    d.axes = positions.shape[0] if positions is not None else 1
-    if sections is None:
-        sections = [cos.shape[1]]
-    _want(len(sections) == d.axes and len(sections) <= 4,
-          f"{len(sections)} sections for {d.axes} axes (at most 4)")
-    d.section0, d.section1, d.section2, d.section3 = list(sections) + [0] * (4 - len(sections))
+    d.axes, d._tokens = 1, None
+    if positions is not None:
+        d.positions = _device_array(positions, "positions", torch.int32, positions.shape, device)
+        d.axes, d._tokens = positions.shape
+    sections = [cos.shape[1]] if sections is None else list(sections)
+    if len(sections) != d.axes or len(sections) > 4:
+        _refuse(f"{len(sections)} sections for {d.axes} axes (at most 4)")
+    d.section0, d.section1, d.section2, d.section3 = sections + [0] * (4 - len(sections))
     d.interleaved = int(interleaved)
-    d._keep = (cos, sin, positions)
+    d._keep, d._device = (cos, sin, positions), device
     return d
 
 
@@ -434,11 +449,9 @@ class Context:
             tokens_out.numel() if tokens_out is not None else 0), "aexq_decode_advance")
 
     # ---- many sequences
-    def _paged(self, kv: _abi.PagedKv) -> torch.device:
-        _want(isinstance(kv, _abi.PagedKv) and hasattr(kv, "_keep"), "kv is not from paged_kv()")
-        device = torch.device("cuda", self.device)
-        _want(kv._keep[0].device == device, f"the cache is on {kv._keep[0].device}, not {device}")
-        return device
+    def _on_device(self, d, kind):
+        if not isinstance(d, kind) or getattr(d, "_device", None) != self.device:
+            _refuse(f"{d!r} is not a {kind.__name__} of GPU {self.device}'s tensors")
 
     def rope_append_paged(self, kv: _abi.PagedKv, rope: _abi.Rope, offsets: torch.Tensor,
                           q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -448,22 +461,21 @@ class Context:
         [tokens][heads_kv][head_dim] to the paged cache.  offsets [sequences + 1]
         (int32): where each sequence's new tokens start; they become its last
         positions, before kv's lengths."""
-        device, tokens = self._paged(kv), q.shape[0]
-        _want(isinstance(rope, _abi.Rope) and hasattr(rope, "_keep"), "rope is not from rope()")
-        _want(rope._keep[0].device == device, f"the tables are on {rope._keep[0].device}")
-        positions = rope._keep[2]
-        _want(positions is None or positions.shape[1] == tokens,
-              f"positions of {None if positions is None else positions.shape[1]} tokens, not {tokens}")
+        device = self.device
+        self._on_device(kv, _abi.PagedKv)
+        self._on_device(rope, _abi.Rope)
+        tokens, heads, _ = _head_shape(q, "q")
+        if rope._tokens is not None and rope._tokens != tokens:
+            _refuse(f"positions of {rope._tokens} tokens, q of {tokens}")
         off = _device_array(offsets, "offsets", torch.int32, (kv.sequences + 1,), device)
-        d, hkv = kv.head_dim, kv.heads_kv
-        qs = _head_rows(q, "q", tokens, None, d, device)
-        ks = _head_rows(k, "k", tokens, hkv, d, device)
-        vs = _head_rows(v, "v", tokens, hkv, d, device)
-        os_ = _head_rows(q_out, "q_out", tokens, q.shape[1], d, device)
+        d = kv.head_dim
+        qs = _head_rows(q, "q", (tokens, heads, d), device)
+        ks = _head_rows(k, "k", (tokens, kv.heads_kv, d), device)
+        vs = _head_rows(v, "v", (tokens, kv.heads_kv, d), device)
+        os_ = _head_rows(q_out, "q_out", (tokens, heads, d), device)
         check(self._lib.aexq_rope_append_paged(
-            self.handle, ctypes.byref(kv), ctypes.byref(rope), off, tokens, q.shape[1],
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, q_out.data_ptr(), os_),
-            "aexq_rope_append_paged")
+            self.handle, kv, rope, off, tokens, heads, q.data_ptr(), qs, k.data_ptr(), ks,
+            v.data_ptr(), vs, q_out.data_ptr(), os_), "aexq_rope_append_paged")
 
     def attention_prompt(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                          offsets: torch.Tensor, scale: float, out: torch.Tensor, *,
@@ -472,45 +484,50 @@ class Context:
         [kv tokens][heads_kv][head_dim] (fp16), sequence s in rows offsets[s] ..
         offsets[s + 1] - 1 (int32 [sequences + 1]; of k and v by kv_offsets where
         given).  causal: the queries are the last positions of their sequence."""
-        device = torch.device("cuda", self.device)
-        _want(offsets.dim() == 1 and offsets.shape[0] >= 2, "offsets holds no sequence")
-        n, tokens, kv_tokens = offsets.shape[0] - 1, q.shape[0], k.shape[0]
+        device = self.device
+        tokens, heads, d = _head_shape(q, "q")
+        kv_tokens, heads_kv, _ = _head_shape(k, "k")
+        n = offsets.numel() - 1 if isinstance(offsets, torch.Tensor) else 0
         off = _device_array(offsets, "offsets", torch.int32, (n + 1,), device)
-        kvo = (_device_array(kv_offsets, "kv_offsets", torch.int32, (n + 1,), device)
-               if kv_offsets is not None else None)
-        _want(q.dim() == 3 and k.dim() == 3, "q and k are [tokens][heads][head_dim]")
-        d = q.shape[2]
-        qs = _head_rows(q, "q", tokens, None, d, device)
-        ks = _head_rows(k, "k", kv_tokens, None, d, device)
-        vs = _head_rows(v, "v", kv_tokens, k.shape[1], d, device)
-        os_ = _head_rows(out, "out", tokens, q.shape[1], d, device)
+        kvo = None
+        if kv_offsets is not None:
+            kvo = _device_array(kv_offsets, "kv_offsets", torch.int32, (n + 1,), device)
+        qs = _head_rows(q, "q", (tokens, heads, d), device)
+        ks = _head_rows(k, "k", (kv_tokens, heads_kv, d), device)
+        vs = _head_rows(v, "v", (kv_tokens, heads_kv, d), device)
+        os_ = _head_rows(out, "out", (tokens, heads, d), device)
         check(self._lib.aexq_attention_prompt(
             self.handle, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, off, kvo, n, tokens,
-            kv_tokens, q.shape[1], k.shape[1], d, int(causal), scale, out.data_ptr(), os_),
+            kv_tokens, heads, heads_kv, d, causal, scale, out.data_ptr(), os_),
             "aexq_attention_prompt")
 
     def attention_prompt_paged(self, kv: _abi.PagedKv, q: torch.Tensor, offsets: torch.Tensor,
                                scale: float, out: torch.Tensor):
         """Causal attention of packed rows over the paged cache; sequence s's rows
         offsets[s] .. offsets[s + 1] - 1 are its last positions."""
-        device, tokens = self._paged(kv), q.shape[0]
+        device = self.device
+        self._on_device(kv, _abi.PagedKv)
+        tokens, heads, _ = _head_shape(q, "q")
         off = _device_array(offsets, "offsets", torch.int32, (kv.sequences + 1,), device)
-        qs = _head_rows(q, "q", tokens, None, kv.head_dim, device)
-        os_ = _head_rows(out, "out", tokens, q.shape[1], kv.head_dim, device)
+        qs = _head_rows(q, "q", (tokens, heads, kv.head_dim), device)
+        os_ = _head_rows(out, "out", (tokens, heads, kv.head_dim), device)
         check(self._lib.aexq_attention_prompt_paged(
-            self.handle, ctypes.byref(kv), q.data_ptr(), qs, off, tokens, q.shape[1], scale,
-            out.data_ptr(), os_), "aexq_attention_prompt_paged")
+            self.handle, kv, q.data_ptr(), qs, off, tokens, heads, scale, out.data_ptr(), os_),
+            "aexq_attention_prompt_paged")
 
     def attention_decode_paged(self, kv: _abi.PagedKv, q: torch.Tensor, scale: float,
                                out: torch.Tensor):
         """Decode attention of one row per sequence, q and out
         [sequences][heads_q][head_dim], over the paged cache."""
-        device = self._paged(kv)
-        qs = _head_rows(q, "q", kv.sequences, None, kv.head_dim, device)
-        os_ = _head_rows(out, "out", kv.sequences, q.shape[1], kv.head_dim, device)
+        device = self.device
+        self._on_device(kv, _abi.PagedKv)
+        _, heads, _ = _head_shape(q, "q")
+        shape = (kv.sequences, heads, kv.head_dim)
+        qs = _head_rows(q, "q", shape, device)
+        os_ = _head_rows(out, "out", shape, device)
         check(self._lib.aexq_attention_decode_paged(
-            self.handle, ctypes.byref(kv), q.data_ptr(), qs, q.shape[1], scale, out.data_ptr(),
-            os_), "aexq_attention_decode_paged")
+            self.handle, kv, q.data_ptr(), qs, heads, scale, out.data_ptr(), os_),
+            "aexq_attention_decode_paged")
 
     def logprobs(self, logits: _abi.Tensor, tokens: Optional[torch.Tensor],
                  logprob: Optional[torch.Tensor], entropy: Optional[torch.Tensor] = None,
@@ -519,20 +536,24 @@ class Context:
         """Log probabilities over rows of logits: of tokens [rows] (int32) into
         logprob [rows], the entropy [rows] (nats), and the top alternatives
         top_ids (int32), top_logprobs [rows][top]; what is None is not computed."""
-        device, rows = torch.device("cuda", self.device), logits.logical.h
-        _want(getattr(logits, "_keep", None) is None or logits._keep.device == device,
-              f"the logits are not on {device}")
-        array = lambda t, name, dtype, shape: (
-            _device_array(t, name, dtype, shape, device) if t is not None else None)
-        tok = array(tokens, "tokens", torch.int32, (rows,))
-        lp = array(logprob, "logprob", torch.float32, (rows,))
-        ent = array(entropy, "entropy", torch.float32, (rows,))
-        some = top_ids if top_ids is not None else top_logprobs
-        top = some.shape[-1] if some is not None else 0
-        ids = array(top_ids, "top_ids", torch.int32, (rows, top))
-        val = array(top_logprobs, "top_logprobs", torch.float32, (rows, top))
-        check(self._lib.aexq_logprobs(self.handle, ctypes.byref(logits), tok, lp, ent, top, ids,
-                                      val), "aexq_logprobs")
+        device, rows, top = self.device, logits.logical.h, 0
+        if logits._keep.get_device() != device:
+            _refuse(f"the logits are on {logits._keep.device}, not on GPU {device}")
+        tok = lp = ent = ids = val = None
+        if tokens is not None:
+            tok = _device_array(tokens, "tokens", torch.int32, (rows,), device)
+        if logprob is not None:
+            lp = _device_array(logprob, "logprob", torch.float32, (rows,), device)
+        if entropy is not None:
+            ent = _device_array(entropy, "entropy", torch.float32, (rows,), device)
+        if top_ids is not None:
+            top = top_ids.shape[-1]
+            ids = _device_array(top_ids, "top_ids", torch.int32, (rows, top), device)
+        if top_logprobs is not None:
+            top = top if top_ids is not None else top_logprobs.shape[-1]
+            val = _device_array(top_logprobs, "top_logprobs", torch.float32, (rows, top), device)
+        check(self._lib.aexq_logprobs(self.handle, logits, tok, lp, ent, top, ids, val),
+              "aexq_logprobs")
 
     def decoder(self, layers, embedding: "QuantWeight", heads_q: int, heads_kv: int,
                 head_dim: int, capacity: int, rms_eps: float, attn_scale: float,

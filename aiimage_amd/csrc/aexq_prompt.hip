@@ -3,6 +3,8 @@
 // paged cache (whose last rows the queries then are).
 #include <math.h>
 
+#include <type_traits>
+
 #include "aexq_paged.hpp"
 
 namespace aexq {
@@ -47,11 +49,11 @@ __device__ __forceinline__ int swz(int r) {
   return (r & 3) << 2 | (r >> 2 & 3);
 }
 
-// Lane i's 16 bytes at its own address to LDS byte lds + 16 i.
-__device__ __forceinline__ void dma_lane(const void* from, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+// Lane i's 16 bytes at byte `off` (its own) of `from` to LDS byte lds + 16 i.
+__device__ __forceinline__ void dma_lane(const void* from, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
-               : "s"(lds), "v"(from)
+               : "s"(lds), "v"(off), "s"(from)
                : "memory", "m0");
 }
 
@@ -133,9 +135,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   for (int s = 0; s < KS; ++s)
     qf[s] = *(const f16x8*)(p.q + token * p.q_stride + qh * D + 16 * s + 8 * h);
   const int vis = seen(rr);
-  // what the wave's rows see at least and at most, and the workgroup's
-  const int w0 = min(tile * kPromptRows + wave * 32, last);
-  const int lo = sreg(seen(w0)), hi = sreg(seen(min(w0 + 31, last)));
+  // what the wave's rows see at most, and the workgroup's at least and at most
+  const int hi = sreg(seen(min(tile * kPromptRows + wave * 32 + 31, last)));
   const int low = sreg(seen(tile * kPromptRows));
   const int most = sreg(seen(min(tile * kPromptRows + kPromptRows - 1, last)));
   const int tiles = (most + KT - 1) / KT;
@@ -145,49 +146,81 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   for (int i = 0; i < DB; ++i) o[i] = f32x16{};
   float m = -INFINITY, l = 0.0f;
 
-  auto fetch = [&](int t, int b) {
-    const int r0 = wave * (KT / 4);
-    long long page_row = 0;
-    if constexpr (PAGED) {
-      // a wave's rows lie in one block of 16 positions, so in one page
-      const int x = min(t * KT + r0, len - 1);
-      page_row = ((long long)sreg(paged_page(p.kv, seq, x >> p.kv.shift)) * p.kv.hkv + head)
-                 << p.kv.shift;
-    }
+  // A wave's rows of a tile lie in one block of 16 positions, so in one page: a
+  // uniform base and an offset of each lane's own, the same for every tile that
+  // ends before the sequence does.
+  const int r0 = wave * (KT / 4);
+  const int kst = PAGED ? D * 2 : (int)p.k_stride * 2, vst = PAGED ? D * 2 : (int)p.v_stride * 2;
+  uint32_t koff[NL], voff[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = r0 + i * RL + lane / CH;
-      const int chunk = lane % CH ^ swz<D>(r);
-      const int x = min(t * KT + r, len - 1);  // rows past the end repeat the last one
-      const uint32_t to = (r0 + i * RL) * D * 2;
-      if constexpr (PAGED) {
-        const long long a = (page_row + (x & ((1 << p.kv.shift) - 1))) * D + 8 * chunk;
-        dma_lane(p.kv.k + a, lds_addr(lds.k[b]) + to);
-        dma_lane(p.kv.v + a, lds_addr(lds.v[b]) + to);
-      } else {
-        const long long a = kv0 + x;
-        dma_lane(p.k + a * p.k_stride + head * D + 8 * chunk, lds_addr(lds.k[b]) + to);
-        dma_lane(p.v + a * p.v_stride + head * D + 8 * chunk, lds_addr(lds.v[b]) + to);
+  for (int i = 0; i < NL; ++i) {
+    const int r = i * RL + lane / CH, chunk = lane % CH ^ swz<D>(r0 + r);
+    koff[i] = r * kst + 16 * chunk;
+    voff[i] = r * vst + 16 * chunk;
+  }
+  const uint32_t lds_base = lds_addr(&lds);
+  auto fetch = [&](int t, int b) {
+    const int x = min(t * KT + r0, len - 1);
+    const f16 *kb, *vb;
+    if constexpr (PAGED) {
+      const long long a =
+          ((((long long)sreg(paged_page(p.kv, seq, x >> p.kv.shift)) * p.kv.hkv + head)
+            << p.kv.shift) + (x & ((1 << p.kv.shift) - 1))) * D;
+      kb = p.kv.k + a;
+      vb = p.kv.v + a;
+    } else {
+      kb = p.k + (long long)(kv0 + x) * p.k_stride + head * D;
+      vb = p.v + (long long)(kv0 + x) * p.v_stride + head * D;
+    }
+    kb = sreg(kb);
+    vb = sreg(vb);
+    const uint32_t kl = lds_base + (b * KT + r0) * D * 2, vl = kl + 2 * KT * D * 2;
+    if ((t + 1) * KT <= len) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        dma_lane(kb, koff[i], kl + i * 1024);
+        dma_lane(vb, voff[i], vl + i * 1024);
+      }
+    } else {
+      // rows past the end repeat the last one
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = i * RL + lane / CH, back = max(r - (len - 1 - x), 0);
+        dma_lane(kb, koff[i] - back * kst, kl + i * 1024);
+        dma_lane(vb, voff[i] - back * vst, vl + i * 1024);
       }
     }
   };
 
-  const int ksw = swz<D>(j);
-  const int tg = lane >> 4 & 1, ti = lane & 15;  // transposed reads: 16-dim half, lane of 16
+  // Where the lane's operands lie in a tile: step s of K (16 dims), and of V the
+  // four positions z of 16 and the 32 dims i (the 16-dim half tg, lane ti of 16).
+  // Everything else of an address is the instruction's own offset.
+  int kat[KS], vat[2][DB];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) kat[s] = j * D + 8 * ((2 * s + h) ^ swz<D>(j));
+#pragma unroll
+  for (int z = 0; z < 2; ++z)
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+      const int tg = lane >> 4 & 1, ti = lane & 15, r = 8 * z + 4 * h + ti / 4;
+      vat[z][i] = r * D + 8 * ((2 * tg + (ti & 3) / 2) ^ (4 * i) ^ swz<D>(r)) + 4 * (ti & 1);
+    }
 
-  if (tiles > 0) fetch(0, 0);
-  for (int t = 0; t < tiles; ++t) {
-    const int b = t & 1, x0 = t * KT;
+  // One tile; EDGE: some row of the workgroup does not see all of it.  `buf`: its
+  // buffer where the code is for one of them, else -1.
+  auto take = [&](int t, auto edge, auto buf) {
+    constexpr bool EDGE = decltype(edge)::value;
+    constexpr int BUF = decltype(buf)::value;
+    const int b = BUF >= 0 ? BUF : t & 1, x0 = t * KT;
     wait_vm<0>();
-    const bool edge = x0 + KT > low;  // some row of the workgroup does not see all of it
-    if (edge) {
+    if constexpr (EDGE) {
       // An infinity or a NaN in V reaches, through 0 * V, the rows that do not
       // see it: each wave looks through the rows it fetched.
       float z = 0.0f;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const u32x4 y = *(const u32x4*)((const char*)lds.v[b] +
-                                        (wave * (KT / 4) + i * RL) * D * 2 + lane * 16);
+        const u32x4 y =
+            *(const u32x4*)((const char*)lds.v[b] + r0 * D * 2 + i * 1024 + lane * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) z = dot2(y[e], 0u, z);
       }
@@ -197,7 +230,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
     }
     bar();
     if (t + 1 < tiles) fetch(t + 1, b ^ 1);
-    if (x0 >= hi) continue;  // none of the wave's rows sees any of it
+    if (EDGE && x0 >= hi) return;  // none of the wave's rows sees any of it
 
     f32x16 sc[SB];
 #pragma unroll
@@ -206,11 +239,21 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < SB; ++i) {
-        const f16x8 kf = *(const f16x8*)&lds.k[b][(32 * i + j) * D + 8 * ((2 * s + h) ^ ksw)];
+        const f16x8 kf = *(const f16x8*)&lds.k[b][32 * i * D + kat[s]];
         sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], sc[i], 0, 0, 0);
       }
-    const bool masked = x0 + KT > lo;
-    if (masked) {
+    if constexpr (BUF >= 0) {
+      // eight K reads ahead of the products that take them
+      constexpr int N = KS * SB, AHEAD = N < 8 ? N : 8;
+      __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+      for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+    }
+    if constexpr (EDGE) {
       const int left = vis - x0 - 4 * h;
 #pragma unroll
       for (int i = 0; i < SB; ++i)
@@ -242,7 +285,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
         sc[i][r] = exp2_fast(fmaf(sc[i][r], p.scale2, -base));
         l += sc[i][r];
       }
-    if (masked && (lds.odd[b][0] | lds.odd[b][1] | lds.odd[b][2] | lds.odd[b][3])) {
+    if (EDGE && (lds.odd[b][0] | lds.odd[b][1] | lds.odd[b][2] | lds.odd[b][3])) {
       // position by position, for the rows that see it
       for (int x = 0; x < KT && x0 + x < hi; ++x) {
         float w = 0.0f;
@@ -263,7 +306,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
             o[i][r] = in ? fmaf(w, (float)y, o[i][r]) : o[i][r];
           }
       }
-      continue;
+      return;
     }
 #pragma unroll
     for (int y = 0; y < KT / 16; ++y) {
@@ -274,16 +317,20 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
       for (int i = 0; i < DB; ++i) {
         f16x4 a[2];
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int r = 16 * y + 8 * z + 4 * h + ti / 4;
-          const int chunk = (2 * tg + (ti & 3) / 2) ^ (4 * i) ^ swz<D>(8 * z + 4 * h + ti / 4);
-          a[z] = read_transposed(&lds.v[b][r * D + 8 * chunk + 4 * (ti & 1)]);
-        }
+        for (int z = 0; z < 2; ++z) a[z] = read_transposed(&lds.v[b][16 * y * D + vat[z][i]]);
         const f16x8 vf = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7);
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w, o[i], 0, 0, 0);
       }
     }
+  };
+  if (tiles > 0) fetch(0, 0);
+  const int whole = min(low / KT, tiles);
+  int t = 0;
+  for (; t + 1 < whole; t += 2) {
+    take(t, std::false_type{}, std::integral_constant<int, 0>{});
+    take(t + 1, std::false_type{}, std::integral_constant<int, 1>{});
   }
+  for (; t < tiles; ++t) take(t, std::true_type{}, std::integral_constant<int, -1>{});
 
   // 3. the row's two lanes hold half of its sum each; a row that sees nothing is
   // 0, one whose every score was -inf (a sum of 0) NaN
