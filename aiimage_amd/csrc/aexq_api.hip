@@ -2262,7 +2262,7 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
   p.scale2 = scale * 1.4426950408889634f;
   p.min_run = 1;
   const long long bound = (long long)kv->table_width * kv->page_size;
-  const int grid = decode_paged_split(bound) ? decode_paged_grid(ctx->cus) : 0;
+  const int grid = decode_paged_split(bound) ? decode_paged_grid(kv->head_dim, ctx->cus) : 0;
   // runs count units of all sequences in 31 bits
   const long long units =
       (bound / 128 + 1) * kv->sequences * (long long)(kv->heads_kv * p.blocks);

@@ -304,8 +304,11 @@ struct RopeAppendParams {
   const float *cos_table, *sin_table;  // [rows][rot / 2]
   const int32_t* positions;            // [axes][tokens]; null: the cache positions
   int rows, rot, axes, interleaved, sections[4];
+  // set by the launch: waves of a token, and 2^32 over the pieces of a head
+  int waves;
+  uint32_t per_r8, per_c8;
 };
-hipError_t rope_append_launch(const RopeAppendParams& p, hipStream_t stream);
+hipError_t rope_append_launch(RopeAppendParams p, hipStream_t stream);
 // attention of one row per sequence; heads go in blocks of up to 16 of a group
 struct DecodePagedParams {
   PagedView kv;
@@ -318,7 +321,7 @@ struct DecodePagedParams {
   int* plan;          // 1 + n ints
   int min_run;        // units a workgroup takes at least
 };
-int decode_paged_grid(int cus);
+int decode_paged_grid(int head_dim, int cus);
 bool decode_paged_split(long long bound);
 long long decode_paged_part_floats(int head_dim, int grid);
 // grid 0: one workgroup per (head block, sequence)

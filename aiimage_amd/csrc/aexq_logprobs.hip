@@ -14,10 +14,10 @@ namespace aexq {
 // Lanes take 16-byte chunks in turn; what a lane keeps for the alternatives is
 // its best chunk (by its largest logit) and the largest logit of the others.
 //
-// The K best of the row, by logit and then by index: among the 256 lanes' best
-// chunks the K-th is a bound that at least K logits reach, so only chunks that
-// reach it are read again (mostly about K of them), and a lane's whole share
-// only where its second chunk reaches it too.  Those logits go through a sorted
+// The K best of the row, by logit and then by index: a bound that K of the 256
+// lanes' best chunks reach is one that K logits reach, so only chunks that reach
+// it are read again (mostly about K of them), and a lane's whole share only where
+// its second chunk reaches it too.  Those logits go through a sorted
 // list per wave, an entry a lane; the four lists are merged by counting, for
 // each entry, the entries above it.
 //
@@ -92,11 +92,41 @@ __device__ __forceinline__ void list_insert(u64& entry, u64 key) {
   entry = lane < at ? entry : lane == at ? key : up;
 }
 
+// A key that at least `top` of the kThreads keys (0: none) reach, and few more:
+// bit by bit from above until no more than `top` + 8 reach it.  0 where fewer than
+// `top` are there.  By every wave, four keys a lane.
+__device__ __forceinline__ u64 top_bound(const u64* keys, int top) {
+  const int lane = threadIdx.x & 63;
+  u64 k[kThreads / 64];
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) k[i] = keys[i * 64 + lane];
+  uint32_t high = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t c = high | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) n += __popcll(__ballot((uint32_t)(k[i] >> 32) >= c));
+    if (n < top) continue;
+    high = c;
+    if (n <= top + 8) return (u64)high << 32;
+  }
+  uint32_t low = 0;  // many equal logits: by index too
+  for (int bit = 31; bit >= 0; --bit) {
+    const u64 c = (u64)high << 32 | low | 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) n += __popcll(__ballot(k[i] >= c));
+    if (n >= top) low |= 1u << bit;
+  }
+  return (u64)high << 32 | low;
+}
+
 template <typename E>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p) {
   constexpr int VE = 16 / (int)sizeof(E), U = 4;  // logits of a chunk, chunks in flight
   __shared__ Stats wave_stats[kWaves];
-  __shared__ u64 keys[kThreads], sorted[64], bound;
+  __shared__ u64 keys[kThreads], sorted[64];
+  __shared__ int counts[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
   const E* x = (const E*)p.x + (long long)row * p.rstride;
@@ -170,14 +200,9 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
     // some logit of the best chunk is `best`, at the chunk's last index or before
     const u64 mine = any ? top_key(best, min(best_chunk * VE - skew + VE, p.n) - 1) : 0;
     keys[tid] = mine;
-    if (tid == 0) bound = 0;
     if (tid < 64) sorted[tid] = 0;
     __syncthreads();
-    int above = 0;
-    for (int i = 0; i < kThreads; ++i) above += keys[i] > mine;
-    if (any && above == p.top - 1) bound = mine;
-    __syncthreads();
-    const u64 least = bound;  // 0: fewer chunks than alternatives, so all of them
+    const u64 least = top_bound(keys, p.top);  // 0: fewer chunks than alternatives, so all of them
     const bool all = any && argmax_ord(second) >= (uint32_t)(least >> 32);
     const bool one = any && !all && top_key(best, max(best_chunk * VE - skew, 0)) >= least;
     u64 entry = 0;
@@ -206,13 +231,15 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
         take(at, at < c1);
       }
     }
+    const u64 own = lane < p.top ? entry : 0;
     __syncthreads();
-    keys[tid] = lane < p.top ? entry : 0;
+    keys[tid] = own;
+    const int held = __popcll(__ballot(own != 0));
+    if (lane == 0) counts[wave] = held;
     __syncthreads();
-    const u64 own = keys[tid];
-    above = 0;
+    int above = 0;
     for (int w = 0; w < kWaves; ++w)
-      for (int i = 0; i < p.top; ++i) above += keys[w * 64 + i] > own;
+      for (int i = 0; i < counts[w]; ++i) above += keys[w * 64 + i] > own;
     if (own && above < p.top) sorted[above] = own;
   }
   __syncthreads();
@@ -237,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
 template <typename E>
 __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobParams p) {
   __shared__ Stats wave_stats[kWaves];
-  __shared__ u64 first[kThreads], reach[64 * 64], sorted[64], bound;
+  __shared__ u64 first[kThreads], reach[72 * 64], sorted[64];
   __shared__ int count;
   const int row = blockIdx.x, tid = threadIdx.x;
   const u64* keys = p.keys + (long long)row * p.parts * p.top;
@@ -253,18 +280,11 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobPar
   u64 key = 0;
   if (p.top) {
     first[tid] = mine;
-    if (tid == 0) {
-      bound = 0;
-      count = 0;
-    }
+    if (tid == 0) count = 0;
     if (tid < 64) sorted[tid] = 0;
     __syncthreads();
-    int above = 0;
-    for (int i = 0; i < p.parts; ++i) above += first[i] > mine;
-    if (mine && above == p.top - 1) bound = mine;
-    __syncthreads();
-    const u64 least = bound;
-    // keys that reach the bound lie in at most top parts (top - 1 parts in all
+    const u64 least = top_bound(first, p.top);
+    // keys that reach the bound lie in at most top + 8 parts (fewer than top in all
     // where there is no bound): no more than the buffer holds
     for (int i = tid; i < p.parts * p.top; i += kThreads) {
       const u64 k = keys[i];
@@ -274,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobPar
     const int n = count;
     for (int i = tid; i < n; i += kThreads) {
       const u64 own = reach[i];
-      above = 0;
+      int above = 0;
       for (int j = 0; j < n; ++j) above += reach[j] > own;
       if (above < p.top) sorted[above] = own;
     }

@@ -12,108 +12,161 @@
 namespace aexq {
 
 // ---------------------------------------------------------------------------
-// Rotary positions and append.  One workgroup per packed token t: the cos and
-// sin of its head's pairs go to LDS once (pair j from the table row of its
-// axis' position), then each thread moves 16-byte pieces: eight pairs (j, j +
-// rot/2) of a q or k head, eight unrotated elements behind them, or eight of v.
+// Rotary positions and append.  One wave per packed token (or four, where there
+// are few tokens): the cos and sin of a head's pairs go to its LDS once (pair j
+// from the table row of its axis' position), then each lane moves 16-byte pieces,
+// several on the way at a time: first those of eight pairs (j, j + rot/2) of a q
+// or k head, then eight unrotated elements behind them, then eight of v, so that
+// the lanes of a wave mostly do the same.
 //   x'[j] = x[j] cos - x[j + rot/2] sin,  x'[j + rot/2] = x[j] sin + x[j + rot/2] cos
 // in fp32, rounded once to fp16.  Token t of a sequence with n new tokens and
 // length L (after the append) lands at position L - n + (t - first).
 // ---------------------------------------------------------------------------
+template <int U>  // pieces of a lane on the way
 __global__ __launch_bounds__(kThreads) void rope_append_kernel(const RopeAppendParams p) {
-  __shared__ float cs[128], sn[128];
-  const int t = blockIdx.x, tid = threadIdx.x;
+  __shared__ float table[kWaves][2][128];
+  const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6);
+  const int index = blockIdx.x * kWaves + wave;
+  const int t = index / p.waves, lead = index % p.waves * 64 + lane, step = 64 * p.waves;
+  if (t >= p.tokens) return;  // (waves meet nowhere below)
+  float* cs = table[wave][0];
+  float* sn = table[wave][1];
   const int d = p.d, half = p.rot / 2;
-  const int r8 = half / 8, c8 = (d - p.rot) / 8, per_head = r8 + c8;
-  const int rotated = (p.hq + p.kv.hkv) * per_head, total = rotated + p.kv.hkv * (d / 8);
+  const int r8 = half / 8, c8 = (d - p.rot) / 8, heads = p.hq + p.kv.hkv;
+  const int turns = heads * r8, copies = heads * c8, log8 = __builtin_ctz(d) - 3;
+  const int total = turns + copies + (p.kv.hkv << log8);
 
-  struct Piece {
-    u32x4 a, b;
+  // piece id: its head (q's, then k's, then v's), its first element, and whether
+  // that is turned with the one rot/2 behind it
+  struct Place {
+    int head, at;
+    bool turn;
   };
-  auto source = [&](int id) -> const f16* {
-    if (id >= rotated)
-      return p.v + (long long)t * p.v_stride + (long long)(id - rotated) * 8;
-    const int head = id / per_head, sub = id % per_head;
-    const f16* row = head < p.hq ? p.q + (long long)t * p.q_stride + head * d
-                                 : p.k + (long long)t * p.k_stride + (head - p.hq) * d;
-    return row + (sub < r8 ? 8 * sub : p.rot + 8 * (sub - r8));
-  };
-  auto load = [&](int id) {
-    const f16* s = source(id);
-    Piece x;
-    x.a = *(const u32x4*)s;
-    x.b = x.a;
-    if (id < rotated && id % per_head < r8) x.b = *(const u32x4*)(s + half);
+  auto place = [&](int id) {
+    Place x;
+    x.turn = id < turns;
+    if (x.turn) {
+      x.head = r8 == 1 ? id : __umulhi(id, p.per_r8);
+      x.at = 8 * (id - x.head * r8);
+    } else if (id < turns + copies) {
+      x.head = __umulhi(id - turns, p.per_c8);
+      x.at = p.rot + 8 * (id - turns - x.head * c8);
+    } else {
+      const int e = id - turns - copies;
+      x.head = heads + (e >> log8);
+      x.at = 8 * (e & ((1 << log8) - 1));
+    }
     return x;
   };
-  Piece x{};
-  if (tid < total) x = load(tid);  // before anything else is known of the token
+  u32x4 xa[U], xb[U];
+  auto load = [&](int id, u32x4& a, u32x4& b) {
+    id = min(id, total - 1);  // (a lane without a piece reads the last one)
+    const Place x = place(id);
+    const int kv = x.head - p.hq;
+    const f16* row = kv < 0            ? p.q + (long long)t * p.q_stride + x.head * d
+                     : kv < p.kv.hkv ? p.k + (long long)t * p.k_stride + kv * d
+                                     : p.v + (long long)t * p.v_stride + (kv - p.kv.hkv) * d;
+    a = *(const u32x4*)(row + x.at);
+    b = a;
+    if (x.turn) b = *(const u32x4*)(row + x.at + half);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u)  // before anything else is known of the token
+    load(lead + step * u, xa[u], xb[u]);
 
-  const int s = packed_sequence(p.offsets, p.kv.n, t);
-  if (s >= p.kv.n) return;  // rows behind the last sequence stay as they were
-  const int first = p.offsets[s], count = p.offsets[s + 1] - first;
-  if (t < first) return;
-  const int pos = p.kv.lengths[s] - count + (t - first);
+  // where positions are given, the tables' rows wait for nothing else
+  auto turn_by = [&](int pos) {
+    for (int j = lane; j < half; j += 64) {
+      int axis = 0, end = p.sections[0];
+#pragma unroll
+      for (int a = 1; a < 4; ++a) {
+        if (p.interleaved) {
+          if (j % p.axes == a && j < p.axes * p.sections[a]) axis = a;
+        } else {
+          if (a < p.axes && j >= end) axis = a;
+          end += p.sections[a];
+        }
+      }
+      int at = p.positions ? p.positions[(long long)axis * p.tokens + t] : pos;
+      at = min(max(at, 0), p.rows - 1);
+      cs[j] = p.cos_table[(long long)at * half + j];
+      sn[j] = p.sin_table[(long long)at * half + j];
+    }
+  };
+  const PackedRow own = packed_row(p.offsets, p.kv.lengths, p.kv.n, t);
+  if (p.positions) turn_by(0);
+  if (!own.found) return;  // rows behind the last sequence stay as they were
+  const int pos = own.length - (own.end - t);
   // where its k and v rows go; nowhere outside the table or the pool
   int page = -1;
   if (pos >= 0 && pos < p.kv.width << p.kv.shift)
-    page = p.kv.table[(long long)s * p.kv.width + (pos >> p.kv.shift)];
+    page = p.kv.table[(long long)own.seq * p.kv.width + (pos >> p.kv.shift)];
   const bool keep = page >= 0 && page < p.kv.pages;
   const int row = pos & ((1 << p.kv.shift) - 1);
-  if (tid < half) {
-    int axis = 0;
-    if (p.interleaved) {
-      axis = tid % p.axes;
-      if (tid >= p.axes * p.sections[axis]) axis = 0;
-    } else {
-      for (int a = 0, end = p.sections[0]; a + 1 < p.axes && tid >= end; end += p.sections[++a])
-        axis = a + 1;
-    }
-    int at = p.positions ? p.positions[(long long)axis * p.tokens + t] : pos;
-    at = min(max(at, 0), p.rows - 1);
-    cs[tid] = p.cos_table[(long long)at * half + tid];
-    sn[tid] = p.sin_table[(long long)at * half + tid];
-  }
-  __syncthreads();
-  for (int id = tid; id < total; id += kThreads) {
-    if (id != tid) x = load(id);
-    if (id >= rotated) {
-      if (!keep) continue;
-      const int g = (id - rotated) / (d / 8), e = (id - rotated) % (d / 8);
-      f16* to = p.vp + ((((long long)page * p.kv.hkv + g) << p.kv.shift) + row) * d;
-      *(u32x4*)(to + 8 * e) = x.a;
-      continue;
-    }
-    const int head = id / per_head, sub = id % per_head;
-    if (head >= p.hq && !keep) continue;
-    f16* to = head < p.hq
-                  ? p.q_out + (long long)t * p.q_out_stride + head * d
-                  : p.kp + ((((long long)page * p.kv.hkv + (head - p.hq)) << p.kv.shift) + row) * d;
-    if (sub >= r8) {
-      *(u32x4*)(to + p.rot + 8 * (sub - r8)) = x.a;
-      continue;
+  if (!p.positions) turn_by(pos);
+  // the wave's own LDS: its stores before its loads
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  // (stored past the caches: 46 us for the 214 MB above, 57 through them)
+  auto store = [&](int id, const u32x4& xa, const u32x4& xb) {
+    const Place x = place(id);
+    const int kv = x.head - p.hq;
+    if (id >= total || (kv >= 0 && !keep)) return;
+    f16* to;
+    if (kv < 0)
+      to = p.q_out + (long long)t * p.q_out_stride + x.head * d;
+    else if (kv < p.kv.hkv)
+      to = p.kp + ((((long long)page * p.kv.hkv + kv) << p.kv.shift) + row) * d;
+    else
+      to = p.vp + ((((long long)page * p.kv.hkv + (kv - p.kv.hkv)) << p.kv.shift) + row) * d;
+    to += x.at;
+    if (!x.turn) {
+      __builtin_nontemporal_store(xa, (u32x4*)to);
+      return;
     }
     u32x4 lo, hi;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const f16x2 a = as_h2(x.a[e]), b = as_h2(x.b[e]);
+      const f16x2 a = as_h2(xa[e]), b = as_h2(xb[e]);
       f16x2 u, w;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float c = cs[8 * sub + 2 * e + i], z = sn[8 * sub + 2 * e + i];
+        const float c = cs[x.at + 2 * e + i], z = sn[x.at + 2 * e + i];
         u[i] = (f16)((float)a[i] * c - (float)b[i] * z);
         w[i] = (f16)((float)a[i] * z + (float)b[i] * c);
       }
       lo[e] = as_u(u);
       hi[e] = as_u(w);
     }
-    *(u32x4*)(to + 8 * sub) = lo;
-    *(u32x4*)(to + 8 * sub + half) = hi;
+    __builtin_nontemporal_store(lo, (u32x4*)to);
+    __builtin_nontemporal_store(hi, (u32x4*)(to + half));
+  };
+  for (int id = lead;;) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) store(id + step * u, xa[u], xb[u]);
+    id += step * U;
+    if (id - lead >= total) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(id + step * u, xa[u], xb[u]);
   }
 }
 
-hipError_t rope_append_launch(const RopeAppendParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(rope_append_kernel, dim3(p.tokens), dim3(kThreads), 0, stream, p);
+hipError_t rope_append_launch(RopeAppendParams p, hipStream_t stream) {
+  // four waves on a token shorten the way of one (4 tokens of 16/4 heads of 128: 3.9
+  // us, one wave 5.3); a wave with several tokens' worth of loads on the way keeps
+  // memory busy (17383 tokens of 8/2 heads of 256, 214 MB: 46 us, four waves 64; a
+  // copy of as many bytes 43)
+  p.waves = p.tokens <= 1024 ? kWaves : 1;
+  const int r8 = p.rot / 16, c8 = (p.d - p.rot) / 8;
+  // n / r8 of any piece is umulhi(n, per_r8): n stays below 2^32 / r8
+  p.per_r8 = r8 > 1 ? 0xffffffffu / r8 + 1 : 0;
+  p.per_c8 = c8 > 1 ? 0xffffffffu / c8 + 1 : 0;
+  const int per = kWaves / p.waves;
+  const dim3 grid((p.tokens + per - 1) / per);
+  if (p.waves > 1)
+    hipLaunchKernelGGL(rope_append_kernel<2>, grid, dim3(kThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL(rope_append_kernel<6>, grid, dim3(kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -140,6 +193,7 @@ hipError_t rope_append_launch(const RopeAppendParams& p, hipStream_t stream) {
 // joins.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeUnit = 128;
+constexpr int kDecodeMostRuns = 2048;  // workgroups of a launch of runs
 
 template <int D>
 struct DecodeLds {
@@ -311,7 +365,7 @@ __device__ __forceinline__ void decode_piece(const DecodePagedParams& p, DecodeL
 
 // One workgroup per (head block, sequence), nothing to join.
 template <int D>
-__global__ __launch_bounds__(kThreads) void decode_paged_whole(const DecodePagedParams p) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_whole(const DecodePagedParams p) {
   __shared__ DecodeLds<D> lds;
   const int hb = blockIdx.x, s = blockIdx.y;
   const int len = paged_length(p.kv, s);
@@ -332,7 +386,7 @@ __device__ __forceinline__ int decode_units(int len) {
 // Equal runs of units.  plan[0] takes the run's length, plan[1 + s] the first
 // unit of sequence s, for the joining launch.
 template <int D>
-__global__ __launch_bounds__(kThreads) void decode_paged_runs(const DecodePagedParams p) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_runs(const DecodePagedParams p) {
   __shared__ DecodeLds<D> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int n = p.kv.n, heads = p.kv.hkv * p.blocks;
@@ -391,15 +445,15 @@ __global__ __launch_bounds__(kThreads) void decode_paged_runs(const DecodePagedP
 }
 
 // Joins the partial rows of the (sequence, head)s that more than one run holds:
-// M = max m_i, out = sum acc_i 2^(m_i - M) / sum l_i 2^(m_i - M).  Also the zero
-// rows of empty sequences.
+// M = max m_i, out = sum acc_i 2^(m_i - M) / sum l_i 2^(m_i - M), the runs' weights
+// first, so that no row waits for another.  Also the zero rows of empty sequences.
 template <int D>
 __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedParams p) {
   constexpr int T4 = D / 4, R = kThreads / T4;  // threads along a row, rows at a time
-  __shared__ float4 sums[R][T4];
-  __shared__ float tops[R], weights[R];
+  __shared__ f32x4 sums[R][T4];
+  __shared__ float weight[kDecodeMostRuns], tops[kWaves], parts[kWaves];
   const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
-  const int y = tid % T4, r = tid / T4;
+  const int lane = tid & 63, wave = tid >> 6, y = tid % T4, r = tid / T4;
   const int len = paged_length(p.kv, s);
   f16* out = p.out + (long long)s * p.out_stride + head * D;
   if (len == 0) {
@@ -409,47 +463,54 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   const int per = decode_units(len), run = p.plan[0];
   const int h = head / p.group, q = head % p.group;
   const int a = p.plan[1 + s] + (h * p.blocks + q / 16) * per, b = a + per - 1;
-  const int w0 = a / run, w1 = b / run;
-  if (w0 == w1) return;  // its one run wrote the output
-  auto row = [&](int w) {
-    const int side = w == w0 && a % run ? 1 : 0;
-    return p.part + ((2LL * w + side) * 16 + q % 16) * (D + 4);
+  const int w0 = a / run, runs = b / run - w0 + 1;
+  if (runs == 1) return;  // it wrote the output
+  // run i's row; the first one may follow another piece of its workgroup
+  auto row = [&](int i) {
+    const int side = i == 0 && a % run ? 1 : 0;
+    return p.part + ((2LL * (w0 + i) + side) * 16 + q % 16) * (D + 4);
   };
-  float m = -INFINITY, l = 0.0f;
-  f32x4 acc = f32x4{};
-  for (int w = w0 + r; w <= w1; w += R) {
-    const float* x = row(w);
-    const f32x4 o = *(const f32x4*)(x + 4 + 4 * y);
-    const float mx = x[0], lx = x[1];
-    const float next = fmaxf(m, mx), base = next == -INFINITY ? 0.0f : next;
-    const float f = exp2_fast(m - base), fx = exp2_fast(mx - base);
-    l = l * f + lx * fx;
+  float m = -INFINITY;
+  for (int i = tid; i < runs; i += kThreads) {
+    weight[i] = row(i)[0];
+    m = fmaxf(m, weight[i]);
+  }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f + o[e] * fx;
-    m = next;
-  }
-  sums[r][y] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-  if (y == 0) {
-    tops[r] = m;
-    weights[r] = l;
-  }
+  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if (lane == 0) tops[wave] = m;
   __syncthreads();
-  if (r) return;
-  float top = tops[0];
 #pragma unroll
-  for (int i = 1; i < R; ++i) top = fmaxf(top, tops[i]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  acc = f32x4{};
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  for (int i = tid; i < runs; i += kThreads) {  // (its own entries again)
+    const float f = exp2_fast(weight[i] - base);
+    weight[i] = f;
+    l = fmaf(row(i)[1], f, l);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off, 64);
+  if (lane == 0) parts[wave] = l;
+  __syncthreads();
   l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const float f = exp2_fast(tops[i] - base);
-    const float4 o = sums[i][y];
-    l = fmaf(weights[i], f, l);
-    acc[0] = fmaf(o.x, f, acc[0]);
-    acc[1] = fmaf(o.y, f, acc[1]);
-    acc[2] = fmaf(o.z, f, acc[2]);
-    acc[3] = fmaf(o.w, f, acc[3]);
+  for (int w = 0; w < kWaves; ++w) l += parts[w];
+  f32x4 acc = f32x4{};
+#pragma unroll 4
+  for (int i = r; i < runs; i += R) {
+    const f32x4 o = *(const f32x4*)(row(i) + 4 + 4 * y);
+    const float f = weight[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], f, acc[e]);
+  }
+  sums[r][y] = acc;
+  __syncthreads();
+  if (r) return;
+#pragma unroll
+  for (int i = 1; i < R; ++i) {
+    const f32x4 o = sums[i][y];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += o[e];
   }
   const float inv = 1.0f / l;
   f16x4 v;
@@ -460,7 +521,11 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
 
 // Workgroups of the runs' launch, and whether a launch over up to `bound`
 // positions of each sequence is split at all.
-int decode_paged_grid(int cus) { return 4 * cus; }
+int decode_paged_grid(int head_dim, int cus) {
+  // what the registers of a launch let run at once
+  const int per_cu = head_dim == 256 ? 2 : 4;
+  return per_cu * cus < kDecodeMostRuns ? per_cu * cus : kDecodeMostRuns;
+}
 bool decode_paged_split(long long bound) { return bound > 512; }
 long long decode_paged_part_floats(int head_dim, int grid) {
   return 2LL * grid * 16 * (head_dim + 4);

@@ -39,18 +39,26 @@ __device__ __forceinline__ float rows_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// The sequence whose packed rows hold row t: the number of sequences that end
-// at or before t (offsets[1..n] do not decrease); n where t is past the last.
-// Every lane of a wave calls it and gets the answer.
-__device__ __forceinline__ int packed_sequence(const int32_t* offsets, int n, int t) {
+// The sequence whose packed rows hold row t (the one after those that end at or
+// before t; offsets[1..n] do not decrease), where its rows end, and its length.
+// By a whole wave; the answer is uniform, and one load deep for n <= 64.
+struct PackedRow {
+  bool found;
+  int seq, end, length;
+};
+__device__ __forceinline__ PackedRow packed_row(const int32_t* offsets, const int32_t* lengths,
+                                                int n, int t) {
   const int lane = threadIdx.x & 63;
-  int count = 0;
   for (int b = 0; b < n; b += 64) {
-    const int i = b + lane;
-    const bool before = i < n && offsets[i + 1] <= t;
-    count += __popcll(__ballot(before));
+    const int i = min(b + lane, n - 1);
+    const int first = offsets[i], end = offsets[i + 1], length = lengths[i];
+    const uint64_t after = __ballot(end > t);
+    if (!after) continue;
+    const int at = __ffsll((unsigned long long)after) - 1;
+    return PackedRow{__builtin_amdgcn_readlane(first, at) <= t, b + at,
+                     __builtin_amdgcn_readlane(end, at), __builtin_amdgcn_readlane(length, at)};
   }
-  return count;
+  return PackedRow{false, 0, 0, 0};
 }
 
 }  // namespace aexq
