@@ -69,6 +69,11 @@ struct aexq_ctx {
   long long paged_part_cap = 0;
   int* paged_plan = nullptr;
   long long paged_plan_cap = 0;
+  // layout of a prompt attention launch, and the registers of its cut tiles
+  int* prompt_plan = nullptr;
+  long long prompt_plan_cap = 0;
+  float* prompt_part = nullptr;
+  long long prompt_part_cap = 0;
   // per part of a logits row: sums, and its best logits
   float* logprob_stats = nullptr;
   long long logprob_stats_cap = 0;
@@ -209,6 +214,8 @@ extern "C" void aexq_destroy(aexq_ctx* ctx) {
   (void)hipFree(ctx->attn_count);
   (void)hipFree(ctx->paged_part);
   (void)hipFree(ctx->paged_plan);
+  (void)hipFree(ctx->prompt_plan);
+  (void)hipFree(ctx->prompt_part);
   (void)hipFree(ctx->logprob_stats);
   (void)hipFree(ctx->logprob_keys);
   (void)hipFree(ctx->sk_part);
@@ -2160,18 +2167,37 @@ extern "C" aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv
 
 // The two prompt entry points behind their descriptors.
 static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, int heads_q,
-                              int head_dim, float scale) {
+                              int head_dim, long long bound, float scale) {
   if (p.n <= 0 || p.tokens <= 0)
     return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "sequences=%d tokens=%d", p.n, p.tokens);
   p.group = heads_q / p.hkv;
   p.scale2 = scale * 1.4426950408889634f;
   // rows of one sequence are counted in 31 bits, tiles are a grid's second axis
-  if ((long long)p.tokens * p.group > 0x7fffffffLL - 4096 ||
-      prompt_tiles(p.tokens, p.n, p.group) > 65535)
+  const long long tiles = prompt_tiles(p.tokens, p.n, p.group);
+  if ((long long)p.tokens * p.group > 0x7fffffffLL - 4096 || tiles > 65535)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "tokens=%d of %d heads per key head in one call",
                 p.tokens, p.group);
   HIP_TRY(op, hipSetDevice(ctx->device));
-  const hipError_t e = prompt_launch(p, head_dim, ctx->stream);
+  long long pieces = tiles;
+  if (prompt_planned(tiles, p.n, bound)) {
+    const PromptScratch need = prompt_scratch(tiles, p.hkv, head_dim, ctx->cus);
+    aexq_status st = grow_scratch(ctx, (void**)&ctx->prompt_plan, &ctx->prompt_plan_cap,
+                                  (need.counters + need.plan_ints) * (long long)sizeof(int), op,
+                                  "prompt attention plan");
+    if (!st)
+      st = grow_scratch(ctx, (void**)&ctx->prompt_part, &ctx->prompt_part_cap,
+                        need.part_floats * (long long)sizeof(float), op,
+                        "prompt attention partials");
+    if (st) return st;
+    p.plan = ctx->prompt_plan;
+    p.counters = ctx->prompt_plan + need.plan_ints;
+    p.part = ctx->prompt_part;
+    p.target = need.target;
+    p.slots = need.slots;
+    pieces = need.pieces;
+    p.pieces = (int)pieces;
+  }
+  const hipError_t e = prompt_launch(p, head_dim, pieces, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "attention launch");
   return AEXQ_OK;
 }
@@ -2213,7 +2239,7 @@ extern "C" aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64
   p.kv_tokens = kv_tokens;
   p.hkv = heads_kv;
   p.causal = causal != 0;
-  return prompt_run(ctx, op, p, heads_q, head_dim, scale);
+  return prompt_run(ctx, op, p, heads_q, head_dim, kv_tokens, scale);
 }
 
 extern "C" aexq_status aexq_attention_prompt_paged(aexq_ctx* ctx, const aexq_paged_kv* kv,
@@ -2237,7 +2263,8 @@ extern "C" aexq_status aexq_attention_prompt_paged(aexq_ctx* ctx, const aexq_pag
   p.tokens = tokens;
   p.hkv = kv->heads_kv;
   p.causal = 1;
-  return prompt_run(ctx, op, p, heads_q, kv->head_dim, scale);
+  return prompt_run(ctx, op, p, heads_q, kv->head_dim,
+                    (long long)kv->table_width * kv->page_size, scale);
 }
 
 extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_paged_kv* kv,

@@ -336,9 +336,24 @@ struct PromptParams {
   const int32_t *q_offsets, *kv_offsets;  // [n + 1]
   int n, tokens, kv_tokens, hkv, group, causal;
   float scale2;
+  // where the launch is laid out first (else plan is null): its pieces, the
+  // registers of cut tiles (`slots` a kv head), and how many of them are there
+  int* plan;
+  float* part;
+  int* counters;
+  int target, slots, pieces;
+};
+// what that takes: pieces of a kv head at most, and scratch
+struct PromptScratch {
+  int target, slots;
+  long long pieces, plan_ints, counters, part_floats;
 };
 long long prompt_tiles(long long tokens, int n, int group);
-hipError_t prompt_launch(const PromptParams& p, int head_dim, hipStream_t stream);
+bool prompt_planned(long long tiles, int n, long long bound);
+PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus);
+// `pieces`: workgroups of a kv head
+hipError_t prompt_launch(const PromptParams& p, int head_dim, long long pieces,
+                         hipStream_t stream);
 // ---- log probabilities of tokens (aexq_logprobs.hip)
 struct LogprobParams {
   const void* x;  // [rows][rstride] logits, n of each row

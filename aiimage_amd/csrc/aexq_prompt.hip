@@ -28,10 +28,184 @@ namespace aexq {
 //                 (ds_read_b64_tr_b16), 4 positions of 16 dims per 16 lanes.
 // So scores, weights, maximum and sum of a row never leave its two lanes.
 //
-// Sequences and their tiles are found on the device from the offsets; the tiles
-// with the most positions start first.
+// Where a launch has few 128-row tiles for the part, or tiles of very different
+// length, a small launch before it lays out its work (prompt_plan): tiles longer
+// than a share of the whole are cut along the positions, and the longest pieces
+// start first.  The pieces of a cut tile leave their (max, sum, acc) registers in
+// scratch; the last one to finish adds them up, in the order of the positions.
+// Otherwise every workgroup finds its tile from the offsets, last tiles first.
 // ---------------------------------------------------------------------------
 constexpr int kPromptRows = 128;
+constexpr int kPlanThreads = 1024;
+constexpr int kPromptLeast = 6;  // units (KT positions) that a cut leaves at least, about
+constexpr int kPlanMost = 2048;  // sequences, and tiles of a kv head, that are laid out
+constexpr int kCoherent = 16;    // buffer cache policy sc1: through to what all XCDs share
+
+// A sequence as the kernels see it, clamped to what the call holds.
+struct PromptSeq {
+  int q0, rows, queries;  // first query row; (query, head of the group) rows; queries
+  int kv0, len;           // first key row (packed), positions
+};
+__device__ __forceinline__ int prompt_first(const PromptParams& p, int s) {
+  return min(max(p.q_offsets[s], 0), p.tokens);
+}
+__device__ __forceinline__ int prompt_rows(const PromptParams& p, int s) {
+  const int a = prompt_first(p, s);
+  return (min(max(p.q_offsets[s + 1], a), p.tokens) - a) * p.group;
+}
+template <bool PAGED>
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
+  PromptSeq q;
+  q.q0 = prompt_first(p, s);
+  q.rows = prompt_rows(p, s);
+  q.queries = q.rows / p.group;
+  if constexpr (PAGED) {
+    q.kv0 = 0;
+    q.len = paged_length(p.kv, s);
+  } else {
+    q.kv0 = min(max(p.kv_offsets[s], 0), p.kv_tokens);
+    q.len = min(max(p.kv_offsets[s + 1], q.kv0), p.kv_tokens) - q.kv0;
+  }
+  return q;
+}
+// Positions that the token of row r sees.
+__device__ __forceinline__ int prompt_seen(const PromptParams& p, const PromptSeq& q, int r) {
+  return p.causal ? max(q.len - q.queries + r / p.group + 1, 0) : q.len;
+}
+
+// A piece of work: tiles [t0, t1) of positions for a 128-row tile of a sequence.
+// pieces > 1: it leaves registers in slot `slot`, those of its tile are in
+// slot0 .. slot0 + pieces - 1 (per kv head).
+struct PromptPiece {
+  int seq, tile, t0, t1, slot, slot0, pieces, pad;
+};
+
+// Lays out the pieces of every kv head, one workgroup: plan[0] their number, then
+// the pieces from plan + 4 by falling length; and clears the tiles' counters.
+template <bool PAGED>
+__global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(const PromptParams p, int kt) {
+  constexpr int kBuckets = 256, kW = kPlanThreads / 64;
+  // of each sequence: the tiles before it, its rows, and where its queries start
+  // among its positions (causal) or its length
+  __shared__ int before[kPlanMost + 1], rows[kPlanMost], from[kPlanMost];
+  __shared__ int bucket[kBuckets], waves[kW], tops[kW], slots;
+  __shared__ unsigned long long sums[kW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int carry = 0;
+  for (int b = 0; b < p.n; b += kPlanThreads) {
+    const int s = b + tid;
+    int mine = 0;
+    if (s < p.n) {
+      const PromptSeq q = prompt_seq<PAGED>(p, s);
+      rows[s] = q.rows;
+      from[s] = p.causal ? q.len - q.queries : q.len;
+      mine = (q.rows + kPromptRows - 1) / kPromptRows;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += v;
+    }
+    if (b) __syncthreads();
+    if (lane == 63) waves[wave] = upto;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+      if (w < wave) upto += waves[w];
+      sum += waves[w];
+    }
+    if (s < p.n) before[s] = carry + upto - mine;
+    carry += sum;
+  }
+  for (int i = tid; i < p.slots * p.hkv; i += kPlanThreads) p.counters[i] = 0;
+  if (tid < kBuckets) bucket[tid] = 0;
+  if (tid == 0) slots = 0;
+  __syncthreads();
+  const int tiles = carry;  // (the first kPlanMost of them: two a thread)
+  int seq[2], cost[2] = {0, 0};
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = tid + u * kPlanThreads;
+    if (i >= tiles) continue;
+    int a = 0, b = p.n;  // the last sequence with before[s] <= i
+    while (b - a > 1) {
+      const int m = (a + b) / 2;
+      if (before[m] <= i) a = m; else b = m;
+    }
+    const int last = min((i - before[a] + 1) * kPromptRows, rows[a]) - 1;
+    const int seen = p.causal ? max(from[a] + last / p.group + 1, 0) : from[a];
+    seq[u] = a;
+    cost[u] = (seen + kt - 1) / kt;
+  }
+  unsigned long long units = (unsigned long long)cost[0] + cost[1];
+  int longest = max(cost[0], cost[1]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    units += __shfl_xor(units, off, 64);
+    longest = max(longest, __shfl_xor(longest, off, 64));
+  }
+  if (lane == 0) {
+    sums[wave] = units;
+    tops[wave] = longest;
+  }
+  __syncthreads();
+  units = 0;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) {
+    units += sums[w];
+    longest = max(longest, tops[w]);
+  }
+  // the share of a workgroup, where the part's workgroups all have one
+  const int share =
+      max(kPromptLeast, (int)min((units * p.hkv + p.target - 1) / p.target, 0x7fffffffULL));
+  const int most = min(share, max(longest, 1));
+  int pieces[2], size[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    if (tid + u * kPlanThreads >= tiles) continue;
+    // (what adds the pieces up takes longer the more there are)
+    pieces[u] = max(1, min((cost[u] + share - 1) / share, (int)sqrtf(2.0f * cost[u]) + 1));
+    size[u] = max(1, (cost[u] + pieces[u] - 1) / pieces[u]);
+    pieces[u] = max(1, (cost[u] + size[u] - 1) / size[u]);
+    atomicAdd(&bucket[max(0, kBuckets - 1 - (int)((long long)size[u] * (kBuckets - 1) / most))],
+              pieces[u]);
+  }
+  __syncthreads();
+  if (tid < 64) {  // where each bucket's pieces start
+    int own[kBuckets / 64], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kBuckets / 64; ++i) {
+      own[i] = sum;
+      sum += bucket[tid * (kBuckets / 64) + i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += v;
+    }
+#pragma unroll
+    for (int i = 0; i < kBuckets / 64; ++i) bucket[tid * (kBuckets / 64) + i] = upto - sum + own[i];
+    if (tid == 63) p.plan[0] = upto;
+  }
+  __syncthreads();
+  PromptPiece* out = (PromptPiece*)(p.plan + 4);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = tid + u * kPlanThreads;
+    if (i >= tiles) continue;
+    int at = atomicAdd(
+        &bucket[max(0, kBuckets - 1 - (int)((long long)size[u] * (kBuckets - 1) / most))],
+        pieces[u]);
+    const int slot = pieces[u] > 1 ? atomicAdd(&slots, pieces[u]) : 0;
+    // (offsets that decrease may ask for more than the call's rows need: left out)
+    for (int k = 0; k < pieces[u] && at < p.pieces; ++k, ++at)
+      out[at] = PromptPiece{seq[u], i - before[seq[u]], k * size[u],
+                            min((k + 1) * size[u], cost[u]), slot + k, slot, pieces[u], 0};
+  }
+}
 
 template <int D>
 struct PromptLds {
@@ -74,55 +248,52 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   const int tid = threadIdx.x, lane = tid & 63, wave = sreg(tid >> 6);
   const int n = p.n, group = p.group, head = blockIdx.x;
 
-  // 1. the workgroup's sequence and tile, the last tiles first
-  auto first_of = [&](int s) { return min(max(p.q_offsets[s], 0), p.tokens); };
-  auto rows_of = [&](int s) {
-    const int a = first_of(s);
-    return (min(max(p.q_offsets[s + 1], a), p.tokens) - a) * group;
-  };
-  const int share = (n + kThreads - 1) / kThreads;
-  const int sa = min(tid * share, n), sb = min(sa + share, n);
-  int mine = 0;
-  for (int s = sa; s < sb; ++s) mine += (rows_of(s) + kPromptRows - 1) / kPromptRows;
-  int upto = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int v = __shfl_up(upto, off, 64);
-    if (lane >= off) upto += v;
-  }
-  if (lane == 63) lds.count[wave] = upto;
-  __syncthreads();
-  int before = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += lds.count[w];
-    total += lds.count[w];
-  }
-  const int at = total - 1 - (int)blockIdx.y;
-  if (at < 0) return;
-  if (before <= at && at < before + mine) {
-    int s = sa, base = before;
-    for (;; ++s) {
-      const int u = (rows_of(s) + kPromptRows - 1) / kPromptRows;
-      if (at < base + u) break;
-      base += u;
-    }
-    lds.seq = s;
-    lds.tile = at - base;
-  }
-  __syncthreads();
-  const int seq = sreg(lds.seq), tile = sreg(lds.tile);
-  const int q0 = first_of(seq), rows = rows_of(seq), queries = rows / group;
-  int kv0 = 0, len;
-  if constexpr (PAGED) {
-    len = paged_length(p.kv, seq);
+  // 1. the workgroup's sequence, tile and positions
+  int seq, tile;
+  PromptPiece piece{};
+  if (p.plan) {
+    if ((int)blockIdx.y >= p.plan[0]) return;
+    piece = ((const PromptPiece*)(p.plan + 4))[blockIdx.y];
+    seq = piece.seq;
+    tile = piece.tile;
   } else {
-    kv0 = min(max(p.kv_offsets[seq], 0), p.kv_tokens);
-    len = min(max(p.kv_offsets[seq + 1], kv0), p.kv_tokens) - kv0;
+    const int share = (n + kThreads - 1) / kThreads;
+    const int sa = min(tid * share, n), sb = min(sa + share, n);
+    int mine = 0;
+    for (int s = sa; s < sb; ++s) mine += (prompt_rows(p, s) + kPromptRows - 1) / kPromptRows;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int v = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += v;
+    }
+    if (lane == 63) lds.count[wave] = upto;
+    __syncthreads();
+    int before = upto - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) before += lds.count[w];
+      total += lds.count[w];
+    }
+    const int at = total - 1 - (int)blockIdx.y;
+    if (at < 0) return;
+    if (before <= at && at < before + mine) {
+      int s = sa, base = before;
+      for (;; ++s) {
+        const int u = (prompt_rows(p, s) + kPromptRows - 1) / kPromptRows;
+        if (at < base + u) break;
+        base += u;
+      }
+      lds.seq = s;
+      lds.tile = at - base;
+    }
+    __syncthreads();
+    seq = sreg(lds.seq);
+    tile = sreg(lds.tile);
   }
-  len = sreg(len);
-  // positions that the token of row r sees
-  auto seen = [&](int r) { return p.causal ? max(len - queries + r / group + 1, 0) : len; };
+  const PromptSeq sq = prompt_seq<PAGED>(p, seq);
+  const int q0 = sq.q0, rows = sq.rows, kv0 = sq.kv0, len = sreg(sq.len);
+  auto seen = [&](int r) { return prompt_seen(p, sq, r); };
 
   // 2. q: the lane's row as the right operand of S^T
   const int j = lane & 31, h = lane >> 5;
@@ -139,7 +310,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   const int hi = sreg(seen(min(tile * kPromptRows + wave * 32 + 31, last)));
   const int low = sreg(seen(tile * kPromptRows));
   const int most = sreg(seen(min(tile * kPromptRows + kPromptRows - 1, last)));
-  const int tiles = (most + KT - 1) / KT;
+  const int begin = sreg(piece.t0);
+  const int tiles = p.plan ? sreg(piece.t1) : (most + KT - 1) / KT;
+  const bool live = tile * kPromptRows + wave * 32 <= last;  // the wave has a row
 
   f32x16 o[DB];
 #pragma unroll
@@ -211,7 +384,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   auto take = [&](int t, auto edge, auto buf) {
     constexpr bool EDGE = decltype(edge)::value;
     constexpr int BUF = decltype(buf)::value;
-    const int b = BUF >= 0 ? BUF : t & 1, x0 = t * KT;
+    const int b = BUF >= 0 ? BUF : (t - begin) & 1, x0 = t * KT;
     wait_vm<0>();
     if constexpr (EDGE) {
       // An infinity or a NaN in V reaches, through 0 * V, the rows that do not
@@ -230,7 +403,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
     }
     bar();
     if (t + 1 < tiles) fetch(t + 1, b ^ 1);
-    if (EDGE && x0 >= hi) return;  // none of the wave's rows sees any of it
+    // (EDGE: where none of the wave's rows sees any of it)
+    if (!live || (EDGE && x0 >= hi)) return;
 
     f32x16 sc[SB];
 #pragma unroll
@@ -323,14 +497,68 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
       }
     }
   };
-  if (tiles > 0) fetch(0, 0);
+  if (tiles > begin) fetch(begin, 0);
   const int whole = min(low / KT, tiles);
-  int t = 0;
+  int t = begin;
   for (; t + 1 < whole; t += 2) {
     take(t, std::false_type{}, std::integral_constant<int, 0>{});
     take(t + 1, std::false_type{}, std::integral_constant<int, 1>{});
   }
   for (; t < tiles; ++t) take(t, std::true_type{}, std::integral_constant<int, -1>{});
+
+  if (piece.pieces > 1) {
+    // the registers of a piece, [wave][four of them][lane], in its slot; they
+    // travel through coherent stores and loads, the stores done before the count
+    constexpr int REGS = DB * 16 + 4;
+    float* slots = p.part + (long long)head * p.slots * (kThreads * REGS);
+    auto slot = [&](int i) {
+      return __builtin_amdgcn_make_buffer_rsrc(
+          (void*)sreg(slots + (long long)(i * kWaves + wave) * (64 * REGS)), (short)0,
+          64 * REGS * 4, kBufferRsrcWord3);
+    };
+    if (live) {
+      const __amdgpu_buffer_rsrc_t to = slot(piece.slot);
+#pragma unroll
+      for (int i = 0; i < DB * 4; ++i) {
+        const f32x4 y = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2],
+                         o[i / 4][i % 4 * 4 + 3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), to,
+                                               (i * 64 + lane) * 16, 0, kCoherent);
+      }
+      const f32x4 y = {m, l, 0.0f, 0.0f};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), to,
+                                             (DB * 4 * 64 + lane) * 16, 0, kCoherent);
+    }
+    wait_vm<0>();
+    __syncthreads();
+    if (tid == 0)
+      lds.seq = atomicAdd(&p.counters[head * p.slots + piece.slot0], 1) == piece.pieces - 1;
+    __syncthreads();
+    if (!sreg(lds.seq) || !live) return;
+    m = -INFINITY;
+    for (int i = 0; i < piece.pieces; ++i)
+      m = fmaxf(m, as_f32(__builtin_amdgcn_raw_buffer_load_b32(
+                       slot(piece.slot0 + i), (DB * 4 * 64 + lane) * 16, 0, kCoherent)));
+    const float base = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    for (int k = 0; k < piece.pieces; ++k) {
+      const __amdgpu_buffer_rsrc_t from = slot(piece.slot0 + k);
+      const f32x4 ml = __builtin_bit_cast(
+          f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (DB * 4 * 64 + lane) * 16, 0,
+                                                       kCoherent));
+      const float f = exp2_fast(ml[0] - base);
+      l = fmaf(ml[1], f, l);
+#pragma unroll
+      for (int i = 0; i < DB * 4; ++i) {
+        const f32x4 y = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (i * 64 + lane) * 16, 0, kCoherent));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i / 4][i % 4 * 4 + e] = fmaf(y[e], f, o[i / 4][i % 4 * 4 + e]);
+      }
+    }
+  }
 
   // 3. the row's two lanes hold half of its sum each; a row that sees nothing is
   // 0, one whose every score was -inf (a sum of 0) NaN
@@ -354,20 +582,40 @@ long long prompt_tiles(long long tokens, int n, int group) {
   return tokens * group / kPromptRows + n;
 }
 
-template <int D>
-static void prompt_dispatch(const PromptParams& p, dim3 grid, hipStream_t stream) {
-  if (p.kv.k)
-    hipLaunchKernelGGL((prompt_kernel<D, true>), grid, dim3(kThreads), 0, stream, p);
-  else
-    hipLaunchKernelGGL((prompt_kernel<D, false>), grid, dim3(kThreads), 0, stream, p);
+// Whether a launch is laid out first, over sequences of up to `bound` positions
+// each: not where the layout would find nothing to cut or to order.
+bool prompt_planned(long long tiles, int n, long long bound) {
+  return n <= kPlanMost && tiles <= kPlanMost && bound > 512;
+}
+PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus) {
+  PromptScratch r;
+  // two workgroups a CU.  A tile of c units is cut into pieces of at least share / 2,
+  // share >= units / target: no more than 2 target pieces of cut tiles in all
+  r.target = 2 * cus;
+  r.slots = (2 * r.target + hkv - 1) / hkv;
+  r.pieces = tiles + r.slots;
+  r.plan_ints = 4 + r.pieces * (long long)(sizeof(PromptPiece) / 4);
+  r.counters = (long long)r.slots * hkv;
+  r.part_floats = r.counters * kThreads * (head_dim / 2 + 4);
+  return r;
 }
 
-hipError_t prompt_launch(const PromptParams& p, int head_dim, hipStream_t stream) {
-  const dim3 grid(p.hkv, (unsigned)prompt_tiles(p.tokens, p.n, p.group));
+template <int D, bool PAGED>
+static void prompt_dispatch(const PromptParams& p, unsigned rows, hipStream_t stream) {
+  if (p.plan)
+    hipLaunchKernelGGL(prompt_plan_kernel<PAGED>, dim3(1), dim3(kPlanThreads), 0, stream, p,
+                       PromptLds<D>::KT);
+  hipLaunchKernelGGL((prompt_kernel<D, PAGED>), dim3(p.hkv, rows), dim3(kThreads), 0, stream, p);
+}
+
+hipError_t prompt_launch(const PromptParams& p, int head_dim, long long pieces,
+                         hipStream_t stream) {
+  const unsigned rows = (unsigned)pieces;
+  const bool paged = p.kv.k;
   switch (head_dim) {
-    case 64: prompt_dispatch<64>(p, grid, stream); break;
-    case 128: prompt_dispatch<128>(p, grid, stream); break;
-    default: prompt_dispatch<256>(p, grid, stream); break;
+    case 64: (paged ? prompt_dispatch<64, true> : prompt_dispatch<64, false>)(p, rows, stream); break;
+    case 128: (paged ? prompt_dispatch<128, true> : prompt_dispatch<128, false>)(p, rows, stream); break;
+    default: (paged ? prompt_dispatch<256, true> : prompt_dispatch<256, false>)(p, rows, stream); break;
   }
   return hipGetLastError();
 }
