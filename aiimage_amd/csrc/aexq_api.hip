@@ -2193,6 +2193,7 @@ static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, in
     p.counters = ctx->prompt_plan + need.plan_ints;
     p.part = ctx->prompt_part;
     p.target = need.target;
+    p.columns = need.columns;
     p.slots = need.slots;
     pieces = need.pieces;
     p.pieces = (int)pieces;

@@ -336,16 +336,16 @@ struct PromptParams {
   const int32_t *q_offsets, *kv_offsets;  // [n + 1]
   int n, tokens, kv_tokens, hkv, group, causal;
   float scale2;
-  // where the launch is laid out first (else plan is null): its pieces, the
-  // registers of cut tiles (`slots` a kv head), and how many of them are there
+  // where the launch is laid out first (else plan is null): its pieces, and the
+  // registers of cut tiles, `slots` for each column (kv head, or part of one)
   int* plan;
   float* part;
   int* counters;
-  int target, slots, pieces;
+  int target, columns, slots, pieces;
 };
 // what that takes: pieces of a kv head at most, and scratch
 struct PromptScratch {
-  int target, slots;
+  int target, columns, slots;
   long long pieces, plan_ints, counters, part_floats;
 };
 long long prompt_tiles(long long tokens, int n, int group);

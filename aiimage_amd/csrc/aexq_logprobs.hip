@@ -7,10 +7,11 @@
 namespace aexq {
 
 // ---------------------------------------------------------------------------
-// One pass over a row of logits x with a running maximum m, in log2 units:
-//   Z = sum e^(x - m),  T = sum e^(x - m) (x - m) log2 e
-//   log p[t] = (x[t] - m) - ln Z,   H = ln Z - T ln 2 / Z
-// (x - m is taken before anything is rounded, so large logits lose nothing).
+// One pass over a row of logits x with a running reference b, the rounded log2 e
+// times their maximum so far:
+//   y = x log2 e - b (one fma),  Z = sum 2^y,  T = sum 2^y y
+//   log p[t] = ln 2 (y[t] - log2 Z),   H = ln 2 (log2 Z - T / Z)
+// No sum depends on how b was rounded, so large logits lose nothing.
 // Lanes take 16-byte chunks in turn; what a lane keeps for the alternatives is
 // its best chunk (by its largest logit) and the largest logit of the others.
 //
@@ -26,7 +27,7 @@ namespace aexq {
 // ---------------------------------------------------------------------------
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// x - m of a logit that weighs nothing (-inf among them), in log2 units
+// y of a logit that weighs nothing (-inf among them)
 constexpr float kFar = -300.0f;
 
 // Order of the alternatives: the larger logit, then the lower index.  0 is below
@@ -36,29 +37,29 @@ __device__ __forceinline__ u64 top_key(float x, int index) {
 }
 
 struct Stats {
-  float m, z, t;
+  float b, z, t;
 };
-// The sums of two parts on their common maximum; parts of weight 0 add 0.
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-  const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.0f : m;
-  const float da = fmaxf((a.m - base) * kLog2e, kFar), db = fmaxf((b.m - base) * kLog2e, kFar);
-  const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+// The sums of two parts on the larger reference; parts of weight 0 add 0.
+__device__ __forceinline__ Stats join(Stats p, Stats q) {
+  const float b = fmaxf(p.b, q.b), base = b == -INFINITY ? 0.0f : b;
+  const float dp = fmaxf(p.b - base, kFar), dq = fmaxf(q.b - base, kFar);
+  const float fp = __builtin_amdgcn_exp2f(dp), fq = __builtin_amdgcn_exp2f(dq);
   Stats r;
-  r.m = m;
-  r.z = a.z * fa + b.z * fb;
-  r.t = fa * fmaf(a.z, da, a.t) + fb * fmaf(b.z, db, b.t);
+  r.b = b;
+  r.z = p.z * fp + q.z * fq;
+  r.t = fp * fmaf(p.z, dp, p.t) + fq * fmaf(q.z, dq, q.t);
   return r;
 }
-__device__ __forceinline__ Stats join_wave(Stats a) {
+__device__ __forceinline__ Stats join_wave(Stats p) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
-    Stats b;
-    b.m = __shfl_xor(a.m, off, 64);
-    b.z = __shfl_xor(a.z, off, 64);
-    b.t = __shfl_xor(a.t, off, 64);
-    a = join(a, b);
+    Stats q;
+    q.b = __shfl_xor(p.b, off, 64);
+    q.z = __shfl_xor(p.z, off, 64);
+    q.t = __shfl_xor(p.t, off, 64);
+    p = join(p, q);
   }
-  return a;
+  return p;
 }
 
 // A row's outputs by its workgroup: thread r < top has the r-th key.  A row
@@ -68,20 +69,21 @@ template <typename E>
 __device__ __forceinline__ void row_outputs(const LogprobParams& p, int row, const E* x, Stats s,
                                             u64 key) {
   const bool sound = s.z > 0.0f && s.z < INFINITY;
-  const float ln = logf(s.z), nan = __builtin_nanf("");
+  const float log2z = log2f(s.z), nan = __builtin_nanf("");
+  auto log_p = [&](float x) { return (fmaf(x, kLog2e, -s.b) - log2z) * kLn2; };
   if (threadIdx.x == 0) {
     if (p.logprob) {
       const int token = p.tokens[row];
       float v = token == -1 ? 0.0f : nan;
-      if (sound && token >= 0 && token < p.n) v = ((float)x[token] - s.m) - ln;
+      if (sound && token >= 0 && token < p.n) v = log_p((float)x[token]);
       p.logprob[row] = v;
     }
-    if (p.entropy) p.entropy[row] = sound ? ln - s.t * kLn2 / s.z : nan;
+    if (p.entropy) p.entropy[row] = sound ? (log2z - s.t / s.z) * kLn2 : nan;
   }
   if ((int)threadIdx.x < p.top) {
     const long long at = (long long)row * p.top + threadIdx.x;
     if (p.ids) p.ids[at] = sound ? (int)~(uint32_t)key : -1;
-    if (p.values) p.values[at] = sound ? (argmax_unord((uint32_t)(key >> 32)) - s.m) - ln : nan;
+    if (p.values) p.values[at] = sound ? log_p(argmax_unord((uint32_t)(key >> 32))) : nan;
   }
 }
 
@@ -136,57 +138,61 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
   const int c0 = min(part * p.cols, chunks), c1 = min(c0 + p.cols, chunks);
 
   // chunk c; logits before the row's first or past its last read -inf
-  auto read = [&](int c, float* v) {
+  typedef E Chunk __attribute__((ext_vector_type(VE)));
+  auto read = [&](int c) {
     const int i0 = c * VE - skew;
+    Chunk v;
     if (i0 >= 0 && i0 <= p.n - VE) {
-      E e[VE];
-      __builtin_memcpy(e, __builtin_assume_aligned(x + i0, 16), 16);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[i] = (float)e[i];
+      v = *(const Chunk*)(x + i0);
     } else {
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        v[i] = -INFINITY;
-        if (i0 + i >= 0 && i0 + i < p.n) v[i] = (float)x[i0 + i];
+        v[i] = (E)-INFINITY;
+        if (i0 + i >= 0 && i0 + i < p.n) v[i] = x[i0 + i];
       }
     }
+    return v;
   };
+  const Chunk none = (Chunk)(E)-INFINITY;
 
   Stats s = {-INFINITY, 0.0f, 0.0f};
   float best = -INFINITY, second = -INFINITY;
   int best_chunk = c0 + tid;
+  Chunk next[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    next[u] = c0 + tid + u * kThreads < c1 ? read(c0 + tid + u * kThreads) : none;
   for (int c = c0 + tid; c < c1; c += U * kThreads) {
-    float v[U][VE];
+    Chunk v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (c + u * kThreads < c1) {
-        read(c + u * kThreads, v[u]);
-      } else {
+    for (int u = 0; u < U; ++u) v[u] = next[u];
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[u][i] = -INFINITY;
-      }
+    for (int u = 0; u < U; ++u) {  // the next chunks on their way
+      const int n = c + (U + u) * kThreads;
+      next[u] = n < c1 ? read(n) : none;
     }
-    float m = s.m;
+    float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float top = v[u][0];
+      E t = v[u][0];
 #pragma unroll
-      for (int i = 1; i < VE; ++i) top = fmaxf(top, v[u][i]);
+      for (int i = 1; i < VE; ++i) t = __builtin_elementwise_maxnum(t, v[u][i]);
+      const float top = (float)t;
       m = fmaxf(m, top);
       second = fmaxf(second, fminf(best, top));
       best_chunk = top > best ? c + u * kThreads : best_chunk;
       best = fmaxf(best, top);
     }
-    const float base = m == -INFINITY ? 0.0f : m;
-    const float d = fmaxf((s.m - base) * kLog2e, kFar), f = __builtin_amdgcn_exp2f(d);
+    const float b = fmaxf(s.b, m * kLog2e), base = b == -INFINITY ? 0.0f : b;
+    const float d = fmaxf(s.b - base, kFar), f = __builtin_amdgcn_exp2f(d);
     s.t = f * fmaf(s.z, d, s.t);
     s.z *= f;
-    s.m = m;
+    s.b = b;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const float y = (v[u][i] - base) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+        const float y = fmaf((float)v[u][i], kLog2e, -base), e = __builtin_amdgcn_exp2f(y);
         s.z += e;
         s.t = fmaf(e, fmaxf(y, kFar), s.t);
       }
@@ -207,13 +213,13 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
     const bool one = any && !all && top_key(best, max(best_chunk * VE - skew, 0)) >= least;
     u64 entry = 0;
     auto take = [&](int c, bool on) {
-      float v[VE];
-      if (on) read(c, v);
+      const Chunk v = on ? read(c) : none;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         const int at = c * VE - skew + i;
-        const bool in = on && at >= 0 && at < p.n && !__builtin_isnan(v[i]);
-        const u64 k = in ? top_key(v[i], at) : 0;
+        const float y = (float)v[i];
+        const bool in = on && at >= 0 && at < p.n && !__builtin_isnan(y);
+        const u64 k = in ? top_key(y, at) : 0;
         for (u64 left = __ballot(in && k >= least); left; left &= left - 1) {
           const int from = __ffsll((unsigned long long)left) - 1;
           const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(k >> 32), from);
@@ -253,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
   }
   if (tid == 0) {
     float* to = p.stats + 4LL * blockIdx.x;
-    to[0] = s.m;
+    to[0] = s.b;
     to[1] = s.z;
     to[2] = s.t;
   }

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(const PromptP
     if (s < p.n) before[s] = carry + upto - mine;
     carry += sum;
   }
-  for (int i = tid; i < p.slots * p.hkv; i += kPlanThreads) p.counters[i] = 0;
+  for (int i = tid; i < p.slots * p.columns; i += kPlanThreads) p.counters[i] = 0;
   if (tid < kBuckets) bucket[tid] = 0;
   if (tid == 0) slots = 0;
   __syncthreads();
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(const PromptP
   }
   // the share of a workgroup, where the part's workgroups all have one
   const int share =
-      max(kPromptLeast, (int)min((units * p.hkv + p.target - 1) / p.target, 0x7fffffffULL));
+      max(kPromptLeast, (int)min((units * p.columns + p.target - 1) / p.target, 0x7fffffffULL));
   const int most = min(share, max(longest, 1));
   int pieces[2], size[2];
 #pragma unroll
@@ -210,8 +210,9 @@ __global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(const PromptP
 template <int D>
 struct PromptLds {
   static constexpr int KT = D == 256 ? 32 : 64;
+  static constexpr int DV = D == 256 ? 128 : D;  // dims of V and of the output it takes
   alignas(1024) f16 k[2][KT * D];
-  alignas(1024) f16 v[2][KT * D];
+  alignas(1024) f16 v[2][KT * DV];
   int seq, tile, count[kWaves];
   int odd[2][kWaves];  // a V tile holds an infinity or a NaN
 };
@@ -240,13 +241,16 @@ __device__ __forceinline__ f16x4 read_transposed(const f16* p) {
 }
 
 template <int D, bool PAGED>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(const PromptParams p) {
-  constexpr int KT = PromptLds<D>::KT, CH = D / 8, KS = D / 16, DB = D / 32, SB = KT / 32;
-  constexpr int RL = 512 / D;        // tile rows of one LDS-direct load
-  constexpr int NL = KT / 4 / RL;    // loads of a wave per K (or V) tile
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const PromptParams p) {
+  constexpr int KT = PromptLds<D>::KT, DV = PromptLds<D>::DV;
+  constexpr int KS = D / 16, DB = DV / 32, SB = KT / 32;
+  // tile rows of one LDS-direct load, and loads of a wave per tile, of K and of V
+  constexpr int RK = 512 / D, NK = KT / 4 / RK, RV = 512 / DV, NV = KT / 4 / RV;
   __shared__ PromptLds<D> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = sreg(tid >> 6);
-  const int n = p.n, group = p.group, head = blockIdx.x;
+  // (DV < D: the heads' output in parts, a workgroup each)
+  const int n = p.n, group = p.group, column = blockIdx.x, head = column / (D / DV);
+  const int dv0 = column % (D / DV) * DV;
 
   // 1. the workgroup's sequence, tile and positions
   int seq, tile;
@@ -324,12 +328,16 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   // ends before the sequence does.
   const int r0 = wave * (KT / 4);
   const int kst = PAGED ? D * 2 : (int)p.k_stride * 2, vst = PAGED ? D * 2 : (int)p.v_stride * 2;
-  uint32_t koff[NL], voff[NL];
+  uint32_t koff[NK], voff[NV];
 #pragma unroll
-  for (int i = 0; i < NL; ++i) {
-    const int r = i * RL + lane / CH, chunk = lane % CH ^ swz<D>(r0 + r);
-    koff[i] = r * kst + 16 * chunk;
-    voff[i] = r * vst + 16 * chunk;
+  for (int i = 0; i < NK; ++i) {
+    const int r = i * RK + lane / (D / 8);
+    koff[i] = r * kst + 16 * (lane % (D / 8) ^ swz<D>(r0 + r));
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = i * RV + lane / (DV / 8);
+    voff[i] = r * vst + 16 * (lane % (DV / 8) ^ swz<DV>(r0 + r));
   }
   const uint32_t lds_base = lds_addr(&lds);
   auto fetch = [&](int t, int b) {
@@ -340,28 +348,29 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
           ((((long long)sreg(paged_page(p.kv, seq, x >> p.kv.shift)) * p.kv.hkv + head)
             << p.kv.shift) + (x & ((1 << p.kv.shift) - 1))) * D;
       kb = p.kv.k + a;
-      vb = p.kv.v + a;
+      vb = p.kv.v + a + dv0;
     } else {
       kb = p.k + (long long)(kv0 + x) * p.k_stride + head * D;
-      vb = p.v + (long long)(kv0 + x) * p.v_stride + head * D;
+      vb = p.v + (long long)(kv0 + x) * p.v_stride + head * D + dv0;
     }
     kb = sreg(kb);
     vb = sreg(vb);
-    const uint32_t kl = lds_base + (b * KT + r0) * D * 2, vl = kl + 2 * KT * D * 2;
-    if ((t + 1) * KT <= len) {
+    const uint32_t kl = lds_base + (b * KT + r0) * D * 2;
+    const uint32_t vl = lds_base + 2 * KT * D * 2 + (b * KT + r0) * DV * 2;
+    // rows past the end repeat the last one
+    const bool ends = (t + 1) * KT > len;
+    const int keep = len - 1 - x;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        dma_lane(kb, koff[i], kl + i * 1024);
-        dma_lane(vb, voff[i], vl + i * 1024);
-      }
-    } else {
-      // rows past the end repeat the last one
+    for (int i = 0; i < NK; ++i) {
+      uint32_t off = koff[i];
+      if (ends) off -= max(i * RK + lane / (D / 8) - keep, 0) * kst;
+      dma_lane(kb, off, kl + i * 1024);
+    }
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int r = i * RL + lane / CH, back = max(r - (len - 1 - x), 0);
-        dma_lane(kb, koff[i] - back * kst, kl + i * 1024);
-        dma_lane(vb, voff[i] - back * vst, vl + i * 1024);
-      }
+    for (int i = 0; i < NV; ++i) {
+      uint32_t off = voff[i];
+      if (ends) off -= max(i * RV + lane / (DV / 8) - keep, 0) * vst;
+      dma_lane(vb, off, vl + i * 1024);
     }
   };
 
@@ -376,24 +385,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
       const int tg = lane >> 4 & 1, ti = lane & 15, r = 8 * z + 4 * h + ti / 4;
-      vat[z][i] = r * D + 8 * ((2 * tg + (ti & 3) / 2) ^ (4 * i) ^ swz<D>(r)) + 4 * (ti & 1);
+      vat[z][i] = r * DV + 8 * ((2 * tg + (ti & 3) / 2) ^ (4 * i) ^ swz<DV>(r)) + 4 * (ti & 1);
     }
 
-  // One tile; EDGE: some row of the workgroup does not see all of it.  `buf`: its
-  // buffer where the code is for one of them, else -1.
-  auto take = [&](int t, auto edge, auto buf) {
+  // The arrival of tile t in buffer b, and the next one on its way.  EDGE: some row
+  // of the workgroup does not see all of it.
+  auto arrive = [&](int t, int b, auto edge) {
     constexpr bool EDGE = decltype(edge)::value;
-    constexpr int BUF = decltype(buf)::value;
-    const int b = BUF >= 0 ? BUF : (t - begin) & 1, x0 = t * KT;
     wait_vm<0>();
     if constexpr (EDGE) {
       // An infinity or a NaN in V reaches, through 0 * V, the rows that do not
       // see it: each wave looks through the rows it fetched.
       float z = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
+      for (int i = 0; i < NV; ++i) {
         const u32x4 y =
-            *(const u32x4*)((const char*)lds.v[b] + r0 * D * 2 + i * 1024 + lane * 16);
+            *(const u32x4*)((const char*)lds.v[b] + r0 * DV * 2 + i * 1024 + lane * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) z = dot2(y[e], 0u, z);
       }
@@ -403,8 +410,15 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
     }
     bar();
     if (t + 1 < tiles) fetch(t + 1, b ^ 1);
-    // (EDGE: where none of the wave's rows sees any of it)
-    if (!live || (EDGE && x0 >= hi)) return;
+  };
+  // The wave's products with it.  `buf`: its buffer where the code is for one of
+  // them, else -1.
+  auto take = [&](int t, auto edge, auto buf) {
+    constexpr bool EDGE = decltype(edge)::value;
+    constexpr int BUF = decltype(buf)::value;
+    const int b = BUF >= 0 ? BUF : (t - begin) & 1, x0 = t * KT;
+    arrive(t, b, edge);
+    if (EDGE && x0 >= hi) return;  // none of the wave's rows sees any of it
 
     f32x16 sc[SB];
 #pragma unroll
@@ -476,7 +490,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = 32 * i + 8 * (r / 4) + 4 * h + r % 4;
-            const f16 y = lds.v[b][x * D + 8 * ((d / 8) ^ swz<D>(x)) + d % 8];
+            const f16 y = lds.v[b][x * DV + 8 * ((d / 8) ^ swz<DV>(x)) + d % 8];
             o[i][r] = in ? fmaf(w, (float)y, o[i][r]) : o[i][r];
           }
       }
@@ -491,7 +505,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
       for (int i = 0; i < DB; ++i) {
         f16x4 a[2];
 #pragma unroll
-        for (int z = 0; z < 2; ++z) a[z] = read_transposed(&lds.v[b][16 * y * D + vat[z][i]]);
+        for (int z = 0; z < 2; ++z) a[z] = read_transposed(&lds.v[b][16 * y * DV + vat[z][i]]);
         const f16x8 vf = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7);
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, w, o[i], 0, 0, 0);
       }
@@ -500,17 +514,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   if (tiles > begin) fetch(begin, 0);
   const int whole = min(low / KT, tiles);
   int t = begin;
-  for (; t + 1 < whole; t += 2) {
-    take(t, std::false_type{}, std::integral_constant<int, 0>{});
-    take(t + 1, std::false_type{}, std::integral_constant<int, 1>{});
+  if (live) {
+    for (; t + 1 < whole; t += 2) {
+      take(t, std::false_type{}, std::integral_constant<int, 0>{});
+      take(t + 1, std::false_type{}, std::integral_constant<int, 1>{});
+    }
+    for (; t < tiles; ++t) take(t, std::true_type{}, std::integral_constant<int, -1>{});
+  } else {  // it only fetches its rows
+    for (; t + 1 < whole; ++t) arrive(t, (t - begin) & 1, std::false_type{});
+    for (; t < tiles; ++t) arrive(t, (t - begin) & 1, std::true_type{});
   }
-  for (; t < tiles; ++t) take(t, std::true_type{}, std::integral_constant<int, -1>{});
 
   if (piece.pieces > 1) {
     // the registers of a piece, [wave][four of them][lane], in its slot; they
     // travel through coherent stores and loads, the stores done before the count
     constexpr int REGS = DB * 16 + 4;
-    float* slots = p.part + (long long)head * p.slots * (kThreads * REGS);
+    float* slots = p.part + (long long)column * p.slots * (kThreads * REGS);
     auto slot = [&](int i) {
       return __builtin_amdgcn_make_buffer_rsrc(
           (void*)sreg(slots + (long long)(i * kWaves + wave) * (64 * REGS)), (short)0,
@@ -532,7 +551,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
     wait_vm<0>();
     __syncthreads();
     if (tid == 0)
-      lds.seq = atomicAdd(&p.counters[head * p.slots + piece.slot0], 1) == piece.pieces - 1;
+      lds.seq = atomicAdd(&p.counters[column * p.slots + piece.slot0], 1) == piece.pieces - 1;
     __syncthreads();
     if (!sreg(lds.seq) || !live) return;
     m = -INFINITY;
@@ -565,7 +584,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void prompt_kernel(cons
   l += __shfl_xor(l, 32, 64);
   const float inv = vis > 0 ? 1.0f / l : 0.0f;
   if (row > last) return;
-  f16* out = p.out + token * p.out_stride + qh * D;
+  f16* out = p.out + token * p.out_stride + qh * D + dv0;
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -589,14 +608,16 @@ bool prompt_planned(long long tiles, int n, long long bound) {
 }
 PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus) {
   PromptScratch r;
+  const int dv = head_dim == 256 ? 128 : head_dim;
+  r.columns = hkv * (head_dim / dv);
   // two workgroups a CU.  A tile of c units is cut into pieces of at least share / 2,
   // share >= units / target: no more than 2 target pieces of cut tiles in all
   r.target = 2 * cus;
-  r.slots = (2 * r.target + hkv - 1) / hkv;
+  r.slots = (2 * r.target + r.columns - 1) / r.columns;
   r.pieces = tiles + r.slots;
   r.plan_ints = 4 + r.pieces * (long long)(sizeof(PromptPiece) / 4);
-  r.counters = (long long)r.slots * hkv;
-  r.part_floats = r.counters * kThreads * (head_dim / 2 + 4);
+  r.counters = (long long)r.slots * r.columns;
+  r.part_floats = r.counters * kThreads * (dv / 2 + 4);
   return r;
 }
 
@@ -605,7 +626,8 @@ static void prompt_dispatch(const PromptParams& p, unsigned rows, hipStream_t st
   if (p.plan)
     hipLaunchKernelGGL(prompt_plan_kernel<PAGED>, dim3(1), dim3(kPlanThreads), 0, stream, p,
                        PromptLds<D>::KT);
-  hipLaunchKernelGGL((prompt_kernel<D, PAGED>), dim3(p.hkv, rows), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL((prompt_kernel<D, PAGED>), dim3(p.hkv * (D / PromptLds<D>::DV), rows),
+                     dim3(kThreads), 0, stream, p);
 }
 
 hipError_t prompt_launch(const PromptParams& p, int head_dim, long long pieces,
