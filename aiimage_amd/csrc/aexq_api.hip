@@ -2288,19 +2288,22 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
   p.group = heads_q / kv->heads_kv;
   p.blocks = (p.group + 15) / 16;
   p.scale2 = scale * 1.4426950408889634f;
-  p.min_run = 1;
   const long long bound = (long long)kv->table_width * kv->page_size;
-  const int grid = decode_paged_split(bound) ? decode_paged_grid(kv->head_dim, ctx->cus) : 0;
-  // runs count units of all sequences in 31 bits
+  const DecodePlan plan =
+      decode_paged_plan(kv->head_dim, ctx->cus, bound,
+                        (long long)kv->sequences * kv->heads_kv * p.blocks);
+  // units of all sequences are counted in 31 bits
   const long long units =
       (bound / 128 + 1) * kv->sequences * (long long)(kv->heads_kv * p.blocks);
   if (units > 0x7fffffffLL - (1 << 20))
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d sequences of up to %lld positions in one call",
                 kv->sequences, bound);
   HIP_TRY(op, hipSetDevice(ctx->device));
-  if (grid) {
+  if (plan.target) {
+    p.target = plan.target;
+    p.grid = (int)plan.grid;
     st = grow_scratch(ctx, (void**)&ctx->paged_part, &ctx->paged_part_cap,
-                      decode_paged_part_floats(kv->head_dim, grid) * (long long)sizeof(float), op,
+                      plan.grid * 16 * (kv->head_dim + 4) * (long long)sizeof(float), op,
                       "paged attention partials");
     if (!st)
       st = grow_scratch(ctx, (void**)&ctx->paged_plan, &ctx->paged_plan_cap,
@@ -2310,7 +2313,7 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
     p.part = ctx->paged_part;
     p.plan = ctx->paged_plan;
   }
-  const hipError_t e = decode_paged_launch(p, kv->head_dim, grid, ctx->stream);
+  const hipError_t e = decode_paged_launch(p, kv->head_dim, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "attention launch");
   return AEXQ_OK;
 }

@@ -317,16 +317,17 @@ struct DecodePagedParams {
   long long q_stride, out_stride;
   int group, blocks;  // query heads per kv head, and their blocks of 16
   float scale2;       // scale * log2(e)
-  float* part;        // partial rows of the runs
+  int target;         // shares of the work that is cut; 0: nothing is cut
+  int grid;           // pieces at most
+  float* part;        // a piece's partial rows, 16 of head_dim + 4 floats
   int* plan;          // 1 + n ints
-  int min_run;        // units a workgroup takes at least
 };
-int decode_paged_grid(int head_dim, int cus);
-bool decode_paged_split(long long bound);
-long long decode_paged_part_floats(int head_dim, int grid);
-// grid 0: one workgroup per (head block, sequence)
-hipError_t decode_paged_launch(const DecodePagedParams& p, int head_dim, int grid,
-                               hipStream_t stream);
+struct DecodePlan {
+  int target;
+  long long grid;
+};
+DecodePlan decode_paged_plan(int head_dim, int cus, long long bound, long long blocks);
+hipError_t decode_paged_launch(const DecodePagedParams& p, int head_dim, hipStream_t stream);
 // attention of packed rows over packed (kv.k null) or paged keys and values
 struct PromptParams {
   PagedView kv;

@@ -294,10 +294,12 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobPar
     // where there is no bound): no more than the buffer holds
     for (int i = tid; i < p.parts * p.top; i += kThreads) {
       const u64 k = keys[i];
-      if (k && k >= least) reach[atomicAdd(&count, 1)] = k;
+      if (!k || k < least) continue;
+      const int at = atomicAdd(&count, 1);
+      if (at < 72 * 64) reach[at] = k;
     }
     __syncthreads();
-    const int n = count;
+    const int n = min(count, 72 * 64);
     for (int i = tid; i < n; i += kThreads) {
       const u64 own = reach[i];
       int above = 0;

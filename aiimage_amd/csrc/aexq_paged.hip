@@ -185,15 +185,14 @@ hipError_t rope_append_launch(RopeAppendParams p, hipStream_t stream) {
 //                 dims into the left operands: product t has dims (D/16) m + t.
 // The waves of a workgroup take steps in turn and meet in LDS at the end.
 //
-// What bounds it is reading K and V once (HBM).  The work is cut into units of
-// kDecodeUnit positions of one (sequence, head block), laid end to end, and each
-// workgroup takes an equal run of units, so lengths may differ as they like and
-// the host need not know them.  A run that holds all of a (sequence, block)
-// writes its output; the others leave (max, sum, acc) rows that a second launch
-// joins.
+// What bounds it is reading K and V once (HBM).  Lengths may differ as they like
+// and the host need not know them: where it pays, a (sequence, head block) longer
+// than a share of all of them is cut into even pieces of kDecodeUnit positions and
+// more, found on the device.  Pieces leave (max, sum, acc) rows that a second
+// launch joins.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeUnit = 128;
-constexpr int kDecodeMostRuns = 2048;  // workgroups of a launch of runs
+constexpr int kDecodeMost = 2048;  // pieces of a (sequence, head block)
 
 template <int D>
 struct DecodeLds {
@@ -201,7 +200,7 @@ struct DecodeLds {
   static constexpr int W = 16 * HT;                   // dims of one pass
   alignas(16) float o[kWaves][16][W + 4];
   float m[kWaves][16], l[kWaves][16];
-  int seq, base, count[kWaves];
+  int seq, base, count[2][kWaves];
 };
 
 // One (sequence s, head block hb) over positions [p0, p1) of len, by the whole
@@ -378,80 +377,90 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_whole
     p.out[(long long)s * p.out_stride + (h * p.group + first) * D + i] = (f16)0.0f;
 }
 
-// Units of one head block of a sequence.
-__device__ __forceinline__ int decode_units(int len) {
-  return (len + kDecodeUnit - 1) / kDecodeUnit;
-}
+// A (sequence, head block) of `len` positions in even pieces of at most `share`
+// units: their number, and the units of each but the last.
+struct DecodeCut {
+  int pieces, size;
+  __device__ DecodeCut(int len, int share) {
+    const int units = (len + kDecodeUnit - 1) / kDecodeUnit;
+    pieces = (units + share - 1) / share;
+    size = pieces ? (units + pieces - 1) / pieces : 0;
+    pieces = size ? (units + size - 1) / size : 0;
+  }
+};
 
-// Equal runs of units.  plan[0] takes the run's length, plan[1 + s] the first
-// unit of sequence s, for the joining launch.
-template <int D>
-__global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_runs(const DecodePagedParams p) {
-  __shared__ DecodeLds<D> lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n = p.kv.n, heads = p.kv.hkv * p.blocks;
-  // thread t adds up the units of its share of the sequences
-  const int share = (n + kThreads - 1) / kThreads;
-  const int s0 = min(tid * share, n), s1 = min(s0 + share, n);
-  int mine = 0;
-  for (int s = s0; s < s1; ++s) mine += decode_units(paged_length(p.kv, s)) * heads;
+// Sum over the workgroup's threads, and of those before each.
+__device__ __forceinline__ int block_scan(int mine, int* waves, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int upto = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int v = __shfl_up(upto, off, 64);
     if (lane >= off) upto += v;
   }
-  if (lane == 63) lds.count[wave] = upto;
+  if (lane == 63) waves[wave] = upto;
   __syncthreads();
-  int before = upto - mine, total = 0;
+  int before = upto - mine, sum = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += lds.count[w];
-    total += lds.count[w];
+    if (w < wave) before += waves[w];
+    sum += waves[w];
   }
-  const int run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_run);
-  const int u0 = blockIdx.x * run;  // (the host keeps grid * run within 31 bits)
-  if (blockIdx.x == 0 && tid == 0) p.plan[0] = run;
-  if (u0 >= total) return;
-  const int u1 = min(u0 + run, total);
-  if (before <= u0 && u0 < before + mine) {
+  *total = sum;
+  return before;
+}
+
+// A piece per workgroup.  plan[0] takes the share of units that is cut, plan[1 +
+// s] the first piece of sequence s, for the joining launch.  (That the last
+// workgroup of a head block joins it in the same launch was slower: its rows then
+// go past the L2s.  One sequence of 1000 positions 9.4 -> 12.9 us, 64 sequences of
+// 56891 55 -> 63.)
+template <int D>
+__global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_cut(
+    const DecodePagedParams p) {
+  __shared__ DecodeLds<D> lds;
+  const int tid = threadIdx.x, n = p.kv.n, heads = p.kv.hkv * p.blocks;
+  // thread t adds up its share of the sequences
+  const int each = (n + kThreads - 1) / kThreads;
+  const int s0 = min(tid * each, n), s1 = min(s0 + each, n);
+  int units = 0, pieces = 0, total;
+  for (int s = s0; s < s1; ++s)
+    units += (paged_length(p.kv, s) + kDecodeUnit - 1) / kDecodeUnit * heads;
+  block_scan(units, lds.count[0], &total);
+  const int share = max((total + p.target - 1) / p.target, 1);
+  for (int s = s0; s < s1; ++s) pieces += DecodeCut(paged_length(p.kv, s), share).pieces * heads;
+  const int before = block_scan(pieces, lds.count[1], &total);
+  if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
+  const int at = blockIdx.x;
+  if (at >= total) return;
+  if (before <= at && at < before + pieces) {
     int s = s0, base = before;
     for (;; ++s) {
-      const int u = decode_units(paged_length(p.kv, s)) * heads;
-      if (u0 < base + u) break;
-      base += u;
+      const int m = DecodeCut(paged_length(p.kv, s), share).pieces * heads;
+      if (at < base + m) break;
+      base += m;
     }
     lds.seq = s;
     lds.base = base;
+    if (at == base) p.plan[1 + s] = base;
   }
   __syncthreads();
-  int s = sreg(lds.seq), base = sreg(lds.base);
-  for (int u = u0; u < u1;) {
-    const int len = paged_length(p.kv, s), per = decode_units(len);
-    if (u >= base + per * heads) {
-      base += per * heads;
-      ++s;
-      continue;
-    }
-    const int hb = (u - base) / per, at = (u - base) % per;
-    const int take = min(per - at, u1 - u);
-    if (hb == 0 && at == 0 && tid == 0) p.plan[1 + s] = base;
-    float* slot = take == per ? nullptr
-                              : p.part + (2LL * blockIdx.x + (u == u0 ? 0 : 1)) * 16 * (D + 4);
-    decode_piece<D>(p, lds, s, hb, len, at * kDecodeUnit, min(len, (at + take) * kDecodeUnit),
-                    slot);
-    u += take;
-  }
+  const int s = sreg(lds.seq), len = paged_length(p.kv, s);
+  const DecodeCut cut(len, share);
+  const int hb = (at - sreg(lds.base)) / cut.pieces, i = (at - sreg(lds.base)) % cut.pieces;
+  decode_piece<D>(p, lds, s, hb, len, i * cut.size * kDecodeUnit,
+                  min(len, (i + 1) * cut.size * kDecodeUnit),
+                  cut.pieces == 1 ? nullptr : p.part + (long long)at * 16 * (D + 4));
 }
 
-// Joins the partial rows of the (sequence, head)s that more than one run holds:
-// M = max m_i, out = sum acc_i 2^(m_i - M) / sum l_i 2^(m_i - M), the runs' weights
-// first, so that no row waits for another.  Also the zero rows of empty sequences.
+// Joins the partial rows of the (sequence, head)s that were cut:
+// M = max m_i, out = sum acc_i 2^(m_i - M) / sum l_i 2^(m_i - M), the pieces'
+// weights first, so that no row waits for another.  Also the zero rows of empty sequences.
 template <int D>
 __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedParams p) {
   constexpr int T4 = D / 4, R = kThreads / T4;  // threads along a row, rows at a time
   __shared__ f32x4 sums[R][T4];
-  __shared__ float weight[kDecodeMostRuns], tops[kWaves], parts[kWaves];
+  __shared__ float weight[kDecodeMost], tops[kWaves], parts[kWaves];
   const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, y = tid % T4, r = tid / T4;
   const int len = paged_length(p.kv, s);
@@ -460,18 +469,14 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
     if (tid < T4) *(f16x4*)(out + 4 * y) = f16x4{};
     return;
   }
-  const int per = decode_units(len), run = p.plan[0];
+  // (whatever the plan holds, the rows read are the launch's own)
   const int h = head / p.group, q = head % p.group;
-  const int a = p.plan[1 + s] + (h * p.blocks + q / 16) * per, b = a + per - 1;
-  const int w0 = a / run, runs = b / run - w0 + 1;
-  if (runs == 1) return;  // it wrote the output
-  // run i's row; the first one may follow another piece of its workgroup
-  auto row = [&](int i) {
-    const int side = i == 0 && a % run ? 1 : 0;
-    return p.part + ((2LL * (w0 + i) + side) * 16 + q % 16) * (D + 4);
-  };
+  const int pieces = DecodeCut(len, max(p.plan[0], 1)).pieces;
+  const int first = max(p.plan[1 + s], 0) + (h * p.blocks + q / 16) * pieces;
+  if (pieces == 1 || pieces > kDecodeMost || first > p.grid - pieces) return;
+  auto row = [&](int i) { return p.part + ((first + i) * 16LL + q % 16) * (D + 4); };
   float m = -INFINITY;
-  for (int i = tid; i < runs; i += kThreads) {
+  for (int i = tid; i < pieces; i += kThreads) {
     weight[i] = row(i)[0];
     m = fmaxf(m, weight[i]);
   }
@@ -483,7 +488,7 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
   const float base = m == -INFINITY ? 0.0f : m;
   float l = 0.0f;
-  for (int i = tid; i < runs; i += kThreads) {  // (its own entries again)
+  for (int i = tid; i < pieces; i += kThreads) {  // (its own entries again)
     const float f = exp2_fast(weight[i] - base);
     weight[i] = f;
     l = fmaf(row(i)[1], f, l);
@@ -497,7 +502,7 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   for (int w = 0; w < kWaves; ++w) l += parts[w];
   f32x4 acc = f32x4{};
 #pragma unroll 4
-  for (int i = r; i < runs; i += R) {
+  for (int i = r; i < pieces; i += R) {
     const f32x4 o = *(const f32x4*)(row(i) + 4 + 4 * y);
     const float f = weight[i];
 #pragma unroll
@@ -519,26 +524,26 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   *(f16x4*)(out + 4 * y) = v;
 }
 
-// Workgroups of the runs' launch, and whether a launch over up to `bound`
-// positions of each sequence is split at all.
-int decode_paged_grid(int head_dim, int cus) {
-  // what the registers of a launch let run at once
-  const int per_cu = head_dim == 256 ? 2 : 4;
-  return per_cu * cus < kDecodeMostRuns ? per_cu * cus : kDecodeMostRuns;
-}
-bool decode_paged_split(long long bound) { return bound > 512; }
-long long decode_paged_part_floats(int head_dim, int grid) {
-  return 2LL * grid * 16 * (head_dim + 4);
+// The cut of a launch over up to `bound` positions of each sequence in `blocks`
+// head blocks of sequences: one piece for each `target`-th of all units, so that
+// no more than blocks + target are there.  Nothing is cut (target 0) where the
+// steps of a workgroup are few, and where there is a workgroup for every CU whose
+// longest way is not much longer.
+DecodePlan decode_paged_plan(int head_dim, int cus, long long bound, long long blocks) {
+  DecodePlan r;
+  r.target = bound <= 512 || (blocks >= cus && bound <= 1024) ? 0 : (head_dim == 256 ? 2 : 3) * cus;
+  r.grid = blocks + r.target;
+  return r;
 }
 
 template <int D>
-static hipError_t decode_launch(const DecodePagedParams& p, int grid, hipStream_t stream) {
-  if (!grid) {
+static hipError_t decode_launch(const DecodePagedParams& p, hipStream_t stream) {
+  if (!p.target) {
     hipLaunchKernelGGL(decode_paged_whole<D>, dim3(p.kv.hkv * p.blocks, p.kv.n), dim3(kThreads), 0,
                        stream, p);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(decode_paged_runs<D>, dim3(grid), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL(decode_paged_cut<D>, dim3((unsigned)p.grid), dim3(kThreads), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(decode_paged_join<D>, dim3(p.kv.hkv * p.group, p.kv.n), dim3(kThreads), 0,
@@ -546,12 +551,11 @@ static hipError_t decode_launch(const DecodePagedParams& p, int grid, hipStream_
   return hipGetLastError();
 }
 
-hipError_t decode_paged_launch(const DecodePagedParams& p, int head_dim, int grid,
-                               hipStream_t stream) {
+hipError_t decode_paged_launch(const DecodePagedParams& p, int head_dim, hipStream_t stream) {
   switch (head_dim) {
-    case 64: return decode_launch<64>(p, grid, stream);
-    case 128: return decode_launch<128>(p, grid, stream);
-    default: return decode_launch<256>(p, grid, stream);
+    case 64: return decode_launch<64>(p, stream);
+    case 128: return decode_launch<128>(p, stream);
+    default: return decode_launch<256>(p, stream);
   }
 }
 

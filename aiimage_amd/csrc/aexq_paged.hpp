@@ -21,6 +21,8 @@ __device__ __forceinline__ int paged_page(const PagedView& kv, int s, int b) {
   return min(max(kv.table[(long long)s * kv.width + b], 0), kv.pages - 1);
 }
 
+constexpr int kCoherent = 16;  // buffer cache policy sc1: through to what all XCDs share
+
 // Softmax weights are kept as 2^(score - m + kLift), m a running maximum that
 // is moved only where a score passes it by more than kLag: weights stay below
 // 2^(kLift + kLag) = 2^15 in fp16, and those down to 2^-21 of the largest keep

@@ -39,7 +39,6 @@ constexpr int kPromptRows = 128;
 constexpr int kPlanThreads = 1024;
 constexpr int kPromptLeast = 6;  // units (KT positions) that a cut leaves at least, about
 constexpr int kPlanMost = 2048;  // sequences, and tiles of a kv head, that are laid out
-constexpr int kCoherent = 16;    // buffer cache policy sc1: through to what all XCDs share
 
 // A sequence as the kernels see it, clamped to what the call holds.
 struct PromptSeq {
@@ -258,8 +257,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   if (p.plan) {
     if ((int)blockIdx.y >= p.plan[0]) return;
     piece = ((const PromptPiece*)(p.plan + 4))[blockIdx.y];
-    seq = piece.seq;
-    tile = piece.tile;
+    // (whatever the plan holds, reads and writes stay within the call's own rows)
+    seq = min(max(sreg(piece.seq), 0), n - 1);
+    tile = max(sreg(piece.tile), 0);
+    if (tile * (long long)kPromptRows >= prompt_rows(p, seq)) return;
+    piece.pieces = sreg(piece.pieces);
+    piece.slot0 = min(max(sreg(piece.slot0), 0), max(p.slots - piece.pieces, 0));
+    piece.slot = min(max(sreg(piece.slot), 0), p.slots - 1);
+    if (piece.pieces > p.slots) return;
   } else {
     const int share = (n + kThreads - 1) / kThreads;
     const int sa = min(tid * share, n), sb = min(sa + share, n);
@@ -314,8 +319,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   const int hi = sreg(seen(min(tile * kPromptRows + wave * 32 + 31, last)));
   const int low = sreg(seen(tile * kPromptRows));
   const int most = sreg(seen(min(tile * kPromptRows + kPromptRows - 1, last)));
-  const int begin = sreg(piece.t0);
-  const int tiles = p.plan ? sreg(piece.t1) : (most + KT - 1) / KT;
+  const int begin = max(sreg(piece.t0), 0), all = (most + KT - 1) / KT;
+  const int tiles = p.plan ? min(sreg(piece.t1), all) : all;
   const bool live = tile * kPromptRows + wave * 32 <= last;  // the wave has a row
 
   f32x16 o[DB];
