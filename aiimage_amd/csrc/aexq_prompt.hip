@@ -223,9 +223,10 @@ __device__ __forceinline__ int swz(int r) {
   return (r & 3) << 2 | (r >> 2 & 3);
 }
 
-// Lane i's 16 bytes at byte `off` (its own) of `from` to LDS byte lds + 16 i.
+// Lane i's 16 bytes at byte `off` (its own) of `from` to LDS byte lds + 16 i.  (One
+// wait state between the write of M0 and the load that reads it, as for dma().)
 __device__ __forceinline__ void dma_lane(const void* from, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds), "v"(off), "s"(from)
                : "memory", "m0");
@@ -397,7 +398,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   // of the workgroup does not see all of it.
   auto arrive = [&](int t, int b, auto edge) {
     constexpr bool EDGE = decltype(edge)::value;
-    wait_vm<0>();
+    // The wave's rows of tile t are there, and its reads of tile t - 1 are done: the
+    // compiler may leave a product, and the wait for its operands, behind the
+    // barrier, after which the others' next rows overwrite that buffer.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     if constexpr (EDGE) {
       // An infinity or a NaN in V reaches, through 0 * V, the rows that do not
       // see it: each wave looks through the rows it fetched.
