@@ -383,9 +383,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   // Where the lane's operands lie in a tile: step s of K (16 dims), and of V the
   // four positions z of 16 and the 32 dims i (the 16-dim half tg, lane ti of 16).
   // Everything else of an address is the instruction's own offset.
-  int kat[KS], vat[2][DB];
+  // (step s + 8 lies 16 chunks behind step s: swz() exchanges the low 4 bits)
+  constexpr int KA = KS < 8 ? KS : 8;
+  int kat[KA], vat[2][DB];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) kat[s] = j * D + 8 * ((2 * s + h) ^ swz<D>(j));
+  for (int s = 0; s < KA; ++s) kat[s] = j * D + 8 * ((2 * s + h) ^ swz<D>(j));
 #pragma unroll
   for (int z = 0; z < 2; ++z)
 #pragma unroll
@@ -436,7 +438,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int i = 0; i < SB; ++i) {
-        const f16x8 kf = *(const f16x8*)&lds.k[b][32 * i * D + kat[s]];
+        const f16x8 kf = *(const f16x8*)&lds.k[b][32 * i * D + s / KA * 128 + kat[s % KA]];
         sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[s], sc[i], 0, 0, 0);
       }
     if constexpr (BUF >= 0) {
@@ -521,6 +523,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
     }
   };
   if (tiles > begin) fetch(begin, 0);
+  wait_vm<0>();  // q too: the loops below then wait for no load but the tiles'
   const int whole = min(low / KT, tiles);
   int t = begin;
   if (live) {
