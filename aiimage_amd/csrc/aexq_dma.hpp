@@ -23,17 +23,19 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // it would otherwise wait for every outstanding load before each LDS read.
 // The kernel orders them itself -- s_waitcnt vmcnt for its own loads, then a
 // barrier for the other waves' -- and the memory clobber keeps the compiler
-// from moving LDS accesses across a load.
+// from moving LDS accesses across a load.  The load reads M0 one wait state after
+// the write at the earliest (the compiler, which sees into no assembly, keeps that
+// distance for its own ones).
 template <int BYTES>
 __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff) {
   static_assert(BYTES == 16 || BYTES == 4, "dword or dwordx4");
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(r)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(lds), "v"(voff), "s"(r)
                  : "memory", "m0");

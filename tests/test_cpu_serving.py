@@ -198,3 +198,20 @@ def test_structs_match_the_c_compiler_and_the_binding(tmp_path):
         snake = lambda n: re.sub(r"(?<=[a-z])([A-Z])", r"_\1", n).lower()  # noqa: E731
         assert [(k == "IntPtr", snake(n)) for k, n in members] == [
             (t is ctypes.c_void_p, f) for f, t in cls._fields_]
+
+
+def test_a_wait_state_between_m0_and_the_load_that_reads_it():
+    """Loads to LDS take their LDS address from M0.  A scalar write of M0 needs one
+    wait state before such a load on gfx9; the compiler adds it to its own code and
+    not inside assembly."""
+    import glob
+    found = 0
+    for path in glob.glob(os.path.join(ROOT, "aiimage_amd", "csrc", "*.h*")):
+        for text in re.findall(r'asm volatile\(\s*((?:"[^"]*"\s*)+)', open(path).read()):
+            lines = [l.strip() for l in re.sub(r'"\s*"', "", text).strip().strip('"')
+                     .replace("\\t", " ").split("\\n")]
+            for i, line in enumerate(lines):
+                if re.match(r"s_mov_b32 m0\b", line):
+                    found += 1
+                    assert lines[i + 1].startswith("s_nop"), (os.path.basename(path), lines)
+    assert found >= 3
