@@ -2083,6 +2083,10 @@ static aexq_status check_rows(const char* op, const char* name, const void* data
   if ((uintptr_t)data % 16 || stride % 8)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%s rows not 16-byte aligned (stride %lld)", name,
                 (long long)stride);
+  // (a tile's rows are addressed by 32-bit offsets from its first)
+  if (stride > 1 << 24)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%s rows %lld elements apart (at most 2^24)", name,
+                (long long)stride);
   return AEXQ_OK;
 }
 

@@ -355,7 +355,7 @@ aexq_status aexq_decode_advance(aexq_ctx* ctx, int32_t* position, int32_t* token
 /* No counterpart in the reference, which decodes one sequence.  Head dimensions
  * 64, 128 and 256; rows of one token's heads are dense ([heads][head_dim]) and
  * lie `stride` elements apart, so q, k and v may be views into one buffer; bases
- * are 16-byte aligned and strides multiples of 8.  Outputs share no memory with
+ * are 16-byte aligned, strides multiples of 8 up to 2^24.  Outputs share no memory with
  * inputs, but where it says so. */
 
 /* A pool of fp16 pages shared by `sequences` sequences.  Position x of sequence
@@ -413,7 +413,7 @@ aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const
  * queries are the sequence's last positions and see those up to their own.  A
  * row that sees no position is 0; what a row does not see does not reach it,
  * infinities and NaN in k or v included.  Rows behind the last sequence are not
- * touched.  scale > 0. */
+ * touched.  scale > 0.  Uses the context's scratch. */
 aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64_t q_stride, const void* k,
                                   int64_t k_stride, const void* v, int64_t v_stride,
                                   const int32_t* q_offsets, const int32_t* kv_offsets,

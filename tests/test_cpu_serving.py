@@ -72,6 +72,7 @@ def test_cache_descriptors(lib, handle, over, status):
     (dict(scale=float("nan")), _abi.ERR_INVALID_ARGUMENT),
     (dict(scale=float("inf")), _abi.ERR_INVALID_ARGUMENT),
     (dict(q_stride=500), _abi.ERR_SHAPE), (dict(q_stride=516), _abi.ERR_UNSUPPORTED),
+    (dict(q_stride=(1 << 24) + 8), _abi.ERR_UNSUPPORTED),
     (dict(out_stride=8), _abi.ERR_SHAPE), (dict(q=PTR + 8), _abi.ERR_UNSUPPORTED),
     (dict(kv=_kv(sequences=65000, table_width=1 << 14, page_size=4096, heads_kv=4)),
      _abi.ERR_UNSUPPORTED)])
