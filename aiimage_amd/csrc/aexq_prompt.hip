@@ -574,19 +574,32 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
-    for (int k = 0; k < piece.pieces; ++k) {
-      const __amdgpu_buffer_rsrc_t from = slot(piece.slot0 + k);
-      const f32x4 ml = __builtin_bit_cast(
-          f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (DB * 4 * 64 + lane) * 16, 0,
-                                                       kCoherent));
-      const float f = exp2_fast(ml[0] - base);
-      l = fmaf(ml[1], f, l);
+    // two pieces on the way at a time (the last one's twin weighs 0)
+    for (int k = 0; k < piece.pieces; k += 2) {
+      const __amdgpu_buffer_rsrc_t from[2] = {slot(piece.slot0 + k),
+                                              slot(piece.slot0 + min(k + 1, piece.pieces - 1))};
+      f32x4 ml[2], y[2][DB * 4];
 #pragma unroll
-      for (int i = 0; i < DB * 4; ++i) {
-        const f32x4 y = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, (i * 64 + lane) * 16, 0, kCoherent));
+      for (int u = 0; u < 2; ++u) {
+        ml[u] = __builtin_bit_cast(
+            f32x4, __builtin_amdgcn_raw_buffer_load_b128(from[u], (DB * 4 * 64 + lane) * 16, 0,
+                                                         kCoherent));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i / 4][i % 4 * 4 + e] = fmaf(y[e], f, o[i / 4][i % 4 * 4 + e]);
+        for (int i = 0; i < DB * 4; ++i)
+          y[u][i] = __builtin_bit_cast(
+              f32x4,
+              __builtin_amdgcn_raw_buffer_load_b128(from[u], (i * 64 + lane) * 16, 0, kCoherent));
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (u && k + 1 == piece.pieces) break;
+        const float f = exp2_fast(ml[u][0] - base);
+        l = fmaf(ml[u][1], f, l);
+#pragma unroll
+        for (int i = 0; i < DB * 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[i / 4][i % 4 * 4 + e] = fmaf(y[u][i][e], f, o[i / 4][i % 4 * 4 + e]);
       }
     }
   }
@@ -624,7 +637,7 @@ PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus) {
   r.columns = hkv * (head_dim / dv);
   // two workgroups a CU.  A tile of c units is cut into pieces of at least share / 2,
   // share >= units / target: no more than 2 target pieces of cut tiles in all
-  r.target = 2 * cus;
+  r.target = 3 * cus / 2;
   r.slots = (2 * r.target + r.columns - 1) / r.columns;
   r.pieces = tiles + r.slots;
   r.plan_ints = 4 + r.pieces * (long long)(sizeof(PromptPiece) / 4);
