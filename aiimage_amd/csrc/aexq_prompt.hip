@@ -32,7 +32,7 @@ namespace aexq {
 // length, a small launch before it lays out its work (prompt_plan): tiles longer
 // than a share of the whole are cut along the positions, and the longest pieces
 // start first.  The pieces of a cut tile leave their (max, sum, acc) registers in
-// scratch; the last one to finish adds them up, in the order of the positions.
+// scratch and are added up in a tree of fixed shape.
 // Otherwise every workgroup finds its tile from the offsets, last tiles first.
 // ---------------------------------------------------------------------------
 constexpr int kPromptRows = 128;
@@ -164,8 +164,7 @@ __global__ __launch_bounds__(kPlanThreads) void prompt_plan_kernel(const PromptP
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     if (tid + u * kPlanThreads >= tiles) continue;
-    // (what adds the pieces up takes longer the more there are)
-    pieces[u] = max(1, min((cost[u] + share - 1) / share, (int)sqrtf(2.0f * cost[u]) + 1));
+    pieces[u] = max(1, (cost[u] + share - 1) / share);
     size[u] = max(1, (cost[u] + pieces[u] - 1) / pieces[u]);
     pieces[u] = max(1, (cost[u] + size[u] - 1) / size[u]);
     atomicAdd(&bucket[max(0, kBuckets - 1 - (int)((long long)size[u] * (kBuckets - 1) / most))],
@@ -538,70 +537,69 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   }
 
   if (piece.pieces > 1) {
-    // the registers of a piece, [wave][four of them][lane], in its slot; they
-    // travel through coherent stores and loads, the stores done before the count
+    // The pieces of a tile meet in pairs, pairs of pairs and so on: of two siblings
+    // the second to finish adds the first one's registers, [wave][four of them]
+    // [lane] in its slot, and goes on with the sum.  They travel through coherent
+    // stores and loads, the stores done before the count.  The sums do not depend
+    // on who is second.
     constexpr int REGS = DB * 16 + 4;
     float* slots = p.part + (long long)column * p.slots * (kThreads * REGS);
     auto slot = [&](int i) {
       return __builtin_amdgcn_make_buffer_rsrc(
-          (void*)sreg(slots + (long long)(i * kWaves + wave) * (64 * REGS)), (short)0,
-          64 * REGS * 4, kBufferRsrcWord3);
+          (void*)sreg(slots + (long long)((piece.slot0 + i) * kWaves + wave) * (64 * REGS)),
+          (short)0, 64 * REGS * 4, kBufferRsrcWord3);
     };
-    if (live) {
-      const __amdgpu_buffer_rsrc_t to = slot(piece.slot);
+    const int own = piece.slot - piece.slot0;
+    for (int step = 1; step < piece.pieces; step *= 2) {
+      const int node = own / step, right = (node | 1) * step;
+      if (right >= piece.pieces) continue;  // no sibling
+      if (live) {
+        const __amdgpu_buffer_rsrc_t to = slot(node * step);
 #pragma unroll
-      for (int i = 0; i < DB * 4; ++i) {
-        const f32x4 y = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2],
-                         o[i / 4][i % 4 * 4 + 3]};
+        for (int i = 0; i < DB * 4; ++i) {
+          const f32x4 y = {o[i / 4][i % 4 * 4], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2],
+                           o[i / 4][i % 4 * 4 + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), to,
+                                                 (i * 64 + lane) * 16, 0, kCoherent);
+        }
+        const f32x4 y = {m, l, 0.0f, 0.0f};
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), to,
-                                               (i * 64 + lane) * 16, 0, kCoherent);
+                                               (DB * 4 * 64 + lane) * 16, 0, kCoherent);
       }
-      const f32x4 y = {m, l, 0.0f, 0.0f};
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), to,
-                                             (DB * 4 * 64 + lane) * 16, 0, kCoherent);
-    }
-    wait_vm<0>();
-    __syncthreads();
-    if (tid == 0)
-      lds.seq = atomicAdd(&p.counters[column * p.slots + piece.slot0], 1) == piece.pieces - 1;
-    __syncthreads();
-    if (!sreg(lds.seq) || !live) return;
-    m = -INFINITY;
-    for (int i = 0; i < piece.pieces; ++i)
-      m = fmaxf(m, as_f32(__builtin_amdgcn_raw_buffer_load_b32(
-                       slot(piece.slot0 + i), (DB * 4 * 64 + lane) * 16, 0, kCoherent)));
-    const float base = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
-    // two pieces on the way at a time (the last one's twin weighs 0)
-    for (int k = 0; k < piece.pieces; k += 2) {
-      const __amdgpu_buffer_rsrc_t from[2] = {slot(piece.slot0 + k),
-                                              slot(piece.slot0 + min(k + 1, piece.pieces - 1))};
-      f32x4 ml[2], y[2][DB * 4];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        ml[u] = __builtin_bit_cast(
-            f32x4, __builtin_amdgcn_raw_buffer_load_b128(from[u], (DB * 4 * 64 + lane) * 16, 0,
-                                                         kCoherent));
-#pragma unroll
-        for (int i = 0; i < DB * 4; ++i)
-          y[u][i] = __builtin_bit_cast(
+      wait_vm<0>();
+      __syncthreads();
+      if (tid == 0)
+        lds.seq = atomicAdd(&p.counters[column * p.slots + piece.slot0 + right], 1);
+      __syncthreads();
+      if (sreg(lds.seq) == 0) return;
+      if (live) {
+        const __amdgpu_buffer_rsrc_t from = slot((node ^ 1) * step);
+        auto read = [&](int i) {
+          return __builtin_bit_cast(
               f32x4,
-              __builtin_amdgcn_raw_buffer_load_b128(from[u], (i * 64 + lane) * 16, 0, kCoherent));
-      }
+              __builtin_amdgcn_raw_buffer_load_b128(from, (i * 64 + lane) * 16, 0, kCoherent));
+        };
+        const f32x4 ml = read(DB * 4);
+        f32x4 y[DB * 4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (u && k + 1 == piece.pieces) break;
-        const float f = exp2_fast(ml[u][0] - base);
-        l = fmaf(ml[u][1], f, l);
+        for (int i = 0; i < DB * 4; ++i) y[i] = read(i);
+        const float top = fmaxf(m, ml[0]), base = top == -INFINITY ? 0.0f : top;
+        const float f = exp2_fast(m - base), g = exp2_fast(ml[0] - base);
+        m = top;
+        // the lower half first, whichever of the two this is
+        const bool low = !(node & 1);
+        auto add = [&](float x, float y) {
+          return low ? fmaf(y, g, x * f) : fmaf(x, f, y * g);
+        };
+        l = add(l, ml[1]);
 #pragma unroll
         for (int i = 0; i < DB * 4; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            o[i / 4][i % 4 * 4 + e] = fmaf(y[u][i][e], f, o[i / 4][i % 4 * 4 + e]);
+            o[i / 4][i % 4 * 4 + e] = add(o[i / 4][i % 4 * 4 + e], y[i][e]);
       }
     }
+    if (!live) return;
   }
 
   // 3. the row's two lanes hold half of its sum each; a row that sees nothing is

@@ -352,3 +352,24 @@ def test_refusals_leave_the_outputs(aexq, ctx):
         ctx.logprobs(d, off[:2], None)
     torch.cuda.synchronize()
     assert (out == 7).all() and (lp == 7).all()
+
+
+@pytest.mark.parametrize("lens,hq,hkv,d,causal", [
+    ([1613, 300], 16, 16, 64, False), ([900, 1700], 16, 4, 128, True), ([800, 65], 8, 2, 256, True)])
+def test_repeated_calls_give_the_same_bits(ctx, lens, hq, hkv, d, causal):
+    """Tiles follow one another through two buffers; a read that is late, or a row
+    that is early, shows in some of many passes only."""
+    print(f"[gpu-case] repeated prompts {lens} {hq}/{hkv} d={d}", flush=True)
+    n = sum(lens)
+    q, k, v = _randn(n, hq, d, seed=1), _randn(n, hkv, d, seed=2), _randn(n, hkv, d, seed=3)
+    off, first, out = ref.offsets(lens), torch.zeros_like(q), torch.zeros_like(q)
+    other = torch.zeros((), dtype=torch.int64, device="cuda")
+    ctx.attention_prompt(q, k, v, off, 0.1, first, causal=causal)
+    for _ in range(150):
+        ctx.attention_prompt(q, k, v, off, 0.1, out, causal=causal)
+        other += (out != first).sum()
+    torch.cuda.synchronize()
+    assert other.item() == 0
+    at = off.tolist()
+    for a, b in zip(at, at[1:]):
+        ref.check_attention(first[a:b], *ref.attend(q[a:b], k[a:b], v[a:b], 0.1, causal))
