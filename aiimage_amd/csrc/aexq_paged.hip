@@ -460,10 +460,10 @@ template <int D>
 __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedParams p) {
   constexpr int T4 = D / 4, R = kThreads / T4;  // threads along a row, rows at a time
   __shared__ f32x4 sums[R][T4];
-  __shared__ float weight[kDecodeMost], tops[kWaves], parts[kWaves];
+  __shared__ float weight[kDecodeMost], sum[kDecodeMost], tops[kWaves], parts[kWaves];
   const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, y = tid % T4, r = tid / T4;
-  const int len = paged_length(p.kv, s);
+  const int len = paged_length(p.kv, s), share = p.plan[0], base_piece = p.plan[1 + s];
   f16* out = p.out + (long long)s * p.out_stride + head * D;
   if (len == 0) {
     if (tid < T4) *(f16x4*)(out + 4 * y) = f16x4{};
@@ -471,14 +471,24 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   }
   // (whatever the plan holds, the rows read are the launch's own)
   const int h = head / p.group, q = head % p.group;
-  const int pieces = DecodeCut(len, max(p.plan[0], 1)).pieces;
-  const int first = max(p.plan[1 + s], 0) + (h * p.blocks + q / 16) * pieces;
+  const int pieces = DecodeCut(len, max(share, 1)).pieces;
+  const int first = max(base_piece, 0) + (h * p.blocks + q / 16) * pieces;
   if (pieces == 1 || pieces > kDecodeMost || first > p.grid - pieces) return;
   auto row = [&](int i) { return p.part + ((first + i) * 16LL + q % 16) * (D + 4); };
+  // the first rows are on their way before the weights are known
+  constexpr int U = 4;
+  f32x4 o[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    o[u] = f32x4{};
+    if (r + u * R < pieces) o[u] = *(const f32x4*)(row(r + u * R) + 4 + 4 * y);
+  }
   float m = -INFINITY;
   for (int i = tid; i < pieces; i += kThreads) {
-    weight[i] = row(i)[0];
-    m = fmaxf(m, weight[i]);
+    const float2 ml = *(const float2*)row(i);
+    weight[i] = ml.x;
+    sum[i] = ml.y;
+    m = fmaxf(m, ml.x);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   for (int i = tid; i < pieces; i += kThreads) {  // (its own entries again)
     const float f = exp2_fast(weight[i] - base);
     weight[i] = f;
-    l = fmaf(row(i)[1], f, l);
+    l = fmaf(sum[i], f, l);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) l += __shfl_xor(l, off, 64);
@@ -501,12 +511,19 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) l += parts[w];
   f32x4 acc = f32x4{};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (r + u * R >= pieces) break;
+    const float f = weight[r + u * R];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[u][e], f, acc[e]);
+  }
 #pragma unroll 4
-  for (int i = r; i < pieces; i += R) {
-    const f32x4 o = *(const f32x4*)(row(i) + 4 + 4 * y);
+  for (int i = r + U * R; i < pieces; i += R) {
+    const f32x4 x = *(const f32x4*)(row(i) + 4 + 4 * y);
     const float f = weight[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], f, acc[e]);
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(x[e], f, acc[e]);
   }
   sums[r][y] = acc;
   __syncthreads();
