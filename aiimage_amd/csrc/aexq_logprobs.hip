@@ -7,11 +7,13 @@
 namespace aexq {
 
 // ---------------------------------------------------------------------------
-// One pass over a row of logits x with a running reference b, the rounded log2 e
-// times their maximum so far:
-//   y = x log2 e - b (one fma),  Z = sum 2^y,  T = sum 2^y y
+// One pass over a row of logits x with a running reference b:
+//   y = log2 e (x - max so far),  Z = sum 2^y,  T = sum 2^y y
 //   log p[t] = ln 2 (y[t] - log2 Z),   H = ln 2 (log2 Z - T / Z)
-// No sum depends on how b was rounded, so large logits lose nothing.
+// fp16: b is the rounded log2 e times the maximum and y one fma, x log2 e - b; no
+// sum depends on how b was rounded, so large logits lose nothing.  fp32: b is the
+// maximum itself, as a logit of the type's lowest value (a mask) times log2 e is
+// past the type's range.
 // Lanes take 16-byte chunks in turn; what a lane keeps for the alternatives is
 // its best chunk (by its largest logit) and the largest logit of the others.
 //
@@ -39,10 +41,26 @@ __device__ __forceinline__ u64 top_key(float x, int index) {
 struct Stats {
   float b, z, t;
 };
+// The reference for a maximum m, y of logit x, and y's step between references.
+template <typename E>
+constexpr bool kHalf = sizeof(E) == 2;
+template <typename E>
+__device__ __forceinline__ float reference(float m) {
+  return kHalf<E> ? m * kLog2e : m;
+}
+template <typename E>
+__device__ __forceinline__ float away(float x, float b) {
+  return kHalf<E> ? fmaf(x, kLog2e, -b) : (x - b) * kLog2e;
+}
+template <typename E>
+__device__ __forceinline__ float shift(float from, float to) {
+  return fmaxf(kHalf<E> ? from - to : (from - to) * kLog2e, kFar);
+}
 // The sums of two parts on the larger reference; parts of weight 0 add 0.
+template <typename E>
 __device__ __forceinline__ Stats join(Stats p, Stats q) {
   const float b = fmaxf(p.b, q.b), base = b == -INFINITY ? 0.0f : b;
-  const float dp = fmaxf(p.b - base, kFar), dq = fmaxf(q.b - base, kFar);
+  const float dp = shift<E>(p.b, base), dq = shift<E>(q.b, base);
   const float fp = __builtin_amdgcn_exp2f(dp), fq = __builtin_amdgcn_exp2f(dq);
   Stats r;
   r.b = b;
@@ -50,6 +68,7 @@ __device__ __forceinline__ Stats join(Stats p, Stats q) {
   r.t = fp * fmaf(p.z, dp, p.t) + fq * fmaf(q.z, dq, q.t);
   return r;
 }
+template <typename E>
 __device__ __forceinline__ Stats join_wave(Stats p) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
@@ -57,7 +76,7 @@ __device__ __forceinline__ Stats join_wave(Stats p) {
     q.b = __shfl_xor(p.b, off, 64);
     q.z = __shfl_xor(p.z, off, 64);
     q.t = __shfl_xor(p.t, off, 64);
-    p = join(p, q);
+    p = join<E>(p, q);
   }
   return p;
 }
@@ -70,7 +89,9 @@ __device__ __forceinline__ void row_outputs(const LogprobParams& p, int row, con
                                             u64 key) {
   const bool sound = s.z > 0.0f && s.z < INFINITY;
   const float log2z = log2f(s.z), nan = __builtin_nanf("");
-  auto log_p = [&](float x) { return (fmaf(x, kLog2e, -s.b) - log2z) * kLn2; };
+  auto log_p = [&](float x) {
+    return kHalf<E> ? (away<E>(x, s.b) - log2z) * kLn2 : x - s.b - log2z * kLn2;
+  };
   if (threadIdx.x == 0) {
     if (p.logprob) {
       const int token = p.tokens[row];
@@ -183,8 +204,8 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
       best_chunk = top > best ? c + u * kThreads : best_chunk;
       best = fmaxf(best, top);
     }
-    const float b = fmaxf(s.b, m * kLog2e), base = b == -INFINITY ? 0.0f : b;
-    const float d = fmaxf(s.b - base, kFar), f = __builtin_amdgcn_exp2f(d);
+    const float b = fmaxf(s.b, reference<E>(m)), base = b == -INFINITY ? 0.0f : b;
+    const float d = shift<E>(s.b, base), f = __builtin_amdgcn_exp2f(d);
     s.t = f * fmaf(s.z, d, s.t);
     s.z *= f;
     s.b = b;
@@ -192,12 +213,12 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const float y = fmaf((float)v[u][i], kLog2e, -base), e = __builtin_amdgcn_exp2f(y);
+        const float y = away<E>((float)v[u][i], base), e = __builtin_amdgcn_exp2f(y);
         s.z += e;
         s.t = fmaf(e, fmaxf(y, kFar), s.t);
       }
   }
-  s = join_wave(s);
+  s = join_wave<E>(s);
   if (lane == 0) wave_stats[wave] = s;
 
   u64 key = 0;
@@ -252,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
   if (tid < p.top) key = sorted[tid];
   s = wave_stats[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) s = join(s, wave_stats[w]);
+  for (int w = 1; w < kWaves; ++w) s = join<E>(s, wave_stats[w]);
   if (p.parts == 1) {
     row_outputs(p, row, x, s, key);
     return;
@@ -281,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobPar
     s = Stats{from[0], from[1], from[2]};
     if (p.top) mine = keys[(long long)tid * p.top];
   }
-  s = join_wave(s);
+  s = join_wave<E>(s);
   if ((tid & 63) == 0) wave_stats[tid >> 6] = s;
   u64 key = 0;
   if (p.top) {
@@ -311,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void logprob_join_kernel(const LogprobPar
   if (tid < p.top) key = sorted[tid];
   s = wave_stats[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) s = join(s, wave_stats[w]);
+  for (int w = 1; w < kWaves; ++w) s = join<E>(s, wave_stats[w]);
   row_outputs(p, row, (const E*)p.x + (long long)row * p.rstride, s, key);
 }
 

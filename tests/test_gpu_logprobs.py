@@ -116,6 +116,24 @@ def test_more_alternatives_than_finite_logits(aexq, ctx):
         _check(x, tokens, got)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows,n", [(1, 9000), (700, 2500)])
+def test_masks_of_the_lowest_value(aexq, ctx, rows, n, dtype):
+    """A masked logit's own probability, and rows of nothing but masks: finite."""
+    print(f"[gpu-case] logprobs lowest values {rows} x {n} {dtype}", flush=True)
+    low = torch.finfo(dtype).min
+    x = torch.full((rows, n), low, device="cuda", dtype=dtype)
+    tokens = torch.full((rows,), n - 3, dtype=torch.int32, device="cuda")
+    _check(x, tokens, _run(aexq, ctx, x, tokens, 20))
+    x[:, n // 2:n // 2 + 5] = 3.0  # fewer than the alternatives
+    _check(x, tokens, _run(aexq, ctx, x, tokens, 20))
+    x[:, n // 2] = -low / 2 ** 40
+    _check(x, tokens, _run(aexq, ctx, x, tokens, 20))
+    x[:] = -math.inf
+    x[:, 7:9] = low
+    _check(x, tokens, _run(aexq, ctx, x, tokens, 20))
+
+
 @pytest.mark.parametrize("n", [500, 9000])
 def test_rows_without_probabilities(aexq, ctx, n):
     """A NaN, a +inf or nothing but -inf: NaN and ids of -1, the rows beside them
