@@ -2119,6 +2119,9 @@ extern "C" aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv
   if (!st) st = check_rows(op, "k", k, k_stride, kv->heads_kv, kv->head_dim);
   if (!st) st = check_rows(op, "v", v, v_stride, kv->heads_kv, kv->head_dim);
   if (!st) st = check_rows(op, "q_out", q_out, q_out_stride, heads_q, kv->head_dim);
+  if (!st && q_out == q && q_out_stride != q_stride && tokens > 1)
+    st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "q_out is q, with rows %lld apart instead of %lld",
+              (long long)q_out_stride, (long long)q_stride);
   if (st) return st;
   const int half = rope->rotary_dim / 2;
   if (rope->rotary_dim <= 0 || rope->rotary_dim % 16 || rope->rotary_dim > kv->head_dim)
@@ -2181,6 +2184,8 @@ static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, in
   if ((long long)p.tokens * p.group > 0x7fffffffLL - 4096 || tiles > 65535)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "tokens=%d of %d heads per key head in one call",
                 p.tokens, p.group);
+  if (p.out == p.q)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is q, which other workgroups still read");
   HIP_TRY(op, hipSetDevice(ctx->device));
   long long pieces = tiles;
   if (prompt_planned(tiles, p.n, bound)) {

@@ -263,8 +263,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
     if (tile * (long long)kPromptRows >= prompt_rows(p, seq)) return;
     piece.pieces = sreg(piece.pieces);
     piece.slot0 = min(max(sreg(piece.slot0), 0), max(p.slots - piece.pieces, 0));
-    piece.slot = min(max(sreg(piece.slot), 0), p.slots - 1);
     if (piece.pieces > p.slots) return;
+    piece.slot = min(max(sreg(piece.slot), piece.slot0), piece.slot0 + max(piece.pieces, 1) - 1);
   } else {
     const int share = (n + kThreads - 1) / kThreads;
     const int sa = min(tid * share, n), sb = min(sa + share, n);

@@ -394,8 +394,8 @@ typedef struct aexq_rope {
 /* aexq_rope_kv_append for packed tokens of many sequences: the new tokens of
  * sequence s are rows offsets[s] .. offsets[s + 1] - 1 (device int32
  * [sequences + 1], not decreasing) and become its last positions, the ones
- * before lengths[s].  q is rotated into q_out (which may be q), k rotated and v
- * copied into their pages.  A position outside the table, or whose page entry
+ * before lengths[s].  q is rotated into q_out (which may be q, rows as far apart), k
+ * rotated and v copied into their pages.  A position outside the table, or whose page entry
  * lies outside the pool, is not stored.  Rows behind the last sequence are not
  * touched.  Two tokens that name the same cache row in one call leave either's
  * values, piece by piece. */

@@ -112,6 +112,18 @@ def test_prompt_arguments(lib, handle, args, status):
                                      a["os"]) == status
 
 
+def test_outputs_over_inputs(lib, handle):
+    """Attention into its own queries, and rotation in place with other row strides."""
+    kv, bad = _kv(), _abi.ERR_INVALID_ARGUMENT
+    assert lib.aexq_attention_prompt_paged(handle, kv, PTR, 512, PTR, 9, 4, 0.1, PTR, 512) == bad
+    assert lib.aexq_attention_prompt(handle, PTR, 512, PTR + 64, 256, PTR + 64, 256, PTR, None, 2,
+                                     9, 9, 4, 2, 128, 1, 0.1, PTR, 512) == bad
+    assert b"out is q" in lib.aexq_last_error()
+    assert lib.aexq_rope_append_paged(handle, kv, _rope(), PTR, 9, 4, PTR, 520, PTR, 256, PTR, 256,
+                                      PTR, 512) == bad
+    assert b"q_out is q" in lib.aexq_last_error()
+
+
 @pytest.mark.parametrize("over,status", [
     (dict(rotary_dim=24, section0=12), _abi.ERR_UNSUPPORTED),
     (dict(rotary_dim=144, section0=72), _abi.ERR_UNSUPPORTED),
