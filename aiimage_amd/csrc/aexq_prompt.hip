@@ -606,16 +606,25 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   // 0, one whose every score was -inf (a sum of 0) NaN
   l += __shfl_xor(l, 32, 64);
   const float inv = vis > 0 ? 1.0f / l : 0.0f;
-  if (row > last) return;
+  if (row > last) return;  // (a row's two lanes both)
   f16* out = p.out + token * p.out_stride + qh * D + dv0;
+  // dims 8 r + 4 h .. of a lane become 16 bytes, 8 r .. of even r in the lower lane of
+  // the row, of odd r in the upper one
 #pragma unroll
   for (int i = 0; i < DB; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f16x4 y;
+    for (int r = 0; r < 4; r += 2) {
+      f16x4 a, b;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = (f16)(o[i][4 * r + e] * inv);
-      *(f16x4*)(out + 32 * i + 8 * r + 4 * h) = y;
+      for (int e = 0; e < 4; ++e) {
+        a[e] = (f16)(o[i][4 * r + e] * inv);
+        b[e] = (f16)(o[i][4 * r + 4 + e] * inv);
+      }
+      const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+      const auto u = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);
+      const auto w = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+      const u32x4 z = {u[0], w[0], u[1], w[1]};
+      *(u32x4*)(out + 32 * i + 8 * (r + h)) = z;
     }
 }
 
