@@ -222,15 +222,6 @@ __device__ __forceinline__ int swz(int r) {
   return (r & 3) << 2 | (r >> 2 & 3);
 }
 
-// Lane i's 16 bytes at byte `off` (its own) of `from` to LDS byte lds + 16 i.  (One
-// wait state between the write of M0 and the load that reads it, as for dma().)
-__device__ __forceinline__ void dma_lane(const void* from, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds), "v"(off), "s"(from)
-               : "memory", "m0");
-}
-
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 // Of each 16 lanes, lane i reads 4 elements at its address; together a 4 x 16
 // block, row i / 4, columns 4 (i % 4) ..; lane i gets column i.
@@ -329,8 +320,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   float m = -INFINITY, l = 0.0f;
 
   // A wave's rows of a tile lie in one block of 16 positions, so in one page: a
-  // uniform base and an offset of each lane's own, the same for every tile that
-  // ends before the sequence does.
+  // uniform base and an offset of each lane's own, the same for every tile.  Rows past
+  // the sequence's end lie past the resource's and read zeros.
   const int r0 = wave * (KT / 4);
   const int kst = PAGED ? D * 2 : (int)p.k_stride * 2, vst = PAGED ? D * 2 : (int)p.v_stride * 2;
   uint32_t koff[NK], voff[NV];
@@ -346,7 +337,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
   }
   const uint32_t lds_base = lds_addr(&lds);
   auto fetch = [&](int t, int b) {
-    const int x = min(t * KT + r0, len - 1);
+    const int x = min(t * KT + r0, len - 1), keep = min(max(len - t * KT - r0, 0), KT / 4);
     const f16 *kb, *vb;
     if constexpr (PAGED) {
       const long long a =
@@ -358,25 +349,16 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
       kb = p.k + (long long)(kv0 + x) * p.k_stride + head * D;
       vb = p.v + (long long)(kv0 + x) * p.v_stride + head * D + dv0;
     }
-    kb = sreg(kb);
-    vb = sreg(vb);
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)sreg(kb), (short)0, sreg(keep * kst), kBufferRsrcWord3);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)sreg(vb), (short)0, sreg(keep * vst), kBufferRsrcWord3);
     const uint32_t kl = lds_base + (b * KT + r0) * D * 2;
     const uint32_t vl = lds_base + 2 * KT * D * 2 + (b * KT + r0) * DV * 2;
-    // rows past the end repeat the last one
-    const bool ends = (t + 1) * KT > len;
-    const int keep = len - 1 - x;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      uint32_t off = koff[i];
-      if (ends) off -= max(i * RK + lane / (D / 8) - keep, 0) * kst;
-      dma_lane(kb, off, kl + i * 1024);
-    }
+    for (int i = 0; i < NK; ++i) dma<16>(kr, kl + i * 1024, koff[i]);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      uint32_t off = voff[i];
-      if (ends) off -= max(i * RV + lane / (DV / 8) - keep, 0) * vst;
-      dma_lane(vb, off, vl + i * 1024);
-    }
+    for (int i = 0; i < NV; ++i) dma<16>(vr, vl + i * 1024, voff[i]);
   };
 
   // Where the lane's operands lie in a tile: step s of K (16 dims), and of V the
