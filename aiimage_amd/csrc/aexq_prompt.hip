@@ -28,11 +28,21 @@ namespace aexq {
 //                 (ds_read_b64_tr_b16), 4 positions of 16 dims per 16 lanes.
 // So scores, weights, maximum and sum of a row never leave its two lanes.
 //
+// What bounds it: the matrix instructions at the clock that their power leaves.
+// 16384 causal tokens of 32/8 heads of 128 take 2040 us (1.08 PFLOP/s; the matrix
+// units busy 61% of the time, at 1.66 GHz), 8192 of 16/4 heads 290 us (940 TFLOP/s;
+// 64 wide 177 and 256 wide 760 us).  4 x 512 tokens after 6143 take 231 us; the same
+// products alone, without reads, exponentials and loads, 191.  Exponentials put
+// between the products of the next tile, and loads between products, were no faster
+// for that (254 and 239 us).  Short prompts wait: some 7 us of a workgroup's time go
+// to finding its rows, its first tile, the masked tile and its stores.
+//
 // Where a launch has few 128-row tiles for the part, or tiles of very different
-// length, a small launch before it lays out its work (prompt_plan): tiles longer
+// length, a launch of 5 to 6 us before it lays out its work (prompt_plan): tiles longer
 // than a share of the whole are cut along the positions, and the longest pieces
-// start first.  The pieces of a cut tile leave their (max, sum, acc) registers in
-// scratch and are added up in a tree of fixed shape.
+// start first (4 x 512 tokens after up to 16000: 280 -> 126 us).  The pieces of a cut
+// tile leave their (max, sum, acc) registers in scratch and are added up in a tree of
+// fixed shape.
 // Otherwise every workgroup finds its tile from the offsets, last tiles first.
 // ---------------------------------------------------------------------------
 constexpr int kPromptRows = 128;
@@ -624,8 +634,10 @@ PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus) {
   PromptScratch r;
   const int dv = head_dim == 256 ? 128 : head_dim;
   r.columns = hkv * (head_dim / dv);
-  // two workgroups a CU.  A tile of c units is cut into pieces of at least share / 2,
-  // share >= units / target: no more than 2 target pieces of cut tiles in all
+  // A tile of c units is cut into pieces of at least share / 2, share >= units /
+  // target: no more than 2 target pieces of cut tiles in all.  Two workgroups have a
+  // place on a CU; shares for 1, 5/4, 3/2 and 2 per CU took 139, 135, 131 and 145 us
+  // (4 x 512 tokens after up to 16000) and 55.8, 54.4, 55.2 and 58.2 (12 prompts).
   r.target = 3 * cus / 2;
   r.slots = (2 * r.target + r.columns - 1) / r.columns;
   r.pieces = tiles + r.slots;
