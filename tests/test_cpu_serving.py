@@ -227,4 +227,4 @@ def test_a_wait_state_between_m0_and_the_load_that_reads_it():
                 if re.match(r"s_mov_b32 m0\b", line):
                     found += 1
                     assert lines[i + 1].startswith("s_nop"), (os.path.basename(path), lines)
-    assert found >= 3
+    assert found >= 2  # the two widths of dma(), which every kernel calls
