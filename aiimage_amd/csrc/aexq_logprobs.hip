@@ -25,7 +25,7 @@ namespace aexq {
 // each entry, the entries above it.
 //
 // Reading the logits bounds it (HBM): 777 rows of 151936 fp32 logits, 20 alternatives,
-// 102 us (4.6 TB/s), 512 rows of fp16 ones 45.  Few rows are cut into parts of chunks, a
+// 87 us (5.4 TB/s), 512 rows of fp16 ones 41 (3.8).  Few rows are cut into parts of chunks, a
 // workgroup each, whose (m, Z, T, K best) a second launch joins in the same way (one
 // row, 5 alternatives: 7.1 and 4.8 us, each a chain of dependent loads).
 // ---------------------------------------------------------------------------
@@ -146,9 +146,10 @@ __device__ __forceinline__ u64 top_bound(const u64* keys, int top) {
   return (u64)high << 32 | low;
 }
 
-template <typename E>
+// STREAM: the logits do not stay in the caches.
+template <typename E, bool STREAM>
 __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p) {
-  constexpr int VE = 16 / (int)sizeof(E), U = 4;  // logits of a chunk, chunks in flight
+  constexpr int VE = 16 / (int)sizeof(E), U = 3;  // logits of a chunk, chunks in flight
   __shared__ Stats wave_stats[kWaves];
   __shared__ u64 keys[kThreads], sorted[64];
   __shared__ int counts[kWaves];
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(const LogprobParams p
     const int i0 = c * VE - skew;
     Chunk v;
     if (i0 >= 0 && i0 <= p.n - VE) {
-      v = *(const Chunk*)(x + i0);
+      v = STREAM ? __builtin_nontemporal_load((const Chunk*)(x + i0)) : *(const Chunk*)(x + i0);
     } else {
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
@@ -348,8 +349,13 @@ int logprob_parts(long long rows, int n, int esize, int cus) {
 
 template <typename E>
 static hipError_t dispatch(const LogprobParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(logprob_kernel<E>, dim3((unsigned)(p.rows * p.parts)), dim3(kThreads), 0,
-                     stream, p);
+  // Logits of more than the last cache holds are read past the caches (1000 rows of
+  // 151936 fp32 logits 118 -> 106 us, 777 101 -> 92); fewer may still be there since
+  // the linear that wrote them (512 rows of fp16 ones 45 us past the caches, 41 through
+  // them; 300 rows 49 and 46).
+  const bool stream_reads = (long long)p.rows * p.n * sizeof(E) > 256LL << 20;
+  hipLaunchKernelGGL((stream_reads ? logprob_kernel<E, true> : logprob_kernel<E, false>),
+                     dim3((unsigned)(p.rows * p.parts)), dim3(kThreads), 0, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.parts == 1) return e;
   hipLaunchKernelGGL(logprob_join_kernel<E>, dim3((unsigned)p.rows), dim3(kThreads), 0, stream, p);
