@@ -25,9 +25,9 @@ namespace aexq {
 // each entry, the entries above it.
 //
 // Reading the logits bounds it (HBM): 777 rows of 151936 fp32 logits, 20 alternatives,
-// 87 us (5.4 TB/s), 512 rows of fp16 ones 41 (3.8).  Few rows are cut into parts of chunks, a
-// workgroup each, whose (m, Z, T, K best) a second launch joins in the same way (one
-// row, 5 alternatives: 7.1 and 4.8 us, each a chain of dependent loads).
+// 87 us (5.4 TB/s), 512 rows of fp16 ones 41 (3.8).  Few rows are cut into parts of
+// chunks, a workgroup each, whose (m, Z, T, K best) a second launch joins in the same
+// way (one row, 5 alternatives: 7.1 and 4.8 us, each a chain of dependent loads).
 // ---------------------------------------------------------------------------
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

@@ -186,9 +186,9 @@ hipError_t rope_append_launch(RopeAppendParams p, hipStream_t stream) {
 // The waves of a workgroup take steps in turn and meet in LDS at the end.
 //
 // What bounds it is reading K and V once (HBM): 7 sequences of 309146 positions, 2
-// key heads of 256, 633 MB in 112 us (5.7 TB/s); 64 of 56891, 8 of 128, 234 MB in 53
-// (4.4: 2.7 us to find the piece, and memory serves pieces of one length unevenly,
-// the first done after 17 us, the last after 52); one of 300 positions takes 6 us.
+// key heads of 256, 633 MB in 112 us (5.7 TB/s); 64 of 56891, 8 of 128, 234 MB in 44
+// (5.4; 2.7 us of it to find the piece, and memory serves pieces of one length
+// unevenly); one of 300 positions takes 6 us.
 //
 // Lengths may differ as they like and the host need not know them: where it pays, a
 // (sequence, head block) longer than a share of all of them is cut into even pieces
@@ -250,7 +250,17 @@ __device__ __forceinline__ void decode_piece(const DecodePagedParams& p, DecodeL
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const f16* row = p.kv.v + (i < 4 ? r0 : r1) * D + (4 * g + i % 4) * D + DPL * c;
-      __builtin_memcpy(v[i], __builtin_assume_aligned(row, 2 * DPL), 2 * DPL);
+      // Past the caches, where one load covers whole rows: 256 sequences of 1000 to
+      // 3000 positions, 8 key heads of 128, 364 -> 332 us, of 100 to 1000 88 -> 72, 64
+      // of 56891 together cold 59 -> 55, warm 48 -> 49.  The two loads of a row of 256
+      // dims need its lines twice, as K's do (309146 positions cold 117 -> 120).
+      if constexpr (DPL <= 8) {
+        typedef uint32_t Run __attribute__((ext_vector_type(DPL / 2)));
+        const Run run = __builtin_nontemporal_load((const Run*)row);
+        __builtin_memcpy(v[i], &run, sizeof(run));
+      } else {
+        __builtin_memcpy(v[i], __builtin_assume_aligned(row, 2 * DPL), 2 * DPL);
+      }
     }
     f32x4 s0 = f32x4{}, s1 = f32x4{};
 #pragma unroll
