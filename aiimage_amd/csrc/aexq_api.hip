@@ -2038,6 +2038,16 @@ extern "C" aexq_status aexq_decode_advance(aexq_ctx* ctx, int32_t* position, int
 // ---------------------------------------------------------------------------
 // many sequences: a paged cache, prompts, log probabilities
 // ---------------------------------------------------------------------------
+// Scratch of a serving step grows with the batch, a little from step to step, and the
+// buffers it outgrows stay until the context ends (graphs may hold them): powers of
+// two, so that all of them together are no more than the last.
+static aexq_status grow_step_scratch(aexq_ctx* ctx, void** buf, long long* cap, long long bytes,
+                                     const char* op, const char* what) {
+  long long size = 4096;
+  while (size < bytes) size *= 2;
+  return bytes <= *cap ? AEXQ_OK : grow_scratch(ctx, buf, cap, size, op, what);
+}
+
 static bool is_head_dim(int d) { return d == 64 || d == 128 || d == 256; }
 
 // A cache descriptor as the kernels take it.
@@ -2190,13 +2200,13 @@ static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, in
   long long pieces = tiles;
   if (prompt_planned(tiles, p.n, bound)) {
     const PromptScratch need = prompt_scratch(tiles, p.hkv, head_dim, ctx->cus);
-    aexq_status st = grow_scratch(ctx, (void**)&ctx->prompt_plan, &ctx->prompt_plan_cap,
-                                  (need.counters + need.plan_ints) * (long long)sizeof(int), op,
-                                  "prompt attention plan");
+    const long long ints = need.counters + need.plan_ints;
+    aexq_status st = grow_step_scratch(ctx, (void**)&ctx->prompt_plan, &ctx->prompt_plan_cap,
+                                       ints * (long long)sizeof(int), op, "prompt attention plan");
     if (!st)
-      st = grow_scratch(ctx, (void**)&ctx->prompt_part, &ctx->prompt_part_cap,
-                        need.part_floats * (long long)sizeof(float), op,
-                        "prompt attention partials");
+      st = grow_step_scratch(ctx, (void**)&ctx->prompt_part, &ctx->prompt_part_cap,
+                             need.part_floats * (long long)sizeof(float), op,
+                             "prompt attention partials");
     if (st) return st;
     p.plan = ctx->prompt_plan;
     p.counters = ctx->prompt_plan + need.plan_ints;
@@ -2311,13 +2321,13 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
   if (plan.target) {
     p.target = plan.target;
     p.grid = (int)plan.grid;
-    st = grow_scratch(ctx, (void**)&ctx->paged_part, &ctx->paged_part_cap,
-                      plan.grid * 16 * (kv->head_dim + 4) * (long long)sizeof(float), op,
-                      "paged attention partials");
+    st = grow_step_scratch(ctx, (void**)&ctx->paged_part, &ctx->paged_part_cap,
+                           plan.grid * 16 * (kv->head_dim + 4) * (long long)sizeof(float), op,
+                           "paged attention partials");
     if (!st)
-      st = grow_scratch(ctx, (void**)&ctx->paged_plan, &ctx->paged_plan_cap,
-                        (1LL + kv->sequences) * (long long)sizeof(int), op,
-                        "paged attention plan");
+      st = grow_step_scratch(ctx, (void**)&ctx->paged_plan, &ctx->paged_plan_cap,
+                             (1LL + kv->sequences) * (long long)sizeof(int), op,
+                             "paged attention plan");
     if (st) return st;
     p.part = ctx->paged_part;
     p.plan = ctx->paged_plan;
@@ -2368,12 +2378,12 @@ extern "C" aexq_status aexq_logprobs(aexq_ctx* ctx, const aexq_tensor* logits,
   HIP_TRY(op, hipSetDevice(ctx->device));
   if (p.parts > 1) {
     const long long n = p.rows * p.parts;
-    st = grow_scratch(ctx, (void**)&ctx->logprob_stats, &ctx->logprob_stats_cap,
-                      n * 4 * (long long)sizeof(float), op, "log probability sums");
+    st = grow_step_scratch(ctx, (void**)&ctx->logprob_stats, &ctx->logprob_stats_cap,
+                           n * 4 * (long long)sizeof(float), op, "log probability sums");
     if (!st)
-      st = grow_scratch(ctx, (void**)&ctx->logprob_keys, &ctx->logprob_keys_cap,
-                        (n * top + 1) * (long long)sizeof(unsigned long long), op,
-                        "log probability alternatives");
+      st = grow_step_scratch(ctx, (void**)&ctx->logprob_keys, &ctx->logprob_keys_cap,
+                             (n * top + 1) * (long long)sizeof(unsigned long long), op,
+                             "log probability alternatives");
     if (st) return st;
     p.stats = ctx->logprob_stats;
     p.keys = ctx->logprob_keys;
