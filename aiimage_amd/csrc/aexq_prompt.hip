@@ -648,12 +648,18 @@ PromptScratch prompt_scratch(long long tiles, int hkv, int head_dim, int cus) {
 }
 
 template <int D, bool PAGED>
-static void prompt_dispatch(const PromptParams& p, unsigned rows, hipStream_t stream) {
-  if (p.plan)
+static hipError_t prompt_dispatch(const PromptParams& p, unsigned rows, hipStream_t stream) {
+  if (p.plan) {
     hipLaunchKernelGGL(prompt_plan_kernel<PAGED>, dim3(1), dim3(kPlanThreads), 0, stream, p,
                        PromptLds<D>::KT);
+    // (the next launch would run on the layout and the counters of an earlier call, and
+    // clear this error)
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((prompt_kernel<D, PAGED>), dim3(p.hkv * (D / PromptLds<D>::DV), rows),
                      dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
 }
 
 hipError_t prompt_launch(const PromptParams& p, int head_dim, long long pieces,
@@ -661,11 +667,10 @@ hipError_t prompt_launch(const PromptParams& p, int head_dim, long long pieces,
   const unsigned rows = (unsigned)pieces;
   const bool paged = p.kv.k;
   switch (head_dim) {
-    case 64: (paged ? prompt_dispatch<64, true> : prompt_dispatch<64, false>)(p, rows, stream); break;
-    case 128: (paged ? prompt_dispatch<128, true> : prompt_dispatch<128, false>)(p, rows, stream); break;
-    default: (paged ? prompt_dispatch<256, true> : prompt_dispatch<256, false>)(p, rows, stream); break;
+    case 64: return (paged ? prompt_dispatch<64, true> : prompt_dispatch<64, false>)(p, rows, stream);
+    case 128: return (paged ? prompt_dispatch<128, true> : prompt_dispatch<128, false>)(p, rows, stream);
+    default: return (paged ? prompt_dispatch<256, true> : prompt_dispatch<256, false>)(p, rows, stream);
   }
-  return hipGetLastError();
 }
 
 }  // namespace aexq

@@ -1,0 +1,40 @@
+"""What the host side of the operators for many sequences launches and allocates,
+and that a launch that fails is reported (fake_hip.py stands for the runtime)."""
+import pytest
+
+import fake_hip
+
+CALLS = {
+    "prompt": ("lib.aexq_attention_prompt(ctx, PTR, 512, PTR, 256, PTR, 256, PTR, None, 2, 900, 900,"
+               " 4, 2, 128, 1, 0.1, PTR + 64, 512)", 2),
+    "prompt_paged": ("lib.aexq_attention_prompt_paged(ctx, paged(), PTR, 512, PTR, 900, 4, 0.1,"
+                     " PTR + 64, 512)", 2),
+    "decode": ("lib.aexq_attention_decode_paged(ctx, paged(), PTR, 512, 4, 0.1, PTR + 64, 512)", 2),
+    "append": ("lib.aexq_rope_append_paged(ctx, paged(), _abi.Rope(PTR, PTR, PTR, 100, 128, 1, 0,"
+               " 64), PTR, 9, 4, PTR, 512, PTR, 256, PTR, 256, PTR, 512)", 1),
+    "logprobs": ("lib.aexq_logprobs(ctx, logits, PTR, PTR, None, 5, PTR, PTR)", 2),
+}
+LOGITS = """
+logits = _abi.Tensor()
+logits.logical = logits.storage = _abi.Shape(2, 150000, 2, 1, 1)
+logits.layout, logits.dtype, logits.data, logits.batch = (_abi.LAYOUT_LINEAR, _abi.DTYPE_F32,
+                                                          PTR, 1)
+"""
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_a_failed_launch_is_reported(tmp_path, name):
+    """Whichever of a call's launches fails, the call does, and no later one of its
+    launches runs on what the failed one should have left."""
+    call, launches = CALLS[name]
+    fake_hip.run(tmp_path, LOGITS + f"""
+before = fake.fake_launches()
+assert {call} == 0, lib.aexq_last_error()
+assert fake.fake_launches() - before == {launches}
+for n in range({launches}):
+    before = fake.fake_launches()
+    fake.fake_fail(n)
+    assert {call} != 0, f"launch {{n}} failed unseen"
+    assert fake.fake_launches() - before == n + 1, f"launches after the failed {{n}}"
+    assert {call} == 0
+""")
