@@ -2100,14 +2100,16 @@ static aexq_status check_rows(const char* op, const char* name, const void* data
   return AEXQ_OK;
 }
 
-// Query heads over key heads, and the scale.
+// Query heads over key heads, and the scale, which the kernels take in log2 units.
+constexpr float kLog2e = 1.4426950408889634f;
 static aexq_status check_heads(const char* op, int heads_q, int heads_kv, float scale) {
   if (heads_kv <= 0 || heads_q <= 0 || heads_q % heads_kv != 0)
     return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "heads_q=%d heads_kv=%d", heads_q, heads_kv);
   if ((long long)heads_q * 256 > 0x7fffffffLL || heads_kv > 65535)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "heads_q=%d heads_kv=%d", heads_q, heads_kv);
-  if (!(scale > 0.0f) || !(scale <= 3.0e38f))
-    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "scale=%g (positive and finite)", (double)scale);
+  if (!(scale > 0.0f) || !(scale * kLog2e <= 3.4028235e38f))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "scale=%g (positive, at most 2.35e38)",
+                (double)scale);
   return AEXQ_OK;
 }
 
@@ -2188,7 +2190,7 @@ static aexq_status prompt_run(aexq_ctx* ctx, const char* op, PromptParams& p, in
   if (p.n <= 0 || p.tokens <= 0)
     return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "sequences=%d tokens=%d", p.n, p.tokens);
   p.group = heads_q / p.hkv;
-  p.scale2 = scale * 1.4426950408889634f;
+  p.scale2 = scale * kLog2e;
   // rows of one sequence are counted in 31 bits, tiles are a grid's second axis
   const long long tiles = prompt_tiles(p.tokens, p.n, p.group);
   if ((long long)p.tokens * p.group > 0x7fffffffLL - 4096 || tiles > 65535)
@@ -2306,7 +2308,7 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
   p.out_stride = out_stride;
   p.group = heads_q / kv->heads_kv;
   p.blocks = (p.group + 15) / 16;
-  p.scale2 = scale * 1.4426950408889634f;
+  p.scale2 = scale * kLog2e;
   const long long bound = (long long)kv->table_width * kv->page_size;
   const DecodePlan plan =
       decode_paged_plan(kv->head_dim, ctx->cus, bound,

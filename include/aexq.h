@@ -413,7 +413,8 @@ aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const
  * queries are the sequence's last positions and see those up to their own.  A
  * row that sees no position is 0; what a row does not see does not reach it,
  * infinities and NaN in k or v included.  Rows behind the last sequence are not
- * touched.  scale > 0.  Uses the context's scratch. */
+ * touched.  scale is above 0 and at most 2.35e38 (here and below); scores past
+ * fp32's range count as infinite.  Uses the context's scratch. */
 aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64_t q_stride, const void* k,
                                   int64_t k_stride, const void* v, int64_t v_stride,
                                   const int32_t* q_offsets, const int32_t* kv_offsets,

@@ -38,3 +38,18 @@ for n in range({launches}):
     assert fake.fake_launches() - before == n + 1, f"launches after the failed {{n}}"
     assert {call} == 0
 """)
+
+
+@pytest.mark.parametrize("name", ["prompt", "prompt_paged", "decode"])
+def test_scales_whose_log2_form_is_past_fp32_are_refused(tmp_path, name):
+    """Scores are formed in log2 units, by scale * log2 e: past fp32's range from
+    2.36e38 on, where every row would be NaN."""
+    call, launches = CALLS[name]
+    fake_hip.run(tmp_path, f"""
+before = fake.fake_launches()
+assert {call.replace("0.1,", "2.4e38,")} == _abi.ERR_INVALID_ARGUMENT, "2.4e38 taken"
+assert b"scale" in lib.aexq_last_error()
+assert fake.fake_launches() == before
+assert {call.replace("0.1,", "2.3e38,")} == 0, lib.aexq_last_error()
+assert fake.fake_launches() - before == {launches}
+""")
