@@ -96,7 +96,8 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(const RopeAppendP
   const PackedRow own = packed_row(p.offsets, p.kv.lengths, p.kv.n, t);
   if (p.positions) turn_by(0);
   if (!own.found) return;  // rows behind the last sequence stay as they were
-  const int pos = own.length - (own.end - t);
+  // (a length below 0 is 0: its difference to a token does not wrap)
+  const int pos = max(own.length, 0) - (own.end - t);
   // where its k and v rows go; nowhere outside the table or the pool
   int page = -1;
   if (pos >= 0 && pos < p.kv.width << p.kv.shift)
