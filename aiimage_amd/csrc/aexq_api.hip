@@ -2323,8 +2323,10 @@ extern "C" aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_pag
   if (plan.target) {
     p.target = plan.target;
     p.grid = (int)plan.grid;
+    p.slots = plan.slots;
+    p.rows = p.group < 16 ? p.group : 16;
     st = grow_step_scratch(ctx, (void**)&ctx->paged_part, &ctx->paged_part_cap,
-                           plan.grid * 16 * (kv->head_dim + 4) * (long long)sizeof(float), op,
+                           (long long)p.slots * p.rows * (kv->head_dim + 4) * sizeof(float), op,
                            "paged attention partials");
     if (!st)
       st = grow_step_scratch(ctx, (void**)&ctx->paged_plan, &ctx->paged_plan_cap,

@@ -319,11 +319,12 @@ struct DecodePagedParams {
   float scale2;       // scale * log2(e)
   int target;         // shares of the work that is cut; 0: nothing is cut
   int grid;           // pieces at most
-  float* part;        // a piece's partial rows, 16 of head_dim + 4 floats
+  int slots, rows;    // of those of what is cut, and query heads of a block at most
+  float* part;        // a slot's partial rows, each of head_dim + 4 floats
   int* plan;          // 1 + n ints
 };
 struct DecodePlan {
-  int target;
+  int target, slots;
   long long grid;
 };
 DecodePlan decode_paged_plan(int head_dim, int cus, long long bound, long long blocks);

@@ -199,13 +199,25 @@ hipError_t rope_append_launch(RopeAppendParams p, hipStream_t stream) {
 constexpr int kDecodeUnit = 128;
 constexpr int kDecodeMost = 2048;  // pieces of a (sequence, head block)
 
+// Two numbers that are added up together.
+struct Two {
+  int a, b;
+};
+__device__ __forceinline__ Two operator+(Two x, Two y) { return Two{x.a + y.a, x.b + y.b}; }
+__device__ __forceinline__ Two operator-(Two x, Two y) { return Two{x.a - y.a, x.b - y.b}; }
+__device__ __forceinline__ int shuffle_up(int v, int off) { return __shfl_up(v, off, 64); }
+__device__ __forceinline__ Two shuffle_up(Two v, int off) {
+  return Two{__shfl_up(v.a, off, 64), __shfl_up(v.b, off, 64)};
+}
+
 template <int D>
 struct DecodeLds {
   static constexpr int HT = D / 16 < 8 ? D / 16 : 8;  // dims of a lane's run in one pass
   static constexpr int W = 16 * HT;                   // dims of one pass
   alignas(16) float o[kWaves][16][W + 4];
   float m[kWaves][16], l[kWaves][16];
-  int seq, base, count[2][kWaves];
+  int seq, base, slot, units[kWaves];
+  Two pieces[kWaves];
 };
 
 // One (sequence s, head block hb) over positions [p0, p1) of len, by the whole
@@ -405,28 +417,30 @@ struct DecodeCut {
 };
 
 // Sum over the workgroup's threads, and of those before each.
-__device__ __forceinline__ int block_scan(int mine, int* waves, int* total) {
+template <typename T>
+__device__ __forceinline__ T block_scan(T mine, T* waves, T* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int upto = mine;
+  T upto = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int v = __shfl_up(upto, off, 64);
-    if (lane >= off) upto += v;
+    const T v = shuffle_up(upto, off);
+    if (lane >= off) upto = upto + v;
   }
   if (lane == 63) waves[wave] = upto;
   __syncthreads();
-  int before = upto - mine, sum = 0;
+  T before = upto - mine, sum = T{};
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += waves[w];
-    sum += waves[w];
+    if (w < wave) before = before + waves[w];
+    sum = sum + waves[w];
   }
   *total = sum;
   return before;
 }
 
 // A piece per workgroup.  plan[0] takes the share of units that is cut, plan[1 +
-// s] the first piece of sequence s, for the joining launch.  (That the last
+// s] the first slot of partial rows of sequence s, for the joining launch: only the
+// pieces of what is cut have one, fewer than two for each share.  (That the last
 // workgroup of a head block joins it in the same launch was slower: its rows then
 // go past the L2s.  One sequence of 1000 positions 9.4 -> 12.9 us, 64 sequences of
 // 56891 55 -> 63.)
@@ -438,34 +452,44 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 2 : 4) void decode_paged_cut(
   // thread t adds up its share of the sequences
   const int each = (n + kThreads - 1) / kThreads;
   const int s0 = min(tid * each, n), s1 = min(s0 + each, n);
-  int units = 0, pieces = 0, total;
+  int units = 0, all;
   for (int s = s0; s < s1; ++s)
     units += (paged_length(p.kv, s) + kDecodeUnit - 1) / kDecodeUnit * heads;
-  block_scan(units, lds.count[0], &total);
-  const int share = max((total + p.target - 1) / p.target, 1);
-  for (int s = s0; s < s1; ++s) pieces += DecodeCut(paged_length(p.kv, s), share).pieces * heads;
-  const int before = block_scan(pieces, lds.count[1], &total);
+  block_scan(units, lds.units, &all);
+  const int share = max((all + p.target - 1) / p.target, 1);
+  // the pieces of sequence s, and those of them that have a slot
+  auto count = [&](int s) {
+    const int m = DecodeCut(paged_length(p.kv, s), share).pieces;
+    return Two{m * heads, m > 1 ? m * heads : 0};
+  };
+  Two pieces = {0, 0}, total;
+  for (int s = s0; s < s1; ++s) pieces = pieces + count(s);
+  const Two before = block_scan(pieces, lds.pieces, &total);
   if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
   const int at = blockIdx.x;
-  if (at >= total) return;
-  if (before <= at && at < before + pieces) {
-    int s = s0, base = before;
+  if (at >= total.a) return;
+  if (before.a <= at && at < before.a + pieces.a) {
+    int s = s0;
+    Two base = before;
     for (;; ++s) {
-      const int m = DecodeCut(paged_length(p.kv, s), share).pieces * heads;
-      if (at < base + m) break;
-      base += m;
+      const Two m = count(s);
+      if (at < base.a + m.a) break;
+      base = base + m;
     }
     lds.seq = s;
-    lds.base = base;
-    if (at == base) p.plan[1 + s] = base;
+    lds.base = base.a;
+    lds.slot = base.b;
+    if (at == base.a) p.plan[1 + s] = base.b;
   }
   __syncthreads();
   const int s = sreg(lds.seq), len = paged_length(p.kv, s);
   const DecodeCut cut(len, share);
-  const int hb = (at - sreg(lds.base)) / cut.pieces, i = (at - sreg(lds.base)) % cut.pieces;
+  const int mine = at - sreg(lds.base), hb = mine / cut.pieces, i = mine % cut.pieces;
+  // (whatever the lengths do meanwhile, the rows written are the launch's own)
+  const int slot = min(sreg(lds.slot) + mine, p.slots - 1);
   decode_piece<D>(p, lds, s, hb, len, i * cut.size * kDecodeUnit,
                   min(len, (i + 1) * cut.size * kDecodeUnit),
-                  cut.pieces == 1 ? nullptr : p.part + (long long)at * 16 * (D + 4));
+                  cut.pieces == 1 ? nullptr : p.part + (long long)slot * p.rows * (D + 4));
 }
 
 // Joins the partial rows of the (sequence, head)s that were cut:
@@ -478,7 +502,7 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   __shared__ float weight[kDecodeMost], sum[kDecodeMost], tops[kWaves], parts[kWaves];
   const int head = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6, y = tid % T4, r = tid / T4;
-  const int len = paged_length(p.kv, s), share = p.plan[0], base_piece = p.plan[1 + s];
+  const int len = paged_length(p.kv, s), share = p.plan[0], slot = p.plan[1 + s];
   f16* out = p.out + (long long)s * p.out_stride + head * D;
   if (len == 0) {
     if (tid < T4) *(f16x4*)(out + 4 * y) = f16x4{};
@@ -487,9 +511,10 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   // (whatever the plan holds, the rows read are the launch's own)
   const int h = head / p.group, q = head % p.group;
   const int pieces = DecodeCut(len, max(share, 1)).pieces;
-  const int first = max(base_piece, 0) + (h * p.blocks + q / 16) * pieces;
-  if (pieces == 1 || pieces > kDecodeMost || first > p.grid - pieces) return;
-  auto row = [&](int i) { return p.part + ((first + i) * 16LL + q % 16) * (D + 4); };
+  if (pieces == 1 || pieces > kDecodeMost) return;
+  const long long first = max(slot, 0) + (h * p.blocks + q / 16) * (long long)pieces;
+  if (first > p.slots - pieces) return;
+  auto row = [&](int i) { return p.part + ((first + i) * p.rows + q % 16) * (D + 4); };
   // the first rows are on their way before the weights are known
   constexpr int U = 4;
   f32x4 o[U];
@@ -558,13 +583,15 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
 
 // The cut of a launch over up to `bound` positions of each sequence in `blocks`
 // head blocks of sequences: one piece for each `target`-th of all units, so that
-// no more than blocks + target are there.  Nothing is cut (target 0) where the
+// no more than blocks + target are there.  What is cut has more than one share, and
+// less than two pieces for each: fewer than 2 target of them.  Nothing is cut (target 0) where the
 // steps of a workgroup are few, and where there is a workgroup for every CU whose
 // longest way is not much longer.
 DecodePlan decode_paged_plan(int head_dim, int cus, long long bound, long long blocks) {
   DecodePlan r;
   r.target = bound <= 512 || (blocks >= cus && bound <= 1024) ? 0 : (head_dim == 256 ? 2 : 3) * cus;
   r.grid = blocks + r.target;
+  r.slots = 2 * r.target;
   return r;
 }
 

@@ -53,3 +53,18 @@ assert fake.fake_launches() == before
 assert {call.replace("0.1,", "2.3e38,")} == 0, lib.aexq_last_error()
 assert fake.fake_launches() - before == {launches}
 """)
+
+
+@pytest.mark.parametrize("sequences,hq,d", [(1, 4, 128), (1024, 32, 128), (8192, 32, 128),
+                                            (20000, 8, 256), (8192, 128, 64)])
+def test_decode_scratch_does_not_grow_with_the_batch(tmp_path, sequences, hq, d):
+    """Only a (sequence, head block) longer than a share of the work leaves partial
+    rows, and those are few however many sequences there are: 2 * 768 pieces (at most)
+    of 16 rows of 260 floats are 26 MB, rounded up to 32; an int a sequence."""
+    fake_hip.run(tmp_path, f"""
+before = fake.fake_bytes()
+kv = paged(sequences={sequences}, heads_kv=8 if {hq} % 8 == 0 else 2, head_dim={d}, table_width=64)
+assert lib.aexq_attention_decode_paged(ctx, kv, PTR, {hq * d}, {hq}, 0.1, PTR + 64,
+                                       {hq * d}) == 0, lib.aexq_last_error()
+assert fake.fake_bytes() - before <= (32 << 20) + 8 * {sequences} + 4096, fake.fake_bytes() - before
+""")

@@ -54,3 +54,54 @@ def test_append_to_the_lowest_length(aexq, ctx):
     torch.cuda.synchronize()
     assert torch.equal(k, before[0]) and torch.equal(v, before[1])
     assert torch.equal(out, q)
+
+
+# ---------------------------------------------------------------- paged decode
+
+@pytest.mark.parametrize("n,hq,hkv,d", [(257, 8, 2, 128), (700, 4, 1, 64), (300, 20, 1, 128),
+                                        (513, 2, 2, 256), (1500, 6, 2, 64)])
+def test_cut_decode_of_more_sequences_than_threads(aexq, ctx, n, hq, hkv, d):
+    """More sequences than a workgroup has threads, most of them short, some cut into
+    several pieces: at the ends, next to the threads' borders, beside empty ones."""
+    print(f"[gpu-case] cut decode of {n} sequences {hq}/{hkv} d={d}", flush=True)
+    each = -(-n // 256)  # sequences of a thread
+    long = sorted({0, 1, each - 1, each, 128 * each, n // 2, n - 2, n - 1})
+    lens = [(37 * i) % 90 for i in range(n)]
+    for i, s in enumerate(long):
+        lens[s] = 1500 + 61 * i
+    lens[2], lens[n // 2 + 1] = 0, 0
+    k, v, table, lengths = ref.make_cache(lens, hkv, 16, d, 6, width=140, fill=NAN)
+    q = _randn(n, hq, d, seed=1)
+    out, again = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
+    kv, scale = aexq.paged_kv(k, v, table, lengths), 1.0 / math.sqrt(d)
+    ctx.attention_decode_paged(kv, q, scale, out)
+    ctx.attention_decode_paged(kv, q, scale, again)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+    for s in sorted(set(long + [2, n // 2 + 1] + list(range(3, n, 13)))):
+        ref.check_attention(out[s:s + 1], *ref.attend(q[s:s + 1], ref.gather(k, table, s, lens[s]),
+                                                      ref.gather(v, table, s, lens[s]), scale,
+                                                      False))
+    dead = torch.tensor([m == 0 for m in lens], device="cuda")
+    assert (out[dead] == 0).all() and torch.isfinite(out).all()
+
+
+def test_decode_scratch_of_a_large_batch(aexq):
+    """Sequences that are not cut take no scratch: a batch of 2048 in 8 key heads of
+    128 takes the 13 MB of partial rows that one of 4 takes."""
+    print("[gpu-case] decode scratch of 2048 sequences", flush=True)
+    n, hq, hkv, d = 2048, 32, 8, 128
+    lens = [(5 * i) % 40 for i in range(n)]
+    k, v, table, lengths = ref.make_cache(lens, hkv, 16, d, 6, width=80)
+    q = _randn(n, hq, d, seed=1)
+    out, kv = torch.zeros_like(q), aexq.paged_kv(k, v, table, lengths)
+    own = aexq.Context(0)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    own.attention_decode_paged(kv, q, 0.09, out)
+    torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= 64 << 20
+    for s in range(0, n, 97):
+        ref.check_attention(out[s:s + 1], *ref.attend(q[s:s + 1], ref.gather(k, table, s, lens[s]),
+                                                      ref.gather(v, table, s, lens[s]), 0.09, False))
+    own.close()
