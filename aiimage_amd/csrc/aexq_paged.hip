@@ -316,7 +316,9 @@ __device__ __forceinline__ void decode_piece(const DecodePagedParams& p, DecodeL
     for (int i = 0; i < 8; ++i) {
       const float e = exp2_fast(sc[i] - base);
       l += e;
-      w[i] = (f16)e;  // the weights' one rounding below 32 bits
+      // the weights' one rounding below 32 bits, for products in fp16 (a second product
+      // with what is left of them is NaN where v is infinite and nothing is left)
+      w[i] = (f16)e;
     }
 #pragma unroll
     for (int e = 0; e < DPL / 2; ++e) {

@@ -500,7 +500,10 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
     }
 #pragma unroll
     for (int y = 0; y < KT / 16; ++y) {
-      f16x8 w;  // the weights' one rounding below 32 bits
+      // The weights' one rounding below 32 bits: the products take fp16, and a second one
+      // with what is left of the weights would be half as many again, and NaN where v is
+      // infinite and nothing is left.
+      f16x8 w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = (f16)sc[y / 2][8 * (y % 2) + i];
 #pragma unroll

@@ -406,15 +406,19 @@ aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const
                                    int64_t q_out_stride);
 
 /* Attention over packed prompts: out = softmax(scale q k^T) v per sequence and
- * query head (key head h / (heads_q / heads_kv)), the softmax as in
- * aexq_attention_decode.  Sequence s has query rows q_offsets[s] ..
- * q_offsets[s + 1] - 1 and key rows kv_offsets[s] .. kv_offsets[s + 1] - 1
- * (device int32 [sequences + 1]; NULL kv_offsets: the same).  causal: the
- * queries are the sequence's last positions and see those up to their own.  A
- * row that sees no position is 0; what a row does not see does not reach it,
- * infinities and NaN in k or v included.  Rows behind the last sequence are not
- * touched.  scale is above 0 and at most 2.35e38 (here and below); scores past
- * fp32's range count as infinite.  Uses the context's scratch. */
+ * query head (key head h / (heads_q / heads_kv)).  Sequence s has query rows
+ * q_offsets[s] .. q_offsets[s + 1] - 1 and key rows kv_offsets[s] ..
+ * kv_offsets[s + 1] - 1 (device int32 [sequences + 1]; NULL kv_offsets: the
+ * same).  causal: the queries are the sequence's last positions and see those up
+ * to their own.  A row that sees no position is 0; what a row does not see does
+ * not reach it, infinities and NaN in k or v included.  Rows behind the last
+ * sequence are not touched.  tokens and kv_tokens are 1 or more.  scale is above
+ * 0 and at most 2.35e38.  Uses the context's scratch.
+ * Scores, maxima and sums are fp32 (scores past its range infinite).  Unlike in
+ * aexq_attention_decode a weight is rounded to fp16 for its product with v: by
+ * 2^-11 of it, below 2^-21 of the row's largest weight by 2^-32 of that one.  An
+ * infinity in a v that a row sees is that infinity in the row's output while its
+ * weight is 2^-31 of the largest or more, and that or a NaN below. */
 aexq_status aexq_attention_prompt(aexq_ctx* ctx, const void* q, int64_t q_stride, const void* k,
                                   int64_t k_stride, const void* v, int64_t v_stride,
                                   const int32_t* q_offsets, const int32_t* kv_offsets,
@@ -430,9 +434,10 @@ aexq_status aexq_attention_prompt_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, 
                                         int heads_q, float scale, void* out, int64_t out_stride);
 
 /* aexq_attention_decode for every sequence of a paged cache: row s of q attends
- * over the lengths[s] positions of sequence s; no position, a zero row.  Uses
- * the context's scratch (launches on one context run in stream order, replays of
- * graphs captured from it included). */
+ * over the lengths[s] positions of sequence s; no position, a zero row.  Scale,
+ * weights and infinities as in aexq_attention_prompt.  Uses the context's scratch
+ * (launches on one context run in stream order, replays of graphs captured from it
+ * included). */
 aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const void* q,
                                         int64_t q_stride, int heads_q, float scale, void* out,
                                         int64_t out_stride);

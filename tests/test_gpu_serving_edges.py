@@ -105,3 +105,91 @@ def test_decode_scratch_of_a_large_batch(aexq):
         ref.check_attention(out[s:s + 1], *ref.attend(q[s:s + 1], ref.gather(k, table, s, lens[s]),
                                                       ref.gather(v, table, s, lens[s]), 0.09, False))
     own.close()
+
+
+# ---------------------------------------------------------------- infinities and NaN
+
+def _check_exactly(got, want, mass):
+    """ref.check_attention, and NaN where NaN is due, infinities of the due sign."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN elsewhere"
+    for sign in (INF, -INF):
+        assert torch.equal(got == sign, want == sign), f"{sign} elsewhere"
+    ref.check_attention(got, want, mass)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+def test_prompt_odd_values_exactly(ctx, d, bad):
+    """An infinity or a NaN in v: in rows of tiles that are seen in part and whole,
+    both signs in one dim, in the last position."""
+    print(f"[gpu-case] prompt odd values exactly {bad} d={d}", flush=True)
+    n, hq, hkv = 330, 4, 2
+    q, k, v = _randn(n, hq, d, seed=1), _randn(n, hkv, d, seed=2), _randn(n, hkv, d, seed=3)
+    v[20, 0, 5] = bad
+    v[90, 0, 5] = -bad
+    v[130, 1, d - 1] = bad
+    v[n - 1, 0, 0] = bad
+    for causal in (True, False):
+        out = torch.zeros_like(q)
+        ctx.attention_prompt(q, k, v, ref.offsets([n]), 0.06, out, causal=causal)
+        torch.cuda.synchronize()
+        _check_exactly(out, *ref.attend(q, k, v, 0.06, causal))
+
+
+@pytest.mark.parametrize("n", [70, 500, 3000])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("bad", [INF, -INF, NAN])
+def test_decode_odd_values_exactly(aexq, ctx, n, d, bad):
+    """The same in paged decode, whole and cut; rows past the end hold NaN."""
+    print(f"[gpu-case] decode odd values exactly {bad} n={n} d={d}", flush=True)
+    hq, hkv, page = 8, 2, 64
+    k, v, table, lengths = ref.make_cache([n, 40], hkv, page, d, 6, fill=NAN)
+    for x, h, e, y in ((20, 0, 5, bad), (60, 0, 5, -bad), (n - 1, 1, d - 1, bad), (3, 1, 0, bad)):
+        v[table[0, x // page], h, x % page, e] = y
+    q = _randn(2, hq, d, seed=1)
+    out = torch.zeros_like(q)
+    ctx.attention_decode_paged(aexq.paged_kv(k, v, table, lengths), q, 0.06, out)
+    torch.cuda.synchronize()
+    for s, m in enumerate((n, 40)):
+        _check_exactly(out[s:s + 1], *ref.attend(q[s:s + 1], ref.gather(k, table, s, m),
+                                                 ref.gather(v, table, s, m), 0.06, False))
+
+
+@pytest.mark.parametrize("bits", [20.0, 28.0, 30.5, 40.0, 200.0])
+@pytest.mark.parametrize("form", ["prompt", "paged prompt", "decode", "cut decode"])
+def test_infinities_of_little_weight(aexq, ctx, form, bits):
+    """An infinite v whose weight is 2^-bits of the row's largest: that infinity down to
+    2^-31, there or NaN below (weights are fp16); all else of the row as ever.  The
+    largest weight before the infinity and behind it."""
+    print(f"[gpu-case] {form}, infinity of weight 2^-{bits}", flush=True)
+    n, hq, hkv, d, page = 3000 if form == "cut decode" else 400, 4, 2, 128, 64
+    for at, peak in ((70, 0), (200, 0), (70, 300)):
+        k, v, table, lengths = ref.make_cache([n], hkv, page, d, 6)
+        k[..., 0] = -3.0   # the other positions weigh 2^-3 of the largest
+        k[..., 1:] = 0.0
+        for x, y in ((at, -bits), (peak, 0.0)):
+            k[table[0, x // page], :, x % page, 0] = y
+        v[table[0, at // page], 0, at % page, 7] = INF
+        v[table[0, at // page], 1, at % page, 9] = -INF
+        kk, vv = ref.gather(k, table, 0, n), ref.gather(v, table, 0, n)
+        rows = 1 if "decode" in form else n
+        q = torch.zeros((rows, hq, d), dtype=torch.float16, device="cuda")
+        q[:, :, 0] = 1.0
+        out, scale = torch.zeros_like(q), math.log(2.0)
+        kv, off = aexq.paged_kv(k, v, table, lengths), ref.offsets([rows])
+        if "decode" in form:
+            ctx.attention_decode_paged(kv, q, scale, out)
+        elif form == "prompt":
+            ctx.attention_prompt(q, kk.contiguous(), vv.contiguous(), off, scale, out)
+        else:
+            ctx.attention_prompt_paged(kv, q, off, scale, out)
+        torch.cuda.synchronize()
+        want, mass = ref.attend(q, kk, vv, scale, True)
+        if bits > 31:
+            # the rows that see both the infinity and a larger weight: others are sure
+            last = torch.arange(n - rows, n, device="cuda")
+            loose = torch.isinf(want) & (last >= min(at, peak))[:, None, None]
+            assert not torch.isfinite(out[loose]).any()
+            assert (torch.isnan(out) | (out.double() == want))[loose].all()
+            out = torch.where(loose, want.half(), out)
+        _check_exactly(out, want, mass)
