@@ -193,3 +193,153 @@ def test_infinities_of_little_weight(aexq, ctx, form, bits):
             assert (torch.isnan(out) | (out.double() == want))[loose].all()
             out = torch.where(loose, want.half(), out)
         _check_exactly(out, want, mass)
+
+
+# ---------------------------------------------------------------- forms of large calls
+
+def _few_tokens(n):
+    """0 to 2 new tokens of each of n sequences, none around every 64th."""
+    new = [(i * 7 + 1) % 3 for i in range(n)]
+    for b in range(64, n + 1, 64):
+        new[b - 1] = 0
+        if b < n:
+            new[b] = 0
+    if n % 64:
+        new[-1] = 2
+    return new
+
+
+APPENDS = [([1024], [0]), ([1025], [7]), ([700, 0, 801], [40, 3, 0]), ([2, 1101, 200], [5, 0, 300])] + [
+    (_few_tokens(n), [(5 * i) % 23 for i in range(n)]) for n in (64, 65, 130, 600)]
+
+
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+@pytest.mark.parametrize("d,rot,sections,interleaved,hq,hkv", [
+    (128, 128, [64], False, 6, 2), (256, 64, [12, 10, 10], True, 4, 1), (64, 48, [8, 16], False, 9, 3)])
+def test_append_of_many_tokens_and_sequences(aexq, ctx, case, d, rot, sections, interleaved, hq,
+                                             hkv):
+    """More tokens than a workgroup for each takes, not in fours, and more sequences
+    than a wave looks through at a time; apart and in place."""
+    new, past = APPENDS[case]
+    print(f"[gpu-case] append of {sum(new)} tokens of {len(new)} sequences d={d}", flush=True)
+    page, lens = 32, [a + b for a, b in zip(new, past)]
+    k, v, table, lengths = ref.make_cache(lens, hkv, page, d, 4)
+    live, rows = sum(new), 500
+    n = live + 3
+    q, kn, vn = _randn(n, hq, d, seed=1), _randn(n, hkv, d, seed=2), _randn(n, hkv, d, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    angle = torch.rand((rows, rot // 2), generator=g, device="cuda") * 6.28
+    cos, sin = torch.cos(angle), torch.sin(angle)
+    pos = torch.randint(-3, rows + 5, (len(sections), n), generator=g, device="cuda",
+                        dtype=torch.int32)
+    rope = aexq.rope(cos, sin, pos, sections=sections, interleaved=interleaved)
+    kv, off, out = aexq.paged_kv(k, v, table, lengths), ref.offsets(new), torch.full_like(q, 7.0)
+    kb, vb = k.clone(), v.clone()
+    ctx.rope_append_paged(kv, rope, off, q, kn, vn, out)
+    torch.cuda.synchronize()
+    axis, at = ref.axis_of_pair(rot // 2, sections, interleaved), pos.clamp(0, rows - 1)
+    want, near = ref.rotate(q, cos, sin, at, axis)
+    assert ((out.double() - want).abs() <= near)[:live].all()
+    assert torch.equal(out[:live, :, rot:], q[:live, :, rot:]) and (out[live:] == 7).all()
+    # where each token's rows are
+    x = torch.cat([torch.arange(b, b + a) for a, b in zip(new, past)])
+    s = torch.repeat_interleave(torch.arange(len(new)), torch.tensor(new))
+    ids, row = table.cpu()[s, x // page].long().cuda(), (x % page).cuda()
+    want, near = ref.rotate(kn, cos, sin, at, axis)
+    assert ((k[ids, :, row].double() - want[:live]).abs() <= near[:live]).all()
+    kb[ids, :, row], vb[ids, :, row] = k[ids, :, row], vn[:live]
+    assert torch.equal(k, kb) and torch.equal(v, vb)  # the appended rows, and no others
+    buf = torch.cat([q, kn, vn], 1).contiguous()
+    views = buf.split([hq, hkv, hkv], 1)
+    ctx.rope_append_paged(kv, rope, off, *views, views[0])
+    torch.cuda.synchronize()
+    assert torch.equal(views[0][:live], out[:live]) and torch.equal(views[0][live:], q[live:])
+    assert torch.equal(views[1], kn) and torch.equal(views[2], vn)
+    assert torch.equal(k, kb) and torch.equal(v, vb)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_prompt_layout_of_many_sequences(aexq, ctx, paged):
+    """A layout of more sequences, and of more tiles, than it has threads, with long
+    sequences that are cut among them."""
+    print(f"[gpu-case] layout of 1500 sequences, paged={paged}", flush=True)
+    lens = [(7 * i) % 9 for i in range(1500)]
+    long = {3: 700, 1023: 300, 1024: 5000, 1490: 1300}
+    for s, m in long.items():
+        lens[s] = m
+    n, hq, hkv, d, page = sum(lens), 4, 2, 64, 64
+    q, off = _randn(n, hq, d, seed=1), ref.offsets(lens)
+    out = torch.full_like(q, 7.0)
+    if paged:
+        kp, vp, table, lengths = ref.make_cache(lens, hkv, page, d, 6, fill=NAN)
+        ctx.attention_prompt_paged(aexq.paged_kv(kp, vp, table, lengths), q, off, 0.125, out)
+    else:
+        k, v = _randn(n, hkv, d, seed=2), _randn(n, hkv, d, seed=3)
+        ctx.attention_prompt(q, k, v, off, 0.125, out)
+    torch.cuda.synchronize()
+    at = off.tolist()
+    assert torch.isfinite(out).all() and not (out == 7).all(-1).any()
+    for s in sorted(set(list(long) + list(range(1000, 1050)) + list(range(5, 1500, 31)) + [1499])):
+        a, m = slice(at[s], at[s + 1]), lens[s]
+        kk, vv = ((ref.gather(kp, table, s, m), ref.gather(vp, table, s, m)) if paged
+                  else (k[a], v[a]))
+        ref.check_attention(out[a], *ref.attend(q[a], kk, vv, 0.125, True))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("short,long,hq,hkv,d", [(2200, 3000, 4, 2, 64), (2, 5000, 64, 1, 128),
+                                                 (2100, 2500, 4, 2, 256)])
+def test_prompts_of_more_tiles_than_a_layout_takes(ctx, short, long, hq, hkv, d, causal):
+    """Without a layout: sequences of several tiles of keys among many of a few tokens."""
+    print(f"[gpu-case] {short} short prompts and one of {long}, {hq}/{hkv} d={d}", flush=True)
+    lens = [(5 * i) % 4 for i in range(short)]
+    lens.insert(short // 2, long)
+    n = sum(lens)
+    q, k, v = _randn(n, hq, d, seed=1), _randn(n, hkv, d, seed=2), _randn(n, hkv, d, seed=3)
+    off, out, scale = ref.offsets(lens), torch.full_like(q, 7.0), 1.0 / math.sqrt(d)
+    ctx.attention_prompt(q, k, v, off, scale, out, causal=causal)
+    torch.cuda.synchronize()
+    at = off.tolist()
+    assert torch.isfinite(out).all()
+    for s in list(range(0, short, max(1, short // 40))) + [short]:
+        if s != short // 2:
+            a = slice(at[s], at[s + 1])
+            ref.check_attention(out[a], *ref.attend(q[a], k[a], v[a], scale, causal))
+    first, end = at[short // 2], at[short // 2 + 1]
+    for b in (1, 130, long // 2, long):  # rows of the long one, heads at the ends of groups
+        a = slice(first + max(0, b - 70), first + b)
+        heads = sorted({0, hq - 1})
+        kk, vv = (t[first:first + b if causal else end][:, [h // (hq // hkv) for h in heads]]
+                  for t in (k, v))
+        ref.check_attention(out[a][:, heads], *ref.attend(q[a][:, heads], kk, vv, scale, causal))
+
+
+@pytest.mark.parametrize("dtype,rows,n", [
+    (torch.float32, 450, 150001), (torch.float32, 600, 120003), (torch.float16, 900, 150001),
+    (torch.float16, 500, 270001)])
+def test_logprobs_of_more_than_the_caches_hold(aexq, ctx, dtype, rows, n):
+    """Logits read past the caches, in one part a row and in two, rows that start
+    anywhere in a 16-byte chunk."""
+    print(f"[gpu-case] logprobs {rows} x {n} {dtype}, past the caches", flush=True)
+    top = 20
+    g = torch.Generator(device="cuda").manual_seed(n + rows)
+    x = 3 * torch.randn((rows, n), generator=g, device="cuda", dtype=dtype)
+    assert x.numel() * x.element_size() > 256 << 20
+    x[:, 100:140] = -INF
+    x[rows - 1] = torch.floor(x[rows - 1])  # many equal ones
+    tokens = torch.randint(0, n, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    tokens[0] = 120
+    lp, ent, val = (torch.full(s, 7.0, device="cuda") for s in ((rows,), (rows,), (rows, top)))
+    ids = torch.full((rows, top), 7, dtype=torch.int32, device="cuda")
+    ctx.logprobs(aexq.describe(x, rows, n), tokens, lp, ent, ids, val)
+    torch.cuda.synchronize()
+    # the bound of test_gpu_logprobs.py: n / 256 sums of a lane, one after the other
+    eps = (n / 256 + 64) * 2.0 ** -24
+    for a in list(range(0, rows - 1, 61)) + [rows - 1]:
+        want = ref.logprobs(x[a:a + 1], tokens[a:a + 1], top)
+        assert torch.equal(ids[a:a + 1], want[2])
+        for got, w in ((lp[a:a + 1], want[0]), (val[a:a + 1], want[3])):
+            assert torch.equal(torch.isneginf(got.double()), torch.isneginf(w))
+            near = (got.double() - w).abs() <= eps + 2.0 ** -22 * w.abs()
+            assert (near | torch.isneginf(w)).all()
+        assert ((ent[a:a + 1].double() - want[1]).abs() <= 2 * eps * (1 + want[1].abs())).all()
