@@ -343,3 +343,51 @@ def test_logprobs_of_more_than_the_caches_hold(aexq, ctx, dtype, rows, n):
             near = (got.double() - w).abs() <= eps + 2.0 ** -22 * w.abs()
             assert (near | torch.isneginf(w)).all()
         assert ((ent[a:a + 1].double() - want[1]).abs() <= 2 * eps * (1 + want[1].abs())).all()
+
+
+def test_logits_past_32_bit_offsets(aexq, ctx):
+    """Rows whose logits lie past 2^31 elements and 2^32 bytes."""
+    print("[gpu-case] logprobs of more than 2^31 logits", flush=True)
+    n, top = 151937, 5
+    rows = (1 << 31) // n + 9
+    x = torch.zeros((rows, n), dtype=torch.float16, device="cuda")
+    picked = [0, rows // 2, rows - 9, rows - 1]
+    for i, r in enumerate(picked):
+        x[r] = _randn(n, seed=i)
+    tokens = torch.arange(rows, dtype=torch.int32, device="cuda") % n
+    lp, ent, val = (torch.full(s, 7.0, device="cuda") for s in ((rows,), (rows,), (rows, top)))
+    ids = torch.full((rows, top), 7, dtype=torch.int32, device="cuda")
+    ctx.logprobs(aexq.describe(x, rows, n), tokens, lp, ent, ids, val)
+    torch.cuda.synchronize()
+    eps = (n / 256 + 64) * 2.0 ** -24
+    for r in picked + [rows - 2]:
+        want = ref.logprobs(x[r:r + 1], tokens[r:r + 1], top)
+        assert torch.equal(ids[r:r + 1], want[2])
+        for got, w in ((lp[r:r + 1], want[0]), (val[r:r + 1], want[3])):
+            assert ((got.double() - w).abs() <= eps + 2.0 ** -22 * w.abs()).all()
+        assert ((ent[r:r + 1].double() - want[1]).abs() <= 2 * eps * (1 + want[1].abs())).all()
+
+
+@pytest.mark.parametrize("form", ["decode", "cut decode", "paged prompt"])
+def test_rows_that_are_views(aexq, ctx, form):
+    """q and out as views into wider buffers: what lies beside them stays."""
+    print(f"[gpu-case] {form} of views", flush=True)
+    lens = [2500, 0, 700] if form == "cut decode" else [300, 0, 41]
+    hq, hkv, d = 12, 2, 128
+    k, v, table, lengths = ref.make_cache(lens, hkv, 64, d, 6, fill=NAN)
+    kv, new = aexq.paged_kv(k, v, table, lengths), [1, 1, 1] if "decode" in form else [20, 2, 41]
+    n = sum(new)
+    wide_q = _randn(n, hq + 4, d, seed=1)
+    wide = torch.full((n, hq + 6, d), 7.0, dtype=torch.float16, device="cuda")
+    q, out = wide_q[:, 3:hq + 3], wide[:, 2:hq + 2]
+    if "decode" in form:
+        ctx.attention_decode_paged(kv, q, 0.09, out)
+    else:
+        ctx.attention_prompt_paged(kv, q, ref.offsets(new), 0.09, out)
+    torch.cuda.synchronize()
+    at = ref.offsets(new).tolist()
+    for s, m in enumerate(lens):
+        a = slice(at[s], at[s + 1])
+        _check_exactly(out[a], *ref.attend(q[a], ref.gather(k, table, s, m),
+                                           ref.gather(v, table, s, m), 0.09, True))
+    assert (wide[:, :2] == 7).all() and (wide[:, hq + 2:] == 7).all()
