@@ -394,11 +394,11 @@ typedef struct aexq_rope {
 /* aexq_rope_kv_append for packed tokens of many sequences: the new tokens of
  * sequence s are rows offsets[s] .. offsets[s + 1] - 1 (device int32
  * [sequences + 1], not decreasing) and become its last positions, the ones
- * before lengths[s].  q is rotated into q_out (which may be q, rows as far apart), k
- * rotated and v copied into their pages.  A position outside the table, or whose page entry
- * lies outside the pool, is not stored.  Rows behind the last sequence are not
- * touched.  Two tokens that name the same cache row in one call leave either's
- * values, piece by piece. */
+ * before lengths[s].  tokens is 1 to 2^23.  q is rotated into q_out (which may be
+ * q, rows as far apart), k rotated and v copied into their pages.  A position
+ * outside the table, or whose page entry lies outside the pool, is not stored.
+ * Rows behind the last sequence are not touched.  Two tokens that name the same
+ * cache row in one call leave either's values, piece by piece. */
 aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const aexq_rope* rope,
                                    const int32_t* offsets, int tokens, int heads_q, const void* q,
                                    int64_t q_stride, const void* k, int64_t k_stride,
@@ -412,8 +412,9 @@ aexq_status aexq_rope_append_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, const
  * same).  causal: the queries are the sequence's last positions and see those up
  * to their own.  A row that sees no position is 0; what a row does not see does
  * not reach it, infinities and NaN in k or v included.  Rows behind the last
- * sequence are not touched.  tokens and kv_tokens are 1 or more.  scale is above
- * 0 and at most 2.35e38.  Uses the context's scratch.
+ * sequence are not touched.  tokens and kv_tokens are 1 or more, and tokens *
+ * (heads_q / heads_kv) / 128 + sequences is at most 65535.  scale is above 0 and
+ * at most 2.35e38.  Uses the context's scratch.
  * Scores, maxima and sums are fp32 (scores past its range infinite).  Unlike in
  * aexq_attention_decode a weight is rounded to fp16 for its product with v: by
  * 2^-11 of it, below 2^-21 of the row's largest weight by 2^-32 of that one.  An
@@ -442,7 +443,7 @@ aexq_status aexq_attention_decode_paged(aexq_ctx* ctx, const aexq_paged_kv* kv, 
                                         int64_t q_stride, int heads_q, float scale, void* out,
                                         int64_t out_stride);
 
-/* Log probabilities over rows of fp32 or fp16 logits (not head-packed):
+/* Log probabilities over up to 2^23 rows of fp32 or fp16 logits (not head-packed):
  * logprob[r] (nullable) of token tokens[r] (device int32; 0 for token -1, NaN
  * for another one outside the row), entropy[r] (nullable, nats), and the `top`
  * (0 to 64) largest logits of the row, equal ones by the lower index: top_ids
