@@ -383,7 +383,7 @@ __device__ __forceinline__ void decode_piece(const DecodePagedParams& p, DecodeL
         const float inv = 1.0f / sum;
         f16x4 b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = (f16)(a[e] * inv);
+        for (int e = 0; e < 4; ++e) b[e] = average_f16(a[e] * inv);
         *(f16x4*)(p.out + (long long)s * p.out_stride + (h * p.group + first + q) * D + dim) = b;
       }
     }
@@ -579,7 +579,7 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
   const float inv = 1.0f / l;
   f16x4 v;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = (f16)(acc[e] * inv);
+  for (int e = 0; e < 4; ++e) v[e] = average_f16(acc[e] * inv);
   *(f16x4*)(out + 4 * y) = v;
 }
 

@@ -31,6 +31,12 @@ constexpr float kLift = 7.0f, kLag = 8.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// An output in fp16.  An average of finite fp16 values is within them; the weights'
+// rounding may take it up to 2^-11 further, past 65520, where fp16 rounds to infinity.
+__device__ __forceinline__ f16 average_f16(float y) {
+  return (f16)(fabsf(y) < INFINITY ? fminf(fmaxf(y, -65504.0f), 65504.0f) : y);
+}
+
 // Maximum (sum) of v over the four 16-lane rows of the wave, in every lane.
 __device__ __forceinline__ float rows_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, 64));

@@ -612,8 +612,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void prompt_kernel(const
       f16x4 a, b;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        a[e] = (f16)(o[i][4 * r + e] * inv);
-        b[e] = (f16)(o[i][4 * r + 4 + e] * inv);
+        a[e] = average_f16(o[i][4 * r + e] * inv);
+        b[e] = average_f16(o[i][4 * r + 4 + e] * inv);
       }
       const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
       const auto u = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);

@@ -391,3 +391,35 @@ def test_rows_that_are_views(aexq, ctx, form):
         _check_exactly(out[a], *ref.attend(q[a], ref.gather(k, table, s, m),
                                            ref.gather(v, table, s, m), 0.09, True))
     assert (wide[:, :2] == 7).all() and (wide[:, hq + 2:] == 7).all()
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("form", ["prompt", "paged prompt", "decode", "cut decode"])
+def test_finite_values_stay_finite(aexq, ctx, form, d):
+    """v of the type's largest magnitude: an average of 65504s is 65504, also where the
+    weights' rounding to fp16 adds up.  Scores of -(1 - 2^-10) in log2 units, every 32nd
+    of 0: weights of 64.043 in the kernels' scale, rounded to 64.0625, 3.0e-4 more than
+    they are, and 31 to every one of 128: 2.8e-4 more in all, which takes 65504 past
+    65520, where fp16 rounds to infinity."""
+    print(f"[gpu-case] {form} of the largest values d={d}", flush=True)
+    n, hq, hkv, page = 3000 if form == "cut decode" else 460, 4, 2, 64
+    k, v, table, lengths = ref.make_cache([n], hkv, page, d, 6)
+    k[..., 0] = -(1 - 2.0 ** -10)
+    k[..., 1:] = 0.0
+    k[:, :, ::32, 0] = 0.0
+    v[:] = 65504.0
+    v[..., 1::2] = -65504.0
+    kk, vv = ref.gather(k, table, 0, n), ref.gather(v, table, 0, n)
+    rows = 1 if "decode" in form else n
+    q = torch.zeros((rows, hq, d), dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    out, scale = torch.zeros_like(q), math.log(2.0)
+    kv, off = aexq.paged_kv(k, v, table, lengths), ref.offsets([rows])
+    if "decode" in form:
+        ctx.attention_decode_paged(kv, q, scale, out)
+    elif form == "prompt":
+        ctx.attention_prompt(q, kk.contiguous(), vv.contiguous(), off, scale, out)
+    else:
+        ctx.attention_prompt_paged(kv, q, off, scale, out)
+    torch.cuda.synchronize()
+    _check_exactly(out, *ref.attend(q, kk, vv, scale, True))
