@@ -28,11 +28,13 @@ namespace aexq {
 //                 (ds_read_b64_tr_b16), 4 positions of 16 dims per 16 lanes.
 // So scores, weights, maximum and sum of a row never leave its two lanes.
 //
-// What bounds it: the matrix instructions at the clock that their power leaves.
-// 16384 causal tokens of 32/8 heads of 128 take 2040 us (1.08 PFLOP/s; the matrix
-// units busy 61% of the time, at 1.66 GHz), 8192 of 16/4 heads 290 us (940 TFLOP/s;
-// 64 wide 177 and 256 wide 760 us).  4 x 512 tokens after 6143 take 231 us; the same
-// products alone, without reads, exponentials and loads, 191.  Exponentials put
+// What bounds it: the matrix instructions, and what the two waves of a SIMD do not
+// cover for each other.  16384 causal tokens of 32/8 heads of 128 take 2015 to 2064 us
+// (1.07 PFLOP/s): the matrix units are busy 61% of the time, at 1.66 GHz, where
+// products and nothing else keep them busy at 1.39 GHz, the power's limit (1.45
+// PFLOP/s).  8192 of 16/4 heads take 290 us (940 TFLOP/s; 64 wide 177 and 256 wide 760
+// us).  4 x 512 tokens after 6143 take 231 us; the same products alone, without reads,
+// exponentials and loads, 191.  Exponentials put
 // between the products of the next tile, and loads between products, were no faster
 // for that (254 and 239 us).  Short prompts wait: some 7 us of a workgroup's time go
 // to finding its rows, its first tile, the masked tile and its stores.
