@@ -14,6 +14,7 @@
 
 #include "../../include/aexq.h"
 #include "aexq_internal.hpp"
+#include "aexq_serving.hpp"
 #include "aexq_step.hpp"
 
 using namespace aexq;

@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "aexq_device.hpp"
+#include "aexq_serving.hpp"
 
 namespace aexq {
 

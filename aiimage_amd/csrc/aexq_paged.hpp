@@ -3,6 +3,7 @@
 #pragma once
 
 #include "aexq_dma.hpp"
+#include "aexq_serving.hpp"
 
 namespace aexq {
 

@@ -38,9 +38,8 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 TRAFFIC_FILE = os.path.join(ROOT, "profiles", "qmv_q4_layer_config2_traffic.json")
 # the sources the dominant launch's kernel is compiled from: the traffic record
 # holds their hash, and a record of other sources is not this build's traffic
-KERNEL_SOURCES = ("include/aexq.h", "aiimage_amd/csrc/aexq_internal.hpp",
-                  "aiimage_amd/csrc/aexq_device.hpp", "aiimage_amd/csrc/aexq_qmv.hpp",
-                  "aiimage_amd/csrc/aexq_qmv_q4.hip")
+KERNEL_SOURCES = ("aiimage_amd/csrc/aexq_internal.hpp", "aiimage_amd/csrc/aexq_device.hpp",
+                  "aiimage_amd/csrc/aexq_qmv.hpp", "aiimage_amd/csrc/aexq_qmv_q4.hip")
 LAYER_WEIGHT_BYTES = 9_142_272
 LAYER_ACT_BYTES = 46_080
 LAYER_BYTES = LAYER_WEIGHT_BYTES + LAYER_ACT_BYTES
