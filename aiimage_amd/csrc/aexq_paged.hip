@@ -586,9 +586,9 @@ __global__ __launch_bounds__(kThreads) void decode_paged_join(const DecodePagedP
 // The cut of a launch over up to `bound` positions of each sequence in `blocks`
 // head blocks of sequences: one piece for each `target`-th of all units, so that
 // no more than blocks + target are there.  What is cut has more than one share, and
-// less than two pieces for each: fewer than 2 target of them.  Nothing is cut (target 0) where the
-// steps of a workgroup are few, and where there is a workgroup for every CU whose
-// longest way is not much longer.
+// less than two pieces for each: fewer than 2 target in all.  Nothing is cut (target
+// 0) where the steps of a workgroup are few, and where there is a workgroup for every
+// CU whose longest way is not much longer.
 DecodePlan decode_paged_plan(int head_dim, int cus, long long bound, long long blocks) {
   DecodePlan r;
   r.target = bound <= 512 || (blocks >= cus && bound <= 1024) ? 0 : (head_dim == 256 ? 2 : 3) * cus;
