@@ -137,6 +137,12 @@ class Rope(ctypes.Structure):
                 ("section3", ctypes.c_int)]
 
 
+class Slots(ctypes.Structure):
+    _fields_ = [("slot", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("counts", ctypes.c_void_p), ("count", ctypes.c_int),
+                ("sequences", ctypes.c_int), ("read_only", ctypes.c_int)]
+
+
 _lib = None
 
 
@@ -167,6 +173,8 @@ def _declare(L):
     TP = ctypes.POINTER(Tensor)
     AP = ctypes.POINTER(LinearArgs)
     KP, RP, i64 = ctypes.POINTER(PagedKv), ctypes.POINTER(Rope), ctypes.c_int64
+    SP = ctypes.POINTER(Slots)
+    rows = [P, i64, P, i64, P, i64, P, i64, P, i64, P, P, i32, i32, i32, i32, f32, f32, P, i64]
     sig = {
         "aexq_abi_version": (i32, []),
         "aexq_last_error": (ctypes.c_char_p, []),
@@ -208,6 +216,11 @@ def _declare(L):
         "aexq_attention_prompt_paged": (i32, [P, KP, P, i64, P, i32, i32, f32, P, i64]),
         "aexq_attention_decode_paged": (i32, [P, KP, P, i64, i32, f32, P, i64]),
         "aexq_logprobs": (i32, [P, TP, P, P, P, i32, P, P]),
+        "aexq_short_conv": (i32, [P, SP, P, P, i32, P, i64, P, P, i32, i32, i32, P, i64]),
+        "aexq_delta_prompt": (i32, [P, SP, P, P, i32, *rows]),
+        "aexq_delta_decode": (i32, [P, SP, P, *rows]),
+        "aexq_gated_rmsnorm": (i32, [P, P, i64, P, i64, P, f32, i32, i32, i32, P, i64]),
+        "aexq_verify_drafts": (i32, [P, TP, P, i32, P, P, i64, P, P, P, P, P]),
         "aexq_decoder_create": (i32, [P, ctypes.POINTER(DecoderConfig), ctypes.POINTER(DecoderLayer),
                                       i32, P, PP]),
         "aexq_decoder_run": (i32, [P, P, P, P]),

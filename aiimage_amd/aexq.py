@@ -211,6 +211,42 @@ def rope(cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor]
     return d
 
 
+# ---------------------------------------------------------------- recurrent layers
+
+def slots(count: int, sequences: int, *, slot: Optional[torch.Tensor] = None,
+          lengths: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+          read_only: bool = False) -> _abi.Slots:
+    """aexq_slots of `sequences` sequences whose states lie in pools of `count`.  All
+    [sequences] (int32, read on the device when a launch runs): slot (None: sequence
+    s has slot s), lengths (positions, the call's rows included; a sequence that has
+    no others starts from zeros; None: all go on) and counts (so many of a
+    sequence's rows are taken, the first ones; None: all).  read_only: states are
+    read, not stored."""
+    d, device = _abi.Slots(), None
+    for name, t in (("slot", slot), ("lengths", lengths), ("counts", counts)):
+        if t is None:
+            continue
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            _refuse(f"{name} is not an array on a GPU")
+        device = t.get_device() if device is None else device
+        setattr(d, name, _device_array(t, name, torch.int32, (sequences,), device))
+    d.count, d.sequences, d.read_only = count, sequences, int(read_only)
+    d._keep, d._device = (slot, lengths, counts), device
+    return d
+
+
+def _gate_rows(t: torch.Tensor, name: str, rows: int, heads: int, device: int) -> int:
+    """Row stride in elements of fp16 [rows][heads] whose heads are dense."""
+    if isinstance(t, torch.Tensor) and t.shape == (rows, heads):
+        row, one = t.stride()
+        if (t.dtype is torch.float16 and t.get_device() == device
+                and (one == 1 or heads == 1)):
+            return row if rows > 1 else heads
+    what = (f"{t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}"
+            if isinstance(t, torch.Tensor) else type(t).__name__)
+    _refuse(f"{name} is {what}, not fp16 rows {(rows, heads)} on GPU {device}")
+
+
 # ---------------------------------------------------------------- records
 
 @dataclass
@@ -554,6 +590,134 @@ class Context:
             val = _device_array(top_logprobs, "top_logprobs", torch.float32, (rows, top), device)
         check(self._lib.aexq_logprobs(self.handle, logits, tok, lp, ent, top, ids, val),
               "aexq_logprobs")
+
+    # ---- recurrent layers, drafted tokens
+    def _slots(self, d):
+        if not isinstance(d, _abi.Slots) or d._device not in (None, self.device):
+            _refuse(f"{d!r} is not a Slots of GPU {self.device}'s tensors")
+
+    def short_conv(self, slots: _abi.Slots, state: torch.Tensor, offsets: torch.Tensor,
+                   x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor], *,
+                   bias: Optional[torch.Tensor] = None, silu: bool = True):
+        """Causal convolution of packed rows x [tokens][channels] (fp16) along each
+        sequence, channel by channel, by weight [channels][width] (fp32), into out
+        (None: the states alone).  state [slots][width - 1][channels] (fp16): the
+        inputs before the first row, oldest first."""
+        device = self.device
+        self._slots(slots)
+        if not (isinstance(x, torch.Tensor) and x.dim() == 2):
+            _refuse("x is not [tokens][channels]")
+        if not (isinstance(weight, torch.Tensor) and weight.dim() == 2):
+            _refuse("weight is not [channels][width]")
+        tokens, channels = x.shape
+        width = weight.shape[1]
+        off = _device_array(offsets, "offsets", torch.int32, (slots.sequences + 1,), device)
+        st = _device_array(state, "state", torch.float16, (slots.count, width - 1, channels),
+                           device)
+        w = _device_array(weight, "weight", torch.float32, (channels, width), device)
+        b = None
+        if bias is not None:
+            b = _device_array(bias, "bias", torch.float32, (channels,), device)
+        xs, os_, o = _gate_rows(x, "x", tokens, channels, device), 0, None
+        if out is not None:
+            os_, o = _gate_rows(out, "out", tokens, channels, device), out.data_ptr()
+        check(self._lib.aexq_short_conv(self.handle, slots, st, off, tokens, x.data_ptr(), xs, w, b,
+                                        channels, width, silu, o, os_), "aexq_short_conv")
+
+    def _delta_rows(self, slots, state, q, k, v, a, b, a_log, dt_bias, out, scale, eps):
+        device = self.device
+        self._slots(slots)
+        tokens, heads_k, dim_k = _head_shape(q, "q")
+        _, heads_v, dim_v = _head_shape(v, "v")
+        st = _device_array(state, "state", torch.float32, (slots.count, heads_v, dim_k, dim_v),
+                           device)
+        qs = _head_rows(q, "q", (tokens, heads_k, dim_k), device)
+        ks = _head_rows(k, "k", (tokens, heads_k, dim_k), device)
+        vs = _head_rows(v, "v", (tokens, heads_v, dim_v), device)
+        as_ = _gate_rows(a, "a", tokens, heads_v, device)
+        bs = _gate_rows(b, "b", tokens, heads_v, device)
+        al = _device_array(a_log, "a_log", torch.float32, (heads_v,), device)
+        dt = _device_array(dt_bias, "dt_bias", torch.float32, (heads_v,), device)
+        os_, o = 0, None
+        if out is not None:
+            os_, o = _head_rows(out, "out", (tokens, heads_v, dim_v), device), out.data_ptr()
+        return st, tokens, (q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, a.data_ptr(), as_,
+                            b.data_ptr(), bs, al, dt, heads_k, heads_v, dim_k, dim_v, scale, eps, o,
+                            os_)
+
+    def delta_prompt(self, slots: _abi.Slots, state: torch.Tensor, offsets: torch.Tensor,
+                     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tensor,
+                     b: torch.Tensor, a_log: torch.Tensor, dt_bias: torch.Tensor,
+                     out: Optional[torch.Tensor], *, scale: float, eps: float = 1e-6):
+        """The gated delta rule over packed rows: q, k [tokens][heads_k][dim_k], v, out
+        [tokens][heads_v][dim_v], a, b [tokens][heads_v] (fp16), a_log, dt_bias
+        [heads_v] (fp32), state [slots][heads_v][dim_k][dim_v] (fp32), sequence s in
+        rows offsets[s] .. offsets[s + 1] - 1.  q and k are scaled to unit length; out
+        None: the states alone."""
+        st, tokens, rows = self._delta_rows(slots, state, q, k, v, a, b, a_log, dt_bias, out, scale,
+                                            eps)
+        off = _device_array(offsets, "offsets", torch.int32, (slots.sequences + 1,), self.device)
+        check(self._lib.aexq_delta_prompt(self.handle, slots, st, off, tokens, *rows),
+              "aexq_delta_prompt")
+
+    def delta_decode(self, slots: _abi.Slots, state: torch.Tensor, q: torch.Tensor,
+                     k: torch.Tensor, v: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                     a_log: torch.Tensor, dt_bias: torch.Tensor, out: Optional[torch.Tensor], *,
+                     scale: float, eps: float = 1e-6):
+        """delta_prompt where every sequence has one row: row s is sequence s."""
+        st, tokens, rows = self._delta_rows(slots, state, q, k, v, a, b, a_log, dt_bias, out, scale,
+                                            eps)
+        if tokens != slots.sequences:
+            _refuse(f"{tokens} rows of {slots.sequences} sequences")
+        check(self._lib.aexq_delta_decode(self.handle, slots, st, *rows), "aexq_delta_decode")
+
+    def gated_rmsnorm(self, x: torch.Tensor, z: torch.Tensor, gamma: Optional[torch.Tensor],
+                      out: torch.Tensor, eps: float = 1e-6):
+        """Norm of each head's row times silu(z): x, z, out [tokens][heads][dim] (fp16),
+        gamma [dim] (fp32).  out may be x or z."""
+        device = self.device
+        tokens, heads, dim = _head_shape(x, "x")
+        xs = _head_rows(x, "x", (tokens, heads, dim), device)
+        zs = _head_rows(z, "z", (tokens, heads, dim), device)
+        os_ = _head_rows(out, "out", (tokens, heads, dim), device)
+        gm = None
+        if gamma is not None:
+            gm = _device_array(gamma, "gamma", torch.float32, (dim,), device)
+        check(self._lib.aexq_gated_rmsnorm(self.handle, x.data_ptr(), xs, z.data_ptr(), zs, gm, eps,
+                                           tokens, heads, dim, out.data_ptr(), os_),
+              "aexq_gated_rmsnorm")
+
+    def verify_drafts(self, logits: _abi.Tensor, offsets: torch.Tensor, drafts: torch.Tensor,
+                      accept_u: torch.Tensor, sample_u: torch.Tensor, counts: torch.Tensor,
+                      tokens: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
+                      draft_probs: Optional[torch.Tensor] = None):
+        """Drafted tokens against the target's probabilities: row i of a sequence holds
+        the logits behind its i-th token and in drafts [rows] (int32) the token
+        proposed for there (the last row's is not read); a draft stays while accept_u
+        [rows] times its draft probability (draft_probs [rows][vocab] (fp32); None: 1)
+        is below the target's, the token behind is drawn by sample_u [sequences].
+        temperature [sequences] (fp32; None: 1; 0: the largest logit).  Leaves the rows
+        that stay in counts [sequences] and the tokens in tokens [rows] (int32)."""
+        device, rows = self.device, logits.logical.h
+        if logits._keep.get_device() != device:
+            _refuse(f"the logits are on {logits._keep.device}, not on GPU {device}")
+        n = offsets.numel() - 1 if isinstance(offsets, torch.Tensor) else 0
+        f32, i32 = torch.float32, torch.int32
+        off = _device_array(offsets, "offsets", i32, (n + 1,), device)
+        dr = _device_array(drafts, "drafts", i32, (rows,), device)
+        au = _device_array(accept_u, "accept_u", f32, (rows,), device)
+        su = _device_array(sample_u, "sample_u", f32, (n,), device)
+        ct = _device_array(counts, "counts", i32, (n,), device)
+        tk = _device_array(tokens, "tokens", i32, (rows,), device)
+        heat = probs = None
+        stride = 0
+        if temperature is not None:
+            heat = _device_array(temperature, "temperature", f32, (n,), device)
+        if draft_probs is not None:
+            probs = _device_array(draft_probs, "draft_probs", f32, (rows, logits.logical.w), device)
+            stride = logits.logical.w
+        check(self._lib.aexq_verify_drafts(self.handle, logits, off, n, dr, probs, stride, heat, au,
+                                           su, ct, tk), "aexq_verify_drafts")
 
     def decoder(self, layers, embedding: "QuantWeight", heads_q: int, heads_kv: int,
                 head_dim: int, capacity: int, rms_eps: float, attn_scale: float,

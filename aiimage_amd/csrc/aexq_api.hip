@@ -14,6 +14,7 @@
 
 #include "../../include/aexq.h"
 #include "aexq_internal.hpp"
+#include "aexq_recurrent.hpp"
 #include "aexq_serving.hpp"
 #include "aexq_step.hpp"
 
@@ -80,6 +81,9 @@ struct aexq_ctx {
   long long logprob_stats_cap = 0;
   unsigned long long* logprob_keys = nullptr;
   long long logprob_keys_cap = 0;
+  // per part of a row of drafted tokens: sums of weights, and what was decided
+  void* verify_mem = nullptr;
+  long long verify_cap = 0;
   // split-K partial planes of the MFMA kernels
   float* sk_part = nullptr;
   long long sk_cap = 0;
@@ -219,6 +223,7 @@ extern "C" void aexq_destroy(aexq_ctx* ctx) {
   (void)hipFree(ctx->prompt_part);
   (void)hipFree(ctx->logprob_stats);
   (void)hipFree(ctx->logprob_keys);
+  (void)hipFree(ctx->verify_mem);
   (void)hipFree(ctx->sk_part);
   (void)hipFree(ctx->am_tagged);
   (void)hipFree(ctx->am_epoch);
@@ -2395,6 +2400,285 @@ extern "C" aexq_status aexq_logprobs(aexq_ctx* ctx, const aexq_tensor* logits,
   }
   const hipError_t e = logprob_launch(p, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "log probability launch");
+  return AEXQ_OK;
+}
+
+// ---------------------------------------------------------------------------
+// recurrent layers, drafted tokens
+// ---------------------------------------------------------------------------
+// The sequences and states of a call as the kernels take them.
+static aexq_status view_slots(const aexq_slots* s, const char* op, const void* state,
+                              SlotsView* v) {
+  if (!s) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "slots is NULL");
+  if (!state) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "state is NULL");
+  if (s->count <= 0 || s->sequences <= 0)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "count=%d sequences=%d", s->count, s->sequences);
+  if (s->sequences > 65535)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "sequences=%d (at most 65535)", s->sequences);
+  if ((uintptr_t)state % 16)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "state not 16-byte aligned");
+  v->slot = s->slot;
+  v->lengths = s->lengths;
+  v->counts = s->counts;
+  v->count = s->count;
+  v->n = s->sequences;
+  v->store = !s->read_only;
+  return AEXQ_OK;
+}
+
+static aexq_status check_tokens(const char* op, const int32_t* offsets, int tokens) {
+  if (!offsets) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "offsets is NULL");
+  if (tokens <= 0 || tokens > 1 << 23)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens=%d (1 to 2^23)", tokens);
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
+                                       const int32_t* offsets, int tokens, const void* x,
+                                       int64_t x_stride, const float* weight, const float* bias,
+                                       int channels, int width, int silu, void* out,
+                                       int64_t out_stride) {
+  const char* op = "aexq_short_conv";
+  if (!ctx || !weight) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  ShortConvParams p{};
+  aexq_status st = view_slots(slots, op, state, &p.slots);
+  if (!st) st = check_tokens(op, offsets, tokens);
+  if (st) return st;
+  if (channels <= 0 || channels % 8 || channels > 1 << 20)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "channels=%d (a multiple of 8, at most 2^20)", channels);
+  if (width < 2 || width > 5) return fail(AEXQ_ERR_UNSUPPORTED, op, "width=%d (2 to 5)", width);
+  st = check_rows(op, "x", x, x_stride, 1, channels);
+  if (!st && out) st = check_rows(op, "out", out, out_stride, 1, channels);
+  if (!st && out == x)
+    st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is x, which other workgroups still read");
+  if (st) return st;
+  p.state = (_Float16*)state;
+  p.offsets = offsets;
+  p.tokens = tokens;
+  p.channels = channels;
+  p.width = width;
+  p.silu = silu != 0;
+  p.x = (const _Float16*)x;
+  p.out = (_Float16*)out;
+  p.x_stride = x_stride;
+  p.out_stride = out_stride;
+  p.weight = weight;
+  p.bias = bias;
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = short_conv_launch(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "convolution launch");
+  return AEXQ_OK;
+}
+
+// The arguments that both forms of the delta rule take, but the sequences'.
+static aexq_status view_delta(const char* op, const void* q, int64_t q_stride, const void* k,
+                              int64_t k_stride, const void* v, int64_t v_stride, const void* a,
+                              int64_t a_stride, const void* b, int64_t b_stride,
+                              const float* a_log, const float* dt_bias, int heads_k, int heads_v,
+                              int dim_k, int dim_v, float scale, float eps, void* out,
+                              int64_t out_stride, DeltaParams* p) {
+  if (!a || !b || !a_log || !dt_bias)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  if (dim_k != 64 && dim_k != 128)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "dim_k=%d (64 or 128)", dim_k);
+  if (!is_head_dim(dim_v))
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "dim_v=%d (64, 128 or 256)", dim_v);
+  aexq_status st = check_heads(op, heads_v, heads_k, 1.0f);
+  if (st) return st;
+  if (!(eps > 0.0f) || !(eps < INFINITY) || !(fabsf(scale) < INFINITY))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "eps=%g (above 0) scale=%g (finite)", (double)eps,
+                (double)scale);
+  st = check_rows(op, "q", q, q_stride, heads_k, dim_k);
+  if (!st) st = check_rows(op, "k", k, k_stride, heads_k, dim_k);
+  if (!st) st = check_rows(op, "v", v, v_stride, heads_v, dim_v);
+  if (!st && out) st = check_rows(op, "out", out, out_stride, heads_v, dim_v);
+  if (st) return st;
+  if (out && (out == q || out == k || out == v))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is an input that other workgroups still read");
+  if (a_stride < heads_v || b_stride < heads_v || a_stride > 1 << 24 || b_stride > 1 << 24)
+    return fail(AEXQ_ERR_SHAPE, op, "a, b rows %lld, %lld elements apart hold %d heads (at most 2^24)",
+                (long long)a_stride, (long long)b_stride, heads_v);
+  if ((uintptr_t)a % 2 || (uintptr_t)b % 2)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "a, b not 2-byte aligned");
+  p->q = (const _Float16*)q;
+  p->k = (const _Float16*)k;
+  p->v = (const _Float16*)v;
+  p->a = (const _Float16*)a;
+  p->b = (const _Float16*)b;
+  p->out = (_Float16*)out;
+  p->q_stride = q_stride;
+  p->k_stride = k_stride;
+  p->v_stride = v_stride;
+  p->a_stride = a_stride;
+  p->b_stride = b_stride;
+  p->out_stride = out_stride;
+  p->a_log = a_log;
+  p->dt_bias = dt_bias;
+  p->hk = heads_k;
+  p->hv = heads_v;
+  p->group = heads_v / heads_k;
+  p->dk = dim_k;
+  p->dv = dim_v;
+  p->scale = scale;
+  p->eps = eps;
+  // (a workgroup takes 16 columns of a head at least)
+  if ((long long)p->slots.n * heads_v * (dim_v / 16) > 0x7fffffffLL)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d sequences of %d heads of %d in one call", p->slots.n,
+                heads_v, dim_v);
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots, float* state,
+                                         const int32_t* offsets, int tokens, const void* q,
+                                         int64_t q_stride, const void* k, int64_t k_stride,
+                                         const void* v, int64_t v_stride, const void* a,
+                                         int64_t a_stride, const void* b, int64_t b_stride,
+                                         const float* a_log, const float* dt_bias, int heads_k,
+                                         int heads_v, int dim_k, int dim_v, float scale, float eps,
+                                         void* out, int64_t out_stride) {
+  const char* op = "aexq_delta_prompt";
+  if (!ctx) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "ctx is NULL");
+  DeltaParams p{};
+  aexq_status st = view_slots(slots, op, state, &p.slots);
+  if (!st) st = check_tokens(op, offsets, tokens);
+  if (!st)
+    st = view_delta(op, q, q_stride, k, k_stride, v, v_stride, a, a_stride, b, b_stride, a_log,
+                    dt_bias, heads_k, heads_v, dim_k, dim_v, scale, eps, out, out_stride, &p);
+  if (st) return st;
+  p.state = state;
+  p.offsets = offsets;
+  p.tokens = tokens;
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = delta_prompt_launch(p, ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "delta rule launch");
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_delta_decode(aexq_ctx* ctx, const aexq_slots* slots, float* state,
+                                         const void* q, int64_t q_stride, const void* k,
+                                         int64_t k_stride, const void* v, int64_t v_stride,
+                                         const void* a, int64_t a_stride, const void* b,
+                                         int64_t b_stride, const float* a_log,
+                                         const float* dt_bias, int heads_k, int heads_v, int dim_k,
+                                         int dim_v, float scale, float eps, void* out,
+                                         int64_t out_stride) {
+  const char* op = "aexq_delta_decode";
+  if (!ctx) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "ctx is NULL");
+  DeltaParams p{};
+  aexq_status st = view_slots(slots, op, state, &p.slots);
+  if (!st)
+    st = view_delta(op, q, q_stride, k, k_stride, v, v_stride, a, a_stride, b, b_stride, a_log,
+                    dt_bias, heads_k, heads_v, dim_k, dim_v, scale, eps, out, out_stride, &p);
+  if (st) return st;
+  p.state = state;
+  p.tokens = p.slots.n;
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = delta_decode_launch(p, ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "delta rule launch");
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t x_stride,
+                                          const void* z, int64_t z_stride, const float* gamma,
+                                          float eps, int tokens, int heads, int dim, void* out,
+                                          int64_t out_stride) {
+  const char* op = "aexq_gated_rmsnorm";
+  if (!ctx) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "ctx is NULL");
+  if (tokens <= 0 || tokens > 1 << 23 || heads <= 0 || heads > 65535)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens=%d (1 to 2^23) heads=%d (1 to 65535)", tokens,
+                heads);
+  if (dim <= 0 || dim % 8 || dim > 512)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "dim=%d (a multiple of 8, at most 512)", dim);
+  if (!(eps >= 0.0f)) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "eps=%g", (double)eps);
+  aexq_status st = check_rows(op, "x", x, x_stride, heads, dim);
+  if (!st) st = check_rows(op, "z", z, z_stride, heads, dim);
+  if (!st) st = check_rows(op, "out", out, out_stride, heads, dim);
+  if (st) return st;
+  if (tokens > 1 && ((out == x && out_stride != x_stride) || (out == z && out_stride != z_stride)))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is x or z, with rows as far apart as its own");
+  GatedNormParams p{};
+  p.x = (const _Float16*)x;
+  p.z = (const _Float16*)z;
+  p.out = (_Float16*)out;
+  p.x_stride = x_stride;
+  p.z_stride = z_stride;
+  p.out_stride = out_stride;
+  p.gamma = gamma;
+  p.rows = (long long)tokens * heads;
+  p.heads = heads;
+  p.dim = dim;
+  p.eps = eps;
+  if (p.rows > 1LL << 31)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d heads in one call", tokens, heads);
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const hipError_t e = gated_norm_launch(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "norm launch");
+  return AEXQ_OK;
+}
+
+extern "C" aexq_status aexq_verify_drafts(aexq_ctx* ctx, const aexq_tensor* logits,
+                                          const int32_t* offsets, int sequences,
+                                          const int32_t* drafts, const float* draft_probs,
+                                          int64_t draft_stride, const float* temperature,
+                                          const float* accept_u, const float* sample_u,
+                                          int32_t* counts, int32_t* tokens) {
+  const char* op = "aexq_verify_drafts";
+  if (!ctx || !offsets || !drafts || !accept_u || !sample_u || !counts || !tokens)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "NULL argument");
+  TensorView v;
+  aexq_status st = view_tensor(logits, op, "logits", &v);
+  if (st) return st;
+  if (v.head_dim || v.batch > 1)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "head-packed or batched logits | rejectedFallback=layout");
+  if (sequences <= 0 || sequences > 65535)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "sequences=%d (1 to 65535)", sequences);
+  const int esize = v.dtype == AEXQ_DTYPE_F16 ? 2 : 4;
+  if ((uintptr_t)v.data % esize)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "logits not aligned to their type");
+  if (v.width > 1 << 24 || v.rows > 1 << 20)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d rows of %d logits (at most 2^20 of 2^24)", v.rows,
+                v.width);
+  if (draft_probs && (draft_stride < v.width || draft_stride > 1 << 28))
+    return fail(AEXQ_ERR_SHAPE, op, "draft_probs rows %lld elements apart hold %d values",
+                (long long)draft_stride, v.width);
+  if ((const void*)drafts == (const void*)tokens)
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens are drafts, which are still read");
+  VerifyParams p{};
+  p.x = v.data;
+  p.f16 = esize == 2;
+  p.rstride = v.rstride;
+  p.rows = v.rows;
+  p.n = v.width;
+  p.offsets = offsets;
+  p.sequences = sequences;
+  p.drafts = drafts;
+  p.probs = draft_probs;
+  p.probs_stride = draft_stride;
+  p.temperature = temperature;
+  p.accept_u = accept_u;
+  p.sample_u = sample_u;
+  p.counts = counts;
+  p.tokens = tokens;
+  p.parts = verify_parts(p.rows, p.n, esize, ctx->cus);
+  const int ve = 16 / esize;  // chunks of a row that starts anywhere in one
+  p.cols = (int)(((long long)p.n + 2 * ve - 2) / ve / p.parts + 1);
+  p.parts2 = verify_parts(sequences, p.n, 16, ctx->cus);
+  p.run = (p.n + p.parts2 - 1) / p.parts2;
+  HIP_TRY(op, hipSetDevice(ctx->device));
+  const long long parts = (long long)p.rows * p.parts;
+  const long long sums = 2LL * sequences * p.parts2;
+  st = grow_step_scratch(ctx, &ctx->verify_mem, &ctx->verify_cap,
+                         parts * 16 + sums * 8 + sequences * 32LL, op, "draft verification");
+  if (st) return st;
+  char* mem = (char*)ctx->verify_mem;  // (16-byte entries first)
+  p.plan = (int4*)mem;
+  p.norm = (double2*)(mem + sequences * 16LL);
+  p.sums = (double*)(mem + sequences * 32LL);
+  p.z = p.sums + sums;
+  p.m = (float*)(p.z + parts);
+  p.at = (int*)(p.m + parts);
+  const hipError_t e = verify_launch(p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, op, "draft verification launch");
   return AEXQ_OK;
 }
 

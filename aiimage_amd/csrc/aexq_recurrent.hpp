@@ -1,0 +1,80 @@
+// Host/device definitions of the recurrent layers and of drafted tokens (not part of
+// the ABI).
+#pragma once
+
+#include "aexq_internal.hpp"
+
+namespace aexq {
+
+// The sequences of a call and their states (aexq_slots).
+struct SlotsView {
+  const int32_t *slot, *lengths, *counts;  // [n], each may be null
+  int count, n, store;
+};
+// ---- short causal convolution (aexq_mixer.hip)
+struct ShortConvParams {
+  SlotsView slots;
+  _Float16* state;  // [count][width - 1][channels]
+  const int32_t* offsets;
+  int tokens, channels, width, silu;
+  const _Float16* x;
+  _Float16* out;  // may be null
+  long long x_stride, out_stride;
+  const float *weight, *bias;  // [channels][width], [channels] or null
+};
+hipError_t short_conv_launch(const ShortConvParams& p, hipStream_t stream);
+// ---- root-mean-square norm of heads, gated by silu (aexq_mixer.hip)
+struct GatedNormParams {
+  const _Float16 *x, *z;
+  _Float16* out;
+  long long x_stride, z_stride, out_stride;
+  const float* gamma;  // [dim] or null
+  long long rows;      // tokens * heads
+  int heads, dim;
+  float eps;
+};
+hipError_t gated_norm_launch(const GatedNormParams& p, hipStream_t stream);
+// ---- the gated delta rule (aexq_delta.hip)
+struct DeltaParams {
+  SlotsView slots;
+  float* state;            // [count][hv][dk][dv]
+  const int32_t* offsets;  // null: row s is sequence s
+  int tokens, hk, hv, group, dk, dv;
+  const _Float16 *q, *k, *v, *a, *b;
+  _Float16* out;  // may be null
+  long long q_stride, k_stride, v_stride, a_stride, b_stride, out_stride;
+  const float *a_log, *dt_bias;
+  float scale, eps;
+};
+hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream);
+hipError_t delta_decode_launch(const DeltaParams& p, int cus, hipStream_t stream);
+// ---- drafted tokens against the target's probabilities (aexq_verify.hip)
+constexpr int kVerifyParts = 64;  // parts of a row at most: a lane each
+struct VerifyParams {
+  const void* x;  // [rows][rstride] logits, n of each row
+  int f16;
+  long long rstride;
+  int rows, n;
+  const int32_t* offsets;
+  int sequences;
+  const int32_t* drafts;     // [rows]
+  const float* probs;        // [rows][probs_stride], or null
+  long long probs_stride;
+  const float* temperature;  // [sequences] or null
+  const float *accept_u, *sample_u;
+  int32_t *counts, *tokens;
+  int parts, cols;    // parts of a row in the first pass, 16-byte chunks of each
+  int parts2, run;    // parts of a sampled row, and values of each
+  // scratch: of each (row, part) the sum of weights, the largest logit and its
+  // index; of each sequence's sampled row the parts' sums; what was decided
+  double* z;
+  float* m;
+  int* at;
+  double* sums;  // [sequences][parts2][2]
+  int4* plan;    // row, mode, greedy token, accepted rows
+  double2* norm; // largest logit and sum of weights of the sampled row
+};
+int verify_parts(long long rows, int n, int esize, int cus);
+hipError_t verify_launch(const VerifyParams& p, hipStream_t stream);
+
+}  // namespace aexq

@@ -168,6 +168,14 @@ namespace Aexis.Hip
         public int rows, rotaryDim, axes, interleaved, section0, section1, section2, section3;
     }
 
+    /// <summary>aexq_slots: the states of a call's sequences in a pool (device pointers).</summary>
+    [StructLayout(LayoutKind.Sequential)]
+    public struct AexqSlots
+    {
+        public IntPtr slot, lengths, counts;
+        public int count, sequences, readOnly;
+    }
+
     /// <summary>The DllImports of include/aexq.h (one per declared function).</summary>
     public static class Native
     {
@@ -257,6 +265,25 @@ namespace Aexis.Hip
             IntPtr q, long qStride, int headsQ, float scale, IntPtr outF16, long outStride);
         [DllImport(Lib)] public static extern int aexq_logprobs(IntPtr ctx, ref AexqTensor logits,
             IntPtr tokens, IntPtr logprob, IntPtr entropy, int top, IntPtr topIds, IntPtr topLogprobs);
+
+        // ---- recurrent layers, drafted tokens; strides in elements
+        [DllImport(Lib)] public static extern int aexq_short_conv(IntPtr ctx, ref AexqSlots slots, IntPtr state,
+            IntPtr offsets, int tokens, IntPtr x, long xStride, IntPtr weight, IntPtr bias /* or 0 */,
+            int channels, int width, int silu, IntPtr outF16 /* or 0 */, long outStride);
+        [DllImport(Lib)] public static extern int aexq_delta_prompt(IntPtr ctx, ref AexqSlots slots, IntPtr state,
+            IntPtr offsets, int tokens, IntPtr q, long qStride, IntPtr k, long kStride, IntPtr v, long vStride,
+            IntPtr a, long aStride, IntPtr b, long bStride, IntPtr aLog, IntPtr dtBias, int headsK, int headsV,
+            int dimK, int dimV, float scale, float eps, IntPtr outF16 /* or 0 */, long outStride);
+        [DllImport(Lib)] public static extern int aexq_delta_decode(IntPtr ctx, ref AexqSlots slots, IntPtr state,
+            IntPtr q, long qStride, IntPtr k, long kStride, IntPtr v, long vStride, IntPtr a, long aStride,
+            IntPtr b, long bStride, IntPtr aLog, IntPtr dtBias, int headsK, int headsV, int dimK, int dimV,
+            float scale, float eps, IntPtr outF16 /* or 0 */, long outStride);
+        [DllImport(Lib)] public static extern int aexq_gated_rmsnorm(IntPtr ctx, IntPtr x, long xStride, IntPtr z,
+            long zStride, IntPtr gamma /* or 0 */, float eps, int tokens, int heads, int dim, IntPtr outF16,
+            long outStride);
+        [DllImport(Lib)] public static extern int aexq_verify_drafts(IntPtr ctx, ref AexqTensor logits,
+            IntPtr offsets, int sequences, IntPtr drafts, IntPtr draftProbs /* or 0 */, long draftStride,
+            IntPtr temperature /* or 0 */, IntPtr acceptU, IntPtr sampleU, IntPtr counts, IntPtr tokens);
 
         // ---- the decoder layers of a decode step in one launch
         [DllImport(Lib)] public static extern int aexq_decoder_create(IntPtr ctx, ref AexqDecoderConfig cfg,

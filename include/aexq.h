@@ -454,6 +454,101 @@ aexq_status aexq_logprobs(aexq_ctx* ctx, const aexq_tensor* logits, const int32_
                           float* logprob, float* entropy, int top, int32_t* top_ids,
                           float* top_logprobs);
 
+/* ---- recurrent layers, drafted tokens -------------------------------------- */
+/* The layers of the hybrid models between their attention layers, for packed tokens
+ * of many sequences: a short causal convolution, the gated delta rule, and a norm
+ * gated by silu; and the verification of drafted tokens, which says how many of a
+ * sequence's rows its states may keep.  The reference runs their one-sequence forms
+ * on other paths.  Rows are packed as above: sequence s has rows offsets[s] ..
+ * offsets[s + 1] - 1 (device int32 [sequences + 1], not decreasing, kept within the
+ * call's tokens), heads of a row dense, rows `stride` elements apart, bases 16-byte
+ * aligned, strides multiples of 8 up to 2^24.  tokens is 1 to 2^23. */
+
+/* The states of `sequences` sequences in a pool.  The arrays are read on the device
+ * when a launch runs.  A sequence whose slot lies outside the pool starts from
+ * zeros and its state is not stored.  Each slot belongs to one sequence of a call:
+ * sequences that name the same one read and leave either's state, piece by piece. */
+typedef struct aexq_slots {
+  const int32_t* slot;     /* device [sequences]; NULL: sequence s has slot s */
+  const int32_t* lengths;  /* device [sequences]: positions, the call's rows included; one that
+                            * has no others starts from zeros.  NULL: all go on */
+  const int32_t* counts;   /* device [sequences]: so many of a sequence's rows are taken, the
+                            * first ones; the others stay as they were, and so does the state
+                            * of a sequence of none.  NULL: all */
+  int count;               /* states in the pool */
+  int sequences;           /* at most 65535 */
+  int read_only;           /* states are read, not stored */
+} aexq_slots;
+
+/* Short causal convolution along each sequence, channel by channel:
+ *   out[t][c] = act(bias[c] + sum_j weight[c][j] x[t - (width - 1) + j][c])
+ * in fp32, act silu or none.  state: device fp16 [count][width - 1][channels], the
+ * inputs before the first, oldest first.  weight, bias (nullable): device fp32
+ * [channels][width], [channels].  channels a multiple of 8, width 2 to 5.  out NULL:
+ * the states alone.  out is not x. */
+aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
+                            const int32_t* offsets, int tokens, const void* x, int64_t x_stride,
+                            const float* weight, const float* bias, int channels, int width,
+                            int silu, void* out, int64_t out_stride);
+
+/* The gated delta rule, row after row of each sequence, per value head with key head
+ * h / (heads_v / heads_k):
+ *   g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b)
+ *   k^ = k / sqrt(sum k^2 + eps), q^ likewise
+ *   S <- e^g S;  u = beta (v - S^T k^);  S <- S + k^ u^T;  out = scale S^T q^
+ * q, k fp16 [tokens][heads_k][dim_k], v, out fp16 [tokens][heads_v][dim_v], a, b fp16
+ * [tokens][heads_v] (2-byte aligned, any stride), a_log, dt_bias device fp32
+ * [heads_v], state device fp32 [count][heads_v][dim_k][dim_v].  dim_k is 64 or 128,
+ * dim_v 64, 128 or 256, eps above 0, scale finite.  out NULL: the states alone; out is
+ * none of the inputs.  States and sums are fp32.  What follows a value that is not
+ * finite in its column of the state is not finite (an infinity or a NaN); what comes
+ * before it, other columns, heads and sequences do not meet it. */
+aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots, float* state,
+                              const int32_t* offsets, int tokens, const void* q, int64_t q_stride,
+                              const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              const void* a, int64_t a_stride, const void* b, int64_t b_stride,
+                              const float* a_log, const float* dt_bias, int heads_k, int heads_v,
+                              int dim_k, int dim_v, float scale, float eps, void* out,
+                              int64_t out_stride);
+
+/* aexq_delta_prompt where every sequence has one row: row s is sequence s. */
+aexq_status aexq_delta_decode(aexq_ctx* ctx, const aexq_slots* slots, float* state, const void* q,
+                              int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                              int64_t v_stride, const void* a, int64_t a_stride, const void* b,
+                              int64_t b_stride, const float* a_log, const float* dt_bias,
+                              int heads_k, int heads_v, int dim_k, int dim_v, float scale,
+                              float eps, void* out, int64_t out_stride);
+
+/* Root-mean-square norm of each head's row, gated: out = x rsqrt(max(mean(x^2) + eps,
+ * 1e-20)) gamma silu(z) in fp32; x, z, out fp16 [tokens][heads][dim], dim a multiple of
+ * 8 up to 512, gamma device fp32 [dim] or NULL.  out may be x or z, rows as far apart. */
+aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t x_stride, const void* z,
+                               int64_t z_stride, const float* gamma, float eps, int tokens,
+                               int heads, int dim, void* out, int64_t out_stride);
+
+/* Drafted tokens against the target's probabilities p = softmax(logits / T).  Row i of
+ * a sequence holds the fp32 or fp16 logits (not head-packed) behind its i-th token, and
+ * drafts[row] (device int32 [rows]; the last row's is not read) the token proposed for
+ * there.  A draft d stays while those before it do and accept_u[row] q(d) < p(d); q is
+ * row `row` of draft_probs (device fp32, rows draft_stride apart), or 1 where that is
+ * NULL.  The new token comes from the first row whose draft does not stay, by the
+ * weights max(p - q, 0) (p without the draft where draft_probs is NULL; p itself where
+ * nothing is left), or from p of the last row: the first index whose cumulative weight
+ * passes sample_u[s] times all of it.  accept_u (device fp32 [rows]) and sample_u
+ * ([sequences]) lie in [0, 1).  temperature (device fp32 [sequences]; NULL: 1): at 0
+ * or below, the largest logit, the lower index first, is what a draft has to be and
+ * what the new token is.  A row with a NaN, a +inf, or nothing but -inf has no
+ * probabilities: its draft does not stay and its token is -1.
+ * counts[s] (device int32): rows that stay, the new token's included (what slots.counts
+ * takes); tokens (device int32 [rows]): the drafts that stay, the new token, -1 in the
+ * rows behind.  Rows of no sequence are not touched.  Weights and sums are 64 bits.
+ * Up to 2^20 rows.  Uses the context's scratch. */
+aexq_status aexq_verify_drafts(aexq_ctx* ctx, const aexq_tensor* logits, const int32_t* offsets,
+                               int sequences, const int32_t* drafts, const float* draft_probs,
+                               int64_t draft_stride, const float* temperature,
+                               const float* accept_u, const float* sample_u, int32_t* counts,
+                               int32_t* tokens);
+
 /* ---- the decoder layers of a decode step in one launch -------------------- */
 /* Qwen35DecoderSession.DecodeCore's per-layer chain (DEC:463-585: RMSNorm,
  * q/k/v, RoPE, K/V append, SDPA, o_proj + residual, RMSNorm, gate/up + SwiGLU,
