@@ -81,6 +81,9 @@ struct aexq_ctx {
   long long logprob_stats_cap = 0;
   unsigned long long* logprob_keys = nullptr;
   long long logprob_keys_cap = 0;
+  // per block of rows and head of the delta rule: its matrices and factors
+  void* delta_mem = nullptr;
+  long long delta_cap = 0;
   // per part of a row of drafted tokens: sums of weights, and what was decided
   void* verify_mem = nullptr;
   long long verify_cap = 0;
@@ -223,6 +226,7 @@ extern "C" void aexq_destroy(aexq_ctx* ctx) {
   (void)hipFree(ctx->prompt_part);
   (void)hipFree(ctx->logprob_stats);
   (void)hipFree(ctx->logprob_keys);
+  (void)hipFree(ctx->delta_mem);
   (void)hipFree(ctx->verify_mem);
   (void)hipFree(ctx->sk_part);
   (void)hipFree(ctx->am_tagged);
@@ -2549,6 +2553,17 @@ extern "C" aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots,
   p.offsets = offsets;
   p.tokens = tokens;
   HIP_TRY(op, hipSetDevice(ctx->device));
+  // (row_blocks of aexq_rows.hpp)
+  const long long blocks = tokens / kDeltaRows + (long long)p.slots.n;
+  if (blocks * heads_v > 0x7fffffffLL)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d sequences and %d heads in one call",
+                tokens, p.slots.n, heads_v);
+  const long long heads = blocks * heads_v * kDeltaHead;
+  st = grow_step_scratch(ctx, &ctx->delta_mem, &ctx->delta_cap,
+                         heads + blocks * heads_k * delta_key_bytes(dim_k), op, "delta rule blocks");
+  if (st) return st;
+  p.heads = (char*)ctx->delta_mem;
+  p.keys = p.heads + heads;
   const hipError_t e = delta_prompt_launch(p, ctx->cus, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "delta rule launch");
   return AEXQ_OK;

@@ -45,7 +45,16 @@ struct DeltaParams {
   long long q_stride, k_stride, v_stride, a_stride, b_stride, out_stride;
   const float *a_log, *dt_bias;
   float scale, eps;
+  // of each block of 64 rows (aexq_rows.hpp), scratch: per value head the matrices
+  // T and P and the rows' factors, per key head the keys transposed
+  char* heads;
+  char* keys;
 };
+// Scratch of a block and head: six (16 rows, 32 columns) pieces of T in two fp16 parts
+// and of P in one, 1 KB each; four factors a row and the block's decay.
+constexpr int kDeltaRows = 64;
+constexpr int kDeltaHead = 18 * 1024 + 4 * kDeltaRows * 4 + 64;
+inline int delta_key_bytes(int dk) { return dk * kDeltaRows * 2; }
 hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream);
 hipError_t delta_decode_launch(const DeltaParams& p, int cus, hipStream_t stream);
 // ---- drafted tokens against the target's probabilities (aexq_verify.hip)
