@@ -5,6 +5,9 @@
 // States and all sums are fp32.
 #include <math.h>
 
+#include <type_traits>
+
+#include "aexq_dma.hpp"
 #include "aexq_rows.hpp"
 
 namespace aexq {
@@ -21,10 +24,20 @@ __device__ __forceinline__ Gate gate_of(const DeltaParams& p, long long row, int
   return Gate{g < -1e5f ? -1e5f : g, 1.0f / (1.0f + expf(-b))};
 }
 
-// Sum of v over the four 16-lane rows of the wave, in every lane.
+// Sum and maximum of v over the four 16-lane rows of the wave, in every lane: rows swapped
+// between two copies of it (v_permlane), no trip through LDS.
+template <typename F>
+__device__ __forceinline__ float rows_join(float v, F join) {
+  const auto a = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+  v = join(as_f32(a[0]), as_f32(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+  return join(as_f32(b[0]), as_f32(b[1]));
+}
 __device__ __forceinline__ float rows_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  return rows_join(v, [](float x, float y) { return x + y; });
+}
+__device__ __forceinline__ float rows_max(float v) {
+  return rows_join(v, [](float x, float y) { return fmaxf(x, y); });
 }
 
 // ---------------------------------------------------------------------------
@@ -51,7 +64,7 @@ struct DeltaState {
   f32x4 s[NT][NC];
 };
 
-// Row after row of [t0, t1).
+// Row after row of [t0, t1), by the whole workgroup.
 template <int DK, int NC>
 __device__ __forceinline__ void delta_rows(const DeltaParams& p, const Span& span, int head,
                                            int col, int t0, int t1, DeltaState<DK, NC>& S,
@@ -150,66 +163,85 @@ __device__ __forceinline__ void delta_rows(const DeltaParams& p, const Span& spa
 __device__ __forceinline__ int piece_of(int w, int b) { return w < 2 ? w : 2 * w - 2 + b; }
 constexpr float kPieceScale = 2048.0f;  // of T and P: small entries keep their bits
 
+// 2^x of a difference in 64 bits, x <= 0: v_exp_f32 is within 2^-23 of it, the rounding
+// of x takes 2^-24 |x| ln 2 (and the weight is 2^x).
+__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
 // Row factors of a block and head: beta, beta e^G / |k|, scale e^G / |q|, and e^(G_63 - G)
 // over |k| as the transposed keys have it; then e^G_63.
 enum : int { kBeta = 0, kSeen = 1, kAsk = 2, kLeft = 3, kDecay = 4 };
-__device__ __forceinline__ float* factors_of(char* head, int which) {
-  return (float*)(head + 18 * 1024) + which * kDeltaRows;
+
+// The power of two that takes a key of length 1 / rk to a length of 1/2 to 1.
+__device__ __forceinline__ float near_one(float rk) {
+  return as_f32(f32_bits(rk) & 0x7f800000u);
 }
 
-// e^x of a difference in 64 bits, to fp32's precision.
-__device__ __forceinline__ float exp_of(double x) {
-  const float hi = (float)x, e = expf(hi);
-  return fmaf(e, (float)(x - (double)hi), e);
+// v of lane I of each row of 16 lanes.
+template <int I>
+__device__ __forceinline__ float row_value(float v) {
+  return as_f32(__builtin_amdgcn_update_dpp(0u, f32_bits(v), 0x150 + I, 0xF, 0xF, true));
+}
+// f(0), f(1), .. f(N - 1), each number a constant.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(f);
+  }
 }
 
+constexpr int kGateHeads = kWaves;  // heads whose gates are made together, a wave each
 template <int DK>
 struct BlockLds {
   alignas(16) f16 k[kDeltaRows][DK + 8];
-  alignas(16) float a[kDeltaRows][kDeltaRows + 4], t[kDeltaRows][kDeltaRows + 4];
-  alignas(16) f16 p[kDeltaRows][kDeltaRows + 8];
-  double sums[kDeltaRows];
-  float beta[kDeltaRows], rk[kDeltaRows], rq[kDeltaRows];
+  alignas(16) float t[kDeltaRows][kDeltaRows + 4];
+  double sums[kGateHeads][kDeltaRows];  // of log2 of the decays, up to each row
+  float beta[kGateHeads][kDeltaRows], rk[kDeltaRows], rq[kDeltaRows];
 };
 
-// One block and key head; the value heads of its group in turn.
+// One block and key head; the value heads of its group in turn.  Products of keys are
+// formed with the earlier rows on the left: lane (c, g) then has row 16 w + c and columns
+// 16 j + 4 g + r, which is how A and P enter the products behind.
 template <int DK>
-__global__ __launch_bounds__(kThreads) void delta_block_kernel(const DeltaParams p) {
+__global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaParams p) {
   constexpr int KB = DK / 32;
   __shared__ BlockLds<DK> lds;
   const int hk = blockIdx.x % p.hk, id = blockIdx.x / p.hk;
   const int tid = threadIdx.x, lane = tid & 63, wave = sreg(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
+  const int c = lane & 15, g = lane >> 4, own = 16 * wave + c;
   const RowBlock at = row_block<kDeltaRows>(p.offsets, p.tokens, p.slots.n, id);
   const Span span = span_of(p.slots, p.offsets, p.tokens, at.seq);
   const int t0 = at.block * kDeltaRows, live = min(kDeltaRows, span.kept - t0);
   if (live <= 0) return;
   // rows past the last one repeat it; their factors are 0
-  const long long row = span.first + t0 + min(16 * wave + c, live - 1);
+  const long long row = span.first + t0 + min(own, live - 1);
   f16x8 k[KB], q[KB];
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
     k[i] = *(const f16x8*)(p.k + row * p.k_stride + hk * DK + 32 * i + 8 * g);
     q[i] = *(const f16x8*)(p.q + row * p.q_stride + hk * DK + 32 * i + 8 * g);
   }
+  // rows for the next kernel, whose workgroups read them often: heads of one row spread
+  // over memory's channels, rows of one head, a power of two apart, would share one
+  char* keys = p.keys + ((long long)id * p.hk + hk) * delta_key_bytes(DK);
   float kk = 0.0f, qq = 0.0f;
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
-    *(f16x8*)&lds.k[16 * wave + c][32 * i + 8 * g] = k[i];
+    *(f16x8*)&lds.k[own][32 * i + 8 * g] = k[i];
+    *(f16x8*)(keys + ((wave * KB + i) * 64 + lane) * 16) = k[i];
+    *(f16x8*)(keys + ((4 * KB + wave * KB + i) * 64 + lane) * 16) = q[i];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       kk = fmaf((float)k[i][e], (float)k[i][e], kk);
       qq = fmaf((float)q[i][e], (float)q[i][e], qq);
     }
   }
-  kk = rows_sum(kk);
-  qq = rows_sum(qq);
+  const float rk = 1.0f / sqrtf(rows_sum(kk) + p.eps), rq = 1.0f / sqrtf(rows_sum(qq) + p.eps);
   if (g == 0) {
-    lds.rk[16 * wave + c] = 1.0f / sqrtf(kk + p.eps);
-    lds.rq[16 * wave + c] = 1.0f / sqrtf(qq + p.eps);
+    lds.rk[own] = rk;
+    lds.rq[own] = rq;
   }
   __syncthreads();
-  // products of the wave's 16 rows with the rows up to their last one
   f32x4 ak[4], aq[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -217,138 +249,167 @@ __global__ __launch_bounds__(kThreads) void delta_block_kernel(const DeltaParams
     if (j > wave) continue;
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
-      const f16x8 b = *(const f16x8*)&lds.k[16 * j + c][32 * i + 8 * g];
-      ak[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], b, ak[j], 0, 0, 0);
-      aq[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], b, aq[j], 0, 0, 0);
+      const f16x8 x = *(const f16x8*)&lds.k[16 * j + c][32 * i + 8 * g];
+      ak[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, k[i], ak[j], 0, 0, 0);
+      aq[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[i], aq[j], 0, 0, 0);
     }
-  }
-  // the keys transposed, in the products' order, times a power of two that leaves rows a
-  // length of 1/2 to 1 (exact but for values below 2^-14, by 2^-25)
-  auto power = [&](float rk) { return as_f32(f32_bits(rk) & 0x7f800000u); };
-  {
-    f16* to = (f16*)(p.keys + ((long long)id * p.hk + hk) * (DK * kDeltaRows * 2));
-#pragma unroll
-    for (int i = 0; i < DK / 32; ++i) {  // pieces (tile, block): two a tile
-      const int n = wave * (DK / 32) + i, tile = n >> 1, b = n & 1;
-      f16x8 y;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int t = 32 * b + (e < 4 ? 0 : 16) + 4 * g + e % 4;
-        y[e] = (f16)((float)lds.k[t][16 * tile + c] * power(lds.rk[t]));
-      }
-      *(f16x8*)(to + (n * 64 + lane) * 8) = y;
-    }
-  }
-  for (int h = 0; h < p.group; ++h) {
-    const int head = hk * p.group + h;
-    char* to = p.heads + ((long long)id * p.hv + head) * kDeltaHead;
-    if (wave == 0) {
-      // a row a lane: sums of g in 64 bits, as differences of large ones are taken
-      Gate gate = {0.0f, 0.0f};
-      if (lane < live) gate = gate_of(p, span.first + t0 + lane, head);
-      double G = gate.g;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const double up = __shfl_up(G, off, 64);
-        if (lane >= off) G += up;
-      }
-      const double last = __shfl(G, 63, 64);
-      const float rk = lds.rk[lane], e = exp_of(G);
-      lds.sums[lane] = G;
-      lds.beta[lane] = gate.beta;
-      const bool in = lane < live;
-      factors_of(to, kBeta)[lane] = gate.beta;
-      factors_of(to, kSeen)[lane] = in ? gate.beta * e * rk : 0.0f;
-      factors_of(to, kAsk)[lane] = in ? p.scale * e * lds.rq[lane] : 0.0f;
-      factors_of(to, kLeft)[lane] = in ? exp_of(last - G) * (rk / power(rk)) : 0.0f;
-      if (lane == 63) factors_of(to, kDecay)[0] = e;
-    }
-    __syncthreads();
-    f32x4 rowk, rowq, beta;
-    double G[4];
+    const f32x4 rj = *(const f32x4*)&lds.rk[16 * j + 4 * g];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
-      rowk[r] = lds.rk[i];
-      rowq[r] = lds.rq[i];
-      beta[r] = lds.beta[i];
-      G[r] = lds.sums[i];
+      ak[j][r] *= rk * rj[r];
+      aq[j][r] *= rq * rj[r];
     }
+  }
+  // the keys transposed, times a power of two (exact but for values below 2^-14, by 2^-25)
+#pragma unroll
+  for (int i = 0; i < DK / 32; ++i) {  // pieces (16 of DK, 32 rows): two a tile
+    const int n = wave * (DK / 32) + i, tile = n >> 1, b = n & 1;
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int t = 32 * b + (e < 4 ? 0 : 16) + 4 * g + e % 4;
+      y[e] = (f16)((float)lds.k[t][16 * tile + c] * near_one(lds.rk[t]));
+    }
+    *(f16x8*)(keys + ((8 * KB + n) * 64 + lane) * 16) = y;
+  }
+  for (int h = 0; h < p.group; ++h) {
+    const int head = hk * p.group + h, slot = h % kGateHeads;
+    char* to = p.heads + ((long long)id * p.hv + head) * kDeltaHead;
+    if (slot == 0) {
+      __syncthreads();
+      if (h + wave < p.group) {
+        // a row a lane: sums in 64 bits, as differences of large ones are taken
+        const int mine = head + wave;
+        Gate gate = {0.0f, 0.0f};
+        if (lane < live) gate = gate_of(p, span.first + t0 + lane, mine);
+        double G = (double)gate.g * 1.4426950408889634;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const double up = __shfl_up(G, off, 64);
+          if (lane >= off) G += up;
+        }
+        lds.sums[wave][lane] = G;
+        lds.beta[wave][lane] = gate.beta;
+        float* f = (float*)(to + wave * (long long)kDeltaHead + kDeltaFactors) + lane;
+        const bool in = lane < live;
+        const float rk = lds.rk[lane], e = exp2_of(G), last = exp2_of(__shfl(G, 63, 64) - G);
+        f[kBeta * kDeltaRows] = gate.beta;
+        f[kSeen * kDeltaRows] = in ? gate.beta * e * rk : 0.0f;
+        f[kAsk * kDeltaRows] = in ? p.scale * e * lds.rq[lane] : 0.0f;
+        f[kLeft * kDeltaRows] = in ? last * (rk / near_one(rk)) : 0.0f;
+        if (lane == 63) f[kDecay * kDeltaRows - 63] = e;
+      }
+      __syncthreads();
+    }
+    // (so that comparisons with the lane's row are made here, not kept over the loop)
+    int here = c;
+    asm volatile("" : "+v"(here));
+    // A and P of the wave's rows
+    const double G = lds.sums[slot][own];
+    const float beta = lds.beta[slot][own];
+    f32x4 a[4], own_tile = f32x4{};
+    f16x4 w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int col = 16 * j + c;
-      const float rk = lds.rk[col];
-      const double Gj = lds.sums[col];
+      a[j] = f32x4{};
+      w[j] = f16x4{};
+      if (j > wave) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * wave + 4 * g + r;
-        float a = 0.0f, w = 0.0f;
-        if (col <= i && i < live) {
-          const float e = exp_of(G[r] - Gj) * rk;
-          a = col < i ? ak[j][r] * rowk[r] * e * beta[r] : 0.0f;
-          w = aq[j][r] * rowq[r] * e;
-        }
-        lds.a[i][col] = a;
-        lds.p[i][col] = (f16)(w * kPieceScale);
+        const int ahead = 4 * g + r - here;  // of the wave's own tile: the column less the row
+        const bool seen = own < live && (j < wave || ahead <= 0);
+        const float e = exp2_of(G - lds.sums[slot][16 * j + 4 * g + r]);
+        a[j][r] = seen && (j < wave || ahead < 0) ? ak[j][r] * (e * beta) : 0.0f;
+        w[j][r] = (f16)(seen ? aq[j][r] * e * kPieceScale : 0.0f);
       }
+      if (j == wave) own_tile = a[j];
     }
-    __syncthreads();
-    // T's diagonal tiles, a column a lane (the four rows of lanes do the same)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      if (b <= wave / 2)
+        *(f16x8*)(to + ((12 + piece_of(wave, b)) * 64 + lane) * 16) =
+            __builtin_shufflevector(w[2 * b], w[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+    // T's diagonal tiles by substitution, column c in lane c (the four rows of lanes do the
+    // same): row i of A comes from lane i of each row of lanes
+    *(f32x4*)&lds.t[own][16 * wave + 4 * g] = own_tile;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     {
-      float t[16];
+      float x[16], t[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = i == c ? 1.0f : 0.0f;
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 y = *(const f32x4*)&lds.t[own][16 * wave + i];
 #pragma unroll
-        for (int j = 0; j < i; ++j) v = fmaf(-lds.a[16 * wave + i][16 * wave + j], t[j], v);
-        t[i] = v;
+        for (int r = 0; r < 4; ++r) x[i + r] = y[r];
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      unrolled<16>([&](auto step) {
+        constexpr int i = decltype(step)::value;
+        float v = i == here ? 1.0f : 0.0f, u = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i % 4 == g) lds.t[16 * wave + i][16 * wave + c] = t[i];
+        for (int j = 0; j < i; ++j) {
+          const float a = row_value<i>(x[j]);
+          if (j % 2)
+            u = fmaf(-a, t[j], u);
+          else
+            v = fmaf(-a, t[j], v);
+        }
+        t[i] = v + u;
+        asm volatile("" : "+v"(t[i]));  // (computed here, not where it is stored)
+      });
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {  // every row of lanes stores every fourth one
+        const float y = g & 2 ? (g & 1 ? t[i + 3] : t[i + 2]) : (g & 1 ? t[i + 1] : t[i]);
+        lds.t[16 * wave + i + g][16 * wave + c] = y;
+      }
     }
     __syncthreads();
     // the tiles below them: T_wj = -T_ww sum_l A_wl T_lj, step k of a product taking row
     // 4 g + k of its right operand
+    const f32x4 diagonal = *(const f32x4*)&lds.t[own][16 * wave + 4 * g];
+#pragma unroll
     for (int d = 1; d < 4; ++d) {
       const int j = wave - d;
       if (j >= 0) {
         f32x4 x = f32x4{}, y = f32x4{};
-        for (int l = j; l < wave; ++l) {
-          const f32x4 a = *(const f32x4*)&lds.a[16 * wave + c][16 * l + 4 * g];
+#pragma unroll
+        for (int l = 0; l < 3; ++l) {
+          if (l < j || l >= wave) continue;
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], lds.t[16 * l + 4 * g + s][16 * j + c], x,
-                                                     0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                a[l][s], lds.t[16 * l + 4 * g + s][16 * j + c], x, 0, 0, 0);
         }
-        const f32x4 t = *(const f32x4*)&lds.t[16 * wave + c][16 * wave + 4 * g];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
-          y = __builtin_amdgcn_mfma_f32_16x16x4f32(t[s], x[s], y, 0, 0, 0);
+          y = __builtin_amdgcn_mfma_f32_16x16x4f32(diagonal[s], x[s], y, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds.t[16 * wave + 4 * g + r][16 * j + c] = -y[r];
       }
       __syncthreads();
     }
-    // the wave's rows of T and P as the products take them
+    // the wave's rows of T as the products take them
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       if (b > wave / 2) continue;
       const int piece = piece_of(wave, b);
-      f16x8 t0, t1, w;
+      f16x8 t0, t1;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = 32 * b + (e < 4 ? 0 : 16) + 4 * g + e % 4;
-        const float v = col < 16 * (wave + 1) ? lds.t[16 * wave + c][col] * kPieceScale : 0.0f;
-        t0[e] = (f16)v;
-        t1[e] = (f16)(v - (float)t0[e]);
-        w[e] = lds.p[16 * wave + c][col];
+      for (int half = 0; half < 2; ++half) {
+        const int tile = 2 * b + half;
+        f32x4 v = f32x4{};
+        if (tile <= wave) v = *(const f32x4*)&lds.t[own][16 * tile + 4 * g];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float y = v[r] * kPieceScale;
+          t0[4 * half + r] = (f16)y;
+          t1[4 * half + r] = (f16)(y - (float)t0[4 * half + r]);
+        }
       }
       *(f16x8*)(to + ((piece * 2) * 64 + lane) * 16) = t0;
       *(f16x8*)(to + ((piece * 2 + 1) * 64 + lane) * 16) = t1;
-      *(f16x8*)(to + ((12 + piece) * 64 + lane) * 16) = w;
     }
-    __syncthreads();
   }
 }
 
@@ -373,8 +434,18 @@ struct DeltaBlock {
   float decay;
 };
 
+// Two fp16 numbers x0 + x1 for four values.
+__device__ __forceinline__ void split4(const f32x4& x, f16x4& x0, f16x4& x1) {
+  x0 = __builtin_convertvector(x, f16x4);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x1[r] = (f16)(x[r] - (float)x0[r]);
+}
+__device__ __forceinline__ float top4(const f32x4& v) {
+  return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+}
+
 template <int DK, int NC>
-__global__ __launch_bounds__(kThreads) void delta_prompt_kernel(const DeltaParams p) {
+__global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaParams p) {
   constexpr int NT = DK / 64, KB = DK / 32;
   __shared__ DeltaLds<DK, NC> lds;
   // the parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the
@@ -399,126 +470,133 @@ __global__ __launch_bounds__(kThreads) void delta_prompt_kernel(const DeltaParam
       for (int r = 0; r < 4; ++r)
         S.s[i][n][r] = span.fresh ? 0.0f : state[(16 * i + r) * p.dv + 16 * n];
 
-  const int blocks = (span.kept + kDeltaRows - 1) / kDeltaRows;
+  const int blocks = sreg((span.kept + kDeltaRows - 1) / kDeltaRows);
   const int id0 = span.first / kDeltaRows + s;
   DeltaBlock<DK, NC> B;
-  auto head_at = [&](int b) { return p.heads + ((long long)(id0 + b) * p.hv + head) * kDeltaHead; };
+  // v and out are addressed by resources that end with the block's last row: rows behind
+  // it read as zeros and are not stored, and a lane's offsets are the same in every block
+  const int rows4 = 16 * wave + 4 * g;
+  const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
+  const uint32_t at_v = (uint32_t)rows4 * step_v + 2 * c, at_out = (uint32_t)rows4 * step_out + 2 * c;
+  const f16* v0 = sreg(p.v + span.first * p.v_stride + head * p.dv + col);
+  f16* out0 = sreg(p.out + span.first * p.out_stride + head * p.dv + col);
+  auto block_rows = [&](const f16* x, uint32_t step, int b) {
+    const int live = min(kDeltaRows, span.kept - b * kDeltaRows);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)b * kDeltaRows * (step / 2)), 0,
+                                             (uint32_t)(live - 1) * step + 32 * NC,
+                                             kBufferRsrcWord3);
+  };
+  auto head_of = [&](int b) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        p.heads + ((long long)(id0 + b) * p.hv + head) * kDeltaHead, 0, kDeltaHead,
+        kBufferRsrcWord3);
+  };
+  auto keys_of = [&](int b) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        p.keys + ((long long)(id0 + b) * p.hk + hk) * delta_key_bytes(DK), 0, delta_key_bytes(DK),
+        kBufferRsrcWord3);
+  };
+  auto factor = [&](__amdgpu_buffer_rsrc_t at, int which) {
+    return __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                   at, rows4 * 4, kDeltaFactors + which * kDeltaRows * 4, 0));
+  };
+  auto piece = [&](__amdgpu_buffer_rsrc_t at, int number) {
+    return __builtin_bit_cast(
+        f16x8, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, number * 1024, 0));
+  };
+  // (a piece past the resource's end, where the wave's rows have no column in it)
+  auto needed = [&](int i, int number) { return i <= wave / 2 ? number : 64; };
   auto load_rows = [&](int b) {  // k, q and v
-    const int last = min(kDeltaRows, span.kept - b * kDeltaRows) - 1;
-    const long long first = span.first + b * kDeltaRows, row = first + min(16 * wave + c, last);
-    const f16* k = p.k + row * p.k_stride + hk * DK + 4 * g;
-    const f16* q = p.q + row * p.q_stride + hk * DK + 4 * g;
+    const auto rows = keys_of(b), rv = block_rows(v0, step_v, b), h = head_of(b);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        B.v[n][r] = __builtin_bit_cast(
+            f16, __builtin_amdgcn_raw_buffer_load_b16(rv, at_v + r * step_v + 32 * n, 0, 0));
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
-      const f16x4 k0 = *(const f16x4*)(k + 32 * i), k1 = *(const f16x4*)(k + 32 * i + 16);
-      const f16x4 q0 = *(const f16x4*)(q + 32 * i), q1 = *(const f16x4*)(q + 32 * i + 16);
-      B.k[i] = __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7);
-      B.q[i] = __builtin_shufflevector(q0, q1, 0, 1, 2, 3, 4, 5, 6, 7);
+      B.k[i] = piece(rows, wave * KB + i);
+      B.q[i] = piece(rows, 4 * KB + wave * KB + i);
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = 16 * wave + 4 * g + r;
-      const f16* v = p.v + (first + min(t, last)) * p.v_stride + head * p.dv + col + c;
-#pragma unroll
-      for (int n = 0; n < NC; ++n) B.v[n][r] = t <= last ? v[16 * n] : (f16)0.0f;
-    }
-  };
-  auto load_factors = [&](int b) {
-    char* at = head_at(b);
-    const int i = 16 * wave + 4 * g;
-    B.beta = *(const f32x4*)(factors_of(at, kBeta) + i);
-    B.seen = *(const f32x4*)(factors_of(at, kSeen) + i);
-    B.ask = *(const f32x4*)(factors_of(at, kAsk) + i);
-    B.left = *(const f32x4*)(factors_of(at, kLeft) + i);
-    B.decay = factors_of(at, kDecay)[0];
+    B.beta = factor(h, kBeta);
+    B.seen = factor(h, kSeen);
   };
   auto load_t = [&](int b) {
-    const char* at = head_at(b) + lane * 16;
+    const auto h = head_of(b);
+    B.left = factor(h, kLeft);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int piece = piece_of(wave, min(i, wave / 2));
-      B.t[i][0] = *(const f16x8*)(at + piece * 2048);
-      B.t[i][1] = *(const f16x8*)(at + piece * 2048 + 1024);
+      const int number = needed(i, 2 * piece_of(wave, i));
+      B.t[i][0] = piece(h, number);
+      B.t[i][1] = piece(h, number + 1);
     }
   };
   auto load_out = [&](int b) {  // P and the transposed keys
-    const char* at = head_at(b) + 12 * 1024 + lane * 16;
+    const auto h = head_of(b), keys = keys_of(b);
+    B.ask = factor(h, kAsk);
+    B.decay = as_f32(
+        __builtin_amdgcn_raw_buffer_load_b32(h, 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      B.w[i] = *(const f16x8*)(at + piece_of(wave, min(i, wave / 2)) * 1024);
-    const char* keys = p.keys + ((long long)(id0 + b) * p.hk + hk) * (DK * kDeltaRows * 2);
+    for (int i = 0; i < 2; ++i) B.w[i] = piece(h, needed(i, 12 + piece_of(wave, i)));
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        B.kt[i][j] = *(const f16x8*)(keys + (((wave * NT + i) * 2 + j) * 64 + lane) * 16);
+      for (int j = 0; j < 2; ++j) B.kt[i][j] = piece(keys, 8 * KB + (wave * NT + i) * 2 + j);
   };
 
-  // largest |S| of a column, as bits: a NaN is above every number
-  auto state_max = [&](int n) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) m = max(m, f32_bits(S.s[i][n][r]) & 0x7fffffffu);
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
-    return max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
+  // where a wave's values 4 g + r of a column go in a right operand of 32 rows, two fp16
+  // numbers to a value (`half`: which 16 rows)
+  auto put = [&](f16x8* part0, f16x8* part1, int to, int half, const f32x4& x) {
+    f16x4 x0, x1;
+    split4(x, x0, x1);
+    __builtin_memcpy((char*)(part0 + to) + 8 * half, &x0, 8);
+    __builtin_memcpy((char*)(part1 + to) + 8 * half, &x1, 8);
   };
-  auto top4 = [&](const f32x4& v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
-  auto bits4 = [&](const f32x4& v) {
-    return as_f32(max(max(f32_bits(v[0]), f32_bits(v[1])), max(f32_bits(v[2]), f32_bits(v[3]))));
-  };
-  float bound[NC];  // of |S|, by column
-  auto meet = [&]() {
+  auto state_top = [&](int n) {
+    float m = top4(S.s[0][n]);
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      const uint32_t m = state_max(n);
-      if (g == 0) lds.first[n][c][wave] = as_f32(m);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NC; ++n) bound[n] = bits4(*(const f32x4*)lds.first[n][c]);
-    __syncthreads();
+    for (int i = 1; i < NT; ++i) m = fmaxf(m, top4(S.s[i][n]));
+    return rows_max(m);
   };
   load_rows(0);
-  load_factors(0);
+  __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
   load_t(0);
+  __builtin_amdgcn_sched_barrier(0);
   load_out(0);
-  meet();
+  __builtin_amdgcn_sched_barrier(0);
+  float bound[NC], top[NC];  // of |S| by column: at most, and in the wave's rows
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    top[n] = state_top(n);
+    lds.first[n][c][wave] = top[n];  // (the four lanes of a column write the same)
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NC; ++n) bound[n] = top4(*(const f32x4*)lds.first[n][c]);
 
-  for (int b = 0; b < blocks; ++b) {
+  int at_block = 0;
+  for (; at_block < blocks; ++at_block) {
+    const int b = sreg(at_block);
     const int next = min(b + 1, blocks - 1);
     // S in two parts, where all waves read them
     Lift ls[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       ls[n] = lift_of(bound[n]);
-      f16 x0[4 * NT], x1[4 * NT];
+      // rows 16 i + 4 g .. of the wave's are an even or odd half of a lane's eight
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = S.s[i][n][r] * ls[n].by;
-          x0[4 * i + r] = (f16)x;
-          x1[4 * i + r] = (f16)(x - (float)x0[4 * i + r]);
-        }
-      if constexpr (NT == 2) {
-        __builtin_memcpy(&lds.s[0][wave][n][lane], x0, 16);
-        __builtin_memcpy(&lds.s[1][wave][n][lane], x1, 16);
-      } else {
-        __builtin_memcpy((char*)&lds.s[0][wave / 2][n][lane] + 8 * (wave & 1), x0, 8);
-        __builtin_memcpy((char*)&lds.s[1][wave / 2][n][lane] + 8 * (wave & 1), x1, 8);
+      for (int i = 0; i < NT; ++i) {
+        const int row = wave * (DK / 4) + 16 * i + 4 * g;
+        put(lds.s[0][row / 32][n], lds.s[1][row / 32][n], c + row % 32 / 8 * 16, row / 4 % 2,
+            S.s[i][n] * ls[n].by);
       }
-      const uint32_t m = state_max(n);
-      float mv = 0.0f;
+      f32x4 v;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mv = fmaxf(mv, fabsf((float)B.v[n][r]));
-      mv = fmaxf(mv, __shfl_xor(mv, 16, 64));
-      mv = fmaxf(mv, __shfl_xor(mv, 32, 64));
-      if (g == 0) {
-        lds.top_s[n][c][wave] = as_f32(m);
-        lds.top_v[n][c][wave] = mv;
-      }
+      for (int r = 0; r < 4; ++r) v[r] = (float)B.v[n][r];
+      lds.top_s[n][c][wave] = top[n];
+      lds.top_v[n][c][wave] = rows_max(top4(v));
     }
     __syncthreads();
     // S^T k and S^T q of the wave's 16 rows
@@ -526,74 +604,60 @@ __global__ __launch_bounds__(kThreads) void delta_prompt_kernel(const DeltaParam
     float top_s[NC], top_v[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
+      f32x4 seen1 = f32x4{}, asked1 = f32x4{};
       seen[n] = asked[n] = f32x4{};
-      top_s[n] = bits4(*(const f32x4*)lds.top_s[n][c]);
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        const f16x8 y0 = lds.s[0][i][n][lane], y1 = lds.s[1][i][n][lane];
+        seen[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.k[i], y0, seen[n], 0, 0, 0);
+        seen1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.k[i], y1, seen1, 0, 0, 0);
+        asked[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.q[i], y0, asked[n], 0, 0, 0);
+        asked1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.q[i], y1, asked1, 0, 0, 0);
+      }
+      top_s[n] = top4(*(const f32x4*)lds.top_s[n][c]);
       top_v[n] = top4(*(const f32x4*)lds.top_v[n][c]);
+      seen[n] = (seen[n] + seen1) * ls[n].back;
+      asked[n] = (asked[n] + asked1) * ls[n].back;
     }
-#pragma unroll
-    for (int i = 0; i < KB; ++i)
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const f16x8 y = lds.s[x][i][n][lane];
-          seen[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.k[i], y, seen[n], 0, 0, 0);
-          asked[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.q[i], y, asked[n], 0, 0, 0);
-        }
     // R in two parts; |R| is within |v| and the column's length
     Lift lr[NC];
     bool odd = false;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       lr[n] = lift_of(fmaf(top_s[n], 12.0f, top_v[n]));
-      f16 x0[4], x1[4];
-      float m = 0.0f;
+      f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float x =
-            B.beta[r] * (float)B.v[n][r] - B.seen[r] * (seen[n][r] * ls[n].back);
-        // (what is not finite in a column that was)
-        odd |= !(fabsf(x) < INFINITY) && top_s[n] < INFINITY;
-        m = fmaxf(m, fabsf(x));
-        const float y = x * lr[n].by;
-        x0[r] = (f16)y;
-        x1[r] = (f16)(y - (float)x0[r]);
+        x[r] = B.beta[r] * (float)B.v[n][r] - B.seen[r] * seen[n][r];
+        odd |= !(fabsf(x[r]) < INFINITY);
       }
-      __builtin_memcpy((char*)&lds.r[0][wave / 2][n][lane] + 8 * (wave & 1), x0, 8);
-      __builtin_memcpy((char*)&lds.r[1][wave / 2][n][lane] + 8 * (wave & 1), x1, 8);
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      if (g == 0) lds.top_r[n][c][wave] = m;
+      put(lds.r[0][wave / 2][n], lds.r[1][wave / 2][n], lane, wave & 1, x * lr[n].by);
+      lds.top_r[n][c][wave] = rows_max(top4(x));
     }
-    odd = __any(odd);
-    if (lane == 0) lds.odd[wave] = odd;
+    const bool any = __any(odd);
+    if (lane == 0) lds.odd[wave] = any;
     __syncthreads();
-    if (lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]) {
-      // a product with zeros would take what is not finite to the rows before it
-      __syncthreads();
-      delta_rows<DK, NC>(p, span, head, col, b * kDeltaRows,
-                         min(span.kept, (b + 1) * kDeltaRows), S, lds);
-      load_rows(next);
-      load_factors(next);
-      load_t(next);
-      load_out(next);
-      meet();
-      continue;
-    }
+    if (sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3])) break;
+    // each operand of the next block is on its way as soon as the present one is used, and
+    // not before (it takes the same registers)
+    __builtin_amdgcn_sched_barrier(0);
+    load_rows(next);
+    __builtin_amdgcn_sched_barrier(0);
     // U = T R of the wave's rows
     f32x4 u[NC];
 #pragma unroll
-    for (int n = 0; n < NC; ++n) u[n] = f32x4{};
+    for (int n = 0; n < NC; ++n) {
+      f32x4 u1 = f32x4{}, u2 = f32x4{};
+      u[n] = f32x4{};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i > wave / 2) continue;
-#pragma unroll
-      for (int n = 0; n < NC; ++n) {
+      for (int i = 0; i < 2; ++i) {
+        if (i > wave / 2) continue;
         const f16x8 r0 = lds.r[0][i][n][lane], r1 = lds.r[1][i][n][lane];
         u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][0], r0, u[n], 0, 0, 0);
-        u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][0], r1, u[n], 0, 0, 0);
-        u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][1], r0, u[n], 0, 0, 0);
+        u1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][0], r1, u1, 0, 0, 0);
+        u2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][1], r0, u2, 0, 0, 0);
       }
+      u[n] = (u[n] + (u1 + u2)) * (lr[n].back * (1.0f / kPieceScale));
     }
     // U as it is for the outputs, times the rows' factors for the state; |U| is within
     // 64 |R|
@@ -601,75 +665,75 @@ __global__ __launch_bounds__(kThreads) void delta_prompt_kernel(const DeltaParam
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       lu[n] = lift_of(64.0f * top4(*(const f32x4*)lds.top_r[n][c]));
-      f16 x0[4], x1[4], y0[4], y1[4];
-      float m = 0.0f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float x = u[n][r] * (lr[n].back * (1.0f / kPieceScale));
-        const float y = x * B.left[r];
-        m = fmaxf(m, fabsf(y));
-        const float xs = x * lu[n].by, ys = y * lu[n].by;
-        x0[r] = (f16)xs;
-        x1[r] = (f16)(xs - (float)x0[r]);
-        y0[r] = (f16)ys;
-        y1[r] = (f16)(ys - (float)y0[r]);
-      }
-      __builtin_memcpy((char*)&lds.u[0][wave / 2][n][lane] + 8 * (wave & 1), x0, 8);
-      __builtin_memcpy((char*)&lds.u[1][wave / 2][n][lane] + 8 * (wave & 1), x1, 8);
-      __builtin_memcpy((char*)&lds.u[2][wave / 2][n][lane] + 8 * (wave & 1), y0, 8);
-      __builtin_memcpy((char*)&lds.u[3][wave / 2][n][lane] + 8 * (wave & 1), y1, 8);
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      if (g == 0) lds.top_u[n][c][wave] = m;
+      const f32x4 y = u[n] * B.left;
+      put(lds.u[2][wave / 2][n], lds.u[3][wave / 2][n], lane, wave & 1, y * lu[n].by);
+      put(lds.u[0][wave / 2][n], lds.u[1][wave / 2][n], lane, wave & 1, u[n] * lu[n].by);
+      lds.top_u[n][c][wave] = rows_max(top4(y));
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_t(next);
     __syncthreads();
-    // the state behind the block
+    // the state behind the block, and the outputs
+    f32x4 y[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 add[NT];
+      f32x4 add[NT][2], o[2];
+      o[0] = o[1] = f32x4{};
 #pragma unroll
-      for (int i = 0; i < NT; ++i) add[i] = f32x4{};
+      for (int i = 0; i < NT; ++i) add[i][0] = add[i][1] = f32x4{};
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const f16x8 y = lds.u[2 + x][j][n][lane];
+          const f16x8 z = lds.u[2 + x][j][n][lane];
 #pragma unroll
           for (int i = 0; i < NT; ++i)
-            add[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.kt[i][j], y, add[i], 0, 0, 0);
+            add[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.kt[i][j], z, add[i][x], 0, 0, 0);
         }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j > wave / 2) continue;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          o[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.w[j], lds.u[x][j][n][lane], o[x], 0, 0, 0);
+      }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          S.s[i][n][r] = fmaf(S.s[i][n][r], B.decay, add[i][r] * lu[n].back);
+          S.s[i][n][r] =
+              fmaf(S.s[i][n][r], B.decay, (add[i][0][r] + add[i][1][r]) * lu[n].back);
       bound[n] = fmaf(128.0f, top4(*(const f32x4*)lds.top_u[n][c]), top_s[n] * B.decay);
+      top[n] = state_top(n);
+      const float back = p.scale * lu[n].back * (1.0f / kPieceScale);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        y[n][r] = fmaf(o[0][r] + o[1][r], back, B.ask[r] * asked[n][r]);
     }
-    if (p.out) {
+    // (what the old operands are for is done before the new ones take their registers)
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        f32x4 o = f32x4{};
+    for (int n = 0; n < NC; ++n) {
+      asm volatile("" : "+v"(y[n]), "+v"(bound[n]));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (i > wave / 2) continue;
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.w[i], lds.u[0][i][n][lane], o, 0, 0, 0);
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.w[i], lds.u[1][i][n][lane], o, 0, 0, 0);
-        }
-        const float back = p.scale * lu[n].back * (1.0f / kPieceScale);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = b * kDeltaRows + 16 * wave + 4 * g + r;
-          const float y = fmaf(o[r], back, B.ask[r] * (asked[n][r] * ls[n].back));
-          if (t < span.kept)
-            p.out[(span.first + t) * p.out_stride + head * p.dv + col + 16 * n + c] = (f16)y;
-        }
-      }
+      for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(S.s[i][n]));
     }
-    load_rows(next);
-    load_factors(next);
-    load_t(next);
+    __builtin_amdgcn_sched_barrier(0);
     load_out(next);
+    __builtin_amdgcn_sched_barrier(0);
+    if (p.out) {
+      const auto to = block_rows(out0, step_out, b);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)y[n][r]), to,
+                                                at_out + r * step_out + 32 * n, 0, 0);
+    }
   }
+  // Where something is not finite, a product with zeros would take it to the rows before
+  // it: from that block on, row after row.
+  if (at_block < blocks)
+    delta_rows<DK, NC>(p, span, head, col, at_block * kDeltaRows, span.kept, S, lds);
   if (!p.slots.store || span.slot < 0) return;
 #pragma unroll
   for (int i = 0; i < NT; ++i)

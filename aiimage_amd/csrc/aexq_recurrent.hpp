@@ -46,15 +46,17 @@ struct DeltaParams {
   const float *a_log, *dt_bias;
   float scale, eps;
   // of each block of 64 rows (aexq_rows.hpp), scratch: per value head the matrices
-  // T and P and the rows' factors, per key head the keys transposed
+  // T and P and the rows' factors, per key head keys, queries and the keys transposed
   char* heads;
   char* keys;
 };
-// Scratch of a block and head: six (16 rows, 32 columns) pieces of T in two fp16 parts
-// and of P in one, 1 KB each; four factors a row and the block's decay.
+// Scratch of a block and value head: six (16 rows, 32 columns) pieces of T in two fp16
+// parts and of P in one, 1 KB each; four factors a row and the block's decay.  Of a block
+// and key head: three times its rows.
 constexpr int kDeltaRows = 64;
-constexpr int kDeltaHead = 18 * 1024 + 4 * kDeltaRows * 4 + 64;
-inline int delta_key_bytes(int dk) { return dk * kDeltaRows * 2; }
+constexpr int kDeltaFactors = 18 * 1024;
+constexpr int kDeltaHead = kDeltaFactors + 4 * kDeltaRows * 4 + 64;
+constexpr int delta_key_bytes(int dk) { return 3 * dk * kDeltaRows * 2; }
 hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream);
 hipError_t delta_decode_launch(const DeltaParams& p, int cus, hipStream_t stream);
 // ---- drafted tokens against the target's probabilities (aexq_verify.hip)
