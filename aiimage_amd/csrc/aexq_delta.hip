@@ -54,6 +54,7 @@ struct DeltaLds {
   // the waves' largest magnitudes by column
   alignas(16) float first[NC][16][kWaves], top_s[NC][16][kWaves], top_v[NC][16][kWaves];
   alignas(16) float top_r[NC][16][kWaves], top_u[NC][16][kWaves];
+  float back_s[NC][16];  // what the parts of S are to be multiplied by
   int odd[kWaves];
   float sums[2][kWaves][2][NC][16];
 };
@@ -64,7 +65,7 @@ struct DeltaState {
   f32x4 s[NT][NC];
 };
 
-// Row after row of [t0, t1), by the whole workgroup.
+// Row after row of [t0, t1), by four waves; a barrier a row.
 template <int DK, int NC>
 __device__ __forceinline__ void delta_rows(const DeltaParams& p, const Span& span, int head,
                                            int col, int t0, int t1, DeltaState<DK, NC>& S,
@@ -422,18 +423,6 @@ __device__ __forceinline__ Lift lift_of(float bound) {
   return Lift{as_f32((uint32_t)(267 - e) << 23), as_f32((uint32_t)(e - 13) << 23)};
 }
 
-// A wave's part of the blocks' operands; each is loaded for the next block as soon as
-// the present one has used it.
-template <int DK, int NC>
-struct DeltaBlock {
-  f16x8 k[DK / 32], q[DK / 32];     // 16 rows
-  f16x8 t[2][2], w[2];              // of T and P, by 32 columns
-  f16x8 kt[DK / 64][2];             // keys transposed: DK / 4 rows, by 32 of the block's
-  f32x4 beta, seen, ask, left;      // of rows 4 g + r
-  f16 v[NC][4];
-  float decay;
-};
-
 // Two fp16 numbers x0 + x1 for four values.
 __device__ __forceinline__ void split4(const f32x4& x, f16x4& x0, f16x4& x1) {
   x0 = __builtin_convertvector(x, f16x4);
@@ -444,24 +433,70 @@ __device__ __forceinline__ float top4(const f32x4& v) {
   return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 }
 
+// Where a wave's values 4 g + r of a column go in a right operand of 32 rows, two fp16
+// numbers to a value (`half`: which 16 rows).
+__device__ __forceinline__ void put_split(f16x8* part0, f16x8* part1, int to, int half,
+                                          const f32x4& x) {
+  f16x4 x0, x1;
+  split4(x, x0, x1);
+  __builtin_memcpy((char*)(part0 + to) + 8 * half, &x0, 8);
+  __builtin_memcpy((char*)(part1 + to) + 8 * half, &x1, 8);
+}
+
+// What the two halves of a workgroup have in common.
+struct DeltaPlace {
+  Span span;
+  int part, head, hk, col, blocks, id0;
+};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t head_of(const DeltaParams& p,
+                                                          const DeltaPlace& at, int b) {
+  return __builtin_amdgcn_make_buffer_rsrc(
+      p.heads + ((long long)(at.id0 + b) * p.hv + at.head) * kDeltaHead, 0, kDeltaHead,
+      kBufferRsrcWord3);
+}
+template <int DK>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_of(const DeltaParams& p,
+                                                          const DeltaPlace& at, int b) {
+  return __builtin_amdgcn_make_buffer_rsrc(
+      p.keys + ((long long)(at.id0 + b) * p.hk + at.hk) * delta_key_bytes(DK), 0,
+      delta_key_bytes(DK), kBufferRsrcWord3);
+}
+// Rows of v and out (x: the sequence's first) are addressed by resources that end with the
+// block's last row: rows behind it read as zeros and are not stored, and a lane's offsets
+// are the same in every block.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const DeltaPlace& at, const f16* x,
+                                                          uint32_t step, int width, int b) {
+  const int live = min(kDeltaRows, at.span.kept - b * kDeltaRows);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)b * kDeltaRows * (step / 2)), 0,
+                                           (uint32_t)(live - 1) * step + 2 * width,
+                                           kBufferRsrcWord3);
+}
+__device__ __forceinline__ f32x4 factor_of(__amdgpu_buffer_rsrc_t head, int which, int row) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                       head, row * 4, kDeltaFactors + which * kDeltaRows * 4, 0));
+}
+__device__ __forceinline__ f16x8 piece_at(__amdgpu_buffer_rsrc_t at, int number) {
+  const int lane = threadIdx.x & 63;
+  return __builtin_bit_cast(
+      f16x8, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, number * 1024, 0));
+}
+// (a piece past the resource's end, where the wave's rows have no column in it)
+__device__ __forceinline__ int needed(int wave, int b, int number) {
+  return b <= wave / 2 ? number : 64;
+}
+
+// The first four waves: the state from block to block.  Wave w has 16 rows of each block
+// and DK / 4 of the state.
 template <int DK, int NC>
-__global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaParams p) {
+__device__ __forceinline__ void delta_chain(const DeltaParams& p, const DeltaPlace& at,
+                                            DeltaLds<DK, NC>& lds) {
   constexpr int NT = DK / 64, KB = DK / 32;
-  __shared__ DeltaLds<DK, NC> lds;
-  // the parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the
-  // same rows and pieces
-  const int parts = p.dv / (16 * NC), units = p.slots.n * p.hv;
-  const int unit = blockIdx.x / (8 * parts) * 8 + blockIdx.x % 8;
-  const int part = blockIdx.x / 8 % parts;
-  if (unit >= units) return;
-  const int head = unit % p.hv, s = unit / p.hv, hk = head / p.group;
   const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, col = part * 16 * NC;
-  const Span span = span_of(p.slots, p.offsets, p.tokens, s);
-  if (!span.kept) return;
+  const int c = lane & 15, g = lane >> 4, rows4 = 16 * wave + 4 * g;
+  const Span& span = at.span;
   DeltaState<DK, NC> S;
-  float* state = p.state + ((long long)max(span.slot, 0) * p.hv + head) * DK * p.dv +
-                 (wave * (DK / 4) + 4 * g) * p.dv + col + c;
+  float* state = p.state + ((long long)max(span.slot, 0) * p.hv + at.head) * DK * p.dv +
+                 (wave * (DK / 4) + 4 * g) * p.dv + at.col + c;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -470,89 +505,48 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
       for (int r = 0; r < 4; ++r)
         S.s[i][n][r] = span.fresh ? 0.0f : state[(16 * i + r) * p.dv + 16 * n];
 
-  const int blocks = sreg((span.kept + kDeltaRows - 1) / kDeltaRows);
-  const int id0 = span.first / kDeltaRows + s;
-  DeltaBlock<DK, NC> B;
-  // v and out are addressed by resources that end with the block's last row: rows behind
-  // it read as zeros and are not stored, and a lane's offsets are the same in every block
-  const int rows4 = 16 * wave + 4 * g;
-  const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
-  const uint32_t at_v = (uint32_t)rows4 * step_v + 2 * c, at_out = (uint32_t)rows4 * step_out + 2 * c;
-  const f16* v0 = sreg(p.v + span.first * p.v_stride + head * p.dv + col);
-  f16* out0 = sreg(p.out + span.first * p.out_stride + head * p.dv + col);
-  auto block_rows = [&](const f16* x, uint32_t step, int b) {
-    const int live = min(kDeltaRows, span.kept - b * kDeltaRows);
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)b * kDeltaRows * (step / 2)), 0,
-                                             (uint32_t)(live - 1) * step + 32 * NC,
-                                             kBufferRsrcWord3);
+  // Each operand of the next block is on its way as soon as the present one is used, and
+  // not before (it takes the same registers), a few at a time.
+  f16x8 k[KB], t[2][2], kt[NT][2];
+  f32x4 beta, seen_by, left;
+  f16 v[NC][4];
+  float decay;
+  const uint32_t step = 2 * (uint32_t)p.v_stride, at_v = (uint32_t)rows4 * step + 2 * c;
+  const f16* v0 = sreg(p.v + span.first * p.v_stride + at.head * p.dv + at.col);
+  auto load_k = [&](int b) {
+    const auto keys = keys_of<DK>(p, at, b);
+#pragma unroll
+    for (int i = 0; i < KB; ++i) k[i] = piece_at(keys, wave * KB + i);
   };
-  auto head_of = [&](int b) {
-    return __builtin_amdgcn_make_buffer_rsrc(
-        p.heads + ((long long)(id0 + b) * p.hv + head) * kDeltaHead, 0, kDeltaHead,
-        kBufferRsrcWord3);
-  };
-  auto keys_of = [&](int b) {
-    return __builtin_amdgcn_make_buffer_rsrc(
-        p.keys + ((long long)(id0 + b) * p.hk + hk) * delta_key_bytes(DK), 0, delta_key_bytes(DK),
-        kBufferRsrcWord3);
-  };
-  auto factor = [&](__amdgpu_buffer_rsrc_t at, int which) {
-    return __builtin_bit_cast(
-        f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                   at, rows4 * 4, kDeltaFactors + which * kDeltaRows * 4, 0));
-  };
-  auto piece = [&](__amdgpu_buffer_rsrc_t at, int number) {
-    return __builtin_bit_cast(
-        f16x8, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, number * 1024, 0));
-  };
-  // (a piece past the resource's end, where the wave's rows have no column in it)
-  auto needed = [&](int i, int number) { return i <= wave / 2 ? number : 64; };
-  auto load_rows = [&](int b) {  // k, q and v
-    const auto rows = keys_of(b), rv = block_rows(v0, step_v, b), h = head_of(b);
+  auto load_v = [&](int b) {
+    const auto rows = rows_of(at, v0, step, 16 * NC, b), head = head_of(p, at, b);
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int n = 0; n < NC; ++n)
-        B.v[n][r] = __builtin_bit_cast(
-            f16, __builtin_amdgcn_raw_buffer_load_b16(rv, at_v + r * step_v + 32 * n, 0, 0));
-#pragma unroll
-    for (int i = 0; i < KB; ++i) {
-      B.k[i] = piece(rows, wave * KB + i);
-      B.q[i] = piece(rows, 4 * KB + wave * KB + i);
-    }
-    B.beta = factor(h, kBeta);
-    B.seen = factor(h, kSeen);
+        v[n][r] = __builtin_bit_cast(
+            f16, __builtin_amdgcn_raw_buffer_load_b16(rows, at_v + r * step + 32 * n, 0, 0));
+    beta = factor_of(head, kBeta, rows4);
+    seen_by = factor_of(head, kSeen, rows4);
   };
   auto load_t = [&](int b) {
-    const auto h = head_of(b);
-    B.left = factor(h, kLeft);
+    const auto head = head_of(p, at, b);
+    left = factor_of(head, kLeft, rows4);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int number = needed(i, 2 * piece_of(wave, i));
-      B.t[i][0] = piece(h, number);
-      B.t[i][1] = piece(h, number + 1);
+      const int number = needed(wave, i, 2 * piece_of(wave, i));
+      t[i][0] = piece_at(head, number);
+      t[i][1] = piece_at(head, number + 1);
     }
   };
-  auto load_out = [&](int b) {  // P and the transposed keys
-    const auto h = head_of(b), keys = keys_of(b);
-    B.ask = factor(h, kAsk);
-    B.decay = as_f32(
-        __builtin_amdgcn_raw_buffer_load_b32(h, 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) B.w[i] = piece(h, needed(i, 12 + piece_of(wave, i)));
+  auto load_kt = [&](int b) {
+    const auto keys = keys_of<DK>(p, at, b);
+    decay = as_f32(__builtin_amdgcn_raw_buffer_load_b32(
+        head_of(p, at, b), 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) B.kt[i][j] = piece(keys, 8 * KB + (wave * NT + i) * 2 + j);
-  };
-
-  // where a wave's values 4 g + r of a column go in a right operand of 32 rows, two fp16
-  // numbers to a value (`half`: which 16 rows)
-  auto put = [&](f16x8* part0, f16x8* part1, int to, int half, const f32x4& x) {
-    f16x4 x0, x1;
-    split4(x, x0, x1);
-    __builtin_memcpy((char*)(part0 + to) + 8 * half, &x0, 8);
-    __builtin_memcpy((char*)(part1 + to) + 8 * half, &x1, 8);
+      for (int j = 0; j < 2; ++j) kt[i][j] = piece_at(keys, 8 * KB + (wave * NT + i) * 2 + j);
   };
   auto state_top = [&](int n) {
     float m = top4(S.s[0][n]);
@@ -560,11 +554,13 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
     for (int i = 1; i < NT; ++i) m = fmaxf(m, top4(S.s[i][n]));
     return rows_max(m);
   };
-  load_rows(0);
+  load_k(0);
   __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
+  load_v(0);
+  __builtin_amdgcn_sched_barrier(0);
   load_t(0);
   __builtin_amdgcn_sched_barrier(0);
-  load_out(0);
+  load_kt(0);
   __builtin_amdgcn_sched_barrier(0);
   float bound[NC], top[NC];  // of |S| by column: at most, and in the wave's rows
 #pragma unroll
@@ -576,10 +572,14 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
 #pragma unroll
   for (int n = 0; n < NC; ++n) bound[n] = top4(*(const f32x4*)lds.first[n][c]);
 
-  int at_block = 0;
-  for (; at_block < blocks; ++at_block) {
-    const int b = sreg(at_block);
-    const int next = min(b + 1, blocks - 1);
+  // The first block in which something is not finite, and the state before it: a product
+  // with zeros takes it to rows before it, so that from there on the blocks are passed a
+  // second time, row after row.  (No way out of the loop: the waits of one that has another
+  // end are those of its worst path.)
+  int odd_block = at.blocks;
+  DeltaState<DK, NC> before = S;
+  for (int b = 0; b < at.blocks; ++b) {
+    const int next = min(b + 1, at.blocks - 1);
     // S in two parts, where all waves read them
     Lift ls[NC];
 #pragma unroll
@@ -589,36 +589,36 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int row = wave * (DK / 4) + 16 * i + 4 * g;
-        put(lds.s[0][row / 32][n], lds.s[1][row / 32][n], c + row % 32 / 8 * 16, row / 4 % 2,
-            S.s[i][n] * ls[n].by);
+        put_split(lds.s[0][row / 32][n], lds.s[1][row / 32][n], c + row % 32 / 8 * 16, row / 4 % 2,
+                  S.s[i][n] * ls[n].by);
       }
-      f32x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = (float)B.v[n][r];
+      lds.back_s[n][c] = ls[n].back;
       lds.top_s[n][c][wave] = top[n];
-      lds.top_v[n][c][wave] = rows_max(top4(v));
+      f32x4 x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = (float)v[n][r];
+      lds.top_v[n][c][wave] = rows_max(top4(x));
     }
     __syncthreads();
-    // S^T k and S^T q of the wave's 16 rows
-    f32x4 seen[NC], asked[NC];
+    // S^T k of the wave's 16 rows
+    f32x4 seen[NC];
     float top_s[NC], top_v[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 seen1 = f32x4{}, asked1 = f32x4{};
-      seen[n] = asked[n] = f32x4{};
+      f32x4 seen1 = f32x4{};
+      seen[n] = f32x4{};
 #pragma unroll
       for (int i = 0; i < KB; ++i) {
-        const f16x8 y0 = lds.s[0][i][n][lane], y1 = lds.s[1][i][n][lane];
-        seen[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.k[i], y0, seen[n], 0, 0, 0);
-        seen1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.k[i], y1, seen1, 0, 0, 0);
-        asked[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.q[i], y0, asked[n], 0, 0, 0);
-        asked1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.q[i], y1, asked1, 0, 0, 0);
+        seen[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], lds.s[0][i][n][lane], seen[n], 0, 0, 0);
+        seen1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], lds.s[1][i][n][lane], seen1, 0, 0, 0);
       }
       top_s[n] = top4(*(const f32x4*)lds.top_s[n][c]);
       top_v[n] = top4(*(const f32x4*)lds.top_v[n][c]);
       seen[n] = (seen[n] + seen1) * ls[n].back;
-      asked[n] = (asked[n] + asked1) * ls[n].back;
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(next);
+    __builtin_amdgcn_sched_barrier(0);
     // R in two parts; |R| is within |v| and the column's length
     Lift lr[NC];
     bool odd = false;
@@ -628,20 +628,21 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
       f32x4 x;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[r] = B.beta[r] * (float)B.v[n][r] - B.seen[r] * seen[n][r];
+        x[r] = beta[r] * (float)v[n][r] - seen_by[r] * seen[n][r];
         odd |= !(fabsf(x[r]) < INFINITY);
       }
-      put(lds.r[0][wave / 2][n], lds.r[1][wave / 2][n], lane, wave & 1, x * lr[n].by);
+      put_split(lds.r[0][wave / 2][n], lds.r[1][wave / 2][n], lane, wave & 1, x * lr[n].by);
       lds.top_r[n][c][wave] = rows_max(top4(x));
     }
     const bool any = __any(odd);
     if (lane == 0) lds.odd[wave] = any;
     __syncthreads();
-    if (sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3])) break;
-    // each operand of the next block is on its way as soon as the present one is used, and
-    // not before (it takes the same registers)
+    if (odd_block == at.blocks && sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3])) {
+      odd_block = b;
+      before = S;
+    }
     __builtin_amdgcn_sched_barrier(0);
-    load_rows(next);
+    load_v(next);
     __builtin_amdgcn_sched_barrier(0);
     // U = T R of the wave's rows
     f32x4 u[NC];
@@ -653,32 +654,30 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
       for (int i = 0; i < 2; ++i) {
         if (i > wave / 2) continue;
         const f16x8 r0 = lds.r[0][i][n][lane], r1 = lds.r[1][i][n][lane];
-        u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][0], r0, u[n], 0, 0, 0);
-        u1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][0], r1, u1, 0, 0, 0);
-        u2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.t[i][1], r0, u2, 0, 0, 0);
+        u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][0], r0, u[n], 0, 0, 0);
+        u1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][0], r1, u1, 0, 0, 0);
+        u2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][1], r0, u2, 0, 0, 0);
       }
       u[n] = (u[n] + (u1 + u2)) * (lr[n].back * (1.0f / kPieceScale));
     }
-    // U as it is for the outputs, times the rows' factors for the state; |U| is within
+    // U times the rows' factors for the state, as it is for the outputs; |U| is within
     // 64 |R|
     Lift lu[NC];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       lu[n] = lift_of(64.0f * top4(*(const f32x4*)lds.top_r[n][c]));
-      const f32x4 y = u[n] * B.left;
-      put(lds.u[2][wave / 2][n], lds.u[3][wave / 2][n], lane, wave & 1, y * lu[n].by);
-      put(lds.u[0][wave / 2][n], lds.u[1][wave / 2][n], lane, wave & 1, u[n] * lu[n].by);
+      const f32x4 y = u[n] * left;
+      put_split(lds.u[2][wave / 2][n], lds.u[3][wave / 2][n], lane, wave & 1, y * lu[n].by);
+      put_split(lds.u[0][wave / 2][n], lds.u[1][wave / 2][n], lane, wave & 1, u[n] * lu[n].by);
       lds.top_u[n][c][wave] = rows_max(top4(y));
     }
     __builtin_amdgcn_sched_barrier(0);
     load_t(next);
     __syncthreads();
-    // the state behind the block, and the outputs
-    f32x4 y[NC];
+    // the state behind the block
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      f32x4 add[NT][2], o[2];
-      o[0] = o[1] = f32x4{};
+      f32x4 add[NT][2];
 #pragma unroll
       for (int i = 0; i < NT; ++i) add[i][0] = add[i][1] = f32x4{};
 #pragma unroll
@@ -688,52 +687,32 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
           const f16x8 z = lds.u[2 + x][j][n][lane];
 #pragma unroll
           for (int i = 0; i < NT; ++i)
-            add[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.kt[i][j], z, add[i][x], 0, 0, 0);
+            add[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kt[i][j], z, add[i][x], 0, 0, 0);
         }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (j > wave / 2) continue;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          o[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(B.w[j], lds.u[x][j][n][lane], o[x], 0, 0, 0);
-      }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          S.s[i][n][r] =
-              fmaf(S.s[i][n][r], B.decay, (add[i][0][r] + add[i][1][r]) * lu[n].back);
-      bound[n] = fmaf(128.0f, top4(*(const f32x4*)lds.top_u[n][c]), top_s[n] * B.decay);
+          S.s[i][n][r] = fmaf(S.s[i][n][r], decay, (add[i][0][r] + add[i][1][r]) * lu[n].back);
+      bound[n] = fmaf(128.0f, top4(*(const f32x4*)lds.top_u[n][c]), top_s[n] * decay);
       top[n] = state_top(n);
-      const float back = p.scale * lu[n].back * (1.0f / kPieceScale);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        y[n][r] = fmaf(o[0][r] + o[1][r], back, B.ask[r] * asked[n][r]);
     }
     // (what the old operands are for is done before the new ones take their registers)
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      asm volatile("" : "+v"(y[n]), "+v"(bound[n]));
+      asm volatile("" : "+v"(bound[n]));
 #pragma unroll
       for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(S.s[i][n]));
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_out(next);
+    load_kt(next);
     __builtin_amdgcn_sched_barrier(0);
-    if (p.out) {
-      const auto to = block_rows(out0, step_out, b);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int n = 0; n < NC; ++n)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)y[n][r]), to,
-                                                at_out + r * step_out + 32 * n, 0, 0);
-    }
   }
-  // Where something is not finite, a product with zeros would take it to the rows before
-  // it: from that block on, row after row.
-  if (at_block < blocks)
-    delta_rows<DK, NC>(p, span, head, col, at_block * kDeltaRows, span.kept, S, lds);
+  if (odd_block < at.blocks) {
+    S = before;
+    __syncthreads();  // the rows' first outputs are in place before the second ones
+    delta_rows<DK, NC>(p, span, at.head, at.col, odd_block * kDeltaRows, span.kept, S, lds);
+  }
   if (!p.slots.store || span.slot < 0) return;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -741,6 +720,151 @@ __global__ __launch_bounds__(kThreads, 2) void delta_prompt_kernel(const DeltaPa
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int r = 0; r < 4; ++r) state[(16 * i + r) * p.dv + 16 * n] = S.s[i][n][r];
+}
+
+// The other four: the outputs, from the parts of S and U that the first four leave in LDS.
+template <int DK, int NC>
+__device__ __forceinline__ void delta_outputs(const DeltaParams& p, const DeltaPlace& at,
+                                              DeltaLds<DK, NC>& lds) {
+  constexpr int KB = DK / 32;
+  const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6) - kWaves;
+  const int c = lane & 15, g = lane >> 4, rows4 = 16 * wave + 4 * g;
+  const Span& span = at.span;
+  f16x8 q[KB], w[2];
+  f32x4 ask;
+  const uint32_t step = 2 * (uint32_t)p.out_stride, at_out = (uint32_t)rows4 * step + 2 * c;
+  const f16* out0 = sreg(p.out + span.first * p.out_stride + at.head * p.dv + at.col);
+  auto load_q = [&](int b) {
+    const auto keys = keys_of<DK>(p, at, b);
+#pragma unroll
+    for (int i = 0; i < KB; ++i) q[i] = piece_at(keys, 4 * KB + wave * KB + i);
+  };
+  auto load_w = [&](int b) {
+    const auto head = head_of(p, at, b);
+    ask = factor_of(head, kAsk, rows4);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = piece_at(head, needed(wave, i, 12 + piece_of(wave, i)));
+  };
+  // What a block takes comes from memory, later than a block takes to pass: a byte of each
+  // of its 128-byte lines is read two blocks ahead, a line a lane over the head's
+  // workgroups, so that the loads find them in the L2 that these share.
+  constexpr int kAhead = 2, key_lines = delta_key_bytes(DK) / 128;
+  constexpr int head_lines = (kDeltaHead + 127) / 128;
+  const int row_lines = p.dv / 64;  // of v
+  const int line = (at.part * kWaves + wave) * 64 + lane, v_line = line - key_lines - head_lines;
+  const char* warm = p.heads + ((long long)at.id0 * p.hv + at.head) * kDeltaHead;
+  long long warm_step = (long long)p.hv * kDeltaHead;
+  if (line < key_lines) {
+    warm = p.keys + ((long long)at.id0 * p.hk + at.hk) * delta_key_bytes(DK) + line * 128;
+    warm_step = (long long)p.hk * delta_key_bytes(DK);
+  } else if (v_line < 0) {
+    warm += (line - key_lines) * 128;
+  } else if (v_line < min(kDeltaRows, span.kept) * row_lines) {
+    warm = (const char*)(p.v + (span.first + v_line / row_lines) * p.v_stride + at.head * p.dv) +
+           v_line % row_lines * 128;
+    warm_step = kDeltaRows * p.v_stride * 2;
+  }
+  uint32_t warmed = 0;
+  auto warm_up = [&](int b) {  // (but the last block, which may have fewer rows)
+    asm volatile("" ::"v"(warmed));
+    warmed = *(const __attribute__((address_space(1))) uint8_t*)(
+        warm + max(min(b, at.blocks - 2), 0) * warm_step);
+  };
+  warm_up(1);
+  load_q(0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(0);
+  __builtin_amdgcn_sched_barrier(0);
+  __syncthreads();
+  int odd_block = at.blocks;
+  for (int b = 0; b < at.blocks; ++b) {
+    const int next = min(b + 1, at.blocks - 1);
+    warm_up(b + kAhead);
+    __syncthreads();
+    f32x4 asked[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 asked1 = f32x4{};
+      asked[n] = f32x4{};
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        asked[n] =
+            __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], lds.s[0][i][n][lane], asked[n], 0, 0, 0);
+        asked1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], lds.s[1][i][n][lane], asked1, 0, 0, 0);
+      }
+      const float back = lds.back_s[n][c];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) asked[n][r] = ask[r] * ((asked[n][r] + asked1[r]) * back);
+      asm volatile("" : "+v"(asked[n]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_q(next);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    if (odd_block == at.blocks && sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]))
+      odd_block = b;
+    float back[NC];
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+      back[n] = p.scale * (1.0f / kPieceScale) *
+                lift_of(64.0f * top4(*(const f32x4*)lds.top_r[n][c])).back;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 o[2];
+      o[0] = o[1] = f32x4{};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j > wave / 2) continue;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          o[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], lds.u[x][j][n][lane], o[x], 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) asked[n][r] = fmaf(o[0][r] + o[1][r], back[n], asked[n][r]);
+      asm volatile("" : "+v"(asked[n]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(next);
+    __builtin_amdgcn_sched_barrier(0);
+    if (p.out) {
+      const auto to = rows_of(at, out0, step, 16 * NC, b);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)asked[n][r]), to,
+                                                at_out + r * step + 32 * n, 0, 0);
+    }
+  }
+  if (odd_block == at.blocks) return;
+  // (the others' second pass, a barrier a row)
+  wait_vm<0>();
+  __syncthreads();
+  for (int t = odd_block * kDeltaRows; t < span.kept; ++t) __syncthreads();
+}
+
+template <int DK, int NC>
+__global__ __launch_bounds__(2 * kThreads, 2) void delta_prompt_kernel(const DeltaParams p) {
+  __shared__ DeltaLds<DK, NC> lds;
+  // the parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the
+  // same rows and pieces
+  const int parts = p.dv / (16 * NC), unit = blockIdx.x / (8 * parts) * 8 + blockIdx.x % 8;
+  if (unit >= p.slots.n * p.hv) return;
+  DeltaPlace at;
+  at.part = blockIdx.x / 8 % parts;
+  at.head = unit % p.hv;
+  at.hk = at.head / p.group;
+  at.col = at.part * 16 * NC;
+  const int s = unit / p.hv;
+  at.span = span_of(p.slots, p.offsets, p.tokens, s);
+  if (!at.span.kept) return;
+  at.blocks = sreg((at.span.kept + kDeltaRows - 1) / kDeltaRows);
+  at.id0 = at.span.first / kDeltaRows + s;
+  if (sreg((int)threadIdx.x >> 6) < kWaves)
+    delta_chain<DK, NC>(p, at, lds);
+  else
+    delta_outputs<DK, NC>(p, at, lds);
 }
 
 template <int DK, int NC>
@@ -752,7 +876,7 @@ static hipError_t prompt_launch(const DeltaParams& p, hipStream_t stream) {
   if (e != hipSuccess) return e;
   const long long units = ((long long)p.slots.n * p.hv + 7) / 8 * 8;
   hipLaunchKernelGGL((delta_prompt_kernel<DK, NC>), dim3((unsigned)(units * (p.dv / (16 * NC)))),
-                     dim3(kThreads), 0, stream, p);
+                     dim3(2 * kThreads), 0, stream, p);
   return hipGetLastError();
 }
 
