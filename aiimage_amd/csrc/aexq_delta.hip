@@ -36,104 +36,9 @@ __device__ __forceinline__ float rows_join(float v, F join) {
 __device__ __forceinline__ float rows_sum(float v) {
   return rows_join(v, [](float x, float y) { return x + y; });
 }
+// (maxima here are NaN where a value is)
 __device__ __forceinline__ float rows_max(float v) {
-  return rows_join(v, [](float x, float y) { return fmaxf(x, y); });
-}
-
-// ---------------------------------------------------------------------------
-// Packed prompts.  A workgroup takes NC blocks of 16 columns of S (columns are
-// independent of one another) of one value head of one sequence; its wave w holds
-// rows w DK / 4 .. of them in the layout of a matrix product's result: lane (c = l %
-// 16, g = l / 16) has rows 16 t + 4 g + r, column c of block n.
-// ---------------------------------------------------------------------------
-template <int DK, int NC>
-struct DeltaLds {
-  f16x8 s[2][DK / 32][NC][64];  // parts of S, R, U and U with the rows' factors
-  f16x8 r[2][2][NC][64];
-  f16x8 u[4][2][NC][64];
-  // the waves' largest magnitudes by column
-  alignas(16) float first[NC][16][kWaves], top_s[NC][16][kWaves], top_v[NC][16][kWaves];
-  alignas(16) float top_r[NC][16][kWaves], top_u[NC][16][kWaves];
-  float back_s[NC][16];  // what the parts of S are to be multiplied by
-  int odd[kWaves];
-  float sums[2][kWaves][2][NC][16];
-};
-
-template <int DK, int NC>
-struct DeltaState {
-  static constexpr int NT = DK / 64;  // 16-row tiles of a wave
-  f32x4 s[NT][NC];
-};
-
-// Row after row of [t0, t1), by four waves; a barrier a row.
-template <int DK, int NC>
-__device__ __forceinline__ void delta_rows(const DeltaParams& p, const Span& span, int head,
-                                           int col, int t0, int t1, DeltaState<DK, NC>& S,
-                                           DeltaLds<DK, NC>& lds) {
-  constexpr int NT = DK / 64;
-  const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  for (int t = t0; t < t1; ++t) {
-    const long long row = span.first + t;
-    const f16* kr = p.k + row * p.k_stride + head / p.group * DK;
-    const f16* qr = p.q + row * p.q_stride + head / p.group * DK;
-    float kk = 0.0f, qq = 0.0f, kq = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DK / 64; ++i) {
-      const float k = (float)kr[lane + 64 * i], q = (float)qr[lane + 64 * i];
-      kk = fmaf(k, k, kk);
-      qq = fmaf(q, q, qq);
-      kq = fmaf(k, q, kq);
-    }
-    const float rk = 1.0f / sqrtf(wave_sum(kk) + p.eps), rq = 1.0f / sqrtf(wave_sum(qq) + p.eps);
-    kq = wave_sum(kq) * rk;
-    const Gate gate = gate_of(p, row, head);
-    const float decay = expf(gate.g);
-    f16x4 k[NT], q[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      k[i] = *(const f16x4*)(kr + wave * (DK / 4) + 16 * i + 4 * g);
-      q[i] = *(const f16x4*)(qr + wave * (DK / 4) + 16 * i + 4 * g);
-    }
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      float sk = 0.0f, sq = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          S.s[i][n][r] *= decay;
-          sk = fmaf(S.s[i][n][r], (float)k[i][r], sk);
-          sq = fmaf(S.s[i][n][r], (float)q[i][r], sq);
-        }
-      sk = rows_sum(sk);
-      sq = rows_sum(sq);
-      if (g == 0) {
-        lds.sums[t & 1][wave][0][n][c] = sk;
-        lds.sums[t & 1][wave][1][n][c] = sq;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      float sk = 0.0f, sq = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        sk += lds.sums[t & 1][w][0][n][c];
-        sq += lds.sums[t & 1][w][1][n][c];
-      }
-      const int at = col + 16 * n + c;
-      const float v = (float)p.v[row * p.v_stride + head * p.dv + at];
-      const float u = gate.beta * (v - rk * sk);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          S.s[i][n][r] = fmaf((float)k[i][r] * rk, u, S.s[i][n][r]);
-      if (p.out && wave == 0 && g == 0)
-        p.out[row * p.out_stride + head * p.dv + at] = (f16)(p.scale * rq * fmaf(u, kq, sq));
-    }
-  }
+  return rows_join(v, [](float x, float y) { return __builtin_elementwise_maximum(x, y); });
 }
 
 // ---------------------------------------------------------------------------
@@ -175,6 +80,12 @@ enum : int { kBeta = 0, kSeen = 1, kAsk = 2, kLeft = 3, kDecay = 4 };
 // The power of two that takes a key of length 1 / rk to a length of 1/2 to 1.
 __device__ __forceinline__ float near_one(float rk) {
   return as_f32(f32_bits(rk) & 0x7f800000u);
+}
+
+// Row of S that row m of tile i of a state in registers is: a lane's rows of a pair of
+// tiles are eight in a row, as the products take them of k and q.
+__device__ __forceinline__ int state_row(int tile, int m) {
+  return tile / 2 * 32 + m / 4 * 8 + tile % 2 * 4 + m % 4;
 }
 
 // v of lane I of each row of 16 lanes.
@@ -269,7 +180,7 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int t = 32 * b + (e < 4 ? 0 : 16) + 4 * g + e % 4;
-      y[e] = (f16)((float)lds.k[t][16 * tile + c] * near_one(lds.rk[t]));
+      y[e] = (f16)((float)lds.k[t][state_row(tile, c)] * near_one(lds.rk[t]));
     }
     *(f16x8*)(keys + ((8 * KB + n) * 64 + lane) * 16) = y;
   }
@@ -422,452 +333,730 @@ __device__ __forceinline__ Lift lift_of(float bound) {
   const int e = min(max((int)(f32_bits(bound) >> 23 & 255), 14), 254);
   return Lift{as_f32((uint32_t)(267 - e) << 23), as_f32((uint32_t)(e - 13) << 23)};
 }
-
-// Two fp16 numbers x0 + x1 for four values.
-__device__ __forceinline__ void split4(const f32x4& x, f16x4& x0, f16x4& x1) {
-  x0 = __builtin_convertvector(x, f16x4);
+// The larger of m and the magnitudes of v.
+__device__ __forceinline__ float top4(float m, const f32x4& v) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) x1[r] = (f16)(x[r] - (float)x0[r]);
+  for (int r = 0; r < 4; r += 2)
+    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(v[r])), fabsf(v[r + 1]));
+  return m;
 }
-__device__ __forceinline__ float top4(const f32x4& v) {
-  return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-}
-
-// Where a wave's values 4 g + r of a column go in a right operand of 32 rows, two fp16
-// numbers to a value (`half`: which 16 rows).
-__device__ __forceinline__ void put_split(f16x8* part0, f16x8* part1, int to, int half,
-                                          const f32x4& x) {
-  f16x4 x0, x1;
-  split4(x, x0, x1);
-  __builtin_memcpy((char*)(part0 + to) + 8 * half, &x0, 8);
-  __builtin_memcpy((char*)(part1 + to) + 8 * half, &x1, 8);
-}
-
-// What the two halves of a workgroup have in common.
-struct DeltaPlace {
-  Span span;
-  int part, head, hk, col, blocks, id0;
+// Eight values as two fp16 numbers x0 + x1 each.
+struct Split {
+  f16x8 x0, x1;
 };
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t head_of(const DeltaParams& p,
-                                                          const DeltaPlace& at, int b) {
-  return __builtin_amdgcn_make_buffer_rsrc(
-      p.heads + ((long long)(at.id0 + b) * p.hv + at.head) * kDeltaHead, 0, kDeltaHead,
-      kBufferRsrcWord3);
-}
-template <int DK>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_of(const DeltaParams& p,
-                                                          const DeltaPlace& at, int b) {
-  return __builtin_amdgcn_make_buffer_rsrc(
-      p.keys + ((long long)(at.id0 + b) * p.hk + at.hk) * delta_key_bytes(DK), 0,
-      delta_key_bytes(DK), kBufferRsrcWord3);
-}
-// Rows of v and out (x: the sequence's first) are addressed by resources that end with the
-// block's last row: rows behind it read as zeros and are not stored, and a lane's offsets
-// are the same in every block.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const DeltaPlace& at, const f16* x,
-                                                          uint32_t step, int width, int b) {
-  const int live = min(kDeltaRows, at.span.kept - b * kDeltaRows);
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(x + (long long)b * kDeltaRows * (step / 2)), 0,
-                                           (uint32_t)(live - 1) * step + 2 * width,
-                                           kBufferRsrcWord3);
-}
-__device__ __forceinline__ f32x4 factor_of(__amdgpu_buffer_rsrc_t head, int which, int row) {
-  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                       head, row * 4, kDeltaFactors + which * kDeltaRows * 4, 0));
-}
-__device__ __forceinline__ f16x8 piece_at(__amdgpu_buffer_rsrc_t at, int number) {
-  const int lane = threadIdx.x & 63;
-  return __builtin_bit_cast(
-      f16x8, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, number * 1024, 0));
-}
-// (a piece past the resource's end, where the wave's rows have no column in it)
-__device__ __forceinline__ int needed(int wave, int b, int number) {
-  return b <= wave / 2 ? number : 64;
-}
-
-// The first four waves: the state from block to block.  Wave w has 16 rows of each block
-// and DK / 4 of the state.
-template <int DK, int NC>
-__device__ __forceinline__ void delta_chain(const DeltaParams& p, const DeltaPlace& at,
-                                            DeltaLds<DK, NC>& lds) {
-  constexpr int NT = DK / 64, KB = DK / 32;
-  const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4, rows4 = 16 * wave + 4 * g;
-  const Span& span = at.span;
-  DeltaState<DK, NC> S;
-  float* state = p.state + ((long long)max(span.slot, 0) * p.hv + at.head) * DK * p.dv +
-                 (wave * (DK / 4) + 4 * g) * p.dv + at.col + c;
+__device__ __forceinline__ Split split8(const f32x4& a, const f32x4& b) {
+  const f16x4 a0 = __builtin_convertvector(a, f16x4), b0 = __builtin_convertvector(b, f16x4);
+  f16x4 a1, b1;
+  float one = 1.0f;  // (a product that is seen as one: v_fma_mix takes x0 as it is, and rounds)
+  asm("" : "+s"(one));
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S.s[i][n][r] = span.fresh ? 0.0f : state[(16 * i + r) * p.dv + 16 * n];
-
-  // Each operand of the next block is on its way as soon as the present one is used, and
-  // not before (it takes the same registers), a few at a time.
-  f16x8 k[KB], t[2][2], kt[NT][2];
-  f32x4 beta, seen_by, left;
-  f16 v[NC][4];
-  float decay;
-  const uint32_t step = 2 * (uint32_t)p.v_stride, at_v = (uint32_t)rows4 * step + 2 * c;
-  const f16* v0 = sreg(p.v + span.first * p.v_stride + at.head * p.dv + at.col);
-  auto load_k = [&](int b) {
-    const auto keys = keys_of<DK>(p, at, b);
-#pragma unroll
-    for (int i = 0; i < KB; ++i) k[i] = piece_at(keys, wave * KB + i);
-  };
-  auto load_v = [&](int b) {
-    const auto rows = rows_of(at, v0, step, 16 * NC, b), head = head_of(p, at, b);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        v[n][r] = __builtin_bit_cast(
-            f16, __builtin_amdgcn_raw_buffer_load_b16(rows, at_v + r * step + 32 * n, 0, 0));
-    beta = factor_of(head, kBeta, rows4);
-    seen_by = factor_of(head, kSeen, rows4);
-  };
-  auto load_t = [&](int b) {
-    const auto head = head_of(p, at, b);
-    left = factor_of(head, kLeft, rows4);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int number = needed(wave, i, 2 * piece_of(wave, i));
-      t[i][0] = piece_at(head, number);
-      t[i][1] = piece_at(head, number + 1);
-    }
-  };
-  auto load_kt = [&](int b) {
-    const auto keys = keys_of<DK>(p, at, b);
-    decay = as_f32(__builtin_amdgcn_raw_buffer_load_b32(
-        head_of(p, at, b), 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) kt[i][j] = piece_at(keys, 8 * KB + (wave * NT + i) * 2 + j);
-  };
-  auto state_top = [&](int n) {
-    float m = top4(S.s[0][n]);
-#pragma unroll
-    for (int i = 1; i < NT; ++i) m = fmaxf(m, top4(S.s[i][n]));
-    return rows_max(m);
-  };
-  load_k(0);
-  __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
-  load_v(0);
-  __builtin_amdgcn_sched_barrier(0);
-  load_t(0);
-  __builtin_amdgcn_sched_barrier(0);
-  load_kt(0);
-  __builtin_amdgcn_sched_barrier(0);
-  float bound[NC], top[NC];  // of |S| by column: at most, and in the wave's rows
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    top[n] = state_top(n);
-    lds.first[n][c][wave] = top[n];  // (the four lanes of a column write the same)
+  for (int r = 0; r < 4; ++r) {
+    a1[r] = (f16)fmaf(a[r], one, -(float)a0[r]);
+    b1[r] = (f16)fmaf(b[r], one, -(float)b0[r]);
   }
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < NC; ++n) bound[n] = top4(*(const f32x4*)lds.first[n][c]);
+  return Split{__builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7),
+               __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+__device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
-  // The first block in which something is not finite, and the state before it: a product
-  // with zeros takes it to rows before it, so that from there on the blocks are passed a
-  // second time, row after row.  (No way out of the loop: the waits of one that has another
-  // end are those of its worst path.)
-  int odd_block = at.blocks;
-  DeltaState<DK, NC> before = S;
-  for (int b = 0; b < at.blocks; ++b) {
-    const int next = min(b + 1, at.blocks - 1);
-    // S in two parts, where all waves read them
-    Lift ls[NC];
+// ---------------------------------------------------------------------------
+// The blocks of a sequence in turn.  A wave takes 16 columns of S of one value head, and
+// nothing passes between waves: columns are independent of one another.  It holds them as
+// a product's result (state_row), which is a product's right operand as it stands, and so
+// are R and U; K, Q, T, P and the transposed keys come from scratch as left operands, each
+// piece for the next block as soon as the present one is done with it.
+//
+// S is kept times a power of two, by column, that takes it to fp16's range; the parts of R
+// and U have theirs, from their largest values.
+// ---------------------------------------------------------------------------
+template <int DK>
+struct DeltaWave {
+  static constexpr int KB = DK / 32;
+  const DeltaParams& p;
+  Span span;
+  int head, hk, col, id0, lane, c, g;
+  f32x4 S[2 * KB];  // times scale.by
+  Lift scale;
+
+  __device__ __forceinline__ DeltaWave(const DeltaParams& p) : p(p) {}
+
+  __device__ __forceinline__ float* state_at(int tile) const {
+    return p.state + ((long long)max(span.slot, 0) * p.hv + head) * DK * p.dv +
+           (long long)state_row(tile, 4 * g) * p.dv + col + c;
+  }
+  __device__ __forceinline__ void rescale(float by) {
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      ls[n] = lift_of(bound[n]);
-      // rows 16 i + 4 g .. of the wave's are an even or odd half of a lane's eight
+    for (int i = 0; i < 2 * KB; ++i) S[i] *= by;
+  }
+  __device__ __forceinline__ float top() const {
+    float m = 0.0f, n = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int row = wave * (DK / 4) + 16 * i + 4 * g;
-        put_split(lds.s[0][row / 32][n], lds.s[1][row / 32][n], c + row % 32 / 8 * 16, row / 4 % 2,
-                  S.s[i][n] * ls[n].by);
-      }
-      lds.back_s[n][c] = ls[n].back;
-      lds.top_s[n][c][wave] = top[n];
-      f32x4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = (float)v[n][r];
-      lds.top_v[n][c][wave] = rows_max(top4(x));
+    for (int i = 0; i < KB; ++i) {
+      m = top4(m, S[2 * i]);
+      n = top4(n, S[2 * i + 1]);
     }
-    __syncthreads();
-    // S^T k of the wave's 16 rows
-    f32x4 seen[NC];
-    float top_s[NC], top_v[NC];
+    return rows_max(__builtin_elementwise_maximum(m, n));
+  }
+  __device__ __forceinline__ void read() {
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      f32x4 seen1 = f32x4{};
-      seen[n] = f32x4{};
+    for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[i][r] = span.fresh ? 0.0f : state_at(i)[r * p.dv];
+    scale = lift_of(top());
+    rescale(scale.by);
+  }
+  __device__ __forceinline__ void write() {
+    if (!p.slots.store || span.slot < 0) return;
+    rescale(scale.back);
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) state_at(i)[r * p.dv] = S[i][r];
+  }
+
+  // Row after row of [t0, t1), S as it is.
+  __device__ __forceinline__ void rows(int t0, int t1) {
+    rescale(scale.back);
+    scale = Lift{1.0f, 1.0f};
+    for (int t = t0; t < t1; ++t) {
+      const long long row = span.first + t;
+      const f16* kr = p.k + row * p.k_stride + hk * DK + 8 * g;
+      const f16* qr = p.q + row * p.q_stride + hk * DK + 8 * g;
+      const Gate gate = gate_of(p, row, head);
+      const float decay = expf(gate.g);
+      float k[2 * KB][4], kk = 0.0f, qq = 0.0f, kq = 0.0f, sk = 0.0f, sq = 0.0f;
 #pragma unroll
       for (int i = 0; i < KB; ++i) {
-        seen[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], lds.s[0][i][n][lane], seen[n], 0, 0, 0);
-        seen1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[i], lds.s[1][i][n][lane], seen1, 0, 0, 0);
-      }
-      top_s[n] = top4(*(const f32x4*)lds.top_s[n][c]);
-      top_v[n] = top4(*(const f32x4*)lds.top_v[n][c]);
-      seen[n] = (seen[n] + seen1) * ls[n].back;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_k(next);
-    __builtin_amdgcn_sched_barrier(0);
-    // R in two parts; |R| is within |v| and the column's length
-    Lift lr[NC];
-    bool odd = false;
+        const f16x8 ki = *(const f16x8*)(kr + 32 * i), qi = *(const f16x8*)(qr + 32 * i);
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      lr[n] = lift_of(fmaf(top_s[n], 12.0f, top_v[n]));
-      f32x4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[r] = beta[r] * (float)v[n][r] - seen_by[r] * seen[n][r];
-        odd |= !(fabsf(x[r]) < INFINITY);
-      }
-      put_split(lds.r[0][wave / 2][n], lds.r[1][wave / 2][n], lane, wave & 1, x * lr[n].by);
-      lds.top_r[n][c][wave] = rows_max(top4(x));
-    }
-    const bool any = __any(odd);
-    if (lane == 0) lds.odd[wave] = any;
-    __syncthreads();
-    if (odd_block == at.blocks && sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3])) {
-      odd_block = b;
-      before = S;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(next);
-    __builtin_amdgcn_sched_barrier(0);
-    // U = T R of the wave's rows
-    f32x4 u[NC];
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      f32x4 u1 = f32x4{}, u2 = f32x4{};
-      u[n] = f32x4{};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i > wave / 2) continue;
-        const f16x8 r0 = lds.r[0][i][n][lane], r1 = lds.r[1][i][n][lane];
-        u[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][0], r0, u[n], 0, 0, 0);
-        u1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][0], r1, u1, 0, 0, 0);
-        u2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t[i][1], r0, u2, 0, 0, 0);
-      }
-      u[n] = (u[n] + (u1 + u2)) * (lr[n].back * (1.0f / kPieceScale));
-    }
-    // U times the rows' factors for the state, as it is for the outputs; |U| is within
-    // 64 |R|
-    Lift lu[NC];
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      lu[n] = lift_of(64.0f * top4(*(const f32x4*)lds.top_r[n][c]));
-      const f32x4 y = u[n] * left;
-      put_split(lds.u[2][wave / 2][n], lds.u[3][wave / 2][n], lane, wave & 1, y * lu[n].by);
-      put_split(lds.u[0][wave / 2][n], lds.u[1][wave / 2][n], lane, wave & 1, u[n] * lu[n].by);
-      lds.top_u[n][c][wave] = rows_max(top4(y));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_t(next);
-    __syncthreads();
-    // the state behind the block
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      f32x4 add[NT][2];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) add[i][0] = add[i][1] = f32x4{};
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const f16x8 z = lds.u[2 + x][j][n][lane];
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-            add[i][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kt[i][j], z, add[i][x], 0, 0, 0);
+        for (int e = 0; e < 8; ++e) {
+          const float x = (float)ki[e], y = (float)qi[e];
+          const float s = S[2 * i + e / 4][e % 4] * decay;
+          S[2 * i + e / 4][e % 4] = s;
+          k[2 * i + e / 4][e % 4] = x;
+          kk = fmaf(x, x, kk);
+          qq = fmaf(y, y, qq);
+          kq = fmaf(x, y, kq);
+          sk = fmaf(s, x, sk);
+          sq = fmaf(s, y, sq);
         }
+      }
+      const float rk = 1.0f / sqrtf(rows_sum(kk) + p.eps), rq = 1.0f / sqrtf(rows_sum(qq) + p.eps);
+      const float v = (float)p.v[row * p.v_stride + head * p.dv + col + c];
+      const float u = gate.beta * (v - rk * rows_sum(sk));
+      const float o = p.scale * rq * fmaf(u, rk * rows_sum(kq), rows_sum(sq));
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+      for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          S.s[i][n][r] = fmaf(S.s[i][n][r], decay, (add[i][0][r] + add[i][1][r]) * lu[n].back);
-      bound[n] = fmaf(128.0f, top4(*(const f32x4*)lds.top_u[n][c]), top_s[n] * decay);
-      top[n] = state_top(n);
+        for (int r = 0; r < 4; ++r) S[i][r] = fmaf(k[i][r] * rk, u, S[i][r]);
+      if (p.out && g == 0) p.out[row * p.out_stride + head * p.dv + col + c] = (f16)o;
     }
-    // (what the old operands are for is done before the new ones take their registers)
+  }
+
+  // ---- what a block takes
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t head_of(int b) const {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        p.heads + ((long long)(id0 + b) * p.hv + head) * kDeltaHead, 0, kDeltaHead,
+        kBufferRsrcWord3);
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_of(int b) const {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        p.keys + ((long long)(id0 + b) * p.hk + hk) * delta_key_bytes(DK), 0, delta_key_bytes(DK),
+        kBufferRsrcWord3);
+  }
+  // Rows of v and out are addressed by resources that end with the block's last row: rows
+  // behind it read as zeros and are not stored, and a lane's offsets are the same in every
+  // block.
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const f16* x, long long stride,
+                                                            int b) const {
+    const int live = min(kDeltaRows, span.kept - b * kDeltaRows);
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(x + (span.first + (long long)b * kDeltaRows) * stride + head * p.dv + col), 0,
+        2 * ((uint32_t)(live - 1) * (uint32_t)stride + 16), kBufferRsrcWord3);
+  }
+  __device__ __forceinline__ f16x8 piece(__amdgpu_buffer_rsrc_t at, int number) const {
+    return __builtin_bit_cast(
+        f16x8, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16, number * 1024, 0));
+  }
+  __device__ __forceinline__ f32x4 factor(__amdgpu_buffer_rsrc_t at, int which, int tile) const {
+    return __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                   at, 16 * g, kDeltaFactors + (which * kDeltaRows + 16 * tile) * 4, 0));
+  }
+};
+
+// The operands of blocks of TILES row tiles.
+template <int DK, int TILES>
+struct DeltaBlock {
+  static constexpr int KB = DK / 32, PAIRS = (TILES + 1) / 2;
+  f16x8 k[TILES][KB], q[TILES][KB];
+  f16x8 t[TILES][PAIRS][2], w[TILES][PAIRS];  // of T and P, by pairs of column tiles
+  f16x8 kt[2 * KB][PAIRS];
+  f32x4 beta[TILES], seen[TILES], ask[TILES], left[TILES];
+  f16 v[TILES][4];
+  float decay;
+  typedef DeltaWave<DK> W;
+
+  __device__ __forceinline__ void load_k(const W& x, int b) {
+    const auto at = x.keys_of(b);
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      asm volatile("" : "+v"(bound[n]));
+    for (int i = 0; i < KB; ++i)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(S.s[i][n]));
+      for (int w = 0; w < TILES; ++w) k[w][i] = x.piece(at, w * KB + i);
+  }
+  __device__ __forceinline__ void load_q(const W& x, int b) {
+    const auto at = x.keys_of(b);
+#pragma unroll
+    for (int i = 0; i < KB; ++i)
+#pragma unroll
+      for (int w = 0; w < TILES; ++w) q[w][i] = x.piece(at, (4 + w) * KB + i);
+  }
+  __device__ __forceinline__ void load_v(const W& x, int b) {
+    const auto at = x.rows_of(x.p.v, x.p.v_stride, b), h = x.head_of(b);
+    const uint32_t step = 2 * (uint32_t)x.p.v_stride, first = 4 * x.g * step + 2 * x.c;
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        v[w][r] = __builtin_bit_cast(
+            f16, __builtin_amdgcn_raw_buffer_load_b16(at, first + r * step, 16 * w * step, 0));
+      beta[w] = x.factor(h, kBeta, w);
+      seen[w] = x.factor(h, kSeen, w);
     }
+  }
+  __device__ __forceinline__ void load_t(const W& x, int b) {
+    const auto h = x.head_of(b);
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) {
+#pragma unroll
+      for (int j = 0; j <= w / 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) t[w][j][i] = x.piece(h, piece_of(w, j) * 2 + i);
+      left[w] = x.factor(h, kLeft, w);
+    }
+  }
+  __device__ __forceinline__ void load_w(const W& x, int b) {
+    const auto h = x.head_of(b);
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) {
+#pragma unroll
+      for (int j = 0; j <= w / 2; ++j) this->w[w][j] = x.piece(h, 12 + piece_of(w, j));
+      ask[w] = x.factor(h, kAsk, w);
+    }
+  }
+  __device__ __forceinline__ void load_kt(const W& x, int b) {
+    const auto at = x.keys_of(b);
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j)
+#pragma unroll
+      for (int i = 0; i < 2 * KB; ++i) kt[i][j] = x.piece(at, 8 * KB + 2 * i + j);
+    decay = as_f32(__builtin_amdgcn_raw_buffer_load_b32(
+        x.head_of(b), 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
+  }
+};
+
+// One block: the outputs, and the state behind it.  `next`: the block whose operands are
+// loaded meanwhile (below 0: none).  True where something is not finite: a product with
+// zeros takes it to the rows before it.
+template <int DK, int TILES>
+__device__ __forceinline__ bool delta_block(DeltaWave<DK>& x, DeltaBlock<DK, TILES>& o, int b,
+                                            int next) {
+  constexpr int KB = DK / 32, PAIRS = (TILES + 1) / 2;
+  const DeltaParams& p = x.p;
+  Split s[KB];
+#pragma unroll
+  for (int i = 0; i < KB; ++i) s[i] = split8(x.S[2 * i], x.S[2 * i + 1]);
+  f32x4 seen[TILES], asked[TILES];
+#pragma unroll
+  for (int w = 0; w < TILES; ++w) seen[w] = asked[w] = f32x4{};
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) seen[w] = mfma(o.k[w][i], s[i].x0, seen[w]);
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) seen[w] = mfma(o.k[w][i], s[i].x1, seen[w]);
+  }
+  if (next >= 0) {
     __builtin_amdgcn_sched_barrier(0);
-    load_kt(next);
+    o.load_k(x, next);
     __builtin_amdgcn_sched_barrier(0);
   }
-  if (odd_block < at.blocks) {
-    S = before;
-    __syncthreads();  // the rows' first outputs are in place before the second ones
-    delta_rows<DK, NC>(p, span, at.head, at.col, odd_block * kDeltaRows, span.kept, S, lds);
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) asked[w] = mfma(o.q[w][i], s[i].x0, asked[w]);
+#pragma unroll
+    for (int w = 0; w < TILES; ++w) asked[w] = mfma(o.q[w][i], s[i].x1, asked[w]);
   }
-  if (!p.slots.store || span.slot < 0) return;
+  // R
+  f32x4 r[2 * PAIRS];
+  float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int w = 0; w < 2 * PAIRS; ++w) {
+    r[w] = f32x4{};
+    if (w >= TILES) continue;
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
+    for (int e = 0; e < 4; ++e) {
+      r[w][e] = o.beta[w][e] * (float)o.v[w][e] - o.seen[w][e] * (seen[w][e] * x.scale.back);
+    }
+    m = top4(m, r[w]);
+  }
+  m = rows_max(m);
+  const bool odd = !(m < INFINITY);
+  const Lift lr = lift_of(m);
+  Split rs[PAIRS];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) state[(16 * i + r) * p.dv + 16 * n] = S.s[i][n][r];
+  for (int j = 0; j < PAIRS; ++j) rs[j] = split8(r[2 * j] * lr.by, r[2 * j + 1] * lr.by);
+  if (next >= 0) {
+    __builtin_amdgcn_sched_barrier(0);
+    o.load_v(x, next);
+    o.load_q(x, next);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // U = T R, by the largest of which and of the state the new scale goes: S is within its
+  // decayed columns and 64 of U's
+  f32x4 u[2 * PAIRS], y[2 * PAIRS];
+  float mu = 0.0f, my = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 2 * PAIRS; ++w) {
+    u[w] = y[w] = f32x4{};
+    if (w >= TILES) continue;
+#pragma unroll
+    for (int j = 0; j <= w / 2; ++j) {
+      u[w] = mfma(o.t[w][j][0], rs[j].x0, u[w]);
+      u[w] = mfma(o.t[w][j][0], rs[j].x1, u[w]);
+      u[w] = mfma(o.t[w][j][1], rs[j].x0, u[w]);
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < TILES; ++w) {
+    u[w] *= lr.back * (1.0f / kPieceScale);
+    y[w] = u[w] * o.left[w];
+    mu = top4(mu, u[w]);
+    my = top4(my, y[w]);
+  }
+  if (next >= 0) {
+    __builtin_amdgcn_sched_barrier(0);
+    o.load_t(x, next);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const Lift lu = lift_of(rows_max(mu));
+  const Lift ls = lift_of(fmaf(64.0f, rows_max(my), x.top() * (x.scale.back * o.decay)));
+  Split us[PAIRS], ys[PAIRS];
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) {
+    ys[j] = split8(y[2 * j] * ls.by, y[2 * j + 1] * ls.by);
+    us[j] = split8(u[2 * j] * lu.by, u[2 * j + 1] * lu.by);
+  }
+  const float keep = o.decay * x.scale.back * ls.by, before = x.scale.back;
+  x.rescale(keep);
+  x.scale = ls;
+#pragma unroll
+  for (int j = 0; j < PAIRS; ++j) {
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) x.S[i] = mfma(o.kt[i][j], ys[j].x0, x.S[i]);
+#pragma unroll
+    for (int i = 0; i < 2 * KB; ++i) x.S[i] = mfma(o.kt[i][j], ys[j].x1, x.S[i]);
+  }
+  f32x4 a[TILES];
+#pragma unroll
+  for (int w = 0; w < TILES; ++w) {
+    a[w] = f32x4{};
+#pragma unroll
+    for (int j = 0; j <= w / 2; ++j) {
+      a[w] = mfma(o.w[w][j], us[j].x0, a[w]);
+      a[w] = mfma(o.w[w][j], us[j].x1, a[w]);
+    }
+  }
+  const float back = p.scale * lu.back * (1.0f / kPieceScale);
+#pragma unroll
+  for (int w = 0; w < TILES; ++w) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      a[w][e] = fmaf(a[w][e], back, o.ask[w][e] * (asked[w][e] * before));
+    asm volatile("" : "+v"(a[w]));  // (before the operands' registers are loaded again)
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * KB; ++i) asm volatile("" : "+v"(x.S[i]));
+  if (next >= 0) {
+    __builtin_amdgcn_sched_barrier(0);
+    o.load_kt(x, next);
+    o.load_w(x, next);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  if (p.out) {
+    const auto to = x.rows_of(p.out, p.out_stride, b);
+    const uint32_t step = 2 * (uint32_t)p.out_stride, first = 4 * x.g * step + 2 * x.c;
+#pragma unroll
+    for (int w = 0; w < TILES; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)a[w][e]), to,
+                                              first + e * step, 16 * w * step, 0);
+  }
+  return odd;
 }
 
-// The other four: the outputs, from the parts of S and U that the first four leave in LDS.
-template <int DK, int NC>
-__device__ __forceinline__ void delta_outputs(const DeltaParams& p, const DeltaPlace& at,
-                                              DeltaLds<DK, NC>& lds) {
+// ---------------------------------------------------------------------------
+// Blocks of more than 16 rows go through two waves: one passes the state from block to
+// block, the other forms the outputs a block behind, from the parts of S and from U that
+// the first one leaves in LDS, and the first one's beta v a block ahead.  One barrier a
+// block.
+// ---------------------------------------------------------------------------
+template <int DK>
+struct DeltaLds {
+  f16x8 s[2][DK / 32][2][64];  // by the block's parity: parts of S
+  f32x4 u[2][4][64], v[2][4][64];
+  float back_s[2][64], back_u[2][64];  // what S and U are to be multiplied by
+};
+
+template <int DK>
+__device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds, int blocks,
+                                            bool& odd) {
   constexpr int KB = DK / 32;
-  const int lane = threadIdx.x & 63, wave = sreg((int)threadIdx.x >> 6) - kWaves;
-  const int c = lane & 15, g = lane >> 4, rows4 = 16 * wave + 4 * g;
-  const Span& span = at.span;
-  f16x8 q[KB], w[2];
-  f32x4 ask;
-  const uint32_t step = 2 * (uint32_t)p.out_stride, at_out = (uint32_t)rows4 * step + 2 * c;
-  const f16* out0 = sreg(p.out + span.first * p.out_stride + at.head * p.dv + at.col);
-  auto load_q = [&](int b) {
-    const auto keys = keys_of<DK>(p, at, b);
-#pragma unroll
-    for (int i = 0; i < KB; ++i) q[i] = piece_at(keys, 4 * KB + wave * KB + i);
+  const int lane = x.lane;
+  // Each operand is on its way as soon as the one before it in its registers is used, and
+  // not earlier; the keys and the transposed keys take turns in `a`.
+  f16x8 a[4 * KB], t[4][2][2];
+  f32x4 seen_by[4], left[4];
+  float decay;
+  auto load_k = [&](__amdgpu_buffer_rsrc_t at, int n) { a[n] = x.piece(at, n % 4 * KB + n / 4); };
+  auto load_kt = [&](__amdgpu_buffer_rsrc_t at, int n) {
+    a[n] = x.piece(at, 8 * KB + 2 * (n % (2 * KB)) + n / (2 * KB));
   };
-  auto load_w = [&](int b) {
-    const auto head = head_of(p, at, b);
-    ask = factor_of(head, kAsk, rows4);
+  auto load_seen = [&](__amdgpu_buffer_rsrc_t h) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) w[i] = piece_at(head, needed(wave, i, 12 + piece_of(wave, i)));
+    for (int w = 0; w < 4; ++w) seen_by[w] = x.factor(h, kSeen, w);
+  };
+  auto load_t = [&](__amdgpu_buffer_rsrc_t h) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int w = 2 * j; w < 4; ++w)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) t[w][j][i] = x.piece(h, piece_of(w, j) * 2 + i);
+  };
+  auto load_left = [&](__amdgpu_buffer_rsrc_t h) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) left[w] = x.factor(h, kLeft, w);
+    decay = as_f32(
+        __builtin_amdgcn_raw_buffer_load_b32(h, 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
+  };
+  {
+    const auto keys = x.keys_of(0), head = x.head_of(0);
+    load_seen(head);
+    __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
+    load_t(head);
+    __builtin_amdgcn_sched_barrier(0);
+    load_left(head);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 4 * KB; ++n) load_k(keys, n);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();  // the first block's v
+  for (int b = 0; b < blocks; ++b) {
+    const int next = min(b + 1, blocks - 1), at = b & 1;
+    const auto keys = x.keys_of(b);
+    f32x4 seen[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) seen[w] = f32x4{};
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+      const Split s = split8(x.S[2 * i], x.S[2 * i + 1]);
+      lds.s[at][i][0][lane] = s.x0;
+      lds.s[at][i][1][lane] = s.x1;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) seen[w] = mfma(a[4 * i + w], s.x0, seen[w]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) seen[w] = mfma(a[4 * i + w], s.x1, seen[w]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) load_kt(keys, 4 * i + w);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // R, times what takes its largest value to fp16's range
+    f32x4 r[4];
+    float m = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const f32x4 v = lds.v[at][w][lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        r[w][e] = fmaf(-seen_by[w][e], seen[w][e] * x.scale.back, v[e]);
+      m = top4(m, r[w]);
+    }
+    m = rows_max(m);
+    odd |= !(m < INFINITY);
+    const float top_s = x.top() * x.scale.back;
+    lds.back_s[at][lane] = x.scale.back;
+    const Lift lr = lift_of(m);
+    Split rs[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) rs[j] = split8(r[2 * j] * lr.by, r[2 * j + 1] * lr.by);
+    const auto head = x.head_of(next);
+    __builtin_amdgcn_sched_barrier(0);
+    load_seen(head);
+    __builtin_amdgcn_sched_barrier(0);
+    // U = T R
+    f32x4 u[4], y[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) u[w] = f32x4{};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int w = 2 * j; w < 4; ++w) u[w] = mfma(t[w][j][0], rs[j].x0, u[w]);
+#pragma unroll
+      for (int w = 2 * j; w < 4; ++w) u[w] = mfma(t[w][j][0], rs[j].x1, u[w]);
+#pragma unroll
+      for (int w = 2 * j; w < 4; ++w) u[w] = mfma(t[w][j][1], rs[j].x0, u[w]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_t(head);
+    __builtin_amdgcn_sched_barrier(0);
+    // U for the outputs, and times the rows' factors for the state, which stays within its
+    // decayed columns and 64 of these
+    const float back_u = lr.back * (1.0f / kPieceScale);
+    float my = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      lds.u[at][w][lane] = u[w];
+      y[w] = u[w] * left[w];
+      my = top4(my, y[w]);
+    }
+    lds.back_u[at][lane] = back_u;
+    const Lift ls = lift_of(fmaf(64.0f, rows_max(my) * back_u, top_s * decay));
+    const float to_y = back_u * ls.by, keep = decay * x.scale.back * ls.by;
+    Split ys[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) ys[j] = split8(y[2 * j] * to_y, y[2 * j + 1] * to_y);
+    x.rescale(keep);
+    x.scale = ls;
+    __builtin_amdgcn_sched_barrier(0);
+    load_left(head);
+    __builtin_amdgcn_sched_barrier(0);
+    const auto after = x.keys_of(next);
+#pragma unroll
+    for (int n = 0; n < 4 * KB; n += 4) {
+      const int j = n / (2 * KB);
+#pragma unroll
+      for (int i = n; i < n + 4; ++i) x.S[i % (2 * KB)] = mfma(a[i], ys[j].x0, x.S[i % (2 * KB)]);
+#pragma unroll
+      for (int i = n; i < n + 4; ++i) x.S[i % (2 * KB)] = mfma(a[i], ys[j].x1, x.S[i % (2 * KB)]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = n; i < n + 4; ++i) load_k(after, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+  }
+}
+
+template <int DK>
+__device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& lds, int blocks) {
+  constexpr int KB = DK / 32;
+  const DeltaParams& p = x.p;
+  const int lane = x.lane;
+  f16x8 q[4][KB], w[4][2];
+  f32x4 ask[4], beta[4];
+  f16 v[4][4];
+  const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
+  const uint32_t at_v = 4 * x.g * step_v + 2 * x.c, at_out = 4 * x.g * step_out + 2 * x.c;
+  auto load_v = [&](int b) {
+    const auto from = x.rows_of(p.v, p.v_stride, b), head = x.head_of(b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[i][e] = __builtin_bit_cast(
+            f16, __builtin_amdgcn_raw_buffer_load_b16(from, at_v + e * step_v, 16 * i * step_v, 0));
+      beta[i] = x.factor(head, kBeta, i);
+    }
+  };
+  auto put_v = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = beta[i][e] * (float)v[i][e];
+      lds.v[b & 1][i][lane] = y;
+    }
+  };
+  auto load_q = [&](__amdgpu_buffer_rsrc_t keys, int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j][i] = x.piece(keys, (4 + j) * KB + i);
+  };
+  auto load_w = [&](__amdgpu_buffer_rsrc_t head) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int j = 0; j <= i / 2; ++j) w[i][j] = x.piece(head, 12 + piece_of(i, j));
+      ask[i] = x.factor(head, kAsk, i);
+    }
   };
   // What a block takes comes from memory, later than a block takes to pass: a byte of each
-  // of its 128-byte lines is read two blocks ahead, a line a lane over the head's
+  // of its 128-byte lines is read some blocks ahead, two lines a lane over the head's
   // workgroups, so that the loads find them in the L2 that these share.
   constexpr int kAhead = 2, key_lines = delta_key_bytes(DK) / 128;
   constexpr int head_lines = (kDeltaHead + 127) / 128;
   const int row_lines = p.dv / 64;  // of v
-  const int line = (at.part * kWaves + wave) * 64 + lane, v_line = line - key_lines - head_lines;
-  const char* warm = p.heads + ((long long)at.id0 * p.hv + at.head) * kDeltaHead;
-  long long warm_step = (long long)p.hv * kDeltaHead;
-  if (line < key_lines) {
-    warm = p.keys + ((long long)at.id0 * p.hk + at.hk) * delta_key_bytes(DK) + line * 128;
-    warm_step = (long long)p.hk * delta_key_bytes(DK);
-  } else if (v_line < 0) {
-    warm += (line - key_lines) * 128;
-  } else if (v_line < min(kDeltaRows, span.kept) * row_lines) {
-    warm = (const char*)(p.v + (span.first + v_line / row_lines) * p.v_stride + at.head * p.dv) +
-           v_line % row_lines * 128;
-    warm_step = kDeltaRows * p.v_stride * 2;
+  const char* warm[2];
+  long long warm_step[2];
+  uint32_t warmed[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int line = (x.col / 16 * 2 + i) * 64 + lane, v_line = line - key_lines - head_lines;
+    warm[i] = p.heads + ((long long)x.id0 * p.hv + x.head) * kDeltaHead;
+    warm_step[i] = (long long)p.hv * kDeltaHead;
+    if (line < key_lines) {
+      warm[i] = p.keys + ((long long)x.id0 * p.hk + x.hk) * delta_key_bytes(DK) + line * 128;
+      warm_step[i] = (long long)p.hk * delta_key_bytes(DK);
+    } else if (v_line < 0) {
+      warm[i] += (line - key_lines) * 128;
+    } else if (v_line < min(kDeltaRows, x.span.kept) * row_lines) {
+      warm[i] = (const char*)(p.v + (x.span.first + v_line / row_lines) * p.v_stride +
+                              x.head * p.dv) + v_line % row_lines * 128;
+      warm_step[i] = kDeltaRows * p.v_stride * 2;
+    }
   }
-  uint32_t warmed = 0;
   auto warm_up = [&](int b) {  // (but the last block, which may have fewer rows)
-    asm volatile("" ::"v"(warmed));
-    warmed = *(const __attribute__((address_space(1))) uint8_t*)(
-        warm + max(min(b, at.blocks - 2), 0) * warm_step);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("" ::"v"(warmed[i]));
+      warmed[i] = *(const __attribute__((address_space(1))) uint8_t*)(
+          warm[i] + max(min(b, blocks - 2), 0) * warm_step[i]);
+    }
   };
   warm_up(1);
-  load_q(0);
+  load_v(0);
   __builtin_amdgcn_sched_barrier(0);
-  load_w(0);
+#pragma unroll
+  for (int i = 0; i < KB; ++i) load_q(x.keys_of(0), i);
+  __builtin_amdgcn_sched_barrier(0);
+  load_w(x.head_of(0));
+  __builtin_amdgcn_sched_barrier(0);
+  put_v(0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(min(1, blocks - 1));
   __builtin_amdgcn_sched_barrier(0);
   __syncthreads();
-  int odd_block = at.blocks;
-  for (int b = 0; b < at.blocks; ++b) {
-    const int next = min(b + 1, at.blocks - 1);
+  for (int b = 0; b < blocks; ++b) {
+    const int next = min(b + 1, blocks - 1), at = b & 1;
+    if (b + 1 < blocks) put_v(b + 1);
+    __builtin_amdgcn_sched_barrier(0);
     warm_up(b + kAhead);
-    __syncthreads();
-    f32x4 asked[NC];
+    load_v(min(b + 2, blocks - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();  // S and U of this block, v of the next
+    const auto keys = x.keys_of(next);
+    f32x4 u[4], o[4], a[4];
+    float m = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      f32x4 asked1 = f32x4{};
-      asked[n] = f32x4{};
+    for (int i = 0; i < 4; ++i) {
+      u[i] = lds.u[at][i][lane];
+      m = top4(m, u[i]);
+      a[i] = o[i] = f32x4{};
+    }
+    const Lift lu = lift_of(rows_max(m));
+    Split us[2];
 #pragma unroll
-      for (int i = 0; i < KB; ++i) {
-        asked[n] =
-            __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], lds.s[0][i][n][lane], asked[n], 0, 0, 0);
-        asked1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[i], lds.s[1][i][n][lane], asked1, 0, 0, 0);
-      }
-      const float back = lds.back_s[n][c];
+    for (int j = 0; j < 2; ++j) us[j] = split8(u[2 * j] * lu.by, u[2 * j + 1] * lu.by);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) asked[n][r] = ask[r] * ((asked[n][r] + asked1[r]) * back);
-      asm volatile("" : "+v"(asked[n]));
+    for (int i = 0; i < KB; ++i) {
+      const f16x8 s0 = lds.s[at][i][0][lane], s1 = lds.s[at][i][1][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = mfma(q[j][i], s0, a[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) a[j] = mfma(q[j][i], s1, a[j]);
+      __builtin_amdgcn_sched_barrier(0);
+      load_q(keys, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j], us[j].x0, o[i]);
+#pragma unroll
+      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j], us[j].x1, o[i]);
+    }
+    const float back_s = lds.back_s[at][lane];
+    const float back = p.scale * lu.back * lds.back_u[at][lane] * (1.0f / kPieceScale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = fmaf(o[i][e], back, ask[i][e] * (a[i][e] * back_s));
+      asm volatile("" : "+v"(o[i]));  // (before the operands' registers are loaded again)
     }
     __builtin_amdgcn_sched_barrier(0);
-    load_q(next);
-    __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
-    if (odd_block == at.blocks && sreg(lds.odd[0] | lds.odd[1] | lds.odd[2] | lds.odd[3]))
-      odd_block = b;
-    float back[NC];
-#pragma unroll
-    for (int n = 0; n < NC; ++n)
-      back[n] = p.scale * (1.0f / kPieceScale) *
-                lift_of(64.0f * top4(*(const f32x4*)lds.top_r[n][c])).back;
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      f32x4 o[2];
-      o[0] = o[1] = f32x4{};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (j > wave / 2) continue;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          o[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[j], lds.u[x][j][n][lane], o[x], 0, 0, 0);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) asked[n][r] = fmaf(o[0][r] + o[1][r], back[n], asked[n][r]);
-      asm volatile("" : "+v"(asked[n]));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_w(next);
+    load_w(x.head_of(next));
     __builtin_amdgcn_sched_barrier(0);
     if (p.out) {
-      const auto to = rows_of(at, out0, step, 16 * NC, b);
+      const auto to = x.rows_of(p.out, p.out_stride, b);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < NC; ++n)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)asked[n][r]), to,
-                                                at_out + r * step + 32 * n, 0, 0);
+        for (int e = 0; e < 4; ++e)
+          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)o[i][e]), to,
+                                                at_out + e * step_out, 16 * i * step_out, 0);
     }
   }
-  if (odd_block == at.blocks) return;
-  // (the others' second pass, a barrier a row)
-  wait_vm<0>();
-  __syncthreads();
-  for (int t = odd_block * kDeltaRows; t < span.kept; ++t) __syncthreads();
 }
 
-template <int DK, int NC>
-__global__ __launch_bounds__(2 * kThreads, 2) void delta_prompt_kernel(const DeltaParams p) {
-  __shared__ DeltaLds<DK, NC> lds;
+template <int DK>
+__global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams p) {
+  __shared__ DeltaLds<DK> lds;
   // the parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the
   // same rows and pieces
-  const int parts = p.dv / (16 * NC), unit = blockIdx.x / (8 * parts) * 8 + blockIdx.x % 8;
+  const int parts = p.dv / 16, unit = blockIdx.x / (8 * parts) * 8 + blockIdx.x % 8;
   if (unit >= p.slots.n * p.hv) return;
-  DeltaPlace at;
-  at.part = blockIdx.x / 8 % parts;
-  at.head = unit % p.hv;
-  at.hk = at.head / p.group;
-  at.col = at.part * 16 * NC;
   const int s = unit / p.hv;
-  at.span = span_of(p.slots, p.offsets, p.tokens, s);
-  if (!at.span.kept) return;
-  at.blocks = sreg((at.span.kept + kDeltaRows - 1) / kDeltaRows);
-  at.id0 = at.span.first / kDeltaRows + s;
-  if (sreg((int)threadIdx.x >> 6) < kWaves)
-    delta_chain<DK, NC>(p, at, lds);
-  else
-    delta_outputs<DK, NC>(p, at, lds);
+  DeltaWave<DK> x(p);
+  x.span = span_of(p.slots, p.offsets, p.tokens, s);
+  if (!x.span.kept) return;
+  x.head = unit % p.hv;
+  x.hk = x.head / p.group;
+  x.col = blockIdx.x / 8 % parts * 16;
+  x.id0 = x.span.first / kDeltaRows + s;
+  x.lane = threadIdx.x & 63;
+  x.c = x.lane & 15;
+  x.g = x.lane >> 4;
+  const int all = (x.span.kept + kDeltaRows - 1) / kDeltaRows;
+  // a last block of up to 16 rows takes a quarter of the products, and one wave
+  const bool short_end = x.span.kept - (all - 1) * kDeltaRows <= 16;
+  const int blocks = sreg(all - short_end);
+  if (sreg((int)threadIdx.x >> 6)) {
+    if (!blocks) return;
+    delta_outputs<DK>(x, lds, blocks);
+    wait_vm<0>();
+    __syncthreads();
+    return;
+  }
+  x.read();
+  bool odd = false;
+  if (blocks) delta_solve<DK>(x, lds, blocks, odd);
+  if (short_end) {
+    DeltaBlock<DK, 1> o;
+    o.load_k(x, blocks);
+    o.load_v(x, blocks);
+    o.load_q(x, blocks);
+    o.load_t(x, blocks);
+    o.load_kt(x, blocks);
+    o.load_w(x, blocks);
+    odd |= delta_block<DK, 1>(x, o, blocks, -1);
+  }
+  if (blocks) __syncthreads();  // the outputs are in place
+  if (__any(odd)) {
+    wait_vm<0>();
+    // from the start again, row after row (the state in memory is still the one before)
+    x.read();
+    x.rows(0, x.span.kept);
+  }
+  x.write();
 }
 
-template <int DK, int NC>
+template <int DK>
 static hipError_t prompt_launch(const DeltaParams& p, hipStream_t stream) {
   const long long blocks = row_blocks(p.tokens, p.slots.n, kDeltaRows);
   hipLaunchKernelGGL(delta_block_kernel<DK>, dim3((unsigned)(blocks * p.hk)), dim3(kThreads), 0,
@@ -875,15 +1064,13 @@ static hipError_t prompt_launch(const DeltaParams& p, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const long long units = ((long long)p.slots.n * p.hv + 7) / 8 * 8;
-  hipLaunchKernelGGL((delta_prompt_kernel<DK, NC>), dim3((unsigned)(units * (p.dv / (16 * NC)))),
-                     dim3(2 * kThreads), 0, stream, p);
+  hipLaunchKernelGGL(delta_prompt_kernel<DK>, dim3((unsigned)(units * (p.dv / 16))), dim3(128), 0,
+                     stream, p);
   return hipGetLastError();
 }
 
 hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream) {
-  const bool few = (long long)p.slots.n * p.hv * (p.dv / 32) < cus;
-  if (p.dk == 64) return few ? prompt_launch<64, 1>(p, stream) : prompt_launch<64, 2>(p, stream);
-  return few ? prompt_launch<128, 1>(p, stream) : prompt_launch<128, 2>(p, stream);
+  return p.dk == 64 ? prompt_launch<64>(p, stream) : prompt_launch<128>(p, stream);
 }
 
 // ---------------------------------------------------------------------------
