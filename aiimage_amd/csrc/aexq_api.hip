@@ -2677,19 +2677,21 @@ extern "C" aexq_status aexq_verify_drafts(aexq_ctx* ctx, const aexq_tensor* logi
   p.parts = verify_parts(p.rows, p.n, esize, ctx->cus);
   const int ve = 16 / esize;  // chunks of a row that starts anywhere in one
   p.cols = (int)(((long long)p.n + 2 * ve - 2) / ve / p.parts + 1);
-  p.parts2 = verify_parts(sequences, p.n, 16, ctx->cus);
-  p.run = (p.n + p.parts2 - 1) / p.parts2;
+  p.runs = verify_runs(p.n);
+  p.run = (p.n + p.runs - 1) / p.runs;
+  p.blocks = verify_blocks(sequences, p.runs, ctx->cus);
   HIP_TRY(op, hipSetDevice(ctx->device));
-  const long long parts = (long long)p.rows * p.parts;
-  const long long sums = 2LL * sequences * p.parts2;
+  const long long parts = (long long)p.rows * p.parts, runs = (long long)sequences * p.runs;
   st = grow_step_scratch(ctx, &ctx->verify_mem, &ctx->verify_cap,
-                         parts * 16 + sums * 8 + sequences * 32LL, op, "draft verification");
+                         sequences * 32LL + p.rows * 16LL + runs * 16 + parts * 16, op,
+                         "draft verification");
   if (st) return st;
   char* mem = (char*)ctx->verify_mem;  // (16-byte entries first)
   p.plan = (int4*)mem;
-  p.norm = (double2*)(mem + sequences * 16LL);
-  p.sums = (double*)(mem + sequences * 32LL);
-  p.z = p.sums + sums;
+  p.norm = (double2*)(p.plan + sequences);
+  p.draft = (VerifyDraft*)(p.norm + sequences);
+  p.sums = (double2*)(p.draft + p.rows);
+  p.z = (double*)(p.sums + runs);
   p.m = (float*)(p.z + parts);
   p.at = (int*)(p.m + parts);
   const hipError_t e = verify_launch(p, ctx->stream);

@@ -60,7 +60,15 @@ constexpr int delta_key_bytes(int dk) { return 3 * dk * kDeltaRows * 2; }
 hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream);
 hipError_t delta_decode_launch(const DeltaParams& p, int cus, hipStream_t stream);
 // ---- drafted tokens against the target's probabilities (aexq_verify.hip)
-constexpr int kVerifyParts = 64;  // parts of a row at most: a lane each
+constexpr int kVerifyParts = 64;   // parts of a row at most: a lane each
+constexpr int kVerifyRuns = 256;   // runs of a sampled row at most: a thread each
+// The draft behind a row, its logit, and what its probability has to pass (+inf where it
+// is none).
+struct VerifyDraft {
+  double need;
+  float x;
+  int token;
+};
 struct VerifyParams {
   const void* x;  // [rows][rstride] logits, n of each row
   int f16;
@@ -75,17 +83,22 @@ struct VerifyParams {
   const float *accept_u, *sample_u;
   int32_t *counts, *tokens;
   int parts, cols;    // parts of a row in the first pass, 16-byte chunks of each
-  int parts2, run;    // parts of a sampled row, and values of each
+  int runs, run;      // runs of a sampled row, and values of each
+  int blocks;         // workgroups that sum the runs of a sequence
   // scratch: of each (row, part) the sum of weights, the largest logit and its
-  // index; of each sequence's sampled row the parts' sums; what was decided
+  // index; of each row its draft; of each sequence's sampled row the runs' sums, all
+  // of it and without the draft's probabilities; what was decided
   double* z;
   float* m;
   int* at;
-  double* sums;  // [sequences][parts2][2]
+  VerifyDraft* draft;
+  double2* sums;  // [sequences][runs]
   int4* plan;    // row, mode, greedy token, accepted rows
   double2* norm; // largest logit and sum of weights of the sampled row
 };
 int verify_parts(long long rows, int n, int esize, int cus);
+int verify_runs(int n);
+int verify_blocks(int sequences, int runs, int cus);
 hipError_t verify_launch(const VerifyParams& p, hipStream_t stream);
 
 }  // namespace aexq

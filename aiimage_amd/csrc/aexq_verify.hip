@@ -1,4 +1,6 @@
 // Verification of drafted tokens against the target's probabilities (gfx950).
+#include <float.h>
+#include <limits.h>
 #include <math.h>
 
 #include "aexq_rows.hpp"
@@ -23,23 +25,25 @@ namespace aexq {
 // ---------------------------------------------------------------------------
 constexpr double kLog2eD = 1.4426950408889634074;
 
-// 2^y for y <= 1000; 0 below -1074.  |error| < 2^-41 of it: the series of 2^f, f in
-// [-1/2, 1/2], has (ln 2 / 2)^11 / 11! = 2^-42 behind its tenth power.
+// 2^y for y <= 1000, |error| < 2^-39 of it; 0 below -1023 and for a NaN.  y = n + f with
+// n whole, f in [-1/2, 1/2]: 2^f is the polynomial of degree 8 that is 1 at 0 and whose
+// largest relative error, 1.07e-12 = 2^-39.8, is least (the exchange method; the series
+// needs degree 10 for that).  Adding 1.5 * 2^52 leaves n in the sum's low bits; n is added
+// to the exponent of 2^f, which at y = -1023 is that of 1: nothing is left.
 __device__ __forceinline__ double exp2_series(double y) {
-  y = fmax(y, -1100.0);
-  const double n = rint(y), f = y - n;
-  double p = 7.054911620801121e-9;
-  p = fma(p, f, 1.0178086009239696e-7);
-  p = fma(p, f, 1.3215486790144305e-6);
-  p = fma(p, f, 1.5252733804059838e-5);
-  p = fma(p, f, 1.5403530393381606e-4);
-  p = fma(p, f, 1.3333558146428441e-3);
-  p = fma(p, f, 9.618129107628477e-3);
-  p = fma(p, f, 5.550410866482157e-2);
-  p = fma(p, f, 2.402265069591007e-1);
-  p = fma(p, f, 6.931471805599453e-1);
+  y = fmax(y, -1023.0);
+  const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);
+  double p = 1.3255224878668817e-6;
+  p = fma(p, f, 1.5310079402249296e-5);
+  p = fma(p, f, 1.5403455852453838e-4);
+  p = fma(p, f, 1.3333450568000645e-3);
+  p = fma(p, f, 9.618129159402558e-3);
+  p = fma(p, f, 5.550410941205933e-2);
+  p = fma(p, f, 2.402265069581299e-1);
+  p = fma(p, f, 6.931471805459335e-1);
   p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) +
+                                        (__builtin_bit_cast(uint64_t, t) << 52));
 }
 
 // What a row's logits are scaled by, in log2 units; 0 or below: the largest one wins.
@@ -47,9 +51,10 @@ __device__ __forceinline__ double heat_of(const VerifyParams& p, int s) {
   const float t = p.temperature ? p.temperature[s] : 1.0f;
   return t > 0.0f ? kLog2eD / (double)t : -1.0;
 }
-// A weight relative to the largest logit's; -inf weighs nothing at any temperature.
+// The weight of logit x relative to that of m; nothing for -inf, above all others if m
+// is -inf.
 __device__ __forceinline__ double weight_of(float x, float m, double heat) {
-  return x == -INFINITY ? 0.0 : exp2_series(((double)x - (double)m) * heat);
+  return exp2_series(((double)x - (double)fmaxf(m, -FLT_MAX)) * heat);
 }
 
 struct Best {
@@ -83,9 +88,50 @@ __device__ __forceinline__ int sequence_of(const VerifyParams& p, int t) {
   return sreg(lo);
 }
 
+// A DPP move of a double; 0 where a lane has no source.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double last_lane(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, 63);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sums up to and with each lane's, without a trip through LDS: inside rows of 16 lanes
+// (row_shr), then the last lane's of a row to the next, of two rows to the next two.
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp64<0x111, 0xF>(v);
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);
+  v += dpp64<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) { return last_lane(wave_scan(v)); }
+// The best of a wave, in every lane.
+__device__ __forceinline__ Best wave_best(Best v) {
+  auto join = [&](auto move) {
+    v = better(v, Best{move(v.m), __builtin_bit_cast(int, move(__builtin_bit_cast(float, v.at)))});
+  };
+  join([](float x) { return dpp<0x128>(x); });
+  join([](float x) { return dpp<0x124>(x); });
+  join([](float x) { return dpp<0x4E>(x); });
+  join([](float x) { return dpp<0xB1>(x); });
+  join([](float x) { return dpp_rows<0x142, 0xA>(x, x); });
+  join([](float x) { return dpp_rows<0x143, 0xC>(x, x); });
+  return Best{__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v.m), 63)),
+              __builtin_amdgcn_readlane(v.at, 63)};
+}
+
 template <typename E>
-__global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParams p) {
-  constexpr int VE = 16 / (int)sizeof(E);
+__global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(const VerifyParams p) {
+  constexpr int VE = 16 / (int)sizeof(E), U = 4;
   __shared__ Best best_of[kWaves];
   __shared__ double sum_of[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -95,54 +141,86 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(const VerifyParam
   if (row < rows.first || row >= rows.first + rows.n) return;
   const double heat = heat_of(p, s);
   const E* x = (const E*)p.x + (long long)row * p.rstride;
+  if (part == 0 && tid == 0) {
+    // the draft behind the row, and what its weight over Z has to pass
+    VerifyDraft d = {INFINITY, -INFINITY, -1};
+    if (row + 1 < rows.first + rows.n) {
+      const int token = p.drafts[row];
+      if (token >= 0 && token < p.n) {
+        const double q = p.probs ? p.probs[row * p.probs_stride + token] : 1.0f;
+        d = VerifyDraft{(double)p.accept_u[row] * q, (float)x[token], token};
+      }
+    }
+    p.draft[row] = d;
+  }
   // chunks lie on 16-byte boundaries: chunk c starts at logit c VE - skew
   const int skew = (int)((uintptr_t)x % 16 / sizeof(E));
   const int chunks = (int)(((long long)p.n + skew + VE - 1) / VE);
   const int c0 = min(part * p.cols, chunks), c1 = min(c0 + p.cols, chunks);
+  const int whole0 = skew ? 1 : 0, whole1 = (int)(((long long)p.n + skew) / VE);
   typedef E Chunk __attribute__((ext_vector_type(VE)));
-  auto read = [&](int c) {
-    const int i0 = c * VE - skew;
-    Chunk v;
-    if (i0 >= 0 && i0 <= p.n - VE) {
-      v = *(const Chunk*)(x + i0);
-    } else {
+  // U chunks of a thread, the ones of neighbours next to each other
+  auto read = [&](int c, Chunk* v) {
+    if (c >= whole0 && c + (U - 1) * kThreads < min(c1, whole1)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = *(const Chunk*)(x + (c + u * kThreads) * VE - skew);
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = c + u * kThreads, i0 = at * VE - skew;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        v[i] = (E)-INFINITY;
-        if (i0 + i >= 0 && i0 + i < p.n) v[i] = x[i0 + i];
+        v[u][i] = (E)-INFINITY;
+        if (at < c1 && i0 + i >= 0 && i0 + i < p.n) v[u][i] = x[i0 + i];
       }
     }
-    return v;
   };
   Best best = {-INFINITY, p.n};
-  bool odd = false;  // a NaN or a +inf: the row has no probabilities
   double z = 0.0;
-  for (int c = c0 + tid; c < c1; c += kThreads) {
-    const Chunk v = read(c);
-    const float old = best.m;
+  float from = -FLT_MAX;  // what the weights are relative to; none is above 2^500
+  if (heat < 0.0) {
+    bool odd = false;  // a NaN or a +inf: the row has no largest logit
+    for (int c = c0 + tid; c < c1; c += U * kThreads) {
+      Chunk v[U];
+      read(c, v);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const float y = (float)v[i];
-      odd |= !(y < INFINITY);
-      if (y > best.m) best = Best{y, c * VE - skew + i};
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float y = (float)v[u][i];
+          odd |= !(y < INFINITY);
+          if (y > best.m) best = Best{y, (c + u * kThreads) * VE - skew + i};
+        }
     }
-    if (heat < 0.0 || best.m == -INFINITY) continue;
-    if (best.m > old) z *= weight_of(old, best.m, heat);
+    if (odd) z = __builtin_nan("");
+  } else {
+    for (int c = c0 + tid; c < c1; c += U * kThreads) {
+      Chunk v[U];
+      read(c, v);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) z += weight_of((float)v[i], best.m, heat);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          best.m = __builtin_elementwise_maximum(best.m, (float)v[u][i]);
+      if (((double)best.m - (double)from) * heat > 500.0) {
+        z *= weight_of(from, best.m, heat);
+        from = best.m;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) z += weight_of((float)v[u][i], from, heat);
+    }
+    if (!(best.m < INFINITY)) z = __builtin_nan("");
   }
-  if (odd) z = __builtin_nan("");
-  const float own = best.m;
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1)
-    best = better(best, Best{__shfl_xor(best.m, off, 64), __shfl_xor(best.at, off, 64)});
+  best = wave_best(best);
   if (lane == 0) best_of[wave] = best;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) best = better(best, best_of[w]);
-  if (best.m > -INFINITY) z *= weight_of(own, best.m, fmax(heat, 0.0));
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) z += __shfl_xor(z, off, 64);
+  if (best.m > -INFINITY) z *= weight_of(from, best.m, fmax(heat, 0.0));
+  z = wave_sum(z);
   if (lane == 0) sum_of[wave] = z;
   __syncthreads();
   if (tid) return;
@@ -162,170 +240,189 @@ struct Chosen {
   float m;
   double z;
 };
-// Rows in turn, by a whole wave; a lane joins a part.
-__device__ __forceinline__ Chosen choose(const VerifyParams& p, int s, const Rows& rows) {
-  const int lane = threadIdx.x & 63;
-  const double heat = heat_of(p, s);
+// By the whole workgroup, two rows a wave at a time; a lane joins a part.
+__device__ __forceinline__ Chosen choose(const VerifyParams& p, const Rows& rows, double heat,
+                                         Chosen* of, int* goes_on) {
+  constexpr int K = 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Chosen r = {rows.first, kNone, -1, 0.0f, 0.0};
-  for (int i = 0; i < rows.n; ++i) {
-    const int row = rows.first + i;
-    Best best = {-INFINITY, p.n};
-    double z = 0.0;
-    if (lane < p.parts) {
-      const long long from = (long long)row * p.parts + lane;
-      best = Best{p.m[from], p.at[from]};
-      z = p.z[from];
+  for (int i0 = 0; i0 < rows.n; i0 += K * kWaves) {
+    Best best[K];
+    double z[K];
+    VerifyDraft d[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int row = rows.first + min(i0 + K * wave + k, rows.n - 1);
+      const long long at = (long long)row * p.parts + min(lane, p.parts - 1);
+      best[k] = Best{p.m[at], p.at[at]};
+      z[k] = p.z[at];
+      d[k] = p.draft[row];
     }
-    const float own = best.m;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1)
-      best = better(best, Best{__shfl_xor(best.m, off, 64), __shfl_xor(best.at, off, 64)});
-    if (best.m > -INFINITY) z *= weight_of(own, best.m, fmax(heat, 0.0));
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) z += __shfl_xor(z, off, 64);
-    r = Chosen{row, kNone, best.at, best.m, z};
-    // (z is NaN where a logit is, and no sum where every one is -inf)
-    if (!(best.m > -INFINITY) || !(z < INFINITY)) return r;
-    const bool last = i == rows.n - 1;
-    r.mode = heat < 0.0 ? kGreedy : last ? kFull : kRest;
-    if (last) return r;
-    const int draft = p.drafts[row];
-    bool stays = false;
-    if (draft >= 0 && draft < p.n) {
-      if (heat < 0.0) {
-        stays = draft == best.at;
-      } else {
-        const long long at = (long long)row * p.rstride + draft;
-        const float x = p.f16 ? (float)((const f16*)p.x)[at] : ((const float*)p.x)[at];
-        const double q = p.probs ? p.probs[row * p.probs_stride + draft] : 1.0f;
-        stays = (double)p.accept_u[row] * q < weight_of(x, best.m, heat) / z;
+    for (int k = 0; k < K; ++k) {
+      const int i = i0 + K * wave + k;
+      if (lane >= p.parts) best[k] = Best{-INFINITY, p.n}, z[k] = 0.0;
+      const float own = best[k].m;
+      best[k] = wave_best(best[k]);
+      if (best[k].m > -INFINITY) z[k] *= weight_of(own, best[k].m, fmax(heat, 0.0));
+      z[k] = wave_sum(z[k]);
+      // (z is NaN where a logit is, and no sum where every one is -inf)
+      const bool none = !(best[k].m > -INFINITY) || !(z[k] < INFINITY);
+      const bool last = i >= rows.n - 1;
+      const bool stays = heat < 0.0 ? d[k].token == best[k].at
+                                    : d[k].need < weight_of(d[k].x, best[k].m, heat) / z[k];
+      if (lane == 0) {
+        const int mode = none ? kNone : heat < 0.0 ? kGreedy : last ? kFull : kRest;
+        of[K * wave + k] = Chosen{rows.first + i, mode, best[k].at, best[k].m, z[k]};
+        goes_on[K * wave + k] = !none && !last && stays;
       }
     }
-    if (!stays) return r;
+    __syncthreads();
+    const uint64_t ends = __ballot(!goes_on[min(lane, K * kWaves - 1)]);
+    const int n = ends ? __ffsll((unsigned long long)ends) - 1 : K * kWaves - 1;
+    r = of[n];
+    const bool on = goes_on[n];
+    __syncthreads();
+    if (!on) return r;
   }
   return r;
 }
 
-// The weights of index j of the sampled row.
+// The weights of index j of the sampled row; none from `end` on.
 struct Weights {
   double full, rest;
 };
-__device__ __forceinline__ Weights weights_of(const VerifyParams& p, const Chosen& r, double heat,
-                                              int draft, int j) {
-  const long long at = (long long)r.row * p.rstride + j;
-  const float x = p.f16 ? (float)((const f16*)p.x)[at] : ((const float*)p.x)[at];
-  Weights w;
-  w.full = weight_of(x, r.m, heat);
-  if (p.probs)
-    w.rest = fmax(w.full - r.z * (double)p.probs[r.row * p.probs_stride + j], 0.0);
-  else
-    w.rest = j == draft ? 0.0 : w.full;
-  return w;
+template <typename E, int N>
+__device__ __forceinline__ void weights_of(const VerifyParams& p, const Chosen& r, double heat,
+                                           int draft, int j0, int step, int end, Weights* w) {
+  const E* x = (const E*)p.x + (long long)r.row * p.rstride;
+  // (where there are no probabilities to take off: some float, and none of it)
+  const bool less = p.probs && r.mode == kRest;
+  const float* q = less ? p.probs + r.row * p.probs_stride : p.accept_u;
+  const int skip = less ? -1 : draft;
+  E v[N];
+  float taken[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = min(j0 + i * step, end - 1);
+    v[i] = x[j];
+    taken[i] = q[less ? j : 0];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = j0 + i * step;
+    w[i].full = weight_of(j < end ? (float)v[i] : -INFINITY, r.m, heat);
+    const double rest = fmax(w[i].full - r.z * (double)(less ? taken[i] : 0.0f), 0.0);
+    w[i].rest = j == skip ? 0.0 : rest;
+  }
 }
 
-// Sum over the workgroup, in every thread.
-__device__ __forceinline__ double block_sum(double v, double* waves) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) v += waves[w];
-  return v;
-}
-
+// A wave sums runs of the sampled row.
+template <typename E>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(const VerifyParams p) {
-  __shared__ double waves[2][kWaves];
-  const int s = blockIdx.x / p.parts2, part = blockIdx.x % p.parts2, tid = threadIdx.x;
+  __shared__ Chosen of[2 * kWaves];
+  __shared__ int goes_on[2 * kWaves];
+  const int s = blockIdx.x / p.blocks, lane = threadIdx.x & 63;
+  const int run0 = blockIdx.x % p.blocks * kWaves + (threadIdx.x >> 6);
   const Rows rows = rows_of(p, s);
-  const Chosen r = choose(p, s, rows);
-  if (part == 0 && tid == 0) {
+  const double heat = heat_of(p, s);
+  const Chosen r = choose(p, rows, heat, of, goes_on);
+  if (run0 == 0 && lane == 0) {
     p.plan[s] = int4{r.row, r.mode, r.token, rows.n ? r.row - rows.first + 1 : 0};
     p.norm[s] = double2{(double)r.m, r.z};
   }
   if (r.mode != kFull && r.mode != kRest) return;
-  const double heat = heat_of(p, s);
-  const int draft = p.drafts[r.row];
-  const long long end = min((long long)p.n, (part + 1LL) * p.run);
-  double full = 0.0, rest = 0.0;
-  for (long long j = (long long)part * p.run + tid; j < end; j += kThreads) {
-    const Weights w = weights_of(p, r, heat, draft, (int)j);
-    full += w.full;
-    rest += w.rest;
-  }
-  full = block_sum(full, waves[0]);
-  rest = block_sum(rest, waves[1]);
-  if (tid == 0) {
-    double* to = p.sums + 2LL * blockIdx.x;
-    to[0] = full;
-    to[1] = rest;
+  const int draft = r.mode == kRest ? p.draft[r.row].token : -1;
+  for (int run = run0; run < p.runs; run += p.blocks * kWaves) {
+    const int end = min(p.n, (run + 1) * p.run);
+    double full = 0.0, rest = 0.0;
+    constexpr int N = 5;
+    for (int j = run * p.run; j < end; j += 64 * N) {
+      Weights w[N];
+      weights_of<E, N>(p, r, heat, draft, j + lane, 64, end, w);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        full += w[i].full;
+        rest += w[i].rest;
+      }
+    }
+    full = wave_sum(full);
+    rest = wave_sum(rest);
+    if (lane == 0) p.sums[(long long)s * p.runs + run] = double2{full, rest};
   }
 }
 
+// Sums up to and with each thread's; `total` is the last one.
+__device__ __forceinline__ double block_scan(double v, double* waves, double* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_scan(v);
+  __syncthreads();
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) v += waves[w];
+    sum += waves[w];
+  }
+  *total = sum;
+  return v;
+}
+
+// The first thread's index for which `hit` holds, in *first, and the last one's for
+// which `some` does, in *last.
+__device__ __forceinline__ void block_find(bool hit, bool some, int at, int* first, int* last) {
+  const uint64_t hits = __ballot(hit), somes = __ballot(some);
+  const int lane = threadIdx.x & 63;
+  if (hits && lane == __ffsll((unsigned long long)hits) - 1) atomicMin(first, at);
+  if (somes && lane == 63 - __clzll((unsigned long long)somes)) atomicMax(last, at);
+  __syncthreads();
+}
+
+template <typename E>
 __global__ __launch_bounds__(kThreads) void verify_token_kernel(const VerifyParams p) {
-  __shared__ double before[kThreads + 1];
-  __shared__ int found, last_one;
-  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  static_assert(kVerifyRuns <= kThreads, "a thread a run");
+  __shared__ double waves[kWaves];
+  __shared__ int first[2], last[2], any_rest;
+  __shared__ double start_of;
+  const int s = blockIdx.x, tid = threadIdx.x;
   const Rows rows = rows_of(p, s);
   const int4 plan = p.plan[s];
   Chosen r = {plan.x, plan.y, plan.z, (float)p.norm[s].x, p.norm[s].y};
   int token = r.mode == kGreedy ? r.token : -1;
   if (r.mode == kFull || r.mode == kRest) {
     const double heat = heat_of(p, s);
-    const int draft = p.drafts[r.row];
-    // the part: every wave, a lane a part
-    double full = 0.0, rest = 0.0;
-    if (lane < p.parts2) {
-      full = p.sums[2LL * (s * p.parts2 + lane)];
-      rest = p.sums[2LL * (s * p.parts2 + lane) + 1];
-    }
-    bool whole = r.mode == kFull || !__any(rest > 0.0);
-    double own = whole ? full : rest, upto = own;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const double v = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += v;
-    }
-    const double total = __shfl(upto, 63, 64), goal = (double)p.sample_u[s] * total;
+    const int draft = r.mode == kRest ? p.draft[r.row].token : -1;
+    if (tid < 2) first[tid] = INT_MAX, last[tid] = -1;
+    if (tid == 0) any_rest = 0;
+    __syncthreads();
+    const double2 sum = tid < p.runs ? p.sums[(long long)s * p.runs + tid] : double2{0.0, 0.0};
+    if (r.mode == kRest && __any(sum.y > 0.0)) any_rest = 1;
+    __syncthreads();
+    const bool whole = !any_rest;
+    double own = whole ? sum.x : sum.y, total;
+    double upto = block_scan(own, waves, &total);
+    const double goal = (double)p.sample_u[s] * total;
     // (the last one that weighs something, where rounding leaves none)
-    const uint64_t over = __ballot(upto > goal && own > 0.0), some = __ballot(own > 0.0);
-    const int part = over ? __ffsll((unsigned long long)over) - 1
-                          : 63 - __clzll((unsigned long long)some);
-    const double start = __shfl(upto - own, max(part, 0), 64);
-    const int j0 = max(part, 0) * p.run, j1 = (int)min((long long)p.n, (long long)j0 + p.run);
-    const int each = (p.run + kThreads - 1) / kThreads;
-    const int a = min(j0 + tid * each, j1), b = min(a + each, j1);
-    auto weight = [&](int j) {
-      const Weights w = weights_of(p, r, heat, draft, j);
-      return whole ? w.full : w.rest;
-    };
-    double sum = 0.0;
-    for (int j = a; j < b; ++j) sum += weight(j);
-    before[tid + 1] = sum;
-    if (tid == 0) {
-      before[0] = start;
-      found = p.n;
-      last_one = -1;
-    }
-    __syncthreads();
-    if (tid == 0)
-      for (int i = 0; i < kThreads; ++i) before[i + 1] += before[i];
-    __syncthreads();
-    double at = before[tid];
-    int hit = p.n, some_one = -1;
-    for (int j = a; j < b; ++j) {
-      const double w = weight(j);
-      at += w;
-      if (w > 0.0) {
-        some_one = j;
-        if (at > goal && hit == p.n) hit = j;
+    block_find(upto > goal && own > 0.0, own > 0.0, tid, first, last);
+    const int run = first[0] < INT_MAX ? first[0] : last[0];
+    if (run >= 0) {
+      if (tid == run) start_of = upto - own;
+      __syncthreads();
+      double start = start_of;
+      const int j0 = run * p.run, end = min(p.n, j0 + p.run);
+#pragma unroll 1
+      for (int j = j0; j < end; j += kThreads) {
+        Weights w;
+        weights_of<E, 1>(p, r, heat, draft, j + tid, 0, end, &w);
+        own = whole ? w.full : w.rest;
+        upto = block_scan(own, waves, &total) + start;
+        start += total;
+        block_find(upto > goal && own > 0.0, own > 0.0, j + tid, first + 1, last + 1);
+        if (first[1] < INT_MAX) break;
       }
+      token = first[1] < INT_MAX ? first[1] : last[1];
     }
-    if (hit < p.n) atomicMin(&found, hit);
-    if (some_one >= 0) atomicMax(&last_one, some_one);
-    __syncthreads();
-    token = found < p.n ? found : last_one;
   }
   if (tid == 0) p.counts[s] = plan.w;
   for (int i = tid; i < rows.n; i += kThreads)
@@ -334,28 +431,42 @@ __global__ __launch_bounds__(kThreads) void verify_token_kernel(const VerifyPara
                                                  : -1;
 }
 
-// Parts of a row: enough for two workgroups per CU, each of at least 512 chunks.
+// Parts of a row: enough for eight workgroups per CU, each of at least 512 chunks.
 int verify_parts(long long rows, int n, int esize, int cus) {
   const long long chunks = ((long long)n * esize + 15) / 16;
-  const long long parts = (2LL * cus + rows - 1) / rows, most = (chunks + 511) / 512;
+  const long long parts = (8LL * cus + rows - 1) / rows, most = (chunks + 511) / 512;
   const long long r = parts < most ? parts : most;
   return (int)(r < 1 ? 1 : r > kVerifyParts ? kVerifyParts : r);
 }
 
-hipError_t verify_launch(const VerifyParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)((long long)p.rows * p.parts));
-  if (p.f16)
-    hipLaunchKernelGGL(verify_rows_kernel<f16>, grid, dim3(kThreads), 0, stream, p);
-  else
-    hipLaunchKernelGGL(verify_rows_kernel<float>, grid, dim3(kThreads), 0, stream, p);
+// Runs of a sampled row: of at least 256 values, whole workgroups of them.
+int verify_runs(int n) {
+  const int runs = (n + 255) / 256;
+  return runs >= kVerifyRuns ? kVerifyRuns : (runs + kWaves - 1) / kWaves * kWaves;
+}
+// Workgroups that sum the runs of a sequence: eight per CU for all sequences.
+int verify_blocks(int sequences, int runs, int cus) {
+  const int most = runs / kWaves, r = (8 * cus + sequences - 1) / sequences;
+  return r < most ? r : most;
+}
+
+template <typename E>
+static hipError_t verify_type(const VerifyParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(verify_rows_kernel<E>, dim3((unsigned)((long long)p.rows * p.parts)),
+                     dim3(kThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_sums_kernel, dim3((unsigned)(p.sequences * p.parts2)), dim3(kThreads), 0,
-                     stream, p);
+  hipLaunchKernelGGL(verify_sums_kernel<E>, dim3((unsigned)(p.sequences * p.blocks)),
+                     dim3(kThreads), 0, stream, p);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(verify_token_kernel, dim3((unsigned)p.sequences), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL(verify_token_kernel<E>, dim3((unsigned)p.sequences), dim3(kThreads), 0, stream,
+                     p);
   return hipGetLastError();
+}
+
+hipError_t verify_launch(const VerifyParams& p, hipStream_t stream) {
+  return p.f16 ? verify_type<f16>(p, stream) : verify_type<float>(p, stream);
 }
 
 }  // namespace aexq
