@@ -6,130 +6,184 @@
 
 namespace aexq {
 
+// x sigmoid(x); the reciprocal is v_rcp's, 1 ulp off at most.
+__device__ __forceinline__ float silu_of(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x));
+}
+__device__ __forceinline__ f16x8 load8(const f16* p) { return *(const f16x8*)p; }
+
 // ---------------------------------------------------------------------------
 // Short causal convolution, channel by channel along a sequence,
 //   y[t][c] = act(bias[c] + sum_j w[c][j] x[t - (W - 1) + j][c])
 // in fp32, rounded once; the inputs before the first are the sequence's state, the
-// last W - 1 ones before.  A thread takes 8 channels over a block of kConvRows rows,
-// its last W - 1 inputs in registers.  The block that starts a sequence reads the
-// state and stores the new one, so no other workgroup meets it.
+// last W - 1 ones before.  A thread takes 4 channels over a block of B rows, the next four
+// on their way while four are computed: each input is read once, but for the W - 1 rows
+// before a block, and what bounds it is memory.  (8 channels a thread left two waves a
+// SIMD of long prompts: 57 us where 4 take 54, and 2 as well.)  The block that starts a sequence reads
+// the state and stores the new one, so no other workgroup meets it.
 // ---------------------------------------------------------------------------
-constexpr int kConvRows = 16;
+constexpr int kConvChannels = 4;
+__host__ __device__ constexpr int conv_groups(int channels) {
+  return (channels / kConvChannels + kThreads - 1) / kThreads;
+}
 
-__device__ __forceinline__ f16x8 load8(const f16* p) { return *(const f16x8*)p; }
-
-template <int W>
+template <int W, int B>
 __global__ __launch_bounds__(kThreads) void short_conv_kernel(const ShortConvParams p) {
-  const int groups = (p.channels / 8 + kThreads - 1) / kThreads;
+  constexpr int kBatch = 4, C = kConvChannels;
+  typedef f16 Row __attribute__((ext_vector_type(C)));
+  auto load = [](const f16* p) { return *(const Row*)p; };
+  const int groups = conv_groups(p.channels);
   const int id = blockIdx.x / groups, group = blockIdx.x % groups;
-  const RowBlock at = row_block<kConvRows>(p.offsets, p.tokens, p.slots.n, id);
+  const RowBlock at = row_block<B>(p.offsets, p.tokens, p.slots.n, id);
   const Span span = span_of(p.slots, p.offsets, p.tokens, at.seq);
-  const int c = 8 * (group * kThreads + threadIdx.x);
-  const int t0 = at.block * kConvRows, t1 = min(t0 + kConvRows, span.kept);
+  const int c = C * (group * kThreads + threadIdx.x);
+  const int t0 = at.block * B, t1 = min(t0 + B, span.kept);
   if (t0 >= span.kept || c >= p.channels) return;
 
   // input of place t among the sequence's rows, the state's below 0
   f16* state = p.state + (long long)max(span.slot, 0) * (W - 1) * p.channels + c;
+  const f16* x = p.x + span.first * p.x_stride + c;
   auto input = [&](int t) {
-    if (t >= 0) return load8(p.x + (span.first + t) * p.x_stride + c);
-    return span.fresh ? f16x8{} : load8(state + (long long)(t + W - 1) * p.channels);
+    if (t >= 0) return load(x + t * p.x_stride);
+    return span.fresh ? Row{} : load(state + (long long)(t + W - 1) * p.channels);
   };
-  f16x8 last[W];  // inputs t - W .. t - 1 (the first unused)
-#pragma unroll
-  for (int j = 1; j < W; ++j) last[j] = input(t0 + j - W);
   if (p.out) {
-    float w[8][W], bias[8];
+    Row row[W - 1 + kBatch], next[kBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int j = 0; j < W - 1; ++j) row[j] = input(t0 + j - (W - 1));
+    // (rows behind the last one: the last one, again)
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) next[b] = load(x + min(t + b, t1 - 1) * p.x_stride);
+    };
+    fetch(t0);
+    float w[C][W], bias[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
 #pragma unroll
       for (int j = 0; j < W; ++j) w[i][j] = p.weight[(long long)(c + i) * W + j];
       bias[i] = p.bias ? p.bias[c + i] : 0.0f;
     }
-    f16x8 row[W];
+    f16* out = p.out + span.first * p.out_stride + c;
+    for (int t = t0; t < t1; t += kBatch) {
 #pragma unroll
-    for (int j = 1; j < W; ++j) row[j] = last[j];
-    for (int t = t0; t < t1; ++t) {
+      for (int b = 0; b < kBatch; ++b) row[W - 1 + b] = next[b];
+      fetch(t + kBatch);
 #pragma unroll
-      for (int j = 0; j + 1 < W; ++j) row[j] = row[j + 1];
-      row[W - 1] = input(t);
-      f16x8 y;
+      for (int b = 0; b < kBatch; ++b) {
+        Row y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float v = bias[i];
+        for (int i = 0; i < C; ++i) {
+          float v = bias[i];
 #pragma unroll
-        for (int j = 0; j < W; ++j) v = fmaf(w[i][j], (float)row[j][i], v);
-        y[i] = (f16)(p.silu ? v / (1.0f + __expf(-v)) : v);
+          for (int j = 0; j < W; ++j) v = fmaf(w[i][j], (float)row[b + j][i], v);
+          y[i] = (f16)(p.silu ? silu_of(v) : v);
+        }
+        if (t + b < t1) *(Row*)(out + (t + b) * p.out_stride) = y;
       }
-      *(f16x8*)(p.out + (span.first + t) * p.out_stride + c) = y;
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) row[j] = row[kBatch + j];
     }
   }
   if (at.block || !p.slots.store || span.slot < 0) return;
   // the last W - 1 inputs; the state's rows that stay move up
-  f16x8 next[W];
+  Row last[W];
 #pragma unroll
-  for (int j = 1; j < W; ++j) next[j] = input(span.kept + j - W);
+  for (int j = 1; j < W; ++j) last[j] = input(span.kept + j - W);
 #pragma unroll
-  for (int j = 1; j < W; ++j) *(f16x8*)(state + (long long)(j - 1) * p.channels) = next[j];
+  for (int j = 1; j < W; ++j) *(Row*)(state + (long long)(j - 1) * p.channels) = last[j];
 }
 
-hipError_t short_conv_launch(const ShortConvParams& p, hipStream_t stream) {
-  const long long groups = (p.channels / 8 + kThreads - 1) / kThreads;
-  const dim3 grid((unsigned)(row_blocks(p.tokens, p.slots.n, kConvRows) * groups));
+template <int B>
+static hipError_t short_conv_rows(const ShortConvParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)(row_blocks(p.tokens, p.slots.n, B) * conv_groups(p.channels)));
   switch (p.width) {
-    case 2: hipLaunchKernelGGL(short_conv_kernel<2>, grid, dim3(kThreads), 0, stream, p); break;
-    case 3: hipLaunchKernelGGL(short_conv_kernel<3>, grid, dim3(kThreads), 0, stream, p); break;
-    case 4: hipLaunchKernelGGL(short_conv_kernel<4>, grid, dim3(kThreads), 0, stream, p); break;
-    default: hipLaunchKernelGGL(short_conv_kernel<5>, grid, dim3(kThreads), 0, stream, p); break;
+    case 2: hipLaunchKernelGGL((short_conv_kernel<2, B>), grid, dim3(kThreads), 0, stream, p); break;
+    case 3: hipLaunchKernelGGL((short_conv_kernel<3, B>), grid, dim3(kThreads), 0, stream, p); break;
+    case 4: hipLaunchKernelGGL((short_conv_kernel<4, B>), grid, dim3(kThreads), 0, stream, p); break;
+    default: hipLaunchKernelGGL((short_conv_kernel<5, B>), grid, dim3(kThreads), 0, stream, p); break;
   }
   return hipGetLastError();
+}
+
+// Blocks of 64 rows where they make two workgroups per CU (256 of them), which read their
+// weights and the rows before the block once for 64 rows: 9600 rows of 6144 channels take
+// 54 us so and 65 with blocks of 16.  Fewer rows are spread over more workgroups.
+hipError_t short_conv_launch(const ShortConvParams& p, hipStream_t stream) {
+  return (long long)p.tokens / 64 * conv_groups(p.channels) >= 512 ? short_conv_rows<64>(p, stream)
+                                                                   : short_conv_rows<16>(p, stream);
 }
 
 // ---------------------------------------------------------------------------
 // Root-mean-square norm of each head, gated by silu:
 //   y = x rsqrt(max(mean(x^2) + eps, 1e-20)) gamma silu(z)
-// in fp32, rounded once.  LPR lanes take a row, 8 values each.
+// in fp32, rounded once.  LPR lanes take a row, 8 values each, and R rows at once, so that
+// long calls have eight loads a lane on their way: 159568 rows of 128 take 25.7 us with
+// R = 4 (122 MB, 4.8 TB/s; a copy of that size runs at 5.3), 27.9 with 2, 42.9 with 1 and
+// 32.1 with 8.  Calls too small to fill the card (below 2^22 values) keep R = 1.
 // ---------------------------------------------------------------------------
 template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if constexpr (LPR == 8) {
+    v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+    v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+    v += dpp<0x141>(v);  // row_half_mirror
+    return v;
+  } else {
+    return group_sum<LPR>(v);
+  }
+}
+
+template <int LPR, int R>
 __global__ __launch_bounds__(kThreads) void gated_norm_kernel(const GatedNormParams p) {
-  const long long row = (long long)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int i = threadIdx.x % LPR * 8;
-  const bool on = row < p.rows && i < p.dim;
-  const long long token = min(row, p.rows - 1) / p.heads;
-  const int head = (int)(min(row, p.rows - 1) % p.heads);
-  f16x8 x = f16x8{}, z = f16x8{};
-  if (on) {
-    x = load8(p.x + token * p.x_stride + (long long)head * p.dim + i);
-    z = load8(p.z + token * p.z_stride + (long long)head * p.dim + i);
+  constexpr int kRows = kThreads / LPR;
+  const int i = threadIdx.x % LPR * 8, at = min(i, p.dim - 8);
+  const long long row0 = (long long)blockIdx.x * (R * kRows) + threadIdx.x / LPR;
+  f16x8 x[R], z[R];
+  f16* out[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const unsigned row = (unsigned)min(row0 + r * kRows, p.rows - 1);
+    const long long token = row / (unsigned)p.heads;
+    const int place = (int)(row % (unsigned)p.heads) * p.dim + at;
+    x[r] = load8(p.x + token * p.x_stride + place);
+    z[r] = load8(p.z + token * p.z_stride + place);
+    out[r] = p.out + token * p.out_stride + place;
   }
-  float sum = 0.0f;
+  float gamma[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum = fmaf((float)x[e], (float)x[e], sum);
+  for (int e = 0; e < 8; ++e) gamma[e] = p.gamma ? p.gamma[at + e] : 1.0f;
 #pragma unroll
-  for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if (!on) return;
-  const float r = 1.0f / sqrtf(fmaxf(sum / p.dim + p.eps, 1e-20f));
-  f16x8 y;
+  for (int r = 0; r < R; ++r) {
+    float sum = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float gate = (float)z[e];
-    const float v = (float)x[e] * r * (p.gamma ? p.gamma[i + e] : 1.0f);
-    y[e] = (f16)(v * (gate / (1.0f + __expf(-gate))));
+    for (int e = 0; e < 8; ++e) sum = fmaf((float)x[r][e], (float)x[r][e], sum);
+    sum = lanes_sum<LPR>(i < p.dim ? sum : 0.0f);
+    const float k = 1.0f / sqrtf(fmaxf(sum / p.dim + p.eps, 1e-20f));
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (f16)((float)x[r][e] * k * gamma[e] * silu_of((float)z[r][e]));
+    if (row0 + r * kRows < p.rows && i < p.dim) *(f16x8*)out[r] = y;
   }
-  *(f16x8*)(p.out + token * p.out_stride + (long long)head * p.dim + i) = y;
+}
+
+template <int R>
+static hipError_t gated_norm_rows(const GatedNormParams& p, hipStream_t stream) {
+  int lpr = 8;
+  while (8 * lpr < p.dim) lpr *= 2;
+  const long long per = kThreads / lpr * R;
+  const dim3 grid((unsigned)((p.rows + per - 1) / per));
+  switch (lpr) {
+    case 8: hipLaunchKernelGGL((gated_norm_kernel<8, R>), grid, dim3(kThreads), 0, stream, p); break;
+    case 16: hipLaunchKernelGGL((gated_norm_kernel<16, R>), grid, dim3(kThreads), 0, stream, p); break;
+    case 32: hipLaunchKernelGGL((gated_norm_kernel<32, R>), grid, dim3(kThreads), 0, stream, p); break;
+    default: hipLaunchKernelGGL((gated_norm_kernel<64, R>), grid, dim3(kThreads), 0, stream, p); break;
+  }
+  return hipGetLastError();
 }
 
 hipError_t gated_norm_launch(const GatedNormParams& p, hipStream_t stream) {
-  int lpr = 8;
-  while (8 * lpr < p.dim) lpr *= 2;
-  const long long per = kThreads / lpr;
-  const dim3 grid((unsigned)((p.rows + per - 1) / per));
-  switch (lpr) {
-    case 8: hipLaunchKernelGGL(gated_norm_kernel<8>, grid, dim3(kThreads), 0, stream, p); break;
-    case 16: hipLaunchKernelGGL(gated_norm_kernel<16>, grid, dim3(kThreads), 0, stream, p); break;
-    case 32: hipLaunchKernelGGL(gated_norm_kernel<32>, grid, dim3(kThreads), 0, stream, p); break;
-    default: hipLaunchKernelGGL(gated_norm_kernel<64>, grid, dim3(kThreads), 0, stream, p); break;
-  }
-  return hipGetLastError();
+  return p.rows * p.dim >= 1 << 22 ? gated_norm_rows<4>(p, stream) : gated_norm_rows<1>(p, stream);
 }
 
 }  // namespace aexq
