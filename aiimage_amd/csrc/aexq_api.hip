@@ -2564,7 +2564,7 @@ extern "C" aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots,
   if (st) return st;
   p.heads = (char*)ctx->delta_mem;
   p.keys = p.heads + heads;
-  const hipError_t e = delta_prompt_launch(p, ctx->cus, ctx->stream);
+  const hipError_t e = delta_prompt_launch(p, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "delta rule launch");
   return AEXQ_OK;
 }

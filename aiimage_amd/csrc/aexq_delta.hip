@@ -114,6 +114,10 @@ struct BlockLds {
 // One block and key head; the value heads of its group in turn.  Products of keys are
 // formed with the earlier rows on the left: lane (c, g) then has row 16 w + c and columns
 // 16 j + 4 g + r, which is how A and P enter the products behind.
+//
+// Bound by memory: a block reads 32 KB of k and q (heads of 128) and writes 48 KB of them
+// in the products' order and 19 KB of T, P and factors for each value head.  16384 rows of
+// 16 key and 32 value heads: 96 us for 490 MB.
 template <int DK>
 __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaParams p) {
   constexpr int KB = DK / 32;
@@ -125,6 +129,9 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
   const Span span = span_of(p.slots, p.offsets, p.tokens, at.seq);
   const int t0 = at.block * kDeltaRows, live = min(kDeltaRows, span.kept - t0);
   if (live <= 0) return;
+  // a block of up to 16 rows has one row tile, its first wave's; the others only share in
+  // the transposed keys
+  const bool small = live <= 16;
   // rows past the last one repeat it; their factors are 0
   const long long row = span.first + t0 + min(own, live - 1);
   f16x8 k[KB], q[KB];
@@ -140,8 +147,10 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
 #pragma unroll
   for (int i = 0; i < KB; ++i) {
     *(f16x8*)&lds.k[own][32 * i + 8 * g] = k[i];
-    *(f16x8*)(keys + ((wave * KB + i) * 64 + lane) * 16) = k[i];
-    *(f16x8*)(keys + ((4 * KB + wave * KB + i) * 64 + lane) * 16) = q[i];
+    if (!small || wave == 0) {
+      *(f16x8*)(keys + ((wave * KB + i) * 64 + lane) * 16) = k[i];
+      *(f16x8*)(keys + ((4 * KB + wave * KB + i) * 64 + lane) * 16) = q[i];
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       kk = fmaf((float)k[i][e], (float)k[i][e], kk);
@@ -176,6 +185,7 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
 #pragma unroll
   for (int i = 0; i < DK / 32; ++i) {  // pieces (16 of DK, 32 rows): two a tile
     const int n = wave * (DK / 32) + i, tile = n >> 1, b = n & 1;
+    if (small && b) continue;
     f16x8 y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -213,6 +223,7 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
       }
       __syncthreads();
     }
+    if (small && wave) continue;
     // (so that comparisons with the lane's row are made here, not kept over the loop)
     int here = c;
     asm volatile("" : "+v"(here));
@@ -276,7 +287,9 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
         lds.t[16 * wave + i + g][16 * wave + c] = y;
       }
     }
-    __syncthreads();
+    if (!small) __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     // the tiles below them: T_wj = -T_ww sum_l A_wl T_lj, step k of a product taking row
     // 4 g + k of its right operand
     const f32x4 diagonal = *(const f32x4*)&lds.t[own][16 * wave + 4 * g];
@@ -299,7 +312,7 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
 #pragma unroll
         for (int r = 0; r < 4; ++r) lds.t[16 * wave + 4 * g + r][16 * j + c] = -y[r];
       }
-      __syncthreads();
+      if (!small) __syncthreads();
     }
     // the wave's rows of T as the products take them
 #pragma unroll
@@ -404,6 +417,8 @@ struct DeltaWave {
     for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[i][r] = span.fresh ? 0.0f : state_at(i)[r * p.dv];
+  }
+  __device__ __forceinline__ void lift() {
     scale = lift_of(top());
     rescale(scale.by);
   }
@@ -485,218 +500,88 @@ struct DeltaWave {
         f32x4, __builtin_amdgcn_raw_buffer_load_b128(
                    at, 16 * g, kDeltaFactors + (which * kDeltaRows + 16 * tile) * 4, 0));
   }
-};
-
-// The operands of blocks of TILES row tiles.
-template <int DK, int TILES>
-struct DeltaBlock {
-  static constexpr int KB = DK / 32, PAIRS = (TILES + 1) / 2;
-  f16x8 k[TILES][KB], q[TILES][KB];
-  f16x8 t[TILES][PAIRS][2], w[TILES][PAIRS];  // of T and P, by pairs of column tiles
-  f16x8 kt[2 * KB][PAIRS];
-  f32x4 beta[TILES], seen[TILES], ask[TILES], left[TILES];
-  f16 v[TILES][4];
-  float decay;
-  typedef DeltaWave<DK> W;
-
-  __device__ __forceinline__ void load_k(const W& x, int b) {
-    const auto at = x.keys_of(b);
-#pragma unroll
-    for (int i = 0; i < KB; ++i)
-#pragma unroll
-      for (int w = 0; w < TILES; ++w) k[w][i] = x.piece(at, w * KB + i);
-  }
-  __device__ __forceinline__ void load_q(const W& x, int b) {
-    const auto at = x.keys_of(b);
-#pragma unroll
-    for (int i = 0; i < KB; ++i)
-#pragma unroll
-      for (int w = 0; w < TILES; ++w) q[w][i] = x.piece(at, (4 + w) * KB + i);
-  }
-  __device__ __forceinline__ void load_v(const W& x, int b) {
-    const auto at = x.rows_of(x.p.v, x.p.v_stride, b), h = x.head_of(b);
-    const uint32_t step = 2 * (uint32_t)x.p.v_stride, first = 4 * x.g * step + 2 * x.c;
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        v[w][r] = __builtin_bit_cast(
-            f16, __builtin_amdgcn_raw_buffer_load_b16(at, first + r * step, 16 * w * step, 0));
-      beta[w] = x.factor(h, kBeta, w);
-      seen[w] = x.factor(h, kSeen, w);
-    }
-  }
-  __device__ __forceinline__ void load_t(const W& x, int b) {
-    const auto h = x.head_of(b);
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) {
-#pragma unroll
-      for (int j = 0; j <= w / 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) t[w][j][i] = x.piece(h, piece_of(w, j) * 2 + i);
-      left[w] = x.factor(h, kLeft, w);
-    }
-  }
-  __device__ __forceinline__ void load_w(const W& x, int b) {
-    const auto h = x.head_of(b);
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) {
-#pragma unroll
-      for (int j = 0; j <= w / 2; ++j) this->w[w][j] = x.piece(h, 12 + piece_of(w, j));
-      ask[w] = x.factor(h, kAsk, w);
-    }
-  }
-  __device__ __forceinline__ void load_kt(const W& x, int b) {
-    const auto at = x.keys_of(b);
-#pragma unroll
-    for (int j = 0; j < PAIRS; ++j)
-#pragma unroll
-      for (int i = 0; i < 2 * KB; ++i) kt[i][j] = x.piece(at, 8 * KB + 2 * i + j);
-    decay = as_f32(__builtin_amdgcn_raw_buffer_load_b32(
-        x.head_of(b), 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
+  __device__ __forceinline__ float decay_of(__amdgpu_buffer_rsrc_t at) const {
+    return as_f32(
+        __builtin_amdgcn_raw_buffer_load_b32(at, 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
   }
 };
 
-// One block: the outputs, and the state behind it.  `next`: the block whose operands are
-// loaded meanwhile (below 0: none).  True where something is not finite: a product with
-// zeros takes it to the rows before it.
-template <int DK, int TILES>
-__device__ __forceinline__ bool delta_block(DeltaWave<DK>& x, DeltaBlock<DK, TILES>& o, int b,
-                                            int next) {
-  constexpr int KB = DK / 32, PAIRS = (TILES + 1) / 2;
+// The last block of a sequence, of up to 16 rows: the outputs, and the state behind it.
+// True where something is not finite: a product with zeros takes it to the rows before it.
+// `first`: the state is as it was read.
+template <int DK>
+__device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
+  constexpr int KB = DK / 32;
   const DeltaParams& p = x.p;
-  Split s[KB];
+  const auto keys = x.keys_of(b), head = x.head_of(b);
+  f16x8 k[KB], q[KB], kt[2 * KB];
+  f16 v[4];
 #pragma unroll
-  for (int i = 0; i < KB; ++i) s[i] = split8(x.S[2 * i], x.S[2 * i + 1]);
-  f32x4 seen[TILES], asked[TILES];
-#pragma unroll
-  for (int w = 0; w < TILES; ++w) seen[w] = asked[w] = f32x4{};
-#pragma unroll
-  for (int i = 0; i < KB; ++i) {
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) seen[w] = mfma(o.k[w][i], s[i].x0, seen[w]);
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) seen[w] = mfma(o.k[w][i], s[i].x1, seen[w]);
-  }
-  if (next >= 0) {
-    __builtin_amdgcn_sched_barrier(0);
-    o.load_k(x, next);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int i = 0; i < KB; ++i) {
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) asked[w] = mfma(o.q[w][i], s[i].x0, asked[w]);
-#pragma unroll
-    for (int w = 0; w < TILES; ++w) asked[w] = mfma(o.q[w][i], s[i].x1, asked[w]);
-  }
-  // R
-  f32x4 r[2 * PAIRS];
-  float m = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 2 * PAIRS; ++w) {
-    r[w] = f32x4{};
-    if (w >= TILES) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      r[w][e] = o.beta[w][e] * (float)o.v[w][e] - o.seen[w][e] * (seen[w][e] * x.scale.back);
-    }
-    m = top4(m, r[w]);
-  }
-  m = rows_max(m);
-  const bool odd = !(m < INFINITY);
-  const Lift lr = lift_of(m);
-  Split rs[PAIRS];
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) rs[j] = split8(r[2 * j] * lr.by, r[2 * j + 1] * lr.by);
-  if (next >= 0) {
-    __builtin_amdgcn_sched_barrier(0);
-    o.load_v(x, next);
-    o.load_q(x, next);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  // U = T R, by the largest of which and of the state the new scale goes: S is within its
-  // decayed columns and 64 of U's
-  f32x4 u[2 * PAIRS], y[2 * PAIRS];
-  float mu = 0.0f, my = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 2 * PAIRS; ++w) {
-    u[w] = y[w] = f32x4{};
-    if (w >= TILES) continue;
-#pragma unroll
-    for (int j = 0; j <= w / 2; ++j) {
-      u[w] = mfma(o.t[w][j][0], rs[j].x0, u[w]);
-      u[w] = mfma(o.t[w][j][0], rs[j].x1, u[w]);
-      u[w] = mfma(o.t[w][j][1], rs[j].x0, u[w]);
-    }
-  }
-#pragma unroll
-  for (int w = 0; w < TILES; ++w) {
-    u[w] *= lr.back * (1.0f / kPieceScale);
-    y[w] = u[w] * o.left[w];
-    mu = top4(mu, u[w]);
-    my = top4(my, y[w]);
-  }
-  if (next >= 0) {
-    __builtin_amdgcn_sched_barrier(0);
-    o.load_t(x, next);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  const Lift lu = lift_of(rows_max(mu));
-  const Lift ls = lift_of(fmaf(64.0f, rows_max(my), x.top() * (x.scale.back * o.decay)));
-  Split us[PAIRS], ys[PAIRS];
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-    ys[j] = split8(y[2 * j] * ls.by, y[2 * j + 1] * ls.by);
-    us[j] = split8(u[2 * j] * lu.by, u[2 * j + 1] * lu.by);
-  }
-  const float keep = o.decay * x.scale.back * ls.by, before = x.scale.back;
-  x.rescale(keep);
-  x.scale = ls;
-#pragma unroll
-  for (int j = 0; j < PAIRS; ++j) {
-#pragma unroll
-    for (int i = 0; i < 2 * KB; ++i) x.S[i] = mfma(o.kt[i][j], ys[j].x0, x.S[i]);
-#pragma unroll
-    for (int i = 0; i < 2 * KB; ++i) x.S[i] = mfma(o.kt[i][j], ys[j].x1, x.S[i]);
-  }
-  f32x4 a[TILES];
-#pragma unroll
-  for (int w = 0; w < TILES; ++w) {
-    a[w] = f32x4{};
-#pragma unroll
-    for (int j = 0; j <= w / 2; ++j) {
-      a[w] = mfma(o.w[w][j], us[j].x0, a[w]);
-      a[w] = mfma(o.w[w][j], us[j].x1, a[w]);
-    }
-  }
-  const float back = p.scale * lu.back * (1.0f / kPieceScale);
-#pragma unroll
-  for (int w = 0; w < TILES; ++w) {
+  for (int i = 0; i < KB; ++i) k[i] = x.piece(keys, i);
+  {
+    const auto from = x.rows_of(p.v, p.v_stride, b);
+    const uint32_t step = 2 * (uint32_t)p.v_stride, at = 4 * x.g * step + 2 * x.c;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      a[w][e] = fmaf(a[w][e], back, o.ask[w][e] * (asked[w][e] * before));
-    asm volatile("" : "+v"(a[w]));  // (before the operands' registers are loaded again)
+      v[e] = __builtin_bit_cast(
+          f16, __builtin_amdgcn_raw_buffer_load_b16(from, at + e * step, 0, 0));
   }
+  const f32x4 beta = x.factor(head, kBeta, 0), seen_by = x.factor(head, kSeen, 0);
 #pragma unroll
-  for (int i = 0; i < 2 * KB; ++i) asm volatile("" : "+v"(x.S[i]));
-  if (next >= 0) {
-    __builtin_amdgcn_sched_barrier(0);
-    o.load_kt(x, next);
-    o.load_w(x, next);
-    __builtin_amdgcn_sched_barrier(0);
+  for (int i = 0; i < KB; ++i) q[i] = x.piece(keys, 4 * KB + i);
+  const f16x8 t0 = x.piece(head, 0), t1 = x.piece(head, 1), w = x.piece(head, 12);
+  const f32x4 left = x.factor(head, kLeft, 0), ask = x.factor(head, kAsk, 0);
+#pragma unroll
+  for (int i = 0; i < 2 * KB; ++i) kt[i] = x.piece(keys, 8 * KB + 2 * i);
+  const float decay = x.decay_of(head);
+  __builtin_amdgcn_sched_barrier(0);  // (all of it on its way together, behind the state)
+  if (first) x.lift();
+  f32x4 seen = f32x4{}, asked = f32x4{};
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    const Split s = split8(x.S[2 * i], x.S[2 * i + 1]);
+    seen = mfma(k[i], s.x0, seen);
+    asked = mfma(q[i], s.x0, asked);
+    seen = mfma(k[i], s.x1, seen);
+    asked = mfma(q[i], s.x1, asked);
   }
+  f32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    r[e] = fmaf(-seen_by[e], seen[e] * x.scale.back, beta[e] * (float)v[e]);
+  const float m = rows_max(top4(0.0f, r));
+  const Lift lr = lift_of(m);
+  const Split rs = split8(r * lr.by, f32x4{});
+  f32x4 u = mfma(t0, rs.x0, f32x4{});
+  u = mfma(t0, rs.x1, u);
+  u = mfma(t1, rs.x0, u);
+  u *= lr.back * (1.0f / kPieceScale);
+  // S is within its decayed columns and 16 of U's, the new scale within that of 64
+  const f32x4 y = u * left;
+  const Lift lu = lift_of(rows_max(top4(0.0f, u)));
+  const Lift ls = lift_of(fmaf(64.0f, rows_max(top4(0.0f, y)), x.top() * (x.scale.back * decay)));
+  const Split us = split8(u * lu.by, f32x4{}), ys = split8(y * ls.by, f32x4{});
+  const float before = x.scale.back;
+  x.rescale(decay * before * ls.by);
+  x.scale = ls;
+#pragma unroll
+  for (int i = 0; i < 2 * KB; ++i) {
+    x.S[i] = mfma(kt[i], ys.x0, x.S[i]);
+    x.S[i] = mfma(kt[i], ys.x1, x.S[i]);
+  }
+  f32x4 a = mfma(w, us.x0, f32x4{});
+  a = mfma(w, us.x1, a);
+  const float back = p.scale * lu.back * (1.0f / kPieceScale);
   if (p.out) {
     const auto to = x.rows_of(p.out, p.out_stride, b);
-    const uint32_t step = 2 * (uint32_t)p.out_stride, first = 4 * x.g * step + 2 * x.c;
+    const uint32_t step = 2 * (uint32_t)p.out_stride, at = 4 * x.g * step + 2 * x.c;
 #pragma unroll
-    for (int w = 0; w < TILES; ++w)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)a[w][e]), to,
-                                              first + e * step, 16 * w * step, 0);
+    for (int e = 0; e < 4; ++e)
+      __builtin_amdgcn_raw_buffer_store_b16(
+          __builtin_bit_cast(short, (f16)fmaf(a[e], back, ask[e] * (asked[e] * before))), to,
+          at + e * step, 0, 0);
   }
-  return odd;
+  return !(m < INFINITY);
 }
 
 // ---------------------------------------------------------------------------
@@ -704,6 +589,14 @@ __device__ __forceinline__ bool delta_block(DeltaWave<DK>& x, DeltaBlock<DK, TIL
 // block, the other forms the outputs a block behind, from the parts of S and from U that
 // the first one leaves in LDS, and the first one's beta v a block ahead.  One barrier a
 // block.
+//
+// A block takes the first wave 1.9 us: 82 matrix products (1300 cycles), 300 vector
+// operations between them (1200) and 52 loads, which it has to issue itself, all in one
+// chain from state to state.  16384 rows of 32 value heads of 128 x 128, one sequence:
+// 490 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 90 us.  One wave for
+// all of it takes 777 and 112 us.  Eight waves that each hold 16 rows of S of 16 columns
+// and add their products through LDS: 450 and 103; blocks of 16 rows 77 us where the last
+// ones go through one wave in 35.
 // ---------------------------------------------------------------------------
 template <int DK>
 struct DeltaLds {
@@ -741,8 +634,7 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
   auto load_left = [&](__amdgpu_buffer_rsrc_t h) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) left[w] = x.factor(h, kLeft, w);
-    decay = as_f32(
-        __builtin_amdgcn_raw_buffer_load_b32(h, 0, kDeltaFactors + kDecay * kDeltaRows * 4, 0));
+    decay = x.decay_of(h);
   };
   {
     const auto keys = x.keys_of(0), head = x.head_of(0);
@@ -1025,8 +917,8 @@ __global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams 
   const int all = (x.span.kept + kDeltaRows - 1) / kDeltaRows;
   // a last block of up to 16 rows takes a quarter of the products, and one wave
   const bool short_end = x.span.kept - (all - 1) * kDeltaRows <= 16;
-  const int blocks = sreg(all - short_end);
-  if (sreg((int)threadIdx.x >> 6)) {
+  const int blocks = sreg(all - short_end), wave = sreg((int)threadIdx.x >> 6);
+  if (wave) {
     if (!blocks) return;
     delta_outputs<DK>(x, lds, blocks);
     wait_vm<0>();
@@ -1035,22 +927,17 @@ __global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams 
   }
   x.read();
   bool odd = false;
-  if (blocks) delta_solve<DK>(x, lds, blocks, odd);
-  if (short_end) {
-    DeltaBlock<DK, 1> o;
-    o.load_k(x, blocks);
-    o.load_v(x, blocks);
-    o.load_q(x, blocks);
-    o.load_t(x, blocks);
-    o.load_kt(x, blocks);
-    o.load_w(x, blocks);
-    odd |= delta_block<DK, 1>(x, o, blocks, -1);
+  if (blocks) {
+    x.lift();
+    delta_solve<DK>(x, lds, blocks, odd);
   }
+  if (short_end) odd |= delta_end<DK>(x, blocks, !blocks);
   if (blocks) __syncthreads();  // the outputs are in place
   if (__any(odd)) {
     wait_vm<0>();
     // from the start again, row after row (the state in memory is still the one before)
     x.read();
+    x.scale = Lift{1.0f, 1.0f};
     x.rows(0, x.span.kept);
   }
   x.write();
@@ -1069,7 +956,7 @@ static hipError_t prompt_launch(const DeltaParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream) {
+hipError_t delta_prompt_launch(const DeltaParams& p, hipStream_t stream) {
   return p.dk == 64 ? prompt_launch<64>(p, stream) : prompt_launch<128>(p, stream);
 }
 

@@ -57,7 +57,7 @@ constexpr int kDeltaRows = 64;
 constexpr int kDeltaFactors = 18 * 1024;
 constexpr int kDeltaHead = kDeltaFactors + 4 * kDeltaRows * 4 + 64;
 constexpr int delta_key_bytes(int dk) { return 3 * dk * kDeltaRows * 2; }
-hipError_t delta_prompt_launch(const DeltaParams& p, int cus, hipStream_t stream);
+hipError_t delta_prompt_launch(const DeltaParams& p, hipStream_t stream);
 hipError_t delta_decode_launch(const DeltaParams& p, int cus, hipStream_t stream);
 // ---- drafted tokens against the target's probabilities (aexq_verify.hip)
 constexpr int kVerifyParts = 64;   // parts of a row at most: a lane each
