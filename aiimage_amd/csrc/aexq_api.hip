@@ -2430,6 +2430,10 @@ static aexq_status view_slots(const aexq_slots* s, const char* op, const void* s
   return AEXQ_OK;
 }
 
+// Workgroups of up to 256 threads that one launch may have: its threads are counted in
+// 32 bits.
+constexpr long long kMostGroups = (1LL << 24) - 1;
+
 static aexq_status check_tokens(const char* op, const int32_t* offsets, int tokens) {
   if (!offsets) return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "offsets is NULL");
   if (tokens <= 0 || tokens > 1 << 23)
@@ -2456,6 +2460,8 @@ extern "C" aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, v
   if (!st && out == x)
     st = fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out is x, which other workgroups still read");
   if (st) return st;
+  if (conv_groups(tokens, p.slots.n, channels) > kMostGroups)
+    return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d channels in one call", tokens, channels);
   p.state = (_Float16*)state;
   p.offsets = offsets;
   p.tokens = tokens;
@@ -2526,7 +2532,7 @@ static aexq_status view_delta(const char* op, const void* q, int64_t q_stride, c
   p->scale = scale;
   p->eps = eps;
   // (a workgroup takes 16 columns of a head at least)
-  if ((long long)p->slots.n * heads_v * (dim_v / 16) > 0x7fffffffLL)
+  if ((long long)p->slots.n * heads_v * (dim_v / 16) > kMostGroups)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d sequences of %d heads of %d in one call", p->slots.n,
                 heads_v, dim_v);
   return AEXQ_OK;
@@ -2555,7 +2561,7 @@ extern "C" aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots,
   HIP_TRY(op, hipSetDevice(ctx->device));
   // (row_blocks of aexq_rows.hpp)
   const long long blocks = tokens / kDeltaRows + (long long)p.slots.n;
-  if (blocks * heads_v > 0x7fffffffLL)
+  if (blocks * heads_v > kMostGroups)  // (heads_k are no more)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d sequences and %d heads in one call",
                 tokens, p.slots.n, heads_v);
   const long long heads = blocks * heads_v * kDeltaHead;
@@ -2623,7 +2629,7 @@ extern "C" aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t 
   p.heads = heads;
   p.dim = dim;
   p.eps = eps;
-  if (p.rows > 1LL << 31)
+  if (gated_norm_groups(p.rows, dim) > kMostGroups)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d heads in one call", tokens, heads);
   HIP_TRY(op, hipSetDevice(ctx->device));
   const hipError_t e = gated_norm_launch(p, ctx->stream);

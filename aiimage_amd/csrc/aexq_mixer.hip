@@ -23,7 +23,7 @@ __device__ __forceinline__ f16x8 load8(const f16* p) { return *(const f16x8*)p; 
 // the state and stores the new one, so no other workgroup meets it.
 // ---------------------------------------------------------------------------
 constexpr int kConvChannels = 4;
-__host__ __device__ constexpr int conv_groups(int channels) {
+__host__ __device__ constexpr int channel_groups(int channels) {
   return (channels / kConvChannels + kThreads - 1) / kThreads;
 }
 
@@ -32,7 +32,7 @@ __global__ __launch_bounds__(kThreads) void short_conv_kernel(const ShortConvPar
   constexpr int kBatch = 4, C = kConvChannels;
   typedef f16 Row __attribute__((ext_vector_type(C)));
   auto load = [](const f16* p) { return *(const Row*)p; };
-  const int groups = conv_groups(p.channels);
+  const int groups = channel_groups(p.channels);
   const int id = blockIdx.x / groups, group = blockIdx.x % groups;
   const RowBlock at = row_block<B>(p.offsets, p.tokens, p.slots.n, id);
   const Span span = span_of(p.slots, p.offsets, p.tokens, at.seq);
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void short_conv_kernel(const ShortConvPar
 
 template <int B>
 static hipError_t short_conv_rows(const ShortConvParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)(row_blocks(p.tokens, p.slots.n, B) * conv_groups(p.channels)));
+  const dim3 grid((unsigned)(row_blocks(p.tokens, p.slots.n, B) * channel_groups(p.channels)));
   switch (p.width) {
     case 2: hipLaunchKernelGGL((short_conv_kernel<2, B>), grid, dim3(kThreads), 0, stream, p); break;
     case 3: hipLaunchKernelGGL((short_conv_kernel<3, B>), grid, dim3(kThreads), 0, stream, p); break;
@@ -106,11 +106,15 @@ static hipError_t short_conv_rows(const ShortConvParams& p, hipStream_t stream) 
   return hipGetLastError();
 }
 
+long long conv_groups(int tokens, int sequences, int channels) {
+  return row_blocks(tokens, sequences, 16) * channel_groups(channels);
+}
+
 // Blocks of 64 rows where they make two workgroups per CU (256 of them), which read their
 // weights and the rows before the block once for 64 rows: 9600 rows of 6144 channels take
 // 54 us so and 65 with blocks of 16.  Fewer rows are spread over more workgroups.
 hipError_t short_conv_launch(const ShortConvParams& p, hipStream_t stream) {
-  return (long long)p.tokens / 64 * conv_groups(p.channels) >= 512 ? short_conv_rows<64>(p, stream)
+  return (long long)p.tokens / 64 * channel_groups(p.channels) >= 512 ? short_conv_rows<64>(p, stream)
                                                                    : short_conv_rows<16>(p, stream);
 }
 
@@ -167,23 +171,34 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(const GatedNormPar
   }
 }
 
+static int norm_lanes(int dim) {
+  int lanes = 8;
+  while (8 * lanes < dim) lanes *= 2;
+  return lanes;
+}
+static int norm_rows_of(long long rows, int dim) { return rows * dim >= 1 << 22 ? 4 : 1; }
+long long gated_norm_groups(long long rows, int dim) {
+  const long long per = kThreads / norm_lanes(dim) * norm_rows_of(rows, dim);
+  return (rows + per - 1) / per;
+}
+
 template <int R>
-static hipError_t gated_norm_rows(const GatedNormParams& p, hipStream_t stream) {
-  int lpr = 8;
-  while (8 * lpr < p.dim) lpr *= 2;
-  const long long per = kThreads / lpr * R;
-  const dim3 grid((unsigned)((p.rows + per - 1) / per));
-  switch (lpr) {
+static void gated_norm_rows(const GatedNormParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)gated_norm_groups(p.rows, p.dim));
+  switch (norm_lanes(p.dim)) {
     case 8: hipLaunchKernelGGL((gated_norm_kernel<8, R>), grid, dim3(kThreads), 0, stream, p); break;
     case 16: hipLaunchKernelGGL((gated_norm_kernel<16, R>), grid, dim3(kThreads), 0, stream, p); break;
     case 32: hipLaunchKernelGGL((gated_norm_kernel<32, R>), grid, dim3(kThreads), 0, stream, p); break;
     default: hipLaunchKernelGGL((gated_norm_kernel<64, R>), grid, dim3(kThreads), 0, stream, p); break;
   }
-  return hipGetLastError();
 }
 
 hipError_t gated_norm_launch(const GatedNormParams& p, hipStream_t stream) {
-  return p.rows * p.dim >= 1 << 22 ? gated_norm_rows<4>(p, stream) : gated_norm_rows<1>(p, stream);
+  if (norm_rows_of(p.rows, p.dim) == 4)
+    gated_norm_rows<4>(p, stream);
+  else
+    gated_norm_rows<1>(p, stream);
+  return hipGetLastError();
 }
 
 }  // namespace aexq

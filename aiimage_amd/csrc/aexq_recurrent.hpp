@@ -22,6 +22,7 @@ struct ShortConvParams {
   long long x_stride, out_stride;
   const float *weight, *bias;  // [channels][width], [channels] or null
 };
+long long conv_groups(int tokens, int sequences, int channels);  // workgroups at most
 hipError_t short_conv_launch(const ShortConvParams& p, hipStream_t stream);
 // ---- root-mean-square norm of heads, gated by silu (aexq_mixer.hip)
 struct GatedNormParams {
@@ -33,6 +34,7 @@ struct GatedNormParams {
   int heads, dim;
   float eps;
 };
+long long gated_norm_groups(long long rows, int dim);  // workgroups
 hipError_t gated_norm_launch(const GatedNormParams& p, hipStream_t stream);
 // ---- the gated delta rule (aexq_delta.hip)
 struct DeltaParams {
