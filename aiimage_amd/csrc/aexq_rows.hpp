@@ -56,7 +56,7 @@ __device__ __forceinline__ RowBlock row_block(const int32_t* offsets, int tokens
   for (;; step /= 64) {
     const int s = lo + lane * step;
     const uint64_t at = __ballot(s < n && base(min(s, n - 1)) <= id);
-    lo += max(__popcll(at) - 1, 0) * step;
+    lo += max((int)__popcll(at) - 1, 0) * step;
     if (step == 1) break;
   }
   lo = sreg(lo);

@@ -82,7 +82,7 @@ __device__ __forceinline__ int sequence_of(const VerifyParams& p, int t) {
   for (;; step /= 64) {
     const int s = lo + lane * step;
     const uint64_t at = __ballot(s < n && p.offsets[min(s, n - 1)] <= t);
-    lo += max(__popcll(at) - 1, 0) * step;
+    lo += max((int)__popcll(at) - 1, 0) * step;
     if (step == 1) break;
   }
   return sreg(lo);
