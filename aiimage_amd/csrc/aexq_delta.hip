@@ -16,12 +16,22 @@ namespace aexq {
 struct Gate {
   float g, beta;
 };
+struct GateInputs {
+  f16 a, b;
+  float dt_bias, a_log;
+  __device__ __forceinline__ Gate gate() const {
+    const float t = (float)a + dt_bias;
+    const float soft = fmaxf(t, 0.0f) + log1pf(expf(-fabsf(t)));
+    const float g = -expf(a_log) * soft;
+    return Gate{g < -1e5f ? -1e5f : g, 1.0f / (1.0f + expf(-(float)b))};
+  }
+};
+__device__ __forceinline__ GateInputs gate_inputs(const DeltaParams& p, long long row, int head) {
+  return GateInputs{p.a[row * p.a_stride + head], p.b[row * p.b_stride + head], p.dt_bias[head],
+                    p.a_log[head]};
+}
 __device__ __forceinline__ Gate gate_of(const DeltaParams& p, long long row, int head) {
-  const float t = (float)p.a[row * p.a_stride + head] + p.dt_bias[head];
-  const float b = (float)p.b[row * p.b_stride + head];
-  const float soft = fmaxf(t, 0.0f) + log1pf(expf(-fabsf(t)));
-  const float g = -expf(p.a_log[head]) * soft;
-  return Gate{g < -1e5f ? -1e5f : g, 1.0f / (1.0f + expf(-b))};
+  return gate_inputs(p, row, head).gate();
 }
 
 // Sum and maximum of v over the four 16-lane rows of the wave, in every lane: rows swapped
@@ -132,6 +142,12 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
   // a block of up to 16 rows has one row tile, its first wave's; the others only share in
   // the transposed keys
   const bool small = live <= 16;
+  // gates of the first heads, a wave each, a row a lane
+  auto gates_from = [&](int h) {
+    return gate_inputs(p, span.first + t0 + min(lane, live - 1),
+                       hk * p.group + min(h + wave, p.group - 1));
+  };
+  GateInputs gates = gates_from(0);
   // rows past the last one repeat it; their factors are 0
   const long long row = span.first + t0 + min(own, live - 1);
   f16x8 k[KB], q[KB];
@@ -201,20 +217,15 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
       __syncthreads();
       if (h + wave < p.group) {
         // a row a lane: sums in 64 bits, as differences of large ones are taken
-        const int mine = head + wave;
-        Gate gate = {0.0f, 0.0f};
-        if (lane < live) gate = gate_of(p, span.first + t0 + lane, mine);
-        double G = (double)gate.g * 1.4426950408889634;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const double up = __shfl_up(G, off, 64);
-          if (lane >= off) G += up;
-        }
+        if (h) gates = gates_from(h);
+        Gate gate = gates.gate();
+        if (lane >= live) gate = Gate{0.0f, 0.0f};
+        const double G = wave_scan((double)gate.g * 1.4426950408889634);
         lds.sums[wave][lane] = G;
         lds.beta[wave][lane] = gate.beta;
         float* f = (float*)(to + wave * (long long)kDeltaHead + kDeltaFactors) + lane;
         const bool in = lane < live;
-        const float rk = lds.rk[lane], e = exp2_of(G), last = exp2_of(__shfl(G, 63, 64) - G);
+        const float rk = lds.rk[lane], e = exp2_of(G), last = exp2_of(last_lane(G) - G);
         f[kBeta * kDeltaRows] = gate.beta;
         f[kSeen * kDeltaRows] = in ? gate.beta * e * rk : 0.0f;
         f[kAsk * kDeltaRows] = in ? p.scale * e * lds.rq[lane] : 0.0f;

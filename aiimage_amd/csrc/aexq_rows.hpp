@@ -64,4 +64,30 @@ __device__ __forceinline__ RowBlock row_block(const int32_t* offsets, int tokens
   return RowBlock{lo, block < 0 ? 1 << 24 : block};
 }
 
+// A DPP move of a double; 0 where a lane has no source.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double last_lane(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, 63);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), 63);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sums up to and with each lane's, without a trip through LDS: inside rows of 16 lanes
+// (row_shr), then the last lane's of a row to the next, of two rows to the next two.
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp64<0x111, 0xF>(v);
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);
+  v += dpp64<0x143, 0xC>(v);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) { return last_lane(wave_scan(v)); }
 }  // namespace aexq
