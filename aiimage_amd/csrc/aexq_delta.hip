@@ -117,7 +117,7 @@ template <int DK>
 struct BlockLds {
   alignas(16) f16 k[kDeltaRows][DK + 8];
   alignas(16) float t[kDeltaRows][kDeltaRows + 4];
-  double sums[kGateHeads][kDeltaRows];  // of log2 of the decays, up to each row
+  alignas(32) double sums[kGateHeads][kDeltaRows];  // of log2 of the decays, up to each row
   float beta[kGateHeads][kDeltaRows], rk[kDeltaRows], rq[kDeltaRows];
 };
 
@@ -193,8 +193,8 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     const f32x4 rj = *(const f32x4*)&lds.rk[16 * j + 4 * g];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      ak[j][r] *= rk * rj[r];
-      aq[j][r] *= rq * rj[r];
+      ak[j][r] = own < live ? ak[j][r] * (rk * rj[r]) : 0.0f;
+      aq[j][r] = own < live ? aq[j][r] * (rq * rj[r]) : 0.0f;
     }
   }
   // the keys transposed, times a power of two (exact but for values below 2^-14, by 2^-25)
@@ -248,13 +248,16 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
       a[j] = f32x4{};
       w[j] = f16x4{};
       if (j > wave) continue;
+      // columns up to the lane's row; of the tiles before the wave's own, all
+      const int upto = j < wave ? 16 : here - 4 * g;
+      typedef double f64x4 __attribute__((ext_vector_type(4)));
+      const f64x4 Gj = *(const f64x4*)&lds.sums[slot][16 * j + 4 * g];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int ahead = 4 * g + r - here;  // of the wave's own tile: the column less the row
-        const bool seen = own < live && (j < wave || ahead <= 0);
-        const float e = exp2_of(G - lds.sums[slot][16 * j + 4 * g + r]);
-        a[j][r] = seen && (j < wave || ahead < 0) ? ak[j][r] * (e * beta) : 0.0f;
-        w[j][r] = (f16)(seen ? aq[j][r] * e * kPieceScale : 0.0f);
+        const float e = exp2_of(G - Gj[r]);
+        const float x = ak[j][r] * (e * beta), y = aq[j][r] * (e * kPieceScale);
+        a[j][r] = r < upto ? x : 0.0f;
+        w[j][r] = (f16)(r <= upto ? y : 0.0f);
       }
       if (j == wave) own_tile = a[j];
     }
