@@ -19,9 +19,14 @@ namespace aexq {
 // some hundreds on the other side.  So weights and sums are 64 bits here, 2^y from a
 // polynomial (v_exp has no such form).
 //   1. parts of rows: largest logit m, its index, Z = sum 2^((x - m) log2 e / T);
-//   2. parts of the sampled rows, which every workgroup finds for itself: their sums of
+//   2. runs of the sampled rows, which every workgroup finds for itself: their sums of
 //      2^((x - m) log2 e / T) and of max(p - q, 0);
-//   3. a workgroup a sequence: the part the number falls into, and the index in it.
+//   3. a workgroup a sequence: the run the number falls into, and the index in it.
+// 64-bit arithmetic bounds the first two: 265 rows of 151936 fp32 logits take 42 us (161
+// MB, 3.8 TB/s), 31 with a plain sum in the weights' place (5.1 TB/s) and 37 with each
+// thread's loads from one place; 64 sampled rows with draft probabilities 23 us (78 MB).
+// The third takes 6 us, and 13 where its scans go through LDS.  One sequence of five rows
+// is three launches of 3 to 6 us.
 // ---------------------------------------------------------------------------
 constexpr double kLog2eD = 1.4426950408889634074;
 
@@ -127,48 +132,52 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(const VerifyPa
     }
     p.draft[row] = d;
   }
-  // chunks lie on 16-byte boundaries: chunk c starts at logit c VE - skew
+  // chunks lie on 16-byte boundaries, chunk c at logit c VE - skew; those that are not
+  // whole go a logit a thread, the first one's with the first part, the last one's with
+  // the last
   const int skew = (int)((uintptr_t)x % 16 / sizeof(E));
-  const int chunks = (int)(((long long)p.n + skew + VE - 1) / VE);
-  const int c0 = min(part * p.cols, chunks), c1 = min(c0 + p.cols, chunks);
   const int whole0 = skew ? 1 : 0, whole1 = (int)(((long long)p.n + skew) / VE);
+  const int c0 = max(part * p.cols, whole0), c1 = min((part + 1) * p.cols, whole1);
+  const int head = skew ? min(VE - skew, p.n) : 0, tail = max(whole1 * VE - skew, head);
   typedef E Chunk __attribute__((ext_vector_type(VE)));
-  // U chunks of a thread, the ones of neighbours next to each other
+  E edge[2] = {(E)-INFINITY, (E)-INFINITY};
+  if (part == 0 && tid < head) edge[0] = x[tid];
+  if (part == p.parts - 1 && tail + tid < p.n) edge[1] = x[tail + tid];
+  // U chunks of a thread, the ones of neighbours next to each other; nothing from c1 on
   auto read = [&](int c, Chunk* v) {
-    if (c >= whole0 && c + (U - 1) * kThreads < min(c1, whole1)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = *(const Chunk*)(x + (c + u * kThreads) * VE - skew);
-      return;
-    }
+    for (int u = 0; u < U; ++u) v[u] = *(const Chunk*)(x + min(c + u * kThreads, c1 - 1) * VE - skew);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = c + u * kThreads, i0 = at * VE - skew;
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        v[u][i] = (E)-INFINITY;
-        if (at < c1 && i0 + i >= 0 && i0 + i < p.n) v[u][i] = x[i0 + i];
-      }
-    }
+    for (int u = 1; u < U; ++u)
+      if (c + u * kThreads >= c1) v[u] = (Chunk)(E)-INFINITY;
   };
   Best best = {-INFINITY, p.n};
   double z = 0.0;
   float from = -FLT_MAX;  // what the weights are relative to; none is above 2^500
   if (heat < 0.0) {
     bool odd = false;  // a NaN or a +inf: the row has no largest logit
+    auto take = [&](float y, int at) {
+      odd |= !(y < INFINITY);
+      if (y > best.m) best = Best{y, at};
+    };
+    take((float)edge[0], tid);
     for (int c = c0 + tid; c < c1; c += U * kThreads) {
       Chunk v[U];
       read(c, v);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const float y = (float)v[u][i];
-          odd |= !(y < INFINITY);
-          if (y > best.m) best = Best{y, (c + u * kThreads) * VE - skew + i};
-        }
+        for (int i = 0; i < VE; ++i) take((float)v[u][i], (c + u * kThreads) * VE - skew + i);
     }
+    take((float)edge[1], tail + tid);
     if (odd) z = __builtin_nan("");
   } else {
+    auto relate = [&]() {
+      if (((double)best.m - (double)from) * heat > 500.0) {
+        z *= weight_of(from, best.m, heat);
+        from = best.m;
+      }
+    };
     for (int c = c0 + tid; c < c1; c += U * kThreads) {
       Chunk v[U];
       read(c, v);
@@ -177,14 +186,17 @@ __global__ __launch_bounds__(kThreads, 4) void verify_rows_kernel(const VerifyPa
 #pragma unroll
         for (int i = 0; i < VE; ++i)
           best.m = __builtin_elementwise_maximum(best.m, (float)v[u][i]);
-      if (((double)best.m - (double)from) * heat > 500.0) {
-        z *= weight_of(from, best.m, heat);
-        from = best.m;
-      }
+      relate();
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < VE; ++i) z += weight_of((float)v[u][i], from, heat);
+    }
+    if (__any(fmaxf((float)edge[0], (float)edge[1]) > -INFINITY || edge[0] != edge[1])) {
+      best.m = __builtin_elementwise_maximum(best.m, (float)edge[0]);
+      best.m = __builtin_elementwise_maximum(best.m, (float)edge[1]);
+      relate();
+      z += weight_of((float)edge[0], from, heat) + weight_of((float)edge[1], from, heat);
     }
     if (!(best.m < INFINITY)) z = __builtin_nan("");
   }
