@@ -2565,11 +2565,14 @@ extern "C" aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots,
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d sequences and %d heads in one call",
                 tokens, p.slots.n, heads_v);
   const long long heads = blocks * heads_v * kDeltaHead;
-  st = grow_step_scratch(ctx, &ctx->delta_mem, &ctx->delta_cap,
-                         heads + blocks * heads_k * delta_key_bytes(dim_k), op, "delta rule blocks");
+  const long long keys = blocks * heads_k * delta_key_bytes(dim_k);
+  const long long longs = delta_splits(p, ctx->cus) ? 4LL * (p.slots.n + 1) : 0;
+  st = grow_step_scratch(ctx, &ctx->delta_mem, &ctx->delta_cap, heads + keys + longs, op,
+                         "delta rule blocks");
   if (st) return st;
   p.heads = (char*)ctx->delta_mem;
   p.keys = p.heads + heads;
+  p.longs = longs ? (int*)(p.keys + keys) : nullptr;
   const hipError_t e = delta_prompt_launch(p, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "delta rule launch");
   return AEXQ_OK;

@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
   if (live <= 0) return;
   // a block of up to 16 rows has one row tile, its first wave's; the others only share in
   // the transposed keys
-  const bool small = live <= 16;
+  const bool small = live <= kDeltaEnd;
   // gates of the first heads, a wave each, a row a lane
   auto gates_from = [&](int h) {
     return gate_inputs(p, span.first + t0 + min(lane, live - 1),
@@ -910,29 +910,52 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
   }
 }
 
+// The parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the same
+// rows and pieces.  A sequence's place and head, and the part, of workgroup `id`.
+struct DeltaPlace {
+  int place, head, part;
+};
+__device__ __forceinline__ DeltaPlace place_of(const DeltaParams& p, int id) {
+  const int parts = p.dv / 16, unit = id / (8 * parts) * 8 + id % 8;
+  return DeltaPlace{unit / p.hv, unit % p.hv, id / 8 % parts};
+}
 template <int DK>
-__global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams p) {
-  __shared__ DeltaLds<DK> lds;
-  // the parts of one head lie on one XCD (workgroup b runs on XCD b % 8): they read the
-  // same rows and pieces
-  const int parts = p.dv / 16, unit = blockIdx.x / (8 * parts) * 8 + blockIdx.x % 8;
-  if (unit >= p.slots.n * p.hv) return;
-  const int s = unit / p.hv;
-  DeltaWave<DK> x(p);
-  x.span = span_of(p.slots, p.offsets, p.tokens, s);
-  if (!x.span.kept) return;
-  x.head = unit % p.hv;
-  x.hk = x.head / p.group;
-  x.col = blockIdx.x / 8 % parts * 16;
+__device__ __forceinline__ void take_place(DeltaWave<DK>& x, int s, const DeltaPlace& at) {
+  x.span = span_of(x.p.slots, x.p.offsets, x.p.tokens, s);
+  x.head = at.head;
+  x.hk = at.head / x.p.group;
+  x.col = at.part * 16;
   x.id0 = x.span.first / kDeltaRows + s;
   x.lane = threadIdx.x & 63;
   x.c = x.lane & 15;
   x.g = x.lane >> 4;
+}
+// From the start again, row after row (the state in memory is still the one before), where
+// something is not finite; then the state behind the rows.
+template <int DK>
+__device__ __forceinline__ void leave(DeltaWave<DK>& x, bool odd) {
+  if (__any(odd)) {
+    wait_vm<0>();
+    x.read();
+    x.scale = Lift{1.0f, 1.0f};
+    x.rows(0, x.span.kept);
+  }
+  x.write();
+}
+
+template <int DK>
+__global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams p) {
+  __shared__ DeltaLds<DK> lds;
+  const DeltaPlace at = place_of(p, blockIdx.x);
+  if (at.place >= (p.longs ? p.longs[0] : p.slots.n)) return;
+  DeltaWave<DK> x(p);
+  take_place(x, p.longs ? p.longs[1 + at.place] : at.place, at);
+  if (!x.span.kept) return;
   const int all = (x.span.kept + kDeltaRows - 1) / kDeltaRows;
   // a last block of up to 16 rows takes a quarter of the products, and one wave
-  const bool short_end = x.span.kept - (all - 1) * kDeltaRows <= 16;
-  const int blocks = sreg(all - short_end), wave = sreg((int)threadIdx.x >> 6);
-  if (wave) {
+  const bool short_end = x.span.kept - (all - 1) * kDeltaRows <= kDeltaEnd;
+  const int blocks = sreg(all - short_end);
+  if (sreg((int)threadIdx.x >> 6)) {
     if (!blocks) return;
     delta_outputs<DK>(x, lds, blocks);
     wait_vm<0>();
@@ -947,14 +970,38 @@ __global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams 
   }
   if (short_end) odd |= delta_end<DK>(x, blocks, !blocks);
   if (blocks) __syncthreads();  // the outputs are in place
-  if (__any(odd)) {
-    wait_vm<0>();
-    // from the start again, row after row (the state in memory is still the one before)
-    x.read();
-    x.scale = Lift{1.0f, 1.0f};
-    x.rows(0, x.span.kept);
+  leave(x, odd);
+}
+
+// Calls of many short sequences: those of up to 16 rows, a wave a part and no LDS, which
+// keeps twice as many on a CU (48 sequences of 2 to 8 rows, 16 heads of 128 x 128: 26 us,
+// where the kernel above takes 35).  One workgroup more lists the longer ones for that
+// kernel, their number first.
+template <int DK>
+__global__ __launch_bounds__(64) void delta_short_kernel(const DeltaParams p) {
+  if (blockIdx.x == 0) {
+    const int lane = threadIdx.x;
+    auto rows_of = [&](int s) {
+      return s < p.slots.n ? span_of(p.slots, p.offsets, p.tokens, s).kept : 0;
+    };
+    int n = 0, rows = rows_of(lane);
+    for (int s = lane; s - lane < p.slots.n; s += 64) {
+      const int next = rows_of(s + 64);
+      const uint64_t at = __ballot(rows > kDeltaEnd);
+      if (rows > kDeltaEnd) p.longs[1 + n + __popcll(at & ((1ull << lane) - 1))] = s;
+      n += (int)__popcll(at);
+      rows = next;
+    }
+    if (lane == 0) p.longs[0] = n;
+    return;
   }
-  x.write();
+  const DeltaPlace at = place_of(p, blockIdx.x - 1);
+  if (at.place >= p.slots.n) return;
+  DeltaWave<DK> x(p);
+  take_place(x, at.place, at);
+  if (!x.span.kept || x.span.kept > kDeltaEnd) return;
+  x.read();
+  leave(x, delta_end<DK>(x, 0, true));
 }
 
 template <int DK>
@@ -962,12 +1009,27 @@ static hipError_t prompt_launch(const DeltaParams& p, hipStream_t stream) {
   const long long blocks = row_blocks(p.tokens, p.slots.n, kDeltaRows);
   hipLaunchKernelGGL(delta_block_kernel<DK>, dim3((unsigned)(blocks * p.hk)), dim3(kThreads), 0,
                      stream, p);
-  const hipError_t e = hipGetLastError();
+  hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const long long units = ((long long)p.slots.n * p.hv + 7) / 8 * 8;
-  hipLaunchKernelGGL(delta_prompt_kernel<DK>, dim3((unsigned)(units * (p.dv / 16))), dim3(128), 0,
-                     stream, p);
+  const int parts = p.dv / 16;
+  auto groups = [&](long long places) { return (unsigned)((places * p.hv + 7) / 8 * 8 * parts); };
+  long long places = p.slots.n;
+  if (p.longs) {
+    hipLaunchKernelGGL(delta_short_kernel<DK>, dim3(1 + groups(places)), dim3(64), 0, stream, p);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const long long most = p.tokens / (kDeltaEnd + 1);  // longer ones
+    if (most < places) places = most;
+    if (!places) return hipSuccess;
+  }
+  hipLaunchKernelGGL(delta_prompt_kernel<DK>, dim3(groups(places)), dim3(128), 0, stream, p);
   return hipGetLastError();
+}
+
+// Sequences of up to 16 rows apart, where the mean is at most 32 and there are more
+// workgroups than the four a CU that LDS lets the longer ones' kernel have.
+bool delta_splits(const DeltaParams& p, int cus) {
+  return (long long)p.slots.n * p.hv * (p.dv / 16) > 4LL * cus && p.tokens <= 32LL * p.slots.n;
 }
 
 hipError_t delta_prompt_launch(const DeltaParams& p, hipStream_t stream) {

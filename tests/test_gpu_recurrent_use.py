@@ -453,6 +453,57 @@ def test_rows_as_far_apart_as_they_may_be(aexq, ctx):
     assert (tokens[:-4] == 0).all()
 
 
+@pytest.mark.parametrize("n,hk,hv,dk,dv", [(100, 2, 4, 128, 128), (300, 1, 2, 64, 256)])
+def test_short_sequences_and_a_few_long_ones(aexq, ctx, n, hk, hv, dk, dv):
+    """Many sequences of 0 to 17 rows with longer ones, a state that is not finite, counts
+    that leave a long one short, slots of no state: each as by itself."""
+    print(f"[gpu-case] {n} sequences, mostly short, {hk}/{hv} {dk}x{dv}", flush=True)
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, 18, (n,), generator=g).tolist()
+    for s, m in ((3, 200), (64, 65), (65, 16), (66, 17), (n - 1, 130), (n - 2, 80)):
+        lens[s] = m
+    kept = list(lens)
+    kept[n - 2], kept[7] = 9, 0
+    total, off = sum(lens), ref.offsets(lens)
+    d = dict(q=_randn(total, hk, dk, seed=1).half(), k=_randn(total, hk, dk, seed=2).half(),
+             v=_randn(total, hv, dv, seed=3).half(), a=_randn(total, hv, seed=4).half(),
+             b=_randn(total, hv, seed=5).half(), a_log=_randn(hv, seed=6),
+             dt_bias=_randn(hv, seed=7) - 1)
+    state = _randn(n, hv, dk, dv, seed=8)
+    state[65, 0, 3, 5], state[3, 1, 7, 9] = math.inf, math.nan
+    before = state.clone()
+    slot = [s if s % 10 != 9 or s in (n - 1,) else -1 for s in range(n)]
+    out = torch.full((total, hv, dv), 7.0, device="cuda").half()
+    ctx.delta_prompt(aexq.slots(n, n, slot=ref.i32(slot), counts=ref.i32(kept)), state, off, **d,
+                     out=out, scale=0.1)
+    torch.cuda.synchronize()
+    at = off.tolist()
+    for s in list(range(0, n, 23)) + [3, 7, 64, 65, 66, n - 2, n - 1]:
+        r = slice(at[s], at[s] + kept[s])
+        assert (out[at[s] + kept[s]:at[s + 1]] == 7).all()
+        if not kept[s]:
+            assert torch.equal(state[s], before[s])
+            continue
+        rows = {k: t if k in ("a_log", "dt_bias") else t[r] for k, t in d.items()}
+        begin = before[s] if slot[s] >= 0 else torch.zeros_like(before[s])
+        y, near, S, err = ref.delta(**rows, state=begin, scale=0.1, eps=1e-6)
+        if s in (3, 65):   # the other columns; this one is not finite from the start
+            h, j = (1, 9) if s == 3 else (0, 5)
+            assert not torch.isfinite(out[r][:, h, j]).any()
+            assert not torch.isfinite(state[s, h, :, j]).any()
+            keep = torch.ones((hv, dv), dtype=torch.bool, device="cuda")
+            keep[h, j] = False
+            ref.check(out[r][:, keep], y[:, keep], near[:, keep], f"sequence {s}")
+            ref.check(state[s].transpose(1, 2)[keep], S.transpose(1, 2)[keep],
+                      err.transpose(1, 2)[keep], f"state {s}")
+            continue
+        ref.check(out[r], y, near, f"sequence {s}")
+        if slot[s] >= 0:
+            ref.check(state[s], S, err, f"state {s}")
+        else:
+            assert torch.equal(state[s], before[s])
+
+
 @pytest.mark.parametrize("n", [65, 4097, 20000])
 def test_thousands_of_sequences(aexq, ctx, n):
     """Sequences of 0 to 3 rows, found by their rows in several steps: the same bits as
