@@ -65,9 +65,10 @@ __device__ __forceinline__ float rows_max(float v) {
 // decays and of 1 - beta k^ k^T, which lengthen nothing, times k^_j.
 //
 // fp32 results from fp16 matrix products: k and q are fp16 already and taken as they
-// are, their lengths put into the rows' factors; S, T, R and U are split into two fp16
+// are, their lengths put into the rows' factors; S, T, P, R and U are split into two fp16
 // numbers, x = x0 + x1 up to 2^-22 of x, scaled by powers of two so that neither part
-// leaves fp16's range.  P is rounded to fp16 once, by 2^-11, as it only enters outputs.
+// leaves fp16's range.  (P in one part, 2^-11 of it, takes outputs half as far again from
+// the exact ones as their own rounding does.)
 //
 // Pieces of T and P lie in scratch in the order in which a lane of a matrix product
 // takes them: 16 rows by 32 columns, lane (m = l % 16, g = l / 16) row m, columns 4 g ..
@@ -112,6 +113,24 @@ __device__ __forceinline__ void unrolled(F f) {
   }
 }
 
+// Eight values as two fp16 numbers x0 + x1 each.
+struct Split {
+  f16x8 x0, x1;
+};
+__device__ __forceinline__ Split split8(const f32x4& a, const f32x4& b) {
+  const f16x4 a0 = __builtin_convertvector(a, f16x4), b0 = __builtin_convertvector(b, f16x4);
+  f16x4 a1, b1;
+  float one = 1.0f;  // (a product that is seen as one: v_fma_mix takes x0 as it is, and rounds)
+  asm("" : "+s"(one));
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    a1[r] = (f16)fmaf(a[r], one, -(float)a0[r]);
+    b1[r] = (f16)fmaf(b[r], one, -(float)b0[r]);
+  }
+  return Split{__builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7),
+               __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7)};
+}
+
 constexpr int kGateHeads = kWaves;  // heads whose gates are made together, a wave each
 template <int DK>
 struct BlockLds {
@@ -126,8 +145,8 @@ struct BlockLds {
 // 16 j + 4 g + r, which is how A and P enter the products behind.
 //
 // Bound by memory: a block reads 32 KB of k and q (heads of 128) and writes 48 KB of them
-// in the products' order and 19 KB of T, P and factors for each value head.  16384 rows of
-// 16 key and 32 value heads: 96 us for 490 MB.
+// in the products' order and 25 KB of T, P and factors for each value head.  16384 rows of
+// 16 key and 32 value heads: 99 us for 540 MB (a copy of that size runs at 5.3 TB/s).
 template <int DK>
 __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaParams p) {
   constexpr int KB = DK / 32;
@@ -241,12 +260,11 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     // A and P of the wave's rows
     const double G = lds.sums[slot][own];
     const float beta = lds.beta[slot][own];
-    f32x4 a[4], own_tile = f32x4{};
-    f16x4 w[4];
+    f32x4 a[4], w[4], own_tile = f32x4{};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       a[j] = f32x4{};
-      w[j] = f16x4{};
+      w[j] = f32x4{};
       if (j > wave) continue;
       // columns up to the lane's row; of the tiles before the wave's own, all
       const int upto = j < wave ? 16 : here - 4 * g;
@@ -257,15 +275,17 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
         const float e = exp2_of(G - Gj[r]);
         const float x = ak[j][r] * (e * beta), y = aq[j][r] * (e * kPieceScale);
         a[j][r] = r < upto ? x : 0.0f;
-        w[j][r] = (f16)(r <= upto ? y : 0.0f);
+        w[j][r] = r <= upto ? y : 0.0f;
       }
       if (j == wave) own_tile = a[j];
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b)
-      if (b <= wave / 2)
-        *(f16x8*)(to + ((12 + piece_of(wave, b)) * 64 + lane) * 16) =
-            __builtin_shufflevector(w[2 * b], w[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+      if (b <= wave / 2) {
+        const Split x = split8(w[2 * b], w[2 * b + 1]);
+        *(f16x8*)(to + ((12 + piece_of(wave, b) * 2) * 64 + lane) * 16) = x.x0;
+        *(f16x8*)(to + ((13 + piece_of(wave, b) * 2) * 64 + lane) * 16) = x.x1;
+      }
     // T's diagonal tiles by substitution, column c in lane c (the four rows of lanes do the
     // same): row i of A comes from lane i of each row of lanes
     *(f32x4*)&lds.t[own][16 * wave + 4 * g] = own_tile;
@@ -333,21 +353,16 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     for (int b = 0; b < 2; ++b) {
       if (b > wave / 2) continue;
       const int piece = piece_of(wave, b);
-      f16x8 t0, t1;
+      f32x4 v[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int tile = 2 * b + half;
-        f32x4 v = f32x4{};
-        if (tile <= wave) v = *(const f32x4*)&lds.t[own][16 * tile + 4 * g];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = v[r] * kPieceScale;
-          t0[4 * half + r] = (f16)y;
-          t1[4 * half + r] = (f16)(y - (float)t0[4 * half + r]);
-        }
+        v[half] = f32x4{};
+        if (tile <= wave) v[half] = *(const f32x4*)&lds.t[own][16 * tile + 4 * g] * kPieceScale;
       }
-      *(f16x8*)(to + ((piece * 2) * 64 + lane) * 16) = t0;
-      *(f16x8*)(to + ((piece * 2 + 1) * 64 + lane) * 16) = t1;
+      const Split x = split8(v[0], v[1]);
+      *(f16x8*)(to + ((piece * 2) * 64 + lane) * 16) = x.x0;
+      *(f16x8*)(to + ((piece * 2 + 1) * 64 + lane) * 16) = x.x1;
     }
   }
 }
@@ -366,23 +381,6 @@ __device__ __forceinline__ float top4(float m, const f32x4& v) {
   for (int r = 0; r < 4; r += 2)
     m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(v[r])), fabsf(v[r + 1]));
   return m;
-}
-// Eight values as two fp16 numbers x0 + x1 each.
-struct Split {
-  f16x8 x0, x1;
-};
-__device__ __forceinline__ Split split8(const f32x4& a, const f32x4& b) {
-  const f16x4 a0 = __builtin_convertvector(a, f16x4), b0 = __builtin_convertvector(b, f16x4);
-  f16x4 a1, b1;
-  float one = 1.0f;  // (a product that is seen as one: v_fma_mix takes x0 as it is, and rounds)
-  asm("" : "+s"(one));
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    a1[r] = (f16)fmaf(a[r], one, -(float)a0[r]);
-    b1[r] = (f16)fmaf(b[r], one, -(float)b0[r]);
-  }
-  return Split{__builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7),
-               __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7)};
 }
 __device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -543,7 +541,8 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
   const f32x4 beta = x.factor(head, kBeta, 0), seen_by = x.factor(head, kSeen, 0);
 #pragma unroll
   for (int i = 0; i < KB; ++i) q[i] = x.piece(keys, 4 * KB + i);
-  const f16x8 t0 = x.piece(head, 0), t1 = x.piece(head, 1), w = x.piece(head, 12);
+  const f16x8 t0 = x.piece(head, 0), t1 = x.piece(head, 1);
+  const f16x8 w0 = x.piece(head, 12), w1 = x.piece(head, 13);
   const f32x4 left = x.factor(head, kLeft, 0), ask = x.factor(head, kAsk, 0);
 #pragma unroll
   for (int i = 0; i < 2 * KB; ++i) kt[i] = x.piece(keys, 8 * KB + 2 * i);
@@ -583,8 +582,9 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
     x.S[i] = mfma(kt[i], ys.x0, x.S[i]);
     x.S[i] = mfma(kt[i], ys.x1, x.S[i]);
   }
-  f32x4 a = mfma(w, us.x0, f32x4{});
-  a = mfma(w, us.x1, a);
+  f32x4 a = mfma(w0, us.x0, f32x4{});
+  a = mfma(w0, us.x1, a);
+  a = mfma(w1, us.x0, a);
   const float back = p.scale * lu.back * (1.0f / kPieceScale);
   if (p.out) {
     const auto to = x.rows_of(p.out, p.out_stride, b);
@@ -607,7 +607,7 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // A block takes the first wave 1.9 us: 82 matrix products (1300 cycles), 300 vector
 // operations between them (1200) and 52 loads, which it has to issue itself, all in one
 // chain from state to state.  16384 rows of 32 value heads of 128 x 128, one sequence:
-// 490 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 90 us.  One wave for
+// 500 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 97 us.  One wave for
 // all of it takes 777 and 112 us.  Eight waves that each hold 16 rows of S of 16 columns
 // and add their products through LDS: 450 and 103; blocks of 16 rows 77 us where the last
 // ones go through one wave in 35.
@@ -765,7 +765,7 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
   constexpr int KB = DK / 32;
   const DeltaParams& p = x.p;
   const int lane = x.lane;
-  f16x8 q[4][KB], w[4][2];
+  f16x8 q[4][KB], w[4][2][2];
   f32x4 ask[4], beta[4];
   f16 v[4][4];
   const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
@@ -798,7 +798,10 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j <= i / 2; ++j) w[i][j] = x.piece(head, 12 + piece_of(i, j));
+      for (int j = 0; j <= i / 2; ++j)
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+          w[i][j][part] = x.piece(head, 12 + piece_of(i, j) * 2 + part);
       ask[i] = x.factor(head, kAsk, i);
     }
   };
@@ -883,9 +886,11 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
-      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j], us[j].x0, o[i]);
+      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j][0], us[j].x0, o[i]);
 #pragma unroll
-      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j], us[j].x1, o[i]);
+      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j][0], us[j].x1, o[i]);
+#pragma unroll
+      for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j][1], us[j].x0, o[i]);
     }
     const float back_s = lds.back_s[at][lane];
     const float back = p.scale * lu.back * lds.back_u[at][lane] * (1.0f / kPieceScale);

@@ -53,12 +53,12 @@ struct DeltaParams {
   char* keys;
   int* longs;  // sequences of more than 16 rows, their number first; null: not apart
 };
-// Scratch of a block and value head: six (16 rows, 32 columns) pieces of T in two fp16
-// parts and of P in one, 1 KB each; four factors a row and the block's decay.  Of a block
+// Scratch of a block and value head: six (16 rows, 32 columns) pieces of T and as many of
+// P, each in two fp16 parts of 1 KB; four factors a row and the block's decay.  Of a block
 // and key head: three times its rows.
 constexpr int kDeltaRows = 64;
 constexpr int kDeltaEnd = 16;  // rows of a last block that go through one row tile
-constexpr int kDeltaFactors = 18 * 1024;
+constexpr int kDeltaFactors = 24 * 1024;
 constexpr int kDeltaHead = kDeltaFactors + 4 * kDeltaRows * 4 + 64;
 constexpr int delta_key_bytes(int dk) { return 3 * dk * kDeltaRows * 2; }
 bool delta_splits(const DeltaParams& p, int cus);

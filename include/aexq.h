@@ -503,7 +503,7 @@ aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
  * none of the inputs.  States and sums are fp32.  What follows a value that is not
  * finite in its column of the state is not finite (an infinity or a NaN); what comes
  * before it, other columns, heads and sequences do not meet it.  Uses the context's
- * scratch, 19 KB for 64 rows of a value head and 3 dim_k fp16 for each of a key head's. */
+ * scratch, 25 KB for 64 rows of a value head and 3 dim_k fp16 for each of a key head's. */
 aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots, float* state,
                               const int32_t* offsets, int tokens, const void* q, int64_t q_stride,
                               const void* k, int64_t k_stride, const void* v, int64_t v_stride,

@@ -71,8 +71,7 @@ def delta(q, k, v, a, b, a_log, dt_bias, state, scale, eps):
     numbers (2^-22 of each factor, in sums over 64 rows and dim_k values, both signs),
     of the column's length and of v.  8 times 2^-22 of both covers either.  The decay
     is off by some 2^-22 of itself for each unit of its logarithm, at most 2^-22 of the
-    column.  In outputs the products of q^ with the keys of up to 64 rows are rounded to
-    fp16, by 2^-11 of what they carry of |u|."""
+    column."""
     n, hk, dk = q.shape
     hv, dv = v.shape[1:]
     group = hv // hk
@@ -87,21 +86,15 @@ def delta(q, k, v, a, b, a_log, dt_bias, state, scale, eps):
     g = -torch.exp(a_log.double()) * soft
     beta = torch.sigmoid(b.double())
     one = 8 * 2.0 ** -22
-    us = torch.zeros((n, hv, dv), dtype=torch.float64, device="cuda")
-    left = torch.ones((n, hv), dtype=torch.float64, device="cuda")   # of row j at row i
     for i in range(n):
         e = torch.exp(g[i])[:, None, None]
-        left[:i] *= e[:, 0, 0]
         S = S * e
         u = beta[i][:, None] * (v[i].double() - (S * kn[i][..., None]).sum(1))
         S = S + kn[i][..., None] * u[:, None]
         size = S.square().sum(1, keepdim=True).sqrt() + v[i].double().abs()[:, None]
         E = E * e + one * size
         out[i] = scale * (S * qn[i][..., None]).sum(1)
-        us[i] = u.abs()
-        j = slice(max(0, i - 63), i + 1)
-        carried = (left[j] * (kn[j] * qn[i]).sum(-1).abs())[..., None] * us[j]
-        near[i] = abs(scale) * ((E + one * size)[:, 0] + 2.0 ** -11 * carried.sum(0))
+        near[i] = abs(scale) * (E + one * size)[:, 0]
     bound = near + _half(out) * (1 + 2.0 ** -10)
     return out, bound, S, E.expand_as(S) + 2.0 ** -24 * S.abs() + 2.0 ** -140
 
