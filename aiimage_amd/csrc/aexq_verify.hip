@@ -22,8 +22,8 @@ namespace aexq {
 //   2. runs of the sampled rows, which every workgroup finds for itself: their sums of
 //      2^((x - m) log2 e / T) and of max(p - q, 0);
 //   3. a workgroup a sequence: the run the number falls into, and the index in it.
-// 64-bit arithmetic bounds the first two: 265 rows of 151936 fp32 logits take 42 us (161
-// MB, 3.8 TB/s), 31 with a plain sum in the weights' place (5.1 TB/s) and 37 with each
+// 64-bit arithmetic bounds the first two: 265 rows of 151936 fp32 logits take 40 us (161
+// MB, 4.0 TB/s), 31 with a plain sum in the weights' place (5.1 TB/s) and 37 with each
 // thread's loads from one place; 64 sampled rows with draft probabilities 23 us (78 MB).
 // The third takes 6 us, and 13 where its scans go through LDS.  One sequence of five rows
 // is three launches of 3 to 6 us.
@@ -47,8 +47,10 @@ __device__ __forceinline__ double exp2_series(double y) {
   p = fma(p, f, 2.402265069581299e-1);
   p = fma(p, f, 6.931471805459335e-1);
   p = fma(p, f, 1.0);
-  return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) +
-                                        (__builtin_bit_cast(uint64_t, t) << 52));
+  typedef uint32_t Words __attribute__((ext_vector_type(2)));
+  Words w = __builtin_bit_cast(Words, p);
+  w.y += __builtin_bit_cast(Words, t).x << 20;
+  return __builtin_bit_cast(double, w);
 }
 
 // What a row's logits are scaled by, in log2 units; 0 or below: the largest one wins.
