@@ -614,9 +614,16 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // ---------------------------------------------------------------------------
 template <int DK>
 struct DeltaLds {
-  f16x8 s[2][DK / 32][2][64];  // by the block's parity: parts of S
+  static constexpr int kPitch = 24;  // of 16 columns: no two rows of a read share banks
+  f16x8 s[2][DK / 32][2][64];        // by the block's parity: parts of S
   f32x4 u[2][4][64], v[2][4][64];
+  f32x4 factors[2][kDecay * kDeltaRows / 4];
   float back_s[2][64], back_u[2][64];  // what S and U are to be multiplied by
+  alignas(16) f16 rows[kDeltaRows][kPitch];  // of v, then of the outputs: the second wave's
+  // Factors of rows 16 tile + 4 g ..
+  __device__ __forceinline__ f32x4 factor(int at, int which, int tile, int g) const {
+    return factors[at][(which * kDeltaRows + 16 * tile) / 4 + g];
+  }
 };
 
 template <int DK>
@@ -633,10 +640,6 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
   auto load_kt = [&](__amdgpu_buffer_rsrc_t at, int n) {
     a[n] = x.piece(at, 8 * KB + 2 * (n % (2 * KB)) + n / (2 * KB));
   };
-  auto load_seen = [&](__amdgpu_buffer_rsrc_t h) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) seen_by[w] = x.factor(h, kSeen, w);
-  };
   auto load_t = [&](__amdgpu_buffer_rsrc_t h) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -645,30 +648,27 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
 #pragma unroll
         for (int i = 0; i < 2; ++i) t[w][j][i] = x.piece(h, piece_of(w, j) * 2 + i);
   };
-  auto load_left = [&](__amdgpu_buffer_rsrc_t h) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) left[w] = x.factor(h, kLeft, w);
-    decay = x.decay_of(h);
-  };
   {
     const auto keys = x.keys_of(0), head = x.head_of(0);
-    load_seen(head);
-    __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
     load_t(head);
-    __builtin_amdgcn_sched_barrier(0);
-    load_left(head);
+    __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
+    decay = x.decay_of(head);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < 4 * KB; ++n) load_k(keys, n);
     __builtin_amdgcn_sched_barrier(0);
   }
-  __syncthreads();  // the first block's v
+  __syncthreads();  // the first block's v and factors
   for (int b = 0; b < blocks; ++b) {
     const int next = min(b + 1, blocks - 1), at = b & 1;
     const auto keys = x.keys_of(b);
     f32x4 seen[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) seen[w] = f32x4{};
+    for (int w = 0; w < 4; ++w) {
+      seen[w] = f32x4{};
+      seen_by[w] = lds.factor(at, kSeen, w, x.g);
+      left[w] = lds.factor(at, kLeft, w, x.g);
+    }
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
       const Split s = split8(x.S[2 * i], x.S[2 * i + 1]);
@@ -703,8 +703,6 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
 #pragma unroll
     for (int j = 0; j < 2; ++j) rs[j] = split8(r[2 * j] * lr.by, r[2 * j + 1] * lr.by);
     const auto head = x.head_of(next);
-    __builtin_amdgcn_sched_barrier(0);
-    load_seen(head);
     __builtin_amdgcn_sched_barrier(0);
     // U = T R
     f32x4 u[4], y[4];
@@ -741,7 +739,7 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
     x.rescale(keep);
     x.scale = ls;
     __builtin_amdgcn_sched_barrier(0);
-    load_left(head);
+    decay = x.decay_of(head);
     __builtin_amdgcn_sched_barrier(0);
     const auto after = x.keys_of(next);
 #pragma unroll
@@ -766,29 +764,40 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
   const DeltaParams& p = x.p;
   const int lane = x.lane;
   f16x8 q[4][KB], w[4][2][2];
-  f32x4 ask[4], beta[4];
-  f16 v[4][4];
+  // v and the outputs move 16 bytes a lane, eight columns of row lane / 2 (and 32 more),
+  // and change places in LDS: 16 loads or stores of two bytes a lane take a CU's address
+  // unit as long as the operands' 16 of 16
+  f16x8 v[2];
+  f32x4 factors;
+  const int row = lane / 2, part = lane % 2 * 8;
   const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
-  const uint32_t at_v = 4 * x.g * step_v + 2 * x.c, at_out = 4 * x.g * step_out + 2 * x.c;
   auto load_v = [&](int b) {
     const auto from = x.rows_of(p.v, p.v_stride, b), head = x.head_of(b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[i][e] = __builtin_bit_cast(
-            f16, __builtin_amdgcn_raw_buffer_load_b16(from, at_v + e * step_v, 16 * i * step_v, 0));
-      beta[i] = x.factor(head, kBeta, i);
-    }
+    for (int i = 0; i < 2; ++i)
+      v[i] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(
+                                           from, row * step_v + 2 * part, 32 * i * step_v, 0));
+    factors = __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(head, 16 * lane, kDeltaFactors, 0));
+  };
+  auto meet = [] {  // LDS written by one lane and read by another
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
   auto put_v = [&](int b) {
+    lds.factors[b & 1][lane] = factors;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) *(f16x8*)&lds.rows[32 * i + row][part] = v[i];
+    meet();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const f32x4 beta = lds.factor(b & 1, kBeta, i, x.g);
       f32x4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = beta[i][e] * (float)v[i][e];
+      for (int e = 0; e < 4; ++e) y[e] = beta[e] * (float)lds.rows[16 * i + 4 * x.g + e][x.c];
       lds.v[b & 1][i][lane] = y;
     }
+    meet();
   };
   auto load_q = [&](__amdgpu_buffer_rsrc_t keys, int i) {
 #pragma unroll
@@ -802,7 +811,6 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
         for (int part = 0; part < 2; ++part)
           w[i][j][part] = x.piece(head, 12 + piece_of(i, j) * 2 + part);
-      ask[i] = x.factor(head, kAsk, i);
     }
   };
   // What a block takes comes from memory, later than a block takes to pass: a byte of each
@@ -892,6 +900,9 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
       for (int i = 2 * j; i < 4; ++i) o[i] = mfma(w[i][j][1], us[j].x0, o[i]);
     }
+    f32x4 ask[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ask[i] = lds.factor(at, kAsk, i, x.g);
     const float back_s = lds.back_s[at][lane];
     const float back = p.scale * lu.back * lds.back_u[at][lane] * (1.0f / kPieceScale);
 #pragma unroll
@@ -908,9 +919,14 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, (f16)o[i][e]), to,
-                                                at_out + e * step_out, 16 * i * step_out, 0);
+        for (int e = 0; e < 4; ++e) lds.rows[16 * i + 4 * x.g + e][x.c] = (f16)o[i][e];
+      meet();
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, *(const f16x8*)&lds.rows[32 * i + row][part]), to,
+            row * step_out + 2 * part, 32 * i * step_out, 0);
+      meet();
     }
   }
 }
