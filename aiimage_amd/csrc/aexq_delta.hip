@@ -605,9 +605,10 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // block.
 //
 // A block takes the first wave 1.9 us: 82 matrix products (1300 cycles), 300 vector
-// operations between them (1200) and 52 loads, which it has to issue itself, all in one
+// operations between them (1200) and 45 loads, which it has to issue itself, all in one
 // chain from state to state.  16384 rows of 32 value heads of 128 x 128, one sequence:
-// 500 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 97 us.  One wave for
+// 500 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 91 us (two parts of
+// a head in one workgroup: 96).  One wave for
 // all of it takes 777 and 112 us.  Eight waves that each hold 16 rows of S of 16 columns
 // and add their products through LDS: 450 and 103; blocks of 16 rows 77 us where the last
 // ones go through one wave in 35.
