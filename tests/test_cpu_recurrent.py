@@ -223,6 +223,12 @@ CALLS = {
              " PTR + 64, 256)", 1),
     "prompt": ("lib.aexq_delta_prompt(ctx, slots(), PTR, PTR, 900, PTR, 256, PTR, 256, PTR, 512, PTR,"
                " 4, PTR, 4, PTR, PTR, 2, 4, 128, 128, 0.1, 1e-6, PTR + 64, 512)", 2),
+    "prompt, mostly short": (
+        "lib.aexq_delta_prompt(ctx, slots(sequences=100, count=100), PTR, PTR, 900, PTR, 256, PTR, 256,"
+        " PTR, 512, PTR, 4, PTR, 4, PTR, PTR, 2, 4, 128, 128, 0.1, 1e-6, PTR + 64, 512)", 3),
+    "prompt, all short": (  # 16 rows: no sequence can have more
+        "lib.aexq_delta_prompt(ctx, slots(sequences=100, count=100), PTR, PTR, 16, PTR, 256, PTR, 256,"
+        " PTR, 512, PTR, 4, PTR, 4, PTR, PTR, 2, 4, 128, 128, 0.1, 1e-6, PTR + 64, 512)", 2),
     "decode": ("lib.aexq_delta_decode(ctx, slots(), PTR, PTR, 256, PTR, 256, PTR, 512, PTR, 4, PTR,"
                " 4, PTR, PTR, 2, 4, 128, 128, 0.1, 1e-6, PTR + 64, 512)", 1),
     "norm": ("lib.aexq_gated_rmsnorm(ctx, PTR, 512, PTR, 512, PTR, 1e-6, 9, 4, 128, PTR, 512)", 1),
