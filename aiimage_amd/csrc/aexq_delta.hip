@@ -198,6 +198,26 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     lds.rq[own] = rq;
   }
   __syncthreads();
+  // Sums of the decays and the rows' factors of heads h .., a wave each, a row a lane: sums
+  // in 64 bits, as differences of large ones are taken
+  auto pass_gates = [&](int h) {
+    if (h + wave >= p.group) return;
+    Gate gate = gates.gate();
+    const bool in = lane < live;
+    if (!in) gate = Gate{0.0f, 0.0f};
+    const double G = wave_scan((double)gate.g * 1.4426950408889634);
+    lds.sums[wave][lane] = G;
+    lds.beta[wave][lane] = gate.beta;
+    const long long head = (long long)id * p.hv + hk * p.group + h + wave;
+    float* f = (float*)(p.heads + head * kDeltaHead + kDeltaFactors) + lane;
+    const float rk = lds.rk[lane], e = exp2_of(G), last = exp2_of(last_lane(G) - G);
+    f[kBeta * kDeltaRows] = gate.beta;
+    f[kSeen * kDeltaRows] = in ? gate.beta * e * rk : 0.0f;
+    f[kAsk * kDeltaRows] = in ? p.scale * e * lds.rq[lane] : 0.0f;
+    f[kLeft * kDeltaRows] = in ? last * (rk / near_one(rk)) : 0.0f;
+    if (lane == 63) f[kDecay * kDeltaRows - 63] = e;
+  };
+  pass_gates(0);  // (the first waves, which have the fewest tiles below)
   f32x4 ak[4], aq[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -234,24 +254,11 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     char* to = p.heads + ((long long)id * p.hv + head) * kDeltaHead;
     if (slot == 0) {
       __syncthreads();
-      if (h + wave < p.group) {
-        // a row a lane: sums in 64 bits, as differences of large ones are taken
-        if (h) gates = gates_from(h);
-        Gate gate = gates.gate();
-        if (lane >= live) gate = Gate{0.0f, 0.0f};
-        const double G = wave_scan((double)gate.g * 1.4426950408889634);
-        lds.sums[wave][lane] = G;
-        lds.beta[wave][lane] = gate.beta;
-        float* f = (float*)(to + wave * (long long)kDeltaHead + kDeltaFactors) + lane;
-        const bool in = lane < live;
-        const float rk = lds.rk[lane], e = exp2_of(G), last = exp2_of(last_lane(G) - G);
-        f[kBeta * kDeltaRows] = gate.beta;
-        f[kSeen * kDeltaRows] = in ? gate.beta * e * rk : 0.0f;
-        f[kAsk * kDeltaRows] = in ? p.scale * e * lds.rq[lane] : 0.0f;
-        f[kLeft * kDeltaRows] = in ? last * (rk / near_one(rk)) : 0.0f;
-        if (lane == 63) f[kDecay * kDeltaRows - 63] = e;
+      if (h) {
+        gates = gates_from(h);
+        pass_gates(h);
+        __syncthreads();
       }
-      __syncthreads();
     }
     if (small && wave) continue;
     // (so that comparisons with the lane's row are made here, not kept over the loop)
