@@ -615,10 +615,9 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // operations between them (1200) and 45 loads, which it has to issue itself, all in one
 // chain from state to state.  16384 rows of 32 value heads of 128 x 128, one sequence:
 // 500 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 91 us (two parts of
-// a head in one workgroup: 96).  One wave for
-// all of it takes 777 and 112 us.  Eight waves that each hold 16 rows of S of 16 columns
-// and add their products through LDS: 450 and 103; blocks of 16 rows 77 us where the last
-// ones go through one wave in 35.
+// a head in one workgroup: 96).  One wave for all of it takes 777 and 112 us.  Eight waves
+// that each hold 16 rows of S of 16 columns and add their products through LDS: 450 and
+// 103; blocks of 16 rows 77 us where the last ones go through one wave in 35.
 // ---------------------------------------------------------------------------
 template <int DK>
 struct DeltaLds {
@@ -1003,11 +1002,12 @@ __global__ __launch_bounds__(128, 2) void delta_prompt_kernel(const DeltaParams 
 }
 
 // Calls of many short sequences: those of up to 16 rows, a wave a part and no LDS, which
-// keeps twice as many on a CU (48 sequences of 2 to 8 rows, 16 heads of 128 x 128: 26 us,
-// where the kernel above takes 35).  One workgroup more lists the longer ones for that
+// keeps three times as many on a CU (48 sequences of 2 to 8 rows, 16 heads of 128 x 128:
+// 23.6 us, where the kernel above takes 35; 26.6 with two waves a SIMD, 41 with four and
+// spilled registers).  One workgroup more lists the longer ones for that
 // kernel, their number first.
 template <int DK>
-__global__ __launch_bounds__(64) void delta_short_kernel(const DeltaParams p) {
+__global__ __launch_bounds__(64, 3) void delta_short_kernel(const DeltaParams p) {
   if (blockIdx.x == 0) {
     const int lane = threadIdx.x;
     auto rows_of = [&](int s) {
