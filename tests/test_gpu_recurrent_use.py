@@ -552,6 +552,31 @@ def test_thousands_of_sequences(aexq, ctx, n):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("layout", ["LAYOUT_PACK4_LINEAR", "LAYOUT_PACK4_TILED"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_logits_as_the_head_leaves_them(aexq, ctx, layout, dtype):
+    """Rows padded to whole packs, rows of an odd width: what lies between them is no
+    token's."""
+    print(f"[gpu-case] verify {layout} {dtype}", flush=True)
+    rows, vocab, lens = 7, 33001, [4, 3]
+    layout = getattr(aexq, layout)
+    buf = aexq.new_activation(rows, vocab, dtype=dtype, layout=layout)
+    wide = buf.view(rows, -1)
+    wide.fill_(50.0)        # above every logit
+    wide[:, :vocab] = 2 * _randn(rows, vocab, seed=1)
+    x = wide[:, :vocab]
+    probs = torch.softmax(x.float() + _randn(rows, vocab, seed=2), -1)
+    drafts = probs.argmax(-1).int()
+    for heat in (None, torch.zeros(2, device="cuda")):
+        au, su = _rand(rows, seed=3), _rand(2, seed=4)
+        counts = torch.zeros(2, dtype=torch.int32, device="cuda")
+        tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        ctx.verify_drafts(aexq.describe(buf, rows, vocab, layout), ref.offsets(lens), drafts, au, su,
+                          counts, tokens, temperature=heat, draft_probs=probs)
+        torch.cuda.synchronize()
+        assert (counts.tolist(), tokens.tolist()) == ref.verify(x, lens, drafts, probs, heat, au, su)
+
+
 def test_rows_before_the_first_sequence(aexq, ctx):
     """Offsets that begin far behind the first row: rows of no sequence are not touched,
     the others have the bits of a call of their own."""
