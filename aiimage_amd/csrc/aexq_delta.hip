@@ -820,40 +820,6 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
           w[i][j][part] = x.piece(head, 12 + piece_of(i, j) * 2 + part);
     }
   };
-  // What a block takes comes from memory, later than a block takes to pass: a byte of each
-  // of its 128-byte lines is read some blocks ahead, two lines a lane over the head's
-  // workgroups, so that the loads find them in the L2 that these share.
-  constexpr int kAhead = 2, key_lines = delta_key_bytes(DK) / 128;
-  constexpr int head_lines = (kDeltaHead + 127) / 128;
-  const int row_lines = p.dv / 64;  // of v
-  const char* warm[2];
-  long long warm_step[2];
-  uint32_t warmed[2] = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int line = (x.col / 16 * 2 + i) * 64 + lane, v_line = line - key_lines - head_lines;
-    warm[i] = p.heads + ((long long)x.id0 * p.hv + x.head) * kDeltaHead;
-    warm_step[i] = (long long)p.hv * kDeltaHead;
-    if (line < key_lines) {
-      warm[i] = p.keys + ((long long)x.id0 * p.hk + x.hk) * delta_key_bytes(DK) + line * 128;
-      warm_step[i] = (long long)p.hk * delta_key_bytes(DK);
-    } else if (v_line < 0) {
-      warm[i] += (line - key_lines) * 128;
-    } else if (v_line < min(kDeltaRows, x.span.kept) * row_lines) {
-      warm[i] = (const char*)(p.v + (x.span.first + v_line / row_lines) * p.v_stride +
-                              x.head * p.dv) + v_line % row_lines * 128;
-      warm_step[i] = kDeltaRows * p.v_stride * 2;
-    }
-  }
-  auto warm_up = [&](int b) {  // (but the last block, which may have fewer rows)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      asm volatile("" ::"v"(warmed[i]));
-      warmed[i] = *(const __attribute__((address_space(1))) uint8_t*)(
-          warm[i] + max(min(b, blocks - 2), 0) * warm_step[i]);
-    }
-  };
-  warm_up(1);
   load_v(0);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -870,7 +836,6 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
     const int next = min(b + 1, blocks - 1), at = b & 1;
     if (b + 1 < blocks) put_v(b + 1);
     __builtin_amdgcn_sched_barrier(0);
-    warm_up(b + kAhead);
     load_v(min(b + 2, blocks - 1));
     __builtin_amdgcn_sched_barrier(0);
     __syncthreads();  // S and U of this block, v of the next
