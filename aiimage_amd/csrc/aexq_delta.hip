@@ -501,14 +501,14 @@ struct DeltaWave {
         kBufferRsrcWord3);
   }
   // Rows of v and out are addressed by resources that end with the block's last row: rows
-  // behind it read as zeros and are not stored, and a lane's offsets are the same in every
-  // block.
+  // behind it read as zeros and are not stored, nor is any where there is no out, and a
+  // lane's offsets are the same in every block.
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const f16* x, long long stride,
                                                             int b) const {
     const int live = min(kDeltaRows, span.kept - b * kDeltaRows);
     return __builtin_amdgcn_make_buffer_rsrc(
         (void*)(x + (span.first + (long long)b * kDeltaRows) * stride + head * p.dv + col), 0,
-        2 * ((uint32_t)(live - 1) * (uint32_t)stride + 16), kBufferRsrcWord3);
+        x ? 2 * ((uint32_t)(live - 1) * (uint32_t)stride + 16) : 0, kBufferRsrcWord3);
   }
   __device__ __forceinline__ f16x8 piece(__amdgpu_buffer_rsrc_t at, int number) const {
     return __builtin_bit_cast(
@@ -639,11 +639,15 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
   constexpr int KB = DK / 32;
   const int lane = x.lane;
   // Each operand is on its way as soon as the one before it in its registers is used, and
-  // not earlier; the keys and the transposed keys take turns in `a`.
-  f16x8 a[4 * KB], t[4][2][2];
+  // not earlier; the keys and the transposed keys take turns in `a`, but for the first
+  // kEarly keys, which a block begins with and which would come too late so.
+  constexpr int kEarly = 8;
+  f16x8 a[4 * KB], begin[kEarly], t[4][2][2];
   f32x4 seen_by[4], left[4];
   float decay;
-  auto load_k = [&](__amdgpu_buffer_rsrc_t at, int n) { a[n] = x.piece(at, n % 4 * KB + n / 4); };
+  auto load_k = [&](__amdgpu_buffer_rsrc_t at, int n) {
+    (n < kEarly ? begin[n] : a[n]) = x.piece(at, n % 4 * KB + n / 4);
+  };
   auto load_kt = [&](__amdgpu_buffer_rsrc_t at, int n) {
     a[n] = x.piece(at, 8 * KB + 2 * (n % (2 * KB)) + n / (2 * KB));
   };
@@ -657,18 +661,21 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
   };
   {
     const auto keys = x.keys_of(0), head = x.head_of(0);
+#pragma unroll
+    for (int n = 0; n < kEarly; ++n) load_k(keys, n);
+    __builtin_amdgcn_sched_barrier(0);  // (in the loop's order)
     load_t(head);
-    __builtin_amdgcn_sched_barrier(0);  // (in the order in which they are waited for)
+    __builtin_amdgcn_sched_barrier(0);
     decay = x.decay_of(head);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int n = 0; n < 4 * KB; ++n) load_k(keys, n);
+    for (int n = kEarly; n < 4 * KB; ++n) load_k(keys, n);
     __builtin_amdgcn_sched_barrier(0);
   }
   __syncthreads();  // the first block's v and factors
   for (int b = 0; b < blocks; ++b) {
     const int next = min(b + 1, blocks - 1), at = b & 1;
-    const auto keys = x.keys_of(b);
+    const auto keys = x.keys_of(b), after = x.keys_of(next);
     f32x4 seen[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -682,12 +689,15 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
       lds.s[at][i][0][lane] = s.x0;
       lds.s[at][i][1][lane] = s.x1;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) seen[w] = mfma(a[4 * i + w], s.x0, seen[w]);
+      for (int w = 0; w < 4; ++w) seen[w] = mfma(4 * i < kEarly ? begin[4 * i + w] : a[4 * i + w], s.x0, seen[w]);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) seen[w] = mfma(a[4 * i + w], s.x1, seen[w]);
+      for (int w = 0; w < 4; ++w) seen[w] = mfma(4 * i < kEarly ? begin[4 * i + w] : a[4 * i + w], s.x1, seen[w]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) load_kt(keys, 4 * i + w);
+      for (int w = 0; w < 4; ++w) {
+        load_kt(keys, 4 * i + w);
+        if (4 * i < kEarly) load_k(after, 4 * i + w);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     // R, times what takes its largest value to fp16's range
@@ -748,7 +758,6 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
     __builtin_amdgcn_sched_barrier(0);
     decay = x.decay_of(head);
     __builtin_amdgcn_sched_barrier(0);
-    const auto after = x.keys_of(next);
 #pragma unroll
     for (int n = 0; n < 4 * KB; n += 4) {
       const int j = n / (2 * KB);
@@ -758,7 +767,8 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
       for (int i = n; i < n + 4; ++i) x.S[i % (2 * KB)] = mfma(a[i], ys[j].x1, x.S[i % (2 * KB)]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = n; i < n + 4; ++i) load_k(after, i);
+      for (int i = n; i < n + 4; ++i)
+        if (n >= kEarly) load_k(after, i);
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
@@ -774,27 +784,29 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
   // v and the outputs move 16 bytes a lane, eight columns of row lane / 2 (and 32 more),
   // and change places in LDS: 16 loads or stores of two bytes a lane take a CU's address
   // unit as long as the operands' 16 of 16
-  f16x8 v[2];
-  f32x4 factors;
+  struct Rows {
+    f16x8 v[2];
+    f32x4 factors;
+  } first, rows;
   const int row = lane / 2, part = lane % 2 * 8;
   const uint32_t step_v = 2 * (uint32_t)p.v_stride, step_out = 2 * (uint32_t)p.out_stride;
-  auto load_v = [&](int b) {
+  auto load_v = [&](Rows& to, int b) {
     const auto from = x.rows_of(p.v, p.v_stride, b), head = x.head_of(b);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      v[i] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(
-                                           from, row * step_v + 2 * part, 32 * i * step_v, 0));
-    factors = __builtin_bit_cast(
+      to.v[i] = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(
+                                              from, row * step_v + 2 * part, 32 * i * step_v, 0));
+    to.factors = __builtin_bit_cast(
         f32x4, __builtin_amdgcn_raw_buffer_load_b128(head, 16 * lane, kDeltaFactors, 0));
   };
   auto meet = [] {  // LDS written by one lane and read by another
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  auto put_v = [&](int b) {
-    lds.factors[b & 1][lane] = factors;
+  auto put_v = [&](const Rows& from, int b) {
+    lds.factors[b & 1][lane] = from.factors;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *(f16x8*)&lds.rows[32 * i + row][part] = v[i];
+    for (int i = 0; i < 2; ++i) *(f16x8*)&lds.rows[32 * i + row][part] = from.v[i];
     meet();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -820,23 +832,25 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
           w[i][j][part] = x.piece(head, 12 + piece_of(i, j) * 2 + part);
     }
   };
-  load_v(0);
+  // (in the loop's order: a wait for the rows at its top leaves what was asked for after
+  // them on its way, which it does only if that holds on both ways there)
+  load_v(first, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  load_v(rows, min(1, blocks - 1));
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < KB; ++i) load_q(x.keys_of(0), i);
   __builtin_amdgcn_sched_barrier(0);
   load_w(x.head_of(0));
   __builtin_amdgcn_sched_barrier(0);
-  put_v(0);
-  __builtin_amdgcn_sched_barrier(0);
-  load_v(min(1, blocks - 1));
+  put_v(first, 0);
   __builtin_amdgcn_sched_barrier(0);
   __syncthreads();
   for (int b = 0; b < blocks; ++b) {
     const int next = min(b + 1, blocks - 1), at = b & 1;
-    if (b + 1 < blocks) put_v(b + 1);
+    put_v(rows, b + 1);  // (behind the last block: of that one again, where nothing reads it)
     __builtin_amdgcn_sched_barrier(0);
-    load_v(min(b + 2, blocks - 1));
+    load_v(rows, min(b + 2, blocks - 1));
     __builtin_amdgcn_sched_barrier(0);
     __syncthreads();  // S and U of this block, v of the next
     const auto keys = x.keys_of(next);
@@ -886,20 +900,18 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
     __builtin_amdgcn_sched_barrier(0);
     load_w(x.head_of(next));
     __builtin_amdgcn_sched_barrier(0);
-    if (p.out) {
-      const auto to = x.rows_of(p.out, p.out_stride, b);
+    const auto to = x.rows_of(p.out, p.out_stride, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) lds.rows[16 * i + 4 * x.g + e][x.c] = (f16)o[i][e];
-      meet();
+      for (int e = 0; e < 4; ++e) lds.rows[16 * i + 4 * x.g + e][x.c] = (f16)o[i][e];
+    meet();
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, *(const f16x8*)&lds.rows[32 * i + row][part]), to,
-            row * step_out + 2 * part, 32 * i * step_out, 0);
-      meet();
-    }
+    for (int i = 0; i < 2; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(
+          __builtin_bit_cast(u32x4, *(const f16x8*)&lds.rows[32 * i + row][part]), to,
+          row * step_out + 2 * part, 32 * i * step_out, 0);
+    meet();
   }
 }
 
