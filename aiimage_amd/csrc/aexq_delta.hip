@@ -681,11 +681,14 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
     for (int w = 0; w < 4; ++w) {
       seen[w] = f32x4{};
       seen_by[w] = lds.factor(at, kSeen, w, x.g);
-      left[w] = lds.factor(at, kLeft, w, x.g);
     }
+    f32x4 v[4];
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
       const Split s = split8(x.S[2 * i], x.S[2 * i + 1]);
+      if (i == KB - 1)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = lds.v[at][w][lane];
       lds.s[at][i][0][lane] = s.x0;
       lds.s[at][i][1][lane] = s.x1;
 #pragma unroll
@@ -705,10 +708,9 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
     float m = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const f32x4 v = lds.v[at][w][lane];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        r[w][e] = fmaf(-seen_by[w][e], seen[w][e] * x.scale.back, v[e]);
+        r[w][e] = fmaf(-seen_by[w][e], seen[w][e] * x.scale.back, v[w][e]);
       m = top4(m, r[w]);
     }
     m = rows_max(m);
@@ -720,6 +722,8 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
 #pragma unroll
     for (int j = 0; j < 2; ++j) rs[j] = split8(r[2 * j] * lr.by, r[2 * j + 1] * lr.by);
     const auto head = x.head_of(next);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) left[w] = lds.factor(at, kLeft, w, x.g);
     __builtin_amdgcn_sched_barrier(0);
     // U = T R
     f32x4 u[4], y[4];
@@ -808,14 +812,18 @@ __device__ __forceinline__ void delta_outputs(DeltaWave<DK>& x, DeltaLds<DK>& ld
 #pragma unroll
     for (int i = 0; i < 2; ++i) *(f16x8*)&lds.rows[32 * i + row][part] = from.v[i];
     meet();
+    f16x4 y[4];
+    f32x4 beta[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x4 beta = lds.factor(b & 1, kBeta, i, x.g);
-      f32x4 y;
+      beta[i] = lds.factor(b & 1, kBeta, i, x.g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = beta[e] * (float)lds.rows[16 * i + 4 * x.g + e][x.c];
-      lds.v[b & 1][i][lane] = y;
+      for (int e = 0; e < 4; ++e) y[i][e] = lds.rows[16 * i + 4 * x.g + e][x.c];
     }
+    __builtin_amdgcn_sched_barrier(0);  // (all of it read before any of it is used)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      lds.v[b & 1][i][lane] = beta[i] * __builtin_convertvector(y[i], f32x4);
     meet();
   };
   auto load_q = [&](__amdgpu_buffer_rsrc_t keys, int i) {
