@@ -633,6 +633,9 @@ struct DeltaLds {
   }
 };
 
+// Kinds of instructions that places in a schedule are kept for.
+enum : int { kSchedValu = 0x2, kSchedMfma = 0x8, kSchedLoad = 0x20, kSchedLds = 0x300 };
+
 template <int DK>
 __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds, int blocks,
                                             bool& odd) {
@@ -683,23 +686,40 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
       seen_by[w] = lds.factor(at, kSeen, w, x.g);
     }
     f32x4 v[4];
+    // (between a step's products: the parts of S for the next one, and loads into the
+    // registers that it is done with)
+    Split s = split8(x.S[0], x.S[1]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < KB; ++i) {
-      const Split s = split8(x.S[2 * i], x.S[2 * i + 1]);
+      Split then = s;
+      if (i + 1 < KB) then = split8(x.S[2 * i + 2], x.S[2 * i + 3]);
       if (i == KB - 1)
 #pragma unroll
         for (int w = 0; w < 4; ++w) v[w] = lds.v[at][w][lane];
       lds.s[at][i][0][lane] = s.x0;
       lds.s[at][i][1][lane] = s.x1;
+      const f16x8* const k = 4 * i < kEarly ? begin : a;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) seen[w] = mfma(4 * i < kEarly ? begin[4 * i + w] : a[4 * i + w], s.x0, seen[w]);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) seen[w] = mfma(4 * i < kEarly ? begin[4 * i + w] : a[4 * i + w], s.x1, seen[w]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int w = 0; w < 4; ++w) seen[w] = mfma(k[4 * i + w], s.x0, seen[w]);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
+        seen[w] = mfma(k[4 * i + w], s.x1, seen[w]);
         load_kt(keys, 4 * i + w);
         if (4 * i < kEarly) load_k(after, 4 * i + w);
+      }
+      s = then;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu | kSchedLds, 3, 0);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedLoad, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu | kSchedLds, 1, 0);
+        if (4 * i < kEarly) __builtin_amdgcn_sched_group_barrier(kSchedLoad, 1, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -757,22 +777,36 @@ __device__ __forceinline__ void delta_solve(DeltaWave<DK>& x, DeltaLds<DK>& lds,
     Split ys[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) ys[j] = split8(y[2 * j] * to_y, y[2 * j + 1] * to_y);
-    x.rescale(keep);
     x.scale = ls;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.S[i] *= keep;
     __builtin_amdgcn_sched_barrier(0);
     decay = x.decay_of(head);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < 4 * KB; n += 4) {
       const int j = n / (2 * KB);
+      if (n + 4 < 2 * KB)
+#pragma unroll
+        for (int i = n + 4; i < n + 8; ++i) x.S[i] *= keep;
 #pragma unroll
       for (int i = n; i < n + 4; ++i) x.S[i % (2 * KB)] = mfma(a[i], ys[j].x0, x.S[i % (2 * KB)]);
 #pragma unroll
-      for (int i = n; i < n + 4; ++i) x.S[i % (2 * KB)] = mfma(a[i], ys[j].x1, x.S[i % (2 * KB)]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = n; i < n + 4; ++i)
+      for (int i = n; i < n + 4; ++i) {
+        x.S[i % (2 * KB)] = mfma(a[i], ys[j].x1, x.S[i % (2 * KB)]);
         if (n >= kEarly) load_k(after, i);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu, 3, 0);
+      }
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        if (n >= kEarly) __builtin_amdgcn_sched_group_barrier(kSchedLoad, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedValu, 1, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
