@@ -611,13 +611,16 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // the first one leaves in LDS, and the first one's beta v a block ahead.  One barrier a
 // block.
 //
-// A block takes the first wave 1.9 us: 82 matrix products (1300 cycles), 300 vector
-// operations between them (1200) and 45 loads, which it has to issue itself, all in one
-// chain from state to state.  16384 rows of 32 value heads of 128 x 128, one sequence:
-// 500 us, 256 blocks in turn; 9600 rows of 12 sequences and 16 heads: 91 us (two parts of
-// a head in one workgroup: 96).  One wave for all of it takes 777 and 112 us.  Eight waves
-// that each hold 16 rows of S of 16 columns and add their products through LDS: 450 and
-// 103; blocks of 16 rows 77 us where the last ones go through one wave in 35.
+// A block takes the first wave 1.8 us: 82 matrix products (1300 cycles), 300 vector
+// operations, which hide behind them in part, and 45 loads, each of which holds it up for
+// 20 to 30 cycles, all in one chain from state to state.  16384 rows of 32 value heads of
+// 128 x 128, one sequence: 462 us, 256 blocks in turn; 9600 rows of 12 sequences and 16
+// heads: 83 us.  Steps on the way, in that order: one wave for all of it 777 and 112 us;
+// eight waves that each hold 16 rows of S of 16 columns and add their products through
+// LDS: 450 and 103 (but 77 for blocks of 16 rows, where the last ones now go through one
+// wave in 35); two waves, each waiting for its own loads: 510 and 97; waits of the second
+// one that leave later loads on their way, keys a block ahead, LDS reads ahead of their
+// use: 478 and 85; parts of S and loads between the products of a step: 462 and 83.
 // ---------------------------------------------------------------------------
 template <int DK>
 struct DeltaLds {
