@@ -163,7 +163,8 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(const GatedNormPar
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum = fmaf((float)x[r][e], (float)x[r][e], sum);
     sum = lanes_sum<LPR>(i < p.dim ? sum : 0.0f);
-    const float k = 1.0f / sqrtf(fmaxf(sum / p.dim + p.eps, 1e-20f));
+    // (a maximum that keeps a NaN: the row's mean is one then, and so are its values)
+    const float k = 1.0f / sqrtf(__builtin_elementwise_maximum(sum / p.dim + p.eps, 1e-20f));
     f16x8 y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = (f16)((float)x[r][e] * k * gamma[e] * silu_of((float)z[r][e]));

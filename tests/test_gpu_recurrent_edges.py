@@ -1,0 +1,85 @@
+"""Edges of the recurrent layers' operators and of the verification of drafted tokens:
+values that are not finite, gates and keys at the ends of their types, rows behind a
+sequence's last, sequences of thousands of rows, numbers beside a border."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import recurrent_ref as ref  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = math.inf, math.nan
+
+
+@pytest.fixture(scope="module")
+def aexq():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from aiimage_amd import aexq as mod
+    return mod
+
+
+@pytest.fixture(scope="module")
+def ctx(aexq):
+    c = aexq.Context(0)
+    yield c
+    torch.cuda.synchronize()
+    c.close()
+
+
+def _randn(*shape, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def _rand(*shape, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.rand(shape, generator=g, device="cuda")
+
+
+def _inputs(n, hk, hv, dk, dv, seed=0):
+    s = 100 * seed
+    return dict(q=_randn(n, hk, dk, seed=s + 1).half(), k=_randn(n, hk, dk, seed=s + 2).half(),
+                v=_randn(n, hv, dv, seed=s + 3).half(), a=_randn(n, hv, seed=s + 4).half(),
+                b=_randn(n, hv, seed=s + 5).half(), a_log=_randn(hv, seed=s + 6),
+                dt_bias=_randn(hv, seed=s + 7) - 1.5)
+
+
+def _rows(d, at):
+    return {x: y if x in ("a_log", "dt_bias") else y[at] for x, y in d.items()}
+
+
+# ---------------------------------------------------------------- gated norm
+
+@pytest.mark.parametrize("tokens,heads,dim", [(3, 2, 8), (5, 3, 64), (4, 2, 128), (6, 1, 200),
+                                              (3, 2, 512), (9000, 4, 128)])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+def test_gated_norm_of_rows_that_are_not_finite(ctx, tokens, heads, dim, bad):
+    """The mean of a row with a NaN is NaN and so is all of it, its zeros and its small
+    values as well; an infinity leaves zeros and a NaN in its own place.  No other row meets
+    either."""
+    print(f"[gpu-case] gated norm with {bad}: {tokens} x {heads} x {dim}", flush=True)
+    x, z = _randn(tokens, heads, dim, seed=1).half(), 2 * _randn(tokens, heads, dim, seed=2).half()
+    x[1, 0] *= 1e-6
+    x[1, 0, ::2] = 0
+    z[1, 0, 1::3] = 0
+    clean, at = x.clone(), dim // 2 + 1
+    x[1, 0, at] = bad
+    gamma = 1 + 0.1 * _randn(dim, seed=3)
+    outs = []
+    for t in (clean, x):
+        outs.append(torch.zeros_like(t))
+        ctx.gated_rmsnorm(t, z, gamma, outs[-1])
+    torch.cuda.synchronize()
+    row = outs[1][1, 0].clone()
+    if math.isnan(bad):
+        assert torch.isnan(row).all()
+    else:
+        assert torch.isnan(row[at])
+        row[at] = 0
+        assert (row == 0).all()
+    outs[1][1, 0] = outs[0][1, 0]
+    assert torch.equal(*outs)
