@@ -21,8 +21,11 @@ struct GateInputs {
   float dt_bias, a_log;
   __device__ __forceinline__ Gate gate() const {
     const float t = (float)a + dt_bias;
-    const float soft = fmaxf(t, 0.0f) + log1pf(expf(-fabsf(t)));
-    const float g = -expf(a_log) * soft;
+    // below -30 the softplus is e^t up to 2^-44 of it and goes into the rate's exponent:
+    // e^a_log may be past fp32 where their product is not (above, both are past 1e5)
+    const bool far = t < -30.0f;
+    const float soft = far ? 1.0f : fmaxf(t, 0.0f) + log1pf(expf(-fabsf(t)));
+    const float g = -expf(far ? a_log + t : a_log) * soft;
     return Gate{g < -1e5f ? -1e5f : g, 1.0f / (1.0f + expf(-(float)b))};
   }
 };

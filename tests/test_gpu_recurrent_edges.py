@@ -83,3 +83,34 @@ def test_gated_norm_of_rows_that_are_not_finite(ctx, tokens, heads, dim, bad):
         assert (row == 0).all()
     outs[1][1, 0] = outs[0][1, 0]
     assert torch.equal(*outs)
+
+
+# ---------------------------------------------------------------- gated delta rule
+
+@pytest.mark.parametrize("decode", [False, True])
+def test_delta_decays_of_large_rates(aexq, ctx, decode):
+    """a_log past the largest logarithm of fp32 with gates that undo it: e^a_log is an
+    infinity and the softplus 0 in fp32, their product is neither.  (a, a_log and their
+    sums are whole quarters: nothing is rounded before the exponential.)"""
+    print(f"[gpu-case] delta rates past fp32 decode={decode}", flush=True)
+    rates = [89.0, 100.0, 128.0, 95.5]
+    n, hv, dk, dv = (40, 4, 64, 64) if decode else (90, 4, 64, 64)
+    d = _inputs(n, 2, hv, dk, dv, seed=1)
+    d["a_log"], d["dt_bias"] = torch.tensor(rates, device="cuda"), torch.zeros(hv, device="cuda")
+    past = torch.tensor([2.0, 1.0, 0.5, -1.5, 8.0, 30.0, -4.0, 0.0], device="cuda").repeat(n // 8 + 1)
+    d["a"] = (-d["a_log"][None] - past[:n, None]).half()
+    if decode:
+        state = _randn(n, hv, dk, dv, seed=2)
+        before, out = state.clone(), torch.zeros((n, hv, dv), device="cuda").half()
+        ctx.delta_decode(aexq.slots(n, n), state, **d, out=out, scale=0.2)
+        spans = [slice(i, i + 1) for i in range(n)]
+    else:
+        state = _randn(2, hv, dk, dv, seed=2)
+        before, out = state.clone(), torch.zeros((n, hv, dv), device="cuda").half()
+        ctx.delta_prompt(aexq.slots(2, 2), state, ref.offsets([n - 9, 9]), **d, out=out, scale=0.2)
+        spans = [slice(0, n - 9), slice(n - 9, n)]
+    torch.cuda.synchronize()
+    for i, r in enumerate(spans):
+        y, near, S, err = ref.delta(**_rows(d, r), state=before[i], scale=0.2, eps=1e-6)
+        ref.check(out[r], y, near, f"sequence {i}")
+        ref.check(state[i], S, err, f"state {i}")
