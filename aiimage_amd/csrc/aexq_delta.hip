@@ -235,8 +235,9 @@ __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaPar
     const f32x4 rj = *(const f32x4*)&lds.rk[16 * j + 4 * g];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      ak[j][r] = own < live ? ak[j][r] * (rk * rj[r]) : 0.0f;
-      aq[j][r] = own < live ? aq[j][r] * (rq * rj[r]) : 0.0f;
+      // (one length at a time: of two rows of zeros their product, 1 / eps, may be past fp32)
+      ak[j][r] = own < live ? ak[j][r] * rk * rj[r] : 0.0f;
+      aq[j][r] = own < live ? aq[j][r] * rq * rj[r] : 0.0f;
     }
   }
   // the keys transposed, times a power of two (exact but for values below 2^-14, by 2^-25)

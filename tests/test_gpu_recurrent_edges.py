@@ -114,3 +114,21 @@ def test_delta_decays_of_large_rates(aexq, ctx, decode):
         y, near, S, err = ref.delta(**_rows(d, r), state=before[i], scale=0.2, eps=1e-6)
         ref.check(out[r], y, near, f"sequence {i}")
         ref.check(state[i], S, err, f"state {i}")
+
+
+@pytest.mark.parametrize("eps", [1e-40, 1e-38, 1e-6])
+@pytest.mark.parametrize("n", [9, 100])
+def test_delta_keys_of_zero_beside_the_smallest_eps(aexq, ctx, n, eps):
+    """Keys and queries of nothing but zeros have length 0 whatever eps is above 0, also
+    where 1 / eps is past fp32."""
+    print(f"[gpu-case] delta zero keys eps={eps}", flush=True)
+    d = _inputs(n, 1, 2, 128, 64, seed=3)
+    d["k"][::3], d["q"][::2] = 0, 0
+    d["k"][4:7] = 0
+    state = _randn(1, 2, 128, 64, seed=4)
+    before, out = state.clone(), torch.zeros((n, 2, 64), device="cuda").half()
+    ctx.delta_prompt(aexq.slots(1, 1), state, ref.offsets([n]), **d, out=out, scale=0.1, eps=eps)
+    torch.cuda.synchronize()
+    y, near, S, err = ref.delta(**d, state=before[0], scale=0.1, eps=eps)
+    ref.check(out, y, near)
+    ref.check(state[0], S, err)
