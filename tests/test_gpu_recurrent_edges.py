@@ -132,3 +132,69 @@ def test_delta_keys_of_zero_beside_the_smallest_eps(aexq, ctx, n, eps):
     y, near, S, err = ref.delta(**d, state=before[0], scale=0.1, eps=eps)
     ref.check(out, y, near)
     ref.check(state[0], S, err)
+
+
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+@pytest.mark.parametrize("n", [1000, 970])
+def test_delta_odd_values_leave_other_columns_alone(aexq, ctx, n, dk, dv):
+    """Values that are not finite in some rows of a long sequence, several in one block
+    among them, and in its last: the outputs before them and every other column's, all of
+    them, and the other columns' states have the bits that they have without."""
+    print(f"[gpu-case] delta odd values in {n} rows {dk}x{dv}", flush=True)
+    hv = 2
+    d = _inputs(n, 1, hv, dk, dv, seed=5)
+    d["a"] -= 2.0
+    state = _randn(1, hv, dk, dv, seed=6)
+    begin = state.clone()
+    odd = {(1, 5): 130, (1, 7): 131, (1, 40): 131, (1, 3): 500, (1, 10): 514, (1, 11): 577,
+           (1, 20): n - 1, (0, 9): n - 3, (0, 33): 0}
+    runs = []
+    for bad in (False, True):
+        s, x = begin.clone(), dict(d, v=d["v"].clone())
+        if bad:
+            for i, ((h, c), t) in enumerate(odd.items()):
+                x["v"][t, h, c] = (NAN, INF, -INF)[i % 3]
+            s[0, 0, 3, 50] = NAN
+        out = torch.zeros((n, hv, dv), device="cuda").half()
+        ctx.delta_prompt(aexq.slots(1, 1), s, ref.offsets([n]), **x, out=out, scale=0.1)
+        torch.cuda.synchronize()
+        runs.append((out, s))
+    (clean, clean_state), (out, left) = runs
+    odd[0, 50] = 0
+    good = torch.ones((hv, dv), dtype=torch.bool, device="cuda")
+    y, near, _, _ = ref.delta(**d, state=begin[0], scale=0.1, eps=1e-6)
+    for (h, c), t in odd.items():
+        good[h, c] = False
+        assert not torch.isfinite(out[t:, h, c]).any() and not torch.isfinite(left[0, h, :, c]).any()
+        ref.check(out[:t, h, c], y[:t, h, c], near[:t, h, c], f"column {c} of head {h}")
+        assert torch.equal(out[:t // 64 * 64, h, c], clean[:t // 64 * 64, h, c])
+    assert torch.equal(out[:, good], clean[:, good])
+    assert torch.equal(left[0].transpose(1, 2)[good], clean_state[0].transpose(1, 2)[good])
+
+
+def test_delta_odd_values_of_short_sequences(aexq, ctx):
+    """The same where there are many sequences of a few rows each."""
+    print("[gpu-case] delta odd values, short sequences", flush=True)
+    n, m, hv, dk, dv = 60, 9, 4, 128, 128
+    d = _inputs(n * m, 2, hv, dk, dv, seed=5)
+    state = _randn(n, hv, dk, dv, seed=6)
+    runs = []
+    for bad in (False, True):
+        s, x = state.clone(), dict(d, v=d["v"].clone())
+        if bad:
+            x["v"][3 * m + 4, 1, 7], x["v"][3 * m + 8, 1, 9], x["v"][59 * m, 0, 127] = NAN, INF, -INF
+        out = torch.zeros((n * m, hv, dv), device="cuda").half()
+        ctx.delta_prompt(aexq.slots(n, n), s, ref.offsets([m] * n), **x, out=out, scale=0.1)
+        torch.cuda.synchronize()
+        runs.append((out.view(n, m, hv, dv), s))
+    (clean, clean_state), (out, left) = runs
+    y, near, _, _ = ref.delta(**_rows(d, slice(3 * m, 4 * m)), state=state[3], scale=0.1, eps=1e-6)
+    odd, odd_state = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(left, dtype=torch.bool)
+    for s, t, h, c in ((3, 4, 1, 7), (3, 8, 1, 9), (59, 0, 0, 127)):
+        odd[s, t:, h, c], odd_state[s, h, :, c] = True, True
+        if t:
+            ref.check(out[s, :t, h, c], y[:t, h, c], near[:t, h, c])
+            out[s, :t, h, c] = clean[s, :t, h, c]
+    assert torch.equal(~torch.isfinite(out), odd) and torch.equal(~torch.isfinite(left), odd_state)
+    assert torch.equal(out.masked_fill(odd, 0), clean.masked_fill(odd, 0))
+    assert torch.equal(left.masked_fill(odd_state, 0), clean_state.masked_fill(odd_state, 0))
