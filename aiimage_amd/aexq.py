@@ -247,6 +247,25 @@ def _gate_rows(t: torch.Tensor, name: str, rows: int, heads: int, device: int) -
     _refuse(f"{name} is {what}, not fp16 rows {(rows, heads)} on GPU {device}")
 
 
+def _rows_meet(a: int, a_stride: int, a_width: int, b: int, b_stride: int, b_width: int,
+               rows: int) -> bool:
+    """Whether some of `rows` fp16 rows from address a, a_width elements of each a_stride,
+    share memory with some of those from b."""
+    at = (b - a) // 2
+    if at >= (rows - 1) * a_stride + a_width or -at >= (rows - 1) * b_stride + b_width:
+        return False
+    if a_stride == b_stride:    # row i of b begins `place` into row i + by of a
+        by, place = divmod(at, a_stride)
+        return ((place < a_width and abs(by) < rows)
+                or (place + b_width > a_stride and abs(by + 1) < rows))
+    for i in range(rows):       # the last row of a that begins before the end of row i of b
+        begin = at + i * b_stride
+        row = min((begin + b_width - 1) // a_stride, rows - 1)
+        if row >= 0 and row * a_stride + a_width > begin:
+            return True
+    return False
+
+
 # ---------------------------------------------------------------- records
 
 @dataclass
@@ -619,9 +638,13 @@ class Context:
         if bias is not None:
             b = _device_array(bias, "bias", torch.float32, (channels,), device)
         xs, os_, o = _gate_rows(x, "x", tokens, channels, device), 0, None
+        xp = x.data_ptr()
         if out is not None:
             os_, o = _gate_rows(out, "out", tokens, channels, device), out.data_ptr()
-        check(self._lib.aexq_short_conv(self.handle, slots, st, off, tokens, x.data_ptr(), xs, w, b,
+            if (o < xp + 2 * tokens * xs and xp < o + 2 * tokens * os_
+                    and _rows_meet(xp, xs, channels, o, os_, channels, tokens)):
+                _refuse("out is or overlaps x, which is still read")
+        check(self._lib.aexq_short_conv(self.handle, slots, st, off, tokens, xp, xs, w, b,
                                         channels, width, silu, o, os_), "aexq_short_conv")
 
     def _delta_rows(self, slots, state, q, k, v, a, b, a_log, dt_bias, out, scale, eps):
@@ -639,11 +662,18 @@ class Context:
         al = _device_array(a_log, "a_log", torch.float32, (heads_v,), device)
         dt = _device_array(dt_bias, "dt_bias", torch.float32, (heads_v,), device)
         os_, o = 0, None
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
         if out is not None:
             os_, o = _head_rows(out, "out", (tokens, heads_v, dim_v), device), out.data_ptr()
-        return st, tokens, (q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, a.data_ptr(), as_,
-                            b.data_ptr(), bs, al, dt, heads_k, heads_v, dim_k, dim_v, scale, eps, o,
-                            os_)
+            end = o + 2 * tokens * os_
+            if ((qp < end and o < qp + 2 * tokens * qs) or (kp < end and o < kp + 2 * tokens * ks)
+                    or (vp < end and o < vp + 2 * tokens * vs)):
+                nk, nv = heads_k * dim_k, heads_v * dim_v
+                for name, p, stride, n in (("q", qp, qs, nk), ("k", kp, ks, nk), ("v", vp, vs, nv)):
+                    if _rows_meet(p, stride, n, o, os_, nv, tokens):
+                        _refuse(f"out is or overlaps {name}, which is still read")
+        return st, tokens, (qp, qs, kp, ks, vp, vs, a.data_ptr(), as_, b.data_ptr(), bs, al, dt,
+                            heads_k, heads_v, dim_k, dim_v, scale, eps, o, os_)
 
     def delta_prompt(self, slots: _abi.Slots, state: torch.Tensor, offsets: torch.Tensor,
                      q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, a: torch.Tensor,

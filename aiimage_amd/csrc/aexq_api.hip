@@ -2602,6 +2602,29 @@ extern "C" aexq_status aexq_delta_decode(aexq_ctx* ctx, const aexq_slots* slots,
   return AEXQ_OK;
 }
 
+// Whether some of `rows` fp16 rows at a share memory with some of those at b: `width`
+// elements of each stride.
+static bool rows_meet(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
+                      long long width, int rows) {
+  const long long at = ((const char*)b - (const char*)a) / 2, last = rows - 1;
+  if (at >= last * a_stride + width || -at >= last * b_stride + width) return false;
+  if (a_stride == b_stride) {  // row i of b begins `place` into row i + by of a
+    const long long by = (at - (at < 0 ? a_stride - 1 : 0)) / a_stride, place = at - by * a_stride;
+    return (place < width && llabs(by) < rows) || (place + width > a_stride && llabs(by + 1) < rows);
+  }
+  for (int i = 0; i < rows; ++i) {  // the last row of a that begins before the end of row i of b
+    const long long begin = at + i * b_stride;
+    if (begin + width <= 0) continue;
+    const long long row = (begin + width - 1) / a_stride;
+    if ((row < last ? row : last) * a_stride + width > begin) return true;
+  }
+  return false;
+}
+// Whether `a` bytes at p and `b` at q share some.
+static bool bytes_meet(const void* p, long long a, const void* q, long long b) {
+  return (const char*)p < (const char*)q + b && (const char*)q < (const char*)p + a;
+}
+
 extern "C" aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t x_stride,
                                           const void* z, int64_t z_stride, const float* gamma,
                                           float eps, int tokens, int heads, int dim, void* out,
@@ -2634,6 +2657,10 @@ extern "C" aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t 
   p.eps = eps;
   if (gated_norm_groups(p.rows, dim) > kMostGroups)
     return fail(AEXQ_ERR_UNSUPPORTED, op, "%d tokens of %d heads in one call", tokens, heads);
+  const long long row = (long long)heads * dim;
+  if ((out != x && rows_meet(x, x_stride, out, out_stride, row, tokens)) ||
+      (out != z && rows_meet(z, z_stride, out, out_stride, row, tokens)))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "out overlaps x or z, rows of which are still read");
   HIP_TRY(op, hipSetDevice(ctx->device));
   const hipError_t e = gated_norm_launch(p, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, op, "norm launch");
@@ -2665,8 +2692,20 @@ extern "C" aexq_status aexq_verify_drafts(aexq_ctx* ctx, const aexq_tensor* logi
   if (draft_probs && (draft_stride < v.width || draft_stride > 1 << 28))
     return fail(AEXQ_ERR_SHAPE, op, "draft_probs rows %lld elements apart hold %d values",
                 (long long)draft_stride, v.width);
-  if ((const void*)drafts == (const void*)tokens)
+  if (bytes_meet(tokens, 4LL * v.rows, drafts, 4LL * v.rows))
     return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens are drafts, which are still read");
+  // (a sequence's are written while others' are read)
+  struct {
+    const void* data;
+    long long values;
+  } const inputs[] = {{offsets, sequences + 1LL}, {accept_u, v.rows}, {sample_u, sequences},
+                      {temperature, temperature ? sequences : 0}, {drafts, v.rows}};
+  for (const auto& in : inputs)
+    if (bytes_meet(tokens, 4LL * v.rows, in.data, 4 * in.values) ||
+        bytes_meet(counts, 4LL * sequences, in.data, 4 * in.values))
+      return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens or counts overlap an input");
+  if (bytes_meet(tokens, 4LL * v.rows, counts, 4LL * sequences))
+    return fail(AEXQ_ERR_INVALID_ARGUMENT, op, "tokens overlap counts");
   VerifyParams p{};
   p.x = v.data;
   p.f16 = esize == 2;

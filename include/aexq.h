@@ -485,7 +485,8 @@ typedef struct aexq_slots {
  * in fp32, act silu or none.  state: device fp16 [count][width - 1][channels], the
  * inputs before the first, oldest first.  weight, bias (nullable): device fp32
  * [channels][width], [channels].  channels a multiple of 8, width 2 to 5.  out NULL:
- * the states alone.  out is not x. */
+ * the states alone.  out shares no memory with x (which is still read when rows of
+ * out are written; views of one buffer may lie beside one another). */
 aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
                             const int32_t* offsets, int tokens, const void* x, int64_t x_stride,
                             const float* weight, const float* bias, int channels, int width,
@@ -499,8 +500,8 @@ aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
  * q, k fp16 [tokens][heads_k][dim_k], v, out fp16 [tokens][heads_v][dim_v], a, b fp16
  * [tokens][heads_v] (2-byte aligned, any stride), a_log, dt_bias device fp32
  * [heads_v], state device fp32 [count][heads_v][dim_k][dim_v].  dim_k is 64 or 128,
- * dim_v 64, 128 or 256, eps above 0, scale finite.  out NULL: the states alone; out is
- * none of the inputs.  States and sums are fp32.  What follows a value that is not
+ * dim_v 64, 128 or 256, eps above 0, scale finite.  out NULL: the states alone; out
+ * shares no memory with the inputs.  States and sums are fp32.  What follows a value that is not
  * finite in its column of the state is not finite (an infinity or a NaN); what comes
  * before it, other columns, heads and sequences do not meet it.  Uses the context's
  * scratch, 25 KB for 64 rows of a value head and 3 dim_k fp16 for each of a key head's. */
@@ -522,7 +523,8 @@ aexq_status aexq_delta_decode(aexq_ctx* ctx, const aexq_slots* slots, float* sta
 
 /* Root-mean-square norm of each head's row, gated: out = x rsqrt(max(mean(x^2) + eps,
  * 1e-20)) gamma silu(z) in fp32; x, z, out fp16 [tokens][heads][dim], dim a multiple of
- * 8 up to 512, gamma device fp32 [dim] or NULL.  out may be x or z, rows as far apart. */
+ * 8 up to 512, gamma device fp32 [dim] or NULL.  out may be x or z, rows as far apart,
+ * and shares no memory with either otherwise. */
 aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t x_stride, const void* z,
                                int64_t z_stride, const float* gamma, float eps, int tokens,
                                int heads, int dim, void* out, int64_t out_stride);
@@ -542,8 +544,9 @@ aexq_status aexq_gated_rmsnorm(aexq_ctx* ctx, const void* x, int64_t x_stride, c
  * probabilities: its draft does not stay and its token is -1.
  * counts[s] (device int32): rows that stay, the new token's included (what slots.counts
  * takes); tokens (device int32 [rows]): the drafts that stay, the new token, -1 in the
- * rows behind.  Rows of no sequence are not touched.  Weights and sums are 64 bits.
- * Up to 2^20 rows.  Uses the context's scratch. */
+ * rows behind.  Rows of no sequence are not touched.  tokens and counts share no memory
+ * with each other or with the inputs.  Weights and sums are 64 bits.  Up to 2^20 rows.
+ * Uses the context's scratch. */
 aexq_status aexq_verify_drafts(aexq_ctx* ctx, const aexq_tensor* logits, const int32_t* offsets,
                                int sequences, const int32_t* drafts, const float* draft_probs,
                                int64_t draft_stride, const float* temperature,

@@ -198,3 +198,41 @@ def test_delta_odd_values_of_short_sequences(aexq, ctx):
     assert torch.equal(~torch.isfinite(out), odd) and torch.equal(~torch.isfinite(left), odd_state)
     assert torch.equal(out.masked_fill(odd, 0), clean.masked_fill(odd, 0))
     assert torch.equal(left.masked_fill(odd_state, 0), clean_state.masked_fill(odd_state, 0))
+
+
+# ---------------------------------------------------------------- refusals
+
+def test_outputs_over_inputs_are_refused(aexq, ctx):
+    """out inside the rows of an input, by rows or by columns; beside them it may lie."""
+    from aiimage_amd import _abi
+    print("[gpu-case] outputs over inputs", flush=True)
+    n, hk, hv, d = 20, 1, 2, 64
+    wide = _randn(n + 1, 8 * d, seed=20).half()
+    part = lambda at, h, row=0: wide[row:row + n, at * d:(at + h) * d].unflatten(1, (h, d))  # noqa: E731
+    g = _inputs(n, hk, hv, d, d, seed=21)
+    args = dict(q=part(0, hk), k=part(1, hk), v=part(2, hv), **{x: g[x] for x in ("a", "b", "a_log",
+                                                                                   "dt_bias")}, scale=0.1)
+    state, conv, w = _randn(n, hv, d, d, seed=22), _randn(1, 3, 2 * d, seed=23).half(), _randn(2 * d, 4)
+    one, off, before = aexq.slots(n, 1), ref.offsets([n]), wide.clone()
+    for at, row in ((0, 0), (1, 0), (2, 0), (3, 0), (2, 1), (0, 1)):
+        with pytest.raises(_abi.ArgumentError, match="overlaps"):
+            ctx.delta_prompt(one, state, off, **args, out=part(at, hv, row))
+        with pytest.raises(_abi.ArgumentError, match="overlaps"):
+            ctx.delta_decode(aexq.slots(n, n), state, **args, out=part(at, hv, row))
+    x = wide[:n, 2 * d:4 * d]
+    for out in (x, wide[1:, 2 * d:4 * d], wide[:n, 2 * d + 8:4 * d + 8], wide[1:, d:3 * d]):
+        with pytest.raises(_abi.ArgumentError, match="overlaps"):
+            ctx.short_conv(aexq.slots(1, 1), conv, off, x, w, out)
+    with pytest.raises(_abi.ArgumentError, match="overlaps"):
+        ctx.gated_rmsnorm(part(2, hv), part(4, hv), None, part(2, hv, 1))
+    assert torch.equal(wide, before)
+    begin = state.clone()
+    ctx.delta_prompt(one, state, off, **args, out=part(4, hv))
+    ctx.short_conv(aexq.slots(1, 1), conv, off, x, w, wide[:n, 6 * d:])
+    torch.cuda.synchronize()
+    y, near, _, _ = ref.delta(**args, state=begin[0], eps=1e-6)
+    ref.check(part(4, hv), y, near)
+    y, near, _ = ref.short_conv(x, _randn(1, 3, 2 * d, seed=23).half()[0], w, None, True)
+    ref.check(wide[:n, 6 * d:], y, near)
+    assert torch.equal(wide[:, :4 * d], before[:, :4 * d])
+    assert torch.equal(wide[n], before[n])
