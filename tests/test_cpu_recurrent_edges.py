@@ -78,3 +78,48 @@ for args in ((PTR, 384, PTR + 256, 384, PTR + 512, 384), (PTR, 128, PTR, 128, PT
 assert lib.aexq_verify_drafts(ctx, logits, PTR, 3, PTR, None, 0, None, PTR, PTR, PTR + 36,
                               PTR + 48) == 0, lib.aexq_last_error()
 """)
+
+
+# ---- scratch: sizes whose need is so little above a power of two that what is allocated
+# for it without any one of its parts does not hold it
+
+@pytest.mark.parametrize("sequences,rows,vocab,f16", [(7, 35, 5000, True), (10, 10, 5000, False),
+                                                      (28, 35, 33000, True)])
+def test_scratch_of_a_verification_holds_all_of_its_parts(tmp_path, sequences, rows, vocab, f16):
+    """Of each sequence what was decided and what its row sums to, of each of its runs two
+    sums; of each row its draft, of each of its parts a sum, a logit and an index."""
+    chunks = (vocab * (2 if f16 else 4) + 15) // 16
+    parts = max(1, min(64, (8 * 256 + rows - 1) // rows, (chunks + 511) // 512))
+    runs = min(256, ((vocab + 255) // 256 + 3) // 4 * 4)
+    held = [16 * sequences, 16 * sequences, 16 * rows, 16 * sequences * runs, 8 * rows * parts,
+            4 * rows * parts, 4 * rows * parts]
+    need, power = sum(held), 4096
+    while 2 * power < need:
+        power *= 2
+    assert need - min(held) <= power < need
+    fake_hip.run(tmp_path, PRELUDE + f"""
+logits.logical = logits.storage = _abi.Shape(2, {vocab}, {rows}, 1, 1)
+logits.dtype = _abi.{"DTYPE_F16" if f16 else "DTYPE_F32"}
+before = fake.fake_bytes()
+assert lib.aexq_verify_drafts(ctx, logits, PTR, {sequences}, PTR, PTR, {vocab}, PTR, PTR, PTR,
+                              PTR + 4096, PTR + 8192) == 0, lib.aexq_last_error()
+got = fake.fake_bytes() - before
+assert {need} <= got <= {2 * need}, got
+""")
+
+
+def test_scratch_of_the_delta_rule_holds_its_list_of_long_sequences(tmp_path):
+    """Blocks that fill a power of two but for 64 bytes, and behind them the number of the
+    sequences of more than 16 rows and their names."""
+    n, tokens, hk, hv, dk, dv = 89, 44 * 64, 1, 3, 128, 128
+    blocks = (tokens // 64 + n) * (hv * (24 * 1024 + 4 * 64 * 4 + 64) + hk * 3 * 64 * dk * 2)
+    assert blocks == 2 ** 24 - 64 and blocks + 4 * (n + 1) > 2 ** 24
+    fake_hip.run(tmp_path, PRELUDE + f"""
+before = fake.fake_bytes(), fake.fake_launches()
+assert lib.aexq_delta_prompt(ctx, slots(sequences={n}, count={n}), PTR, PTR, {tokens}, PTR, {hk * dk}, PTR,
+    {hk * dk}, PTR, {hv * dv}, PTR, {hv}, PTR, {hv}, PTR, PTR, {hk}, {hv}, {dk}, {dv}, 0.1, 1e-6,
+    PTR + 64, {hv * dv}) == 0, lib.aexq_last_error()
+assert fake.fake_launches() - before[1] == 3    # (the sequences of up to 16 rows go apart)
+got = fake.fake_bytes() - before[0]
+assert {blocks + 4 * (n + 1)} <= got, got
+""")
