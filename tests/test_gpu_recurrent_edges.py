@@ -200,6 +200,112 @@ def test_delta_odd_values_of_short_sequences(aexq, ctx):
     assert torch.equal(left.masked_fill(odd_state, 0), clean_state.masked_fill(odd_state, 0))
 
 
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 256)])
+@pytest.mark.parametrize("n", [1, 16, 17, 18, 31, 32, 33, 40, 48, 49, 63, 65, 81, 90, 96, 100])
+def test_delta_rows_behind_the_last_one(aexq, ctx, n, dk, dv):
+    """Rows around a sequence's, more than a block of them, hold NaN: nothing of them is
+    read, and their outputs stay."""
+    print(f"[gpu-case] delta rows behind {n} {dk}x{dv}", flush=True)
+    hk, hv, room = 1, 2, 130
+    total = n + 2 * room
+    d = _inputs(total, hk, hv, dk, dv, seed=7)
+    here = slice(room, room + n)
+    for x in ("q", "k", "v", "a", "b"):
+        d[x][:room], d[x][room + n:] = NAN, NAN
+    state = _randn(1, hv, dk, dv, seed=8)
+    begin, out = state.clone(), torch.full((total, hv, dv), 7.0, device="cuda").half()
+    ctx.delta_prompt(aexq.slots(1, 1), state, ref.offsets([n]) + room, **d, out=out, scale=0.1)
+    torch.cuda.synchronize()
+    y, near, S, err = ref.delta(**_rows(d, here), state=begin[0], scale=0.1, eps=1e-6)
+    ref.check(out[here], y, near)
+    ref.check(state[0], S, err)
+    assert (out[:room] == 7).all() and (out[room + n:] == 7).all()
+
+
+@pytest.mark.parametrize("lens,hk,hv,dk,dv", [([5000, 3001], 1, 2, 128, 128), ([4100], 2, 2, 64, 64)])
+def test_delta_of_thousands_of_rows(aexq, ctx, lens, hk, hv, dk, dv):
+    """Tens of blocks in turn, with decays that forget and decays that keep."""
+    print(f"[gpu-case] delta of {lens} rows", flush=True)
+    n = sum(lens)
+    d = _inputs(n, hk, hv, dk, dv, seed=9)
+    d["dt_bias"][0] = -7.0          # keeps some thousand rows
+    state = _randn(len(lens), hv, dk, dv, seed=10)
+    begin, out = state.clone(), torch.zeros((n, hv, dv), device="cuda").half()
+    ctx.delta_prompt(aexq.slots(len(lens), len(lens)), state, ref.offsets(lens), **d, out=out,
+                     scale=dk ** -0.5)
+    torch.cuda.synchronize()
+    at = 0
+    for i, m in enumerate(lens):
+        y, near, S, err = ref.delta(**_rows(d, slice(at, at + m)), state=begin[i], scale=dk ** -0.5,
+                                    eps=1e-6)
+        ref.check(out[at:at + m], y, near, f"sequence {i}")
+        ref.check(state[i], S, err, f"state {i}")
+        at += m
+
+
+@pytest.mark.parametrize("n,drafted,hk,hv,dk,dv", [
+    (3, 8, 2, 4, 128, 128), (1, 5, 4, 16, 128, 128), (48, 8, 2, 16, 128, 128),
+    (20, 40, 4, 16, 128, 128),     # too long to go apart with their drafts, not without them
+    (20, 100, 4, 16, 64, 256)])
+def test_states_behind_accepted_rows_are_those_of_these_rows_alone(aexq, ctx, n, drafted, hk, hv, dk,
+                                                                  dv):
+    """Bit for bit, whichever kernels either call takes."""
+    print(f"[gpu-case] accepted rows of {n} x {drafted} {hk}/{hv} {dk}x{dv}", flush=True)
+    c = 2 * hk * dk + hv * dv
+    g = torch.Generator().manual_seed(n + drafted)
+    kept = [int(torch.randint(1, min(drafted, 20) + 1, (1,), generator=g)) for _ in range(n)]
+    kept[0] = drafted
+    x, w = _randn(n * drafted, c, seed=11).half(), _randn(c, 4, seed=12)
+    d = _inputs(n * drafted, hk, hv, dk, dv, seed=13)
+    gates = [d.pop(t) for t in ("a_log", "dt_bias")]
+    conv, state = _randn(n, 3, c, seed=14).half(), _randn(n, hv, dk, dv, seed=15)
+    rows = torch.cat([torch.arange(k, device="cuda") + drafted * s for s, k in enumerate(kept)])
+    got = []
+    for whole in (True, False):
+        s, t = conv.clone(), state.clone()
+        off = ref.offsets([drafted] * n if whole else kept)
+        slots = aexq.slots(n, n, counts=ref.i32(kept) if whole else None)
+        y, e = (x, d) if whole else (x[rows], {k: v[rows] for k, v in d.items()})
+        ctx.short_conv(slots, s, off, y, w, None)
+        ctx.delta_prompt(slots, t, off, **e, a_log=gates[0], dt_bias=gates[1], out=None, scale=0.1)
+        torch.cuda.synchronize()
+        got.append((s, t))
+    assert torch.equal(got[0][0], got[1][0])
+    assert torch.equal(got[0][1], got[1][1])
+
+
+# ---------------------------------------------------------------- drafted tokens
+
+def test_verify_numbers_next_to_a_border(aexq, ctx):
+    """A flat row of 151936 logits, and for each row the two numbers of 32 bits on either
+    side of a border between two tokens.  Weights within 2^-39 of theirs place the border,
+    at most 1, within 2^-38 of its place; of 64 borders that one is taken whose nearer
+    neighbour is nearest, but no nearer than 2^-36."""
+    print("[gpu-case] verify numbers next to a border", flush=True)
+    vocab, n, some = 151936, 12, 64
+    x = 0.5 * _randn(n, vocab, seed=16)
+    p = torch.softmax(x.double(), -1).cumsum(-1)
+    p /= p[:, -1:].clone()
+    at = (vocab * _rand(n, some, seed=17)).long().clamp(max=vocab - 2)
+    border = p.gather(1, at)
+    near = border.float()
+    up = torch.where(near.double() > border, near, torch.nextafter(near, torch.full_like(near, 2.0)))
+    down = torch.nextafter(up, torch.zeros_like(up))
+    gap = torch.minimum(up.double() - border, border - down.double())
+    pick = torch.where(gap >= 2.0 ** -36, gap, 1.0).argmin(-1, keepdim=True)
+    at, up, down = (t.gather(1, pick)[:, 0] for t in (at, up, down))
+    assert (gap.gather(1, pick) < 2.0 ** -27).all()
+    for su, step in ((up, 1), (down, 0)):
+        counts = torch.zeros(n, dtype=torch.int32, device="cuda")
+        tokens = torch.zeros(n, dtype=torch.int32, device="cuda")
+        ctx.verify_drafts(aexq.describe(x, n, vocab), ref.offsets([1] * n),
+                          torch.zeros(n, dtype=torch.int32, device="cuda"), _rand(n, seed=18), su,
+                          counts, tokens)
+        torch.cuda.synchronize()
+        assert counts.tolist() == [1] * n
+        assert tokens.tolist() == (at + step).tolist()
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_outputs_over_inputs_are_refused(aexq, ctx):
