@@ -69,8 +69,9 @@ __device__ __forceinline__ float rows_max(float v) {
 //
 // fp32 results from fp16 matrix products: k and q are fp16 already and taken as they
 // are, their lengths put into the rows' factors; S, T, P, R and U are split into two fp16
-// numbers, x = x0 + x1 up to 2^-22 of x, scaled by powers of two so that neither part
-// leaves fp16's range.  (P in one part, 2^-11 of it, takes outputs half as far again from
+// numbers, x = x0 + x1, scaled by powers of two so that neither part leaves fp16's range:
+// up to 2^-22 of x, and where x1 is too small for that (x below 2^-16 of the largest of its
+// column in the block) up to 2^-38 of that one; of T and P, which are at most 1, 2^-36.  (P in one part, 2^-11 of it, takes outputs half as far again from
 // the exact ones as their own rounding does.)
 //
 // Pieces of T and P lie in scratch in the order in which a lane of a matrix product
@@ -149,7 +150,7 @@ struct BlockLds {
 //
 // Bound by memory: a block reads 32 KB of k and q (heads of 128) and writes 48 KB of them
 // in the products' order and 25 KB of T, P and factors for each value head.  16384 rows of
-// 16 key and 32 value heads: 99 us for 540 MB (a copy of that size runs at 5.3 TB/s).
+// 16 key and 32 value heads: 97 us for 560 MB (a copy of that size runs at 5.3 TB/s).
 template <int DK>
 __global__ __launch_bounds__(kThreads, 4) void delta_block_kernel(const DeltaParams p) {
   constexpr int KB = DK / 32;
@@ -621,7 +622,7 @@ __device__ __forceinline__ bool delta_end(DeltaWave<DK>& x, int b, bool first) {
 // A block takes the first wave 1.8 us: 82 matrix products (1300 cycles), 300 vector
 // operations, which hide behind them in part, and 45 loads, each of which holds it up for
 // 20 to 30 cycles, all in one chain from state to state.  16384 rows of 32 value heads of
-// 128 x 128, one sequence: 462 us, 256 blocks in turn; 9600 rows of 12 sequences and 16
+// 128 x 128, one sequence: 462 us, 256 blocks in turn; 6657 rows of 12 sequences and 16
 // heads: 83 us.  Steps on the way, in that order: one wave for all of it 777 and 112 us;
 // eight waves that each hold 16 rows of S of 16 columns and add their products through
 // LDS: 450 and 103 (but 77 for blocks of 16 rows, where the last ones now go through one

@@ -501,10 +501,14 @@ aexq_status aexq_short_conv(aexq_ctx* ctx, const aexq_slots* slots, void* state,
  * [tokens][heads_v] (2-byte aligned, any stride), a_log, dt_bias device fp32
  * [heads_v], state device fp32 [count][heads_v][dim_k][dim_v].  dim_k is 64 or 128,
  * dim_v 64, 128 or 256, eps above 0, scale finite.  out NULL: the states alone; out
- * shares no memory with the inputs.  States and sums are fp32.  What follows a value that is not
- * finite in its column of the state is not finite (an infinity or a NaN); what comes
- * before it, other columns, heads and sequences do not meet it.  Uses the context's
- * scratch, 25 KB for 64 rows of a value head and 3 dim_k fp16 for each of a key head's. */
+ * shares no memory with the inputs.  States and sums are fp32.  What follows a value
+ * that is not finite in its column of the state is not finite (an infinity or a NaN);
+ * what comes before it, other columns, heads and sequences do not meet it.  Uses the
+ * context's scratch: tokens / 64 + sequences blocks (a sequence has one of its own however short),
+ * each 25.06 KB a value head and 384 dim_k bytes a key head, together rounded up to a power
+ * of two; what a larger call outgrows stays until the context ends.  16384 tokens of 16 key
+ * and 32 value heads of 128 take 0.41 GB (0.54 allocated), 2^20 take 26 (34), and so do some
+ * 16000 sequences of a row each, which aexq_delta_decode takes without. */
 aexq_status aexq_delta_prompt(aexq_ctx* ctx, const aexq_slots* slots, float* state,
                               const int32_t* offsets, int tokens, const void* q, int64_t q_stride,
                               const void* k, int64_t k_stride, const void* v, int64_t v_stride,
