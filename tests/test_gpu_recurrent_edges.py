@@ -172,6 +172,39 @@ def test_delta_odd_values_leave_other_columns_alone(aexq, ctx, n, dk, dv):
     assert torch.equal(left[0].transpose(1, 2)[good], clean_state[0].transpose(1, 2)[good])
 
 
+def test_delta_odd_values_in_every_column_and_without_outputs(aexq, ctx):
+    """Each of 16 columns stops being finite in another block, two in the last: the states
+    of a call that has no outputs are those of one that has, and a call that reads states
+    alone leaves them."""
+    print("[gpu-case] delta odd values in every column", flush=True)
+    n, hv, dk, dv = 14 * 64 + 30, 1, 128, 64
+    d = _inputs(n, 1, hv, dk, dv, seed=24)
+    state = _randn(1, hv, dk, dv, seed=25)
+    clean = torch.zeros((n, hv, dv), device="cuda").half()
+    ctx.delta_prompt(aexq.slots(1, 1, read_only=True), state, ref.offsets([n]), **d, out=clean, scale=0.1)
+    place = [min(64 * c + 5 * c, n - 1) for c in range(16)]
+    for c, t in enumerate(place):
+        d["v"][t, 0, 16 + c] = NAN
+    y, near, _, _ = ref.delta(**dict(d, v=d["v"].nan_to_num(0.0)), state=state[0], scale=0.1, eps=1e-6)
+    states, out = [], torch.zeros((n, hv, dv), device="cuda").half()
+    for o, only in ((out, False), (None, False), (out.clone(), True)):
+        s = state.clone()
+        ctx.delta_prompt(aexq.slots(1, 1, read_only=only), s, ref.offsets([n]), **d, out=o, scale=0.1)
+        torch.cuda.synchronize()
+        states.append(s)
+    assert torch.equal(states[2], state)
+    for c, t in enumerate(place):
+        assert not torch.isfinite(out[t:, 0, 16 + c]).any()
+        ref.check(out[:t, 0, 16 + c], y[:t, 0, 16 + c], near[:t, 0, 16 + c], f"column {16 + c}")
+        assert torch.equal(out[:t // 64 * 64, 0, 16 + c], clean[:t // 64 * 64, 0, 16 + c])
+    odd = torch.zeros(dv, dtype=torch.bool, device="cuda")
+    odd[16:32] = True
+    assert torch.equal(out[..., ~odd], clean[..., ~odd])
+    for s in states[:2]:
+        assert torch.equal(~torch.isfinite(s), odd.expand_as(s))
+    assert torch.equal(states[0][..., ~odd], states[1][..., ~odd])
+
+
 def test_delta_odd_values_of_short_sequences(aexq, ctx):
     """The same where there are many sequences of a few rows each."""
     print("[gpu-case] delta odd values, short sequences", flush=True)
